@@ -32,6 +32,8 @@ typedef struct qmlp_activation_s* qmlp_activation_t;
 
 /* qmlp::Tensor::Precision / ::Usage (src_cpp/include/qmlp/tensor.h:25-38) */
 enum { QMLP_FLOAT = 0, QMLP_HALF = 1, QMLP_DOUBLE = 2 };
+/* Further types of the operators on rows of tokens (qmlp_tokens_*); everything else refuses them. */
+enum { QMLP_BFLOAT16 = 3, QMLP_INT32 = 4, QMLP_INT64 = 5 };
 enum { QMLP_INFERENCE = 0, QMLP_GRADIENTS = 1 };
 /* qmlp::FusedNetwork::AdjointMode (src_cpp/include/qmlp/fused_network.h:22-33) */
 enum { QMLP_GRADIENTS_INPUT = 1, QMLP_GRADIENTS_NETWORK_WEIGHTS = 2, QMLP_GRADIENTS_INPUT_ENCODINGS = 4 };
@@ -262,6 +264,45 @@ int qmlp_utils_pullpush_adjoint_in(const qmlp_tensor* mask, const qmlp_tensor* d
 /* Compiles the pull-push kernels for QMLP_FLOAT or QMLP_DOUBLE into the kernel cache without a
  * device (the reference compiles them on first use, src_cpp/src/utils.cpp:12-35 and :145-180). */
 int qmlp_utils_pullpush_precompile(int precision);
+
+/* ---- operators on rows of tokens: no counterpart in the reference ----
+ * Values are float, half or bfloat16; rows are the first dimension, the last one has stride 1. Indices are 32- or 64-bit
+ * integers. Gradients are written as a whole, not added to. These calls allocate nothing and do not synchronise: `memory` is
+ * device memory of the caller, aligned to 256 bytes, of the size that the function beside reports (NULL where that is 0). An
+ * undefined tensor (NULL or ndim = 0) leaves an optional input or output out. */
+/* order (rows) and offsets (groups + 1), both INT32: the rows by the group that index (rows) names, in their own order within a
+ * group; group g has the entries offsets[g] .. offsets[g + 1] - 1. Rows whose index is not in 0 .. groups - 1 come last. */
+int qmlp_tokens_group_memory(long long rows, int groups, size_t* bytes);
+int qmlp_tokens_group(const qmlp_tensor* index, int groups, const qmlp_tensor* order, const qmlp_tensor* offsets, void* memory,
+                      void* stream);
+/* output[i] = scale * table[index[i]], zero where the index names no row: table (vocabulary, channels), output (rows, channels). */
+int qmlp_tokens_embedding(const qmlp_tensor* index, const qmlp_tensor* table, float scale, const qmlp_tensor* output, void* stream);
+/* adj_table[v] = scale * the sum of the adj_output[i] with index[i] = v, bit for bit the same for the same inputs. */
+int qmlp_tokens_embedding_adjoint_memory(long long rows, long long vocabulary, int channels, size_t* bytes);
+int qmlp_tokens_embedding_adjoint(const qmlp_tensor* index, const qmlp_tensor* adj_output, float scale, const qmlp_tensor* adj_table,
+                                  void* memory, void* stream);
+/* output = (input - mean) / sqrt(variance + epsilon) * weight + bias over the channels of every row of input (rows, channels).
+ * weight, bias (channels): of the input's type or FLOAT, both of one type, optional. mean, rstd (rows, FLOAT; rstd = 1 / sqrt(variance +
+ * epsilon)): outputs for the adjoint, optional. */
+int qmlp_tokens_layer_norm(const qmlp_tensor* input, const qmlp_tensor* weight, const qmlp_tensor* bias, float epsilon,
+                           const qmlp_tensor* output, const qmlp_tensor* mean, const qmlp_tensor* rstd, void* stream);
+/* The gradients (each optional); input, mean, rstd as the call above saw and left them. */
+int qmlp_tokens_layer_norm_adjoint_memory(long long rows, int channels, size_t* bytes);
+int qmlp_tokens_layer_norm_adjoint(const qmlp_tensor* input, const qmlp_tensor* weight, const qmlp_tensor* mean, const qmlp_tensor* rstd,
+                                   const qmlp_tensor* adj_output, const qmlp_tensor* adj_input, const qmlp_tensor* adj_weight,
+                                   const qmlp_tensor* adj_bias, void* memory, void* stream);
+/* output[r] = weight[e] input[r] + bias[e] for offsets[e] <= r < offsets[e + 1]: input (rows, inputs), weight (experts, outputs, inputs),
+ * offsets (experts + 1, INT32, device memory, not decreasing, from 0 on), bias (experts, outputs; optional), output (rows, outputs).
+ * Rows behind the last expert's get zeros. */
+int qmlp_tokens_grouped_linear(const qmlp_tensor* input, const qmlp_tensor* weight, const qmlp_tensor* offsets, const qmlp_tensor* bias,
+                               const qmlp_tensor* output, void* stream);
+/* The gradients (each optional; adj_weight and adj_bias contiguous). */
+int qmlp_tokens_grouped_linear_adjoint_memory(long long rows, int experts, int inputs, int outputs, size_t* bytes);
+int qmlp_tokens_grouped_linear_adjoint(const qmlp_tensor* input, const qmlp_tensor* weight, const qmlp_tensor* offsets,
+                                       const qmlp_tensor* adj_output, const qmlp_tensor* adj_input, const qmlp_tensor* adj_weight,
+                                       const qmlp_tensor* adj_bias, void* memory, void* stream);
+/* Compiles the kernels for values of QMLP_FLOAT, QMLP_HALF or QMLP_BFLOAT16 into the kernel cache without a device. */
+int qmlp_tokens_precompile(int precision);
 
 #ifdef __cplusplus
 }

@@ -18,13 +18,13 @@ QUICKMLP_NAMESPACE_BEGIN
 
 /**
  * Describes an N-dimensional strided tensor in device memory.
- * Datatype can be 'float', 'half' or 'double'.
+ * Datatype can be 'float', 'half' or 'double'; the operators on rows of tokens (tokens.h) know 'bfloat16' and integers besides.
  * Either wraps external memory (non-owning) or hosts its own allocation.
  */
 class Tensor
 {
 public:
-    enum Precision { FLOAT, HALF, DOUBLE, _NUM_PRECISION_ };
+    enum Precision { FLOAT, HALF, DOUBLE, BFLOAT16, INT32, INT64, _NUM_PRECISION_ };
     static const int BytesPerEntry[];
     static const std::string DatatypePerEntry[];
     static const std::string NamePerEntry[];
@@ -50,6 +50,12 @@ private:
             throw configuration_error("Illegal type, the tensor stores half data!");
         if (precision_ == DOUBLE && !std::is_same_v<double, U>)
             throw configuration_error("Illegal type, the tensor stores double data!");
+        if (precision_ == BFLOAT16)   // (no type of the host)
+            throw configuration_error("Illegal type, the tensor stores bfloat16 data!");
+        if (precision_ == INT32 && !std::is_same_v<int32_t, U>)
+            throw configuration_error("Illegal type, the tensor stores 32-bit integers!");
+        if (precision_ == INT64 && !std::is_same_v<int64_t, U>)
+            throw configuration_error("Illegal type, the tensor stores 64-bit integers!");
     }
 
 public:
@@ -140,6 +146,8 @@ public:
             std::vector<half> data(n);
             for (int64_t i = 0; i < n; ++i) data[i] = static_cast<half>(distr(rng));
             copyFromHost(data.data(), sizeof(half) * n);
+        } else if (precision_ != DOUBLE) {
+            throw configuration_error("random numbers are for float, half and double tensors");
         } else {
             std::vector<double> data(n);
             for (int64_t i = 0; i < n; ++i) data[i] = distr(rng);

@@ -1,0 +1,403 @@
+#pragma once
+// The linear layer of every expert on its own rows, and its adjoint.
+//
+//   y[r] = W[e] x[r] + b[e]  for the rows r of expert e: offsets[e] <= r < offsets[e + 1];  zero for rows behind the last expert's
+//   dx[r] = W[e]^T dy[r],    dW[e] = sum over the rows of e of dy[r] x[r]^T,    db[e] = sum over the rows of e of dy[r]
+//
+// All three are matrix products C(i, j) = sum over k of A(i, k) B(j, k) in tiles of TI x TJ, with j the index along which the
+// result is consecutive in memory. An operand is consecutive along k (x and W of the first, dy of the second) or along its own
+// index (W of the second, dy and x of the third).
+//
+// How many rows an expert has is known on the device only. The rows of the experts are cut into tiles that begin where the
+// expert does, and the places of the tiles follow without a scan: expert e has the places from e + floor(offsets[e] / TI) on,
+// of which it has always enough, as floor(b / T) - floor(a / T) + 1 >= ceil((b - a) / T). A workgroup finds the expert of its
+// place by a search of 64 steps at a time, and has nothing to do where the expert has fewer tiles than places.
+//
+// Offsets are limited to the rows there are wherever they are read: no access depends on their values.
+
+#include <qmlp/kernels/token_types.h>
+
+QUICKMLP_KERNEL_NAMESPACE_BEGIN
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+// ------------------------------------------------------------------------------------------------ matrix cores
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+/** 16 lanes name 4 consecutive entries each of 4 rows of 16 entries, row by row; each gets the 4 entries of one of the columns. */
+__device__ __forceinline__ s16x4 readTransposed16(const void* p)
+{
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p));
+}
+
+/** Operands of 32 x 32 matrix products: STEP consecutive values of k for two halves of the lanes, 32 rows each. */
+template <typename T>
+struct Matrix;
+template <>
+struct Matrix<f16>
+{
+    typedef f16x8 Operand;
+    typedef f16x4 Quad;
+    static __device__ __forceinline__ f32x16 multiply(Operand a, Operand b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ Quad readTransposed(const f16* p)
+    {
+        return __builtin_bit_cast(Quad, readTransposed16(p));
+    }
+};
+template <>
+struct Matrix<bf16>
+{
+    typedef bf16x8 Operand;
+    typedef bf16x4 Quad;
+    static __device__ __forceinline__ f32x16 multiply(Operand a, Operand b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ Quad readTransposed(const bf16* p)
+    {
+        return __builtin_bit_cast(Quad, readTransposed16(p));
+    }
+};
+template <>
+struct Matrix<float>
+{
+    typedef f32x4 Operand;
+    // the instruction takes one k of each half of the lanes: the operands' k-th ones together
+    static __device__ __forceinline__ f32x16 multiply(Operand a, Operand b, f32x16 c)
+    {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[k], b[k], c, 0, 0, 0);
+        return c;
+    }
+};
+
+// ------------------------------------------------------------------------------------------------ tiles in LDS
+/** Values of k in a tile: 128 bytes of a row. */
+template <typename T>
+constexpr int TILE_K = 128 / static_cast<int>(sizeof(T));
+/** Values of k that an operand of the matrix cores takes of a tile. */
+template <typename T>
+constexpr int STEP_K = 2 * WIDE<T>;
+
+/**
+ * A tile of an operand: SIZE of its indices by TILE_K. ALONG_K: rows of 128 bytes, one for each index; otherwise one row for each k.
+ * It goes from global memory through the registers of all THREADS, 16 bytes at a time, whatever the alignment.
+ * Pieces of a row lie in an order that depends on the row, so that the lanes that read the same piece of different rows find
+ * them in different banks.
+ */
+template <typename T, bool ALONG_K, int SIZE, int THREADS>
+struct Tile
+{
+    static constexpr int PIECE = WIDE<T>;                                  // entries per access
+    static constexpr int ROW = ALONG_K ? TILE_K<T> : SIZE;                 // entries of a row
+    static constexpr int PIECES = ROW / PIECE;                             // of a row
+    static constexpr int EACH = SIZE * 8 / THREADS;                        // pieces per thread
+    static constexpr int BYTES = SIZE * 128;
+    static_assert(SIZE * 8 % THREADS == 0, "every thread moves the same number of pieces");
+
+    T raw[EACH][PIECE];
+
+    /** Place of an entry of the tile. */
+    static __device__ __forceinline__ int place(int row, int column)
+    {
+        if constexpr (ALONG_K) return row * ROW + ((column / PIECE ^ (row & 7)) * PIECE + column % PIECE);
+        else if constexpr (sizeof(T) == 2) {
+            // 32 entries (64 bytes) are read of each of four consecutive rows
+            constexpr int UNITS = ROW / 32;
+            return row * ROW + (((column / 32) ^ (row & (UNITS < 4 ? UNITS - 1 : 3))) * 32 + column % 32);
+        } else
+            return row * ROW + column;
+    }
+
+    /**
+     * Reads the tile whose first index and k are at 'p': 'indices' and 'ks' of them are there (no more than the tile's), the
+     * others are zero. stride: between rows.
+     */
+    __device__ __forceinline__ void read(const T* __restrict__ p, long long stride, int indices, int ks)
+    {
+        const int rows = ALONG_K ? indices : ks, columns = ALONG_K ? ks : indices;
+#pragma unroll
+        for (int n = 0; n < EACH; ++n) {
+            const int piece = n * THREADS + threadIdx.x;
+            const int row = piece / PIECES, column = piece % PIECES * PIECE;
+#pragma unroll
+            for (int k = 0; k < PIECE; ++k) raw[n][k] = static_cast<T>(0);
+            if (row >= rows) continue;
+            const T* from = p + row * stride + column;
+            if (column + PIECE <= columns) __builtin_memcpy(raw[n], from, 16);
+            else {
+#pragma unroll
+                for (int k = 0; k < PIECE; ++k)
+                    if (column + k < columns) raw[n][k] = from[k];
+            }
+        }
+    }
+    __device__ __forceinline__ void write(T* lds) const
+    {
+#pragma unroll
+        for (int n = 0; n < EACH; ++n) {
+            const int piece = n * THREADS + threadIdx.x;
+            __builtin_memcpy(__builtin_assume_aligned(lds + place(piece / PIECES, piece % PIECES * PIECE), 16), raw[n], 16);
+        }
+    }
+
+    /** The operand of the matrix cores for 32 indices from i on and the given step of the tile's k. */
+    static __device__ __forceinline__ typename Matrix<T>::Operand operand(const T* lds, int i, int step)
+    {
+        const int lane = threadIdx.x % 64;
+        if constexpr (ALONG_K) {
+            typename Matrix<T>::Operand v;
+            __builtin_memcpy(&v, __builtin_assume_aligned(lds + place(i + lane % 32, step * STEP_K<T> + lane / 32 * PIECE), 16), 16);
+            return v;
+        } else if constexpr (sizeof(T) == 2) {
+            // of 4 rows by 16 columns that 16 lanes read, each lane gets a column
+            const int row = step * STEP_K<T> + lane / 32 * PIECE + lane % 16 / 4, column = i + lane / 16 % 2 * 16 + lane % 4 * 4;
+            const auto low = Matrix<T>::readTransposed(lds + place(row, column)), high = Matrix<T>::readTransposed(lds + place(row + 4, column));
+            return __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7);
+        } else {
+            typename Matrix<T>::Operand v;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = lds[place(step * STEP_K<T> + lane / 32 * 4 + k, i + lane % 32)];
+            return v;
+        }
+    }
+};
+
+/**
+ * The sums of a tile of TI x TJ by WI x WJ wavefronts. In an accumulator, lane l holds C(i, j) of i = l % 32 and
+ * j = 8 (n / 4) + 4 (l / 32) + n % 4 for n = 0 .. 15: four consecutive j at a time.
+ */
+template <typename T, bool A_ALONG_K, bool B_ALONG_K, int TI, int TJ, int WI, int WJ>
+struct TileProduct
+{
+    static constexpr int THREADS = 64 * WI * WJ;
+    static constexpr int NI = TI / WI / 32, NJ = TJ / WJ / 32;
+    typedef Tile<T, A_ALONG_K, TI, THREADS> TileA;
+    typedef Tile<T, B_ALONG_K, TJ, THREADS> TileB;
+    static constexpr int LDS_BYTES = 2 * (TileA::BYTES + TileB::BYTES);
+
+    f32x16 sums[NI][NJ];
+    f32x16 sumsOfA[NI];   // over k alone
+
+    static __device__ __forceinline__ int firstI() { return threadIdx.x / 64 / WJ * (NI * 32); }
+    static __device__ __forceinline__ int firstJ() { return threadIdx.x / 64 % WJ * (NJ * 32); }
+
+    /** a, b: at the tile's first index and k = 0; ni, nj: indices that are there. sumA: also sums A over k. */
+    __device__ __forceinline__ void run(char* lds, const T* __restrict__ a, long long strideA, int ni, const T* __restrict__ b, long long strideB,
+                                        int nj, int K, bool sumA)
+    {
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            sumsOfA[i] = f32x16{};
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) sums[i][j] = f32x16{};
+        }
+        const long long advanceA = A_ALONG_K ? TILE_K<T> : TILE_K<T> * strideA, advanceB = B_ALONG_K ? TILE_K<T> : TILE_K<T> * strideB;
+        const int fromI = firstI(), fromJ = firstJ();
+        TileA tileA;
+        TileB tileB;
+        int buffer = 0;
+        tileA.read(a, strideA, ni, min(K, TILE_K<T>));
+        tileB.read(b, strideB, nj, min(K, TILE_K<T>));
+        for (int k = 0; k < K; k += TILE_K<T>) {
+            T* const ldsA = reinterpret_cast<T*>(lds + buffer * (TileA::BYTES + TileB::BYTES));
+            T* const ldsB = reinterpret_cast<T*>(lds + buffer * (TileA::BYTES + TileB::BYTES) + TileA::BYTES);
+            tileA.write(ldsA);
+            tileB.write(ldsB);
+            __syncthreads();   // (and the other buffer's readers of the step before are done)
+            if (k + TILE_K<T> < K) {
+                a += advanceA;
+                b += advanceB;
+                const int left = min(K - k - TILE_K<T>, TILE_K<T>);
+                tileA.read(a, strideA, ni, left);
+                tileB.read(b, strideB, nj, left);
+            }
+#pragma unroll
+            for (int step = 0; step < TILE_K<T> / STEP_K<T>; ++step) {
+                typename Matrix<T>::Operand x[NI], w[NJ];
+#pragma unroll
+                for (int i = 0; i < NI; ++i) x[i] = TileA::operand(ldsA, fromI + i * 32, step);
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) w[j] = TileB::operand(ldsB, fromJ + j * 32, step);
+#pragma unroll
+                for (int i = 0; i < NI; ++i)
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) sums[i][j] = Matrix<T>::multiply(w[j], x[i], sums[i][j]);
+                if (sumA) {
+                    typename Matrix<T>::Operand ones;
+#pragma unroll
+                    for (int n = 0; n < static_cast<int>(sizeof(ones) / sizeof(T)); ++n) ones[n] = static_cast<T>(1);
+#pragma unroll
+                    for (int i = 0; i < NI; ++i) sumsOfA[i] = Matrix<T>::multiply(ones, x[i], sumsOfA[i]);
+                }
+            }
+            buffer ^= 1;
+        }
+    }
+
+    /** Hands every four consecutive results to put(i, j, values), with i and j counted from the tile's first ones. */
+    template <typename Put>
+    __device__ __forceinline__ void results(Put put) const
+    {
+        const int lane = threadIdx.x % 64;
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                for (int n = 0; n < 16; n += 4) {
+                    float v[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) v[k] = sums[i][j][n + k];
+                    put(firstI() + i * 32 + lane % 32, firstJ() + j * 32 + n * 2 + lane / 32 * 4, v);
+                }
+    }
+};
+
+/** Up to four consecutive values, as many as are left before 'end'. */
+template <typename T>
+__device__ __forceinline__ void storeUpToFour(T* __restrict__ p, const float (&v)[4], int left)
+{
+    if (left >= 4) storeFloats(p, v);
+    else
+#pragma unroll
+        for (int k = 0; k < 3; ++k)
+            if (k < left) p[k] = static_cast<T>(v[k]);
+}
+
+// ------------------------------------------------------------------------------------------------ experts
+/** offsets[e], never outside of the rows there are; the first expert begins at row 0. */
+__device__ __forceinline__ int expertBegin(const int* __restrict__ offsets, int e, int rows)
+{
+    return e == 0 ? 0 : min(max(offsets[e], 0), rows);
+}
+
+struct ExpertTile
+{
+    int expert;       // the number of experts: rows behind the last one's
+    int index;        // of the tile among the expert's
+    int from, to;     // rows
+    int expertRows;
+};
+
+/** What the given place has; to <= from: nothing. */
+__device__ __forceinline__ ExpertTile expertTile(const int* __restrict__ offsets, int experts, int rows, int tileRows, int place)
+{
+    // the last e of 0 .. experts with e + floor(begin / tileRows) <= place; the first one has that
+    int from = 0, count = experts + 1;
+    while (count > 1) {
+        const int step = (count + 63) / 64;
+        const int e = from + min(static_cast<int>(threadIdx.x % 64) * step, count - 1);
+        const unsigned long long votes = __ballot(e + expertBegin(offsets, e, rows) / tileRows <= place);
+        // (the first lane votes yes: e = from; where the offsets are in order, so do the lanes up to the one looked for)
+        const int lane = max(0, 63 - __clzll(votes));
+        const int chosen = min(lane * step, count - 1);
+        from += chosen;
+        count = min(step, count - chosen);
+    }
+    from = __builtin_amdgcn_readfirstlane(from);
+    const int begin = expertBegin(offsets, from, rows), end = from < experts ? expertBegin(offsets, from + 1, rows) : rows;
+    ExpertTile t;
+    t.expert = from;
+    t.index = place - (from + begin / tileRows);
+    const long long first = begin + static_cast<long long>(max(t.index, 0)) * tileRows;
+    t.from = static_cast<int>(min(first, static_cast<long long>(rows)));
+    t.to = min(end, static_cast<int>(min(first + tileRows, static_cast<long long>(rows))));
+    if (t.index < 0) t.to = t.from;   // (offsets out of order)
+    t.expertRows = max(0, end - begin);
+    return t;
+}
+
+// ------------------------------------------------------------------------------------------------ kernels
+/**
+ * Rows times the experts' matrices: y[r][j] = sum over k of x[r][k] B(j, k) + bias[e][j]. B_ALONG_K: weights[e][j][k] (the layer),
+ * otherwise weights[e][k][j] (its adjoint). Workgroups: places of tiles x tiles of J.
+ */
+template <typename T, bool B_ALONG_K, int TI, int TJ, int WI, int WJ>
+__global__ void __launch_bounds__(64 * WI * WJ)
+GroupedRowsKernel(const T* __restrict__ x, long long strideX, const T* __restrict__ weights, long long strideExpert, long long strideWeights,
+                  const T* __restrict__ bias, long long strideBias, const int* __restrict__ offsets, int experts, T* __restrict__ y, long long strideY,
+                  int rows, int J, int K, int tilesJ)
+{
+    typedef TileProduct<T, true, B_ALONG_K, TI, TJ, WI, WJ> Product;
+    extern __shared__ __attribute__((aligned(16))) char groupedLds[];
+    const ExpertTile at = expertTile(offsets, experts, rows, TI, blockIdx.x / tilesJ);
+    if (at.to <= at.from) return;
+    const int j0 = blockIdx.x % tilesJ * TJ;
+    const int ni = at.to - at.from, nj = min(J - j0, TJ);
+    Product product;
+    const bool none = at.expert >= experts;
+    const T* w = weights + (none ? 0 : at.expert) * strideExpert;
+    product.run(groupedLds, x + at.from * strideX, strideX, ni, w + (B_ALONG_K ? j0 * strideWeights : j0), strideWeights, nj, none ? 0 : K, false);
+    const T* b = bias && !none ? bias + at.expert * strideBias + j0 : nullptr;
+    product.results([&](int i, int j, float (&v)[4]) {
+        if (i >= ni || j >= nj) return;
+        if (b)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (j + k < nj) v[k] += static_cast<float>(b[j + k]);
+        storeUpToFour(y + (at.from + i) * strideY + j0 + j, v, nj - j);
+    });
+}
+
+/**
+ * The adjoint of the weights: adjWeights[e][i][j] = sum over the rows r of e of adjY[r][i] x[r][j], and of the biases, the sums of
+ * adjY (null: not wanted). Workgroups: places of 'chunk' rows x tiles of I x tiles of J. An expert with more rows than a chunk has
+ * its sums per chunk in partial[place], I x J and I floats, for GroupedSumKernel.
+ */
+template <typename T, int TI, int TJ, int WI, int WJ>
+__global__ void __launch_bounds__(64 * WI * WJ)
+GroupedWeightsKernel(const T* __restrict__ adjY, long long strideAdjY, const T* __restrict__ x, long long strideX, const int* __restrict__ offsets,
+                     int experts, T* __restrict__ adjWeights, T* __restrict__ adjBias, float* __restrict__ partial, int rows, int I, int J, int tilesI,
+                     int tilesJ, int chunk)
+{
+    typedef TileProduct<T, false, false, TI, TJ, WI, WJ> Product;
+    extern __shared__ __attribute__((aligned(16))) char groupedLds[];
+    const int tile = blockIdx.x % (tilesI * tilesJ);
+    const ExpertTile at = expertTile(offsets, experts, rows, chunk, blockIdx.x / (tilesI * tilesJ));
+    if (at.expert >= experts || (at.to <= at.from && at.index != 0)) return;   // (the first place of an expert without rows writes zeros)
+    const int i0 = tile / tilesJ * TI, j0 = tile % tilesJ * TJ;
+    const int ni = min(I - i0, TI), nj = min(J - j0, TJ);
+    const bool whole = at.expertRows <= chunk;
+    const bool sumA = adjBias && j0 == 0;
+    Product product;
+    product.run(groupedLds, adjY + at.from * strideAdjY + i0, strideAdjY, ni, x + at.from * strideX + j0, strideX, nj, max(0, at.to - at.from), sumA);
+    const long long size = static_cast<long long>(I) * J;
+    float* sums = whole ? nullptr : partial + (blockIdx.x / (tilesI * tilesJ)) * (size + I);
+    T* out = adjWeights + at.expert * size;
+    if (adjWeights || !whole)
+        product.results([&](int i, int j, float (&v)[4]) {
+            if (i >= ni || j >= nj) return;
+            const long long to = static_cast<long long>(i0 + i) * J + j0 + j;
+            if (whole) storeUpToFour(out + to, v, nj - j);
+            else storeUpToFour(sums + to, v, nj - j);
+        });
+    if (sumA && Product::firstJ() == 0 && threadIdx.x % 64 < 32)
+#pragma unroll
+        for (int n = 0; n < Product::NI; ++n) {
+            const int i = Product::firstI() + n * 32 + threadIdx.x % 32;
+            if (i >= ni) continue;
+            if (whole) adjBias[static_cast<long long>(at.expert) * I + i0 + i] = static_cast<T>(product.sumsOfA[n][0]);
+            else sums[size + i0 + i] = product.sumsOfA[n][0];
+        }
+}
+
+/** Adds up the sums per chunk of the experts that have several. Workgroups: experts x pieces of 256 of their size + I sums. */
+template <typename T>
+__global__ void __launch_bounds__(256)
+GroupedSumKernel(const float* __restrict__ partial, const int* __restrict__ offsets, T* __restrict__ adjWeights, T* __restrict__ adjBias, int rows,
+                 long long size, int I, int chunk, int pieces)
+{
+    const int e = blockIdx.x / pieces;
+    const int begin = expertBegin(offsets, e, rows), end = expertBegin(offsets, e + 1, rows);
+    if (end - begin <= chunk) return;
+    const long long at = static_cast<long long>(blockIdx.x % pieces) * 256 + threadIdx.x;
+    if (at >= size + (adjBias ? I : 0)) return;
+    const float* p = partial + static_cast<long long>(e + begin / chunk) * (size + I) + at;
+    const int chunks = (end - begin + chunk - 1) / chunk;
+    float sum = 0;
+#pragma unroll 4
+    for (int n = 0; n < chunks; ++n) sum += p[n * (size + I)];
+    if (at >= size) adjBias[static_cast<long long>(e) * I + at - size] = static_cast<T>(sum);
+    else if (adjWeights) adjWeights[e * size + at] = static_cast<T>(sum);
+}
+
+QUICKMLP_KERNEL_NAMESPACE_END

@@ -1,0 +1,303 @@
+#pragma once
+// Rows in the order of the group that they belong to: a stable counting sort by one or more digits of the group's number.
+//
+// The sort reads an index per row and writes a place per row; what bounds it is the latency of its launches, not its bytes
+// (2^20 rows: 8 MB). So a digit has up to 13 bits, which makes one pass of up to 8191 groups, and a batch that fits the
+// registers of a workgroup is sorted by one workgroup in one launch.
+//
+// The place of a row among those of its digit is found by ballots: of the lanes of a wavefront with the same digit, those
+// with lower numbers come first; wavefronts and tiles follow in the order of their rows. No atomic decides an order.
+
+#include <qmlp/kernels/token_types.h>
+
+QUICKMLP_KERNEL_NAMESPACE_BEGIN
+
+constexpr int GROUP_SMALL_THREADS = 1024, GROUP_SMALL_ITEMS = 8, GROUP_SMALL_BITS = 8;
+constexpr int GROUP_SMALL_ROWS = GROUP_SMALL_THREADS * GROUP_SMALL_ITEMS;
+constexpr int GROUP_THREADS = 256, GROUP_ITEMS = 16, GROUP_TILE = GROUP_THREADS * GROUP_ITEMS;
+constexpr int GROUP_MAX_BITS = 13;
+constexpr int GROUP_SCAN_DIGITS = 64, GROUP_SCAN_SLICES = 16;
+
+/** The group of a row; 'groups' for rows whose index names none. */
+template <typename I>
+__device__ __forceinline__ unsigned groupOf(const I* __restrict__ index, long long stride, long long row, unsigned groups)
+{
+    const I g = index[row * stride];
+    return g >= 0 && g < static_cast<I>(groups) ? static_cast<unsigned>(g) : groups;
+}
+
+/** The lanes of the wavefront, among those of 'active', whose 'bits' lowest bits of d are this lane's. */
+__device__ __forceinline__ unsigned long long lanesLike(unsigned d, int bits, unsigned long long active)
+{
+    unsigned long long same = active;
+    for (int b = 0; b < bits; ++b) {
+        const bool set = (d >> b) & 1;
+        const unsigned long long votes = __ballot(set);
+        same &= set ? votes : ~votes;
+    }
+    return same;
+}
+
+__device__ __forceinline__ int lanesBelow(unsigned long long lanes)
+{
+    return __popcll(lanes & ((1ull << (threadIdx.x % 64)) - 1));
+}
+
+/**
+ * Exclusive scan of n values in LDS by the whole workgroup of THREADS; 'sums' holds a value per wavefront.
+ * Every thread takes n / THREADS consecutive values.
+ */
+template <int THREADS>
+__device__ __forceinline__ void scanInLds(unsigned* values, int n, unsigned* sums)
+{
+    constexpr int WAVES = THREADS / 64;
+    const int each = (n + THREADS - 1) / THREADS;
+    const int from = min(static_cast<int>(threadIdx.x) * each, n), to = min(from + each, n);
+    unsigned own = 0;
+    for (int i = from; i < to; ++i) own += values[i];
+    unsigned before = own;
+#pragma unroll
+    for (int m = 1; m < 64; m *= 2) {
+        const unsigned other = __shfl_up(before, m);
+        if (static_cast<int>(threadIdx.x) % 64 >= m) before += other;
+    }
+    if (threadIdx.x % 64 == 63) sums[threadIdx.x / 64] = before;
+    before -= own;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < WAVES; ++k)
+        if (k < static_cast<int>(threadIdx.x) / 64) before += sums[k];
+    for (int i = from; i < to; ++i) {
+        const unsigned v = values[i];
+        values[i] = before;
+        before += v;
+    }
+    __syncthreads();
+}
+
+/** The first of n sorted keys that is not below g. */
+__device__ __forceinline__ unsigned lowerBound(const unsigned* keys, unsigned n, unsigned g)
+{
+    unsigned from = 0;
+    while (n > 0) {
+        const unsigned half = n / 2;
+        if (keys[from + half] < g) {
+            from += half + 1;
+            n -= half + 1;
+        } else
+            n = half;
+    }
+    return from;
+}
+
+/**
+ * All of up to GROUP_SMALL_ROWS rows by one workgroup. bits: of the number 'groups'. keys (the groups in order) and offsets (groups + 1
+ * of them) may be null. LDS: GROUP_SMALL_ROWS keys and rows, the counters of the wavefronts.
+ */
+template <typename I>
+__global__ void __launch_bounds__(GROUP_SMALL_THREADS)
+GroupSmallKernel(const I* __restrict__ index, long long stride, int rows, unsigned groups, int bits, int* __restrict__ order,
+                 unsigned* __restrict__ keys, int* __restrict__ offsets)
+{
+    constexpr int WAVES = GROUP_SMALL_THREADS / 64;
+    extern __shared__ unsigned groupLds[];
+    unsigned* const keysLds = groupLds;
+    unsigned* const counters = groupLds + rows;   // [digit][wavefront]
+    unsigned* const sums = counters + (WAVES << (bits < GROUP_SMALL_BITS ? bits : GROUP_SMALL_BITS));
+    unsigned short* const rowsLds = reinterpret_cast<unsigned short*>(sums + WAVES);
+    const int wave = threadIdx.x / 64;
+    // a wavefront takes consecutive rows, 64 at a time
+    const int items = (rows + GROUP_SMALL_THREADS - 1) / GROUP_SMALL_THREADS;
+    unsigned key[GROUP_SMALL_ITEMS];
+    int row[GROUP_SMALL_ITEMS];
+#pragma unroll
+    for (int i = 0; i < GROUP_SMALL_ITEMS; ++i) {
+        row[i] = (wave * items + i) * 64 + threadIdx.x % 64;
+        if (i < items && row[i] < rows) key[i] = groupOf(index, stride, row[i], groups);
+    }
+    for (int shift = 0; shift < bits; shift += GROUP_SMALL_BITS) {
+        const int digitBits = min(GROUP_SMALL_BITS, bits - shift);
+        const int digits = 1 << digitBits;
+        for (int i = threadIdx.x; i < digits * WAVES; i += GROUP_SMALL_THREADS) counters[i] = 0;
+        __syncthreads();
+        unsigned place[GROUP_SMALL_ITEMS];
+#pragma unroll
+        for (int i = 0; i < GROUP_SMALL_ITEMS; ++i) {
+            if (i >= items) break;
+            const bool has = (wave * items + i) * 64 + static_cast<int>(threadIdx.x) % 64 < rows;
+            const unsigned d = has ? (key[i] >> shift) & (digits - 1) : 0;
+            const unsigned long long same = lanesLike(d, digitBits, __ballot(has));
+            unsigned* const counter = counters + d * WAVES + wave;
+            const unsigned before = has ? *counter : 0;
+            place[i] = before + lanesBelow(same);
+            waveLdsSync();
+            if (has && lanesBelow(same) == 0) *counter = before + __popcll(same);
+            waveLdsSync();
+        }
+        __syncthreads();
+        scanInLds<GROUP_SMALL_THREADS>(counters, digits * WAVES, sums);
+#pragma unroll
+        for (int i = 0; i < GROUP_SMALL_ITEMS; ++i) {
+            if (i >= items) break;
+            if ((wave * items + i) * 64 + static_cast<int>(threadIdx.x) % 64 >= rows) continue;
+            const unsigned d = (key[i] >> shift) & (digits - 1);
+            const unsigned p = counters[d * WAVES + wave] + place[i];
+            keysLds[p] = key[i];
+            rowsLds[p] = static_cast<unsigned short>(row[i]);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < GROUP_SMALL_ITEMS; ++i) {
+            const int p = (wave * items + i) * 64 + threadIdx.x % 64;
+            if (i < items && p < rows) {
+                key[i] = keysLds[p];
+                row[i] = rowsLds[p];
+            }
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < GROUP_SMALL_ITEMS; ++i) {
+        const int p = (wave * items + i) * 64 + threadIdx.x % 64;
+        if (i < items && p < rows) {
+            order[p] = row[i];
+            if (keys) keys[p] = key[i];
+        }
+    }
+    if (offsets)   // (keysLds: as the last pass left them)
+        for (unsigned g = threadIdx.x; g <= groups; g += GROUP_SMALL_THREADS) offsets[g] = static_cast<int>(lowerBound(keysLds, rows, g));
+}
+
+/** What a pass of the sort of many rows reads: the index itself (first pass) or the keys and rows of the pass before. */
+template <typename I>
+struct GroupSource
+{
+    const I* index;
+    long long stride;
+    const unsigned* keys;
+    const int* order;
+    unsigned groups;
+    __device__ __forceinline__ unsigned key(long long i) const { return keys ? keys[i] : groupOf(index, stride, i, groups); }
+    __device__ __forceinline__ int row(long long i) const { return order ? order[i] : static_cast<int>(i); }
+};
+
+/** Rows per digit of every tile: counts[tile][digit]; digits: as many as there are, their bits in 'mask'. LDS: a counter per digit. */
+template <typename I>
+__global__ void __launch_bounds__(GROUP_THREADS)
+GroupCountKernel(GroupSource<I> source, long long rows, int shift, unsigned mask, int digits, unsigned* __restrict__ counts)
+{
+    extern __shared__ unsigned groupLds[];
+    for (int d = threadIdx.x; d < digits; d += GROUP_THREADS) groupLds[d] = 0;
+    __syncthreads();
+    const long long first = static_cast<long long>(blockIdx.x) * GROUP_TILE;
+    unsigned key[GROUP_ITEMS];
+#pragma unroll
+    for (int i = 0; i < GROUP_ITEMS; ++i) {
+        const long long r = first + i * GROUP_THREADS + threadIdx.x;
+        if (r < rows) key[i] = source.key(r);
+    }
+#pragma unroll
+    for (int i = 0; i < GROUP_ITEMS; ++i)
+        if (first + i * GROUP_THREADS + threadIdx.x < rows) atomicAdd(groupLds + ((key[i] >> shift) & mask), 1u);
+    __syncthreads();
+    unsigned* out = counts + static_cast<long long>(blockIdx.x) * digits;
+    for (int d = threadIdx.x; d < digits; d += GROUP_THREADS) out[d] = groupLds[d];
+}
+
+/** counts[tile][digit] becomes the rows of the digit in the tiles before; totals[digit]: in all tiles. */
+__global__ void __launch_bounds__(GROUP_SCAN_DIGITS* GROUP_SCAN_SLICES)
+GroupScanKernel(unsigned* __restrict__ counts, int tiles, int digits, unsigned* __restrict__ totals)
+{
+    __shared__ unsigned sums[GROUP_SCAN_SLICES][GROUP_SCAN_DIGITS];
+    const int column = threadIdx.x % GROUP_SCAN_DIGITS, slice = threadIdx.x / GROUP_SCAN_DIGITS;
+    const int d = blockIdx.x * GROUP_SCAN_DIGITS + column;
+    const int each = (tiles + GROUP_SCAN_SLICES - 1) / GROUP_SCAN_SLICES;
+    const int from = min(slice * each, tiles), to = d < digits ? min(from + each, tiles) : from;
+    unsigned sum = 0;
+#pragma unroll 8
+    for (int t = from; t < to; ++t) sum += counts[static_cast<long long>(t) * digits + d];
+    sums[slice][column] = sum;
+    __syncthreads();
+    unsigned before = 0;
+    for (int s = 0; s < slice; ++s) before += sums[s][column];
+    if (d < digits && slice == GROUP_SCAN_SLICES - 1) totals[d] = before + sum;
+#pragma unroll 8
+    for (int t = from; t < to; ++t) {
+        unsigned* const at = counts + static_cast<long long>(t) * digits + d;
+        const unsigned v = *at;
+        *at = before;
+        before += v;
+    }
+}
+
+/**
+ * Writes the rows of a tile to their places. keysOut, offsets: may be null; offsets for a sort of one pass only, whose digits are
+ * the groups. LDS: a start per digit, the counters of the wavefronts.
+ */
+template <typename I>
+__global__ void __launch_bounds__(GROUP_THREADS)
+GroupScatterKernel(GroupSource<I> source, long long rows, int shift, int digitBits, int digits, const unsigned* __restrict__ counts,
+                   const unsigned* __restrict__ totals, int* __restrict__ orderOut, unsigned* __restrict__ keysOut, int* __restrict__ offsets)
+{
+    constexpr int WAVES = GROUP_THREADS / 64;
+    const unsigned mask = (1u << digitBits) - 1;
+    extern __shared__ unsigned groupLds[];
+    unsigned* const starts = groupLds;
+    unsigned short* const counters = reinterpret_cast<unsigned short*>(groupLds + digits);   // [wavefront][digit]
+    __shared__ unsigned sums[WAVES];
+    const int wave = threadIdx.x / 64;
+    for (int d = threadIdx.x; d < digits; d += GROUP_THREADS) {
+        starts[d] = totals[d];
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) counters[w * digits + d] = 0;
+    }
+    // a wavefront takes consecutive rows, 64 at a time
+    const long long first = static_cast<long long>(blockIdx.x) * GROUP_TILE + wave * (64 * GROUP_ITEMS) + threadIdx.x % 64;
+    unsigned key[GROUP_ITEMS];
+    int row[GROUP_ITEMS];
+    unsigned short place[GROUP_ITEMS];
+#pragma unroll
+    for (int i = 0; i < GROUP_ITEMS; ++i)
+        if (first + i * 64 < rows) {
+            key[i] = source.key(first + i * 64);
+            row[i] = source.row(first + i * 64);
+        }
+    __syncthreads();
+    scanInLds<GROUP_THREADS>(starts, digits, sums);
+    if (offsets && blockIdx.x == 0)
+        for (unsigned g = threadIdx.x; g <= source.groups; g += GROUP_THREADS) offsets[g] = static_cast<int>(starts[g]);
+#pragma unroll
+    for (int i = 0; i < GROUP_ITEMS; ++i) {
+        const bool has = first + i * 64 < rows;
+        const unsigned d = has ? (key[i] >> shift) & mask : 0;
+        const unsigned long long same = lanesLike(d, digitBits, __ballot(has));
+        unsigned short* const counter = counters + wave * digits + d;
+        const unsigned before = has ? *counter : 0;
+        place[i] = static_cast<unsigned short>(before + lanesBelow(same));
+        waveLdsSync();
+        if (has && lanesBelow(same) == 0) *counter = static_cast<unsigned short>(before + __popcll(same));
+        waveLdsSync();
+    }
+    __syncthreads();
+    const unsigned* before = counts + static_cast<long long>(blockIdx.x) * digits;
+#pragma unroll
+    for (int i = 0; i < GROUP_ITEMS; ++i) {
+        if (first + i * 64 >= rows) continue;
+        const unsigned d = (key[i] >> shift) & mask;
+        unsigned p = starts[d] + before[d] + place[i];
+#pragma unroll
+        for (int w = 0; w < WAVES - 1; ++w)
+            if (w < wave) p += counters[w * digits + d];
+        orderOut[p] = row[i];
+        if (keysOut) keysOut[p] = key[i];
+    }
+}
+
+/** Where every group begins among sorted keys. */
+__global__ void __launch_bounds__(256) GroupOffsetsKernel(const unsigned* __restrict__ keys, long long rows, unsigned groups, int* __restrict__ offsets)
+{
+    const long long g = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+    if (g <= groups) offsets[g] = static_cast<int>(lowerBound(keys, static_cast<unsigned>(rows), static_cast<unsigned>(g)));
+}
+
+QUICKMLP_KERNEL_NAMESPACE_END

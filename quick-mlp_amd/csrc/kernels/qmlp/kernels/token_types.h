@@ -1,0 +1,70 @@
+#pragma once
+// Element types and vector accesses shared by the operators on rows of tokens (layer_norm.h, embedding.h, row_groups.h,
+// grouped_linear.h). Values are read and written in float, half or bfloat16 and computed in float.
+
+#include <qmlp/kernels/common.h>
+
+QUICKMLP_KERNEL_NAMESPACE_BEGIN
+
+typedef __bf16 bf16;
+
+/** Entries of T in an access of 16 bytes. */
+template <typename T>
+constexpr int WIDE = 16 / static_cast<int>(sizeof(T));
+
+/**
+ * N consecutive entries as floats. The address needs the alignment of one entry only: the hardware takes wide accesses at any
+ * address, so rows of odd lengths are moved 16 bytes at a time as well.
+ */
+template <int N, typename T>
+__device__ __forceinline__ void loadFloats(const T* __restrict__ p, float (&v)[N])
+{
+    T raw[N];
+    __builtin_memcpy(raw, p, sizeof(raw));
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = static_cast<float>(raw[i]);
+}
+
+/** N consecutive entries from floats, each rounded once to nearest even. */
+template <int N, typename T>
+__device__ __forceinline__ void storeFloats(T* __restrict__ p, const float (&v)[N])
+{
+    if constexpr (N == 1) {
+        *p = static_cast<T>(v[0]);
+    } else {
+        typedef T Pair __attribute__((ext_vector_type(2)));
+        Pair raw[N / 2];
+#pragma unroll
+        for (int i = 0; i < N; i += 2) raw[i / 2] = __builtin_convertvector(f32x2{v[i], v[i + 1]}, Pair);
+        __builtin_memcpy(p, raw, sizeof(raw));
+    }
+}
+
+/** Sum over the G (a power of two up to 64) consecutive lanes that a lane belongs to, in all of them. */
+template <int G>
+__device__ __forceinline__ float sumOfLanes(float v)
+{
+#pragma unroll
+    for (int m = 1; m < G; m *= 2) v += __shfl_xor(v, m);
+    return v;
+}
+
+/**
+ * The places of a row of C entries that one of the G lanes of the row holds: CHUNKS pieces of VEC entries. The last piece of
+ * a row whose length is no multiple of VEC starts earlier, so that it ends with the row: its first entries are the piece's before
+ * too, read and written twice with the same values, and 'first' tells how many to leave out of sums. C >= VEC.
+ */
+template <int VEC, int G>
+struct RowPieces
+{
+    int C, lane;
+    __device__ __forceinline__ bool has(int j) const { return (j * G + lane) * VEC < C; }
+    __device__ __forceinline__ int start(int j) const
+    {
+        const int c = (j * G + lane) * VEC;
+        return VEC == 1 ? c : min(c, C - VEC);
+    }
+    __device__ __forceinline__ int first(int j) const { return (j * G + lane) * VEC - start(j); }
+};
+
+QUICKMLP_KERNEL_NAMESPACE_END

@@ -7,6 +7,7 @@
 #include <qmlp/fused_network.h>
 #include <qmlp/iencoding.h>
 #include <qmlp/qmlp.h>
+#include <qmlp/tokens.h>
 #include <qmlp/utils.h>
 
 #include <cstdlib>
@@ -67,17 +68,19 @@ int handleException()
     }                \
     catch (...) { return handleException(); }
 
-Tensor wrap(const qmlp_tensor* t)
+Tensor wrap(const qmlp_tensor* t, int lastPrecision = QMLP_DOUBLE)
 {
     if (!t || t->ndim <= 0) return {};
     bool empty = false;
     for (int i = 0; i < t->ndim && i < 4; ++i) empty = empty || t->sizes[i] == 0;
     if (t->data == nullptr && !empty) return {};   // a null pointer is only a tensor if it has no entries
     if (t->ndim > 4) throw std::runtime_error("tensors with more than 4 dimensions are not supported");
-    if (t->precision < 0 || t->precision > QMLP_DOUBLE) throw std::runtime_error("unknown tensor precision");
+    if (t->precision < 0 || t->precision > lastPrecision) throw std::runtime_error("unknown tensor precision");
     std::vector<int32_t> sizes(t->sizes, t->sizes + t->ndim), strides(t->strides, t->strides + t->ndim);
     return Tensor(t->data, static_cast<Tensor::Precision>(t->precision), sizes, strides);
 }
+/** Of the operators on rows of tokens, which know more types. */
+Tensor wrapToken(const qmlp_tensor* t) { return wrap(t, QMLP_INT64); }
 
 void unwrap(const Tensor& t, qmlp_tensor* out)
 {
@@ -681,6 +684,109 @@ int qmlp_utils_pullpush_precompile(int precision)
     QMLP_API_BEGIN
     if (precision != QMLP_FLOAT && precision != QMLP_DOUBLE) throw std::runtime_error("precision must be float or double");
     Utils::precompile(static_cast<Tensor::Precision>(precision));
+    QMLP_API_END
+}
+
+// ---------------------------------------------------------------- rows of tokens
+
+int qmlp_tokens_group_memory(long long rows, int groups, size_t* bytes)
+{
+    QMLP_API_BEGIN
+    *bytes = Tokens::groupMemory(rows, groups);
+    QMLP_API_END
+}
+
+int qmlp_tokens_group(const qmlp_tensor* index, int groups, const qmlp_tensor* order, const qmlp_tensor* offsets, void* memory, void* stream)
+{
+    QMLP_API_BEGIN
+    Tensor o = wrapToken(order), f = wrapToken(offsets);
+    Tokens::group(wrapToken(index), groups, o, f, memory, static_cast<stream_t>(stream));
+    QMLP_API_END
+}
+
+int qmlp_tokens_embedding(const qmlp_tensor* index, const qmlp_tensor* table, float scale, const qmlp_tensor* output, void* stream)
+{
+    QMLP_API_BEGIN
+    Tensor out = wrapToken(output);
+    Tokens::embedding(wrapToken(index), wrapToken(table), scale, out, static_cast<stream_t>(stream));
+    QMLP_API_END
+}
+
+int qmlp_tokens_embedding_adjoint_memory(long long rows, long long vocabulary, int channels, size_t* bytes)
+{
+    QMLP_API_BEGIN
+    *bytes = Tokens::embeddingAdjointMemory(rows, vocabulary, channels);
+    QMLP_API_END
+}
+
+int qmlp_tokens_embedding_adjoint(const qmlp_tensor* index, const qmlp_tensor* adj_output, float scale, const qmlp_tensor* adj_table, void* memory,
+                                  void* stream)
+{
+    QMLP_API_BEGIN
+    Tensor adjTable = wrapToken(adj_table);
+    Tokens::embeddingAdjoint(wrapToken(index), wrapToken(adj_output), scale, adjTable, memory, static_cast<stream_t>(stream));
+    QMLP_API_END
+}
+
+int qmlp_tokens_layer_norm(const qmlp_tensor* input, const qmlp_tensor* weight, const qmlp_tensor* bias, float epsilon, const qmlp_tensor* output,
+                           const qmlp_tensor* mean, const qmlp_tensor* rstd, void* stream)
+{
+    QMLP_API_BEGIN
+    Tensor out = wrapToken(output), m = wrapToken(mean), r = wrapToken(rstd);
+    Tokens::layerNorm(wrapToken(input), wrapToken(weight), wrapToken(bias), epsilon, out, m, r, static_cast<stream_t>(stream));
+    QMLP_API_END
+}
+
+int qmlp_tokens_layer_norm_adjoint_memory(long long rows, int channels, size_t* bytes)
+{
+    QMLP_API_BEGIN
+    *bytes = Tokens::layerNormAdjointMemory(rows, channels);
+    QMLP_API_END
+}
+
+int qmlp_tokens_layer_norm_adjoint(const qmlp_tensor* input, const qmlp_tensor* weight, const qmlp_tensor* mean, const qmlp_tensor* rstd,
+                                   const qmlp_tensor* adj_output, const qmlp_tensor* adj_input, const qmlp_tensor* adj_weight,
+                                   const qmlp_tensor* adj_bias, void* memory, void* stream)
+{
+    QMLP_API_BEGIN
+    Tensor adjInput = wrapToken(adj_input), adjWeight = wrapToken(adj_weight), adjBias = wrapToken(adj_bias);
+    Tokens::layerNormAdjoint(wrapToken(input), wrapToken(weight), wrapToken(mean), wrapToken(rstd), wrapToken(adj_output), adjInput, adjWeight, adjBias,
+                             memory, static_cast<stream_t>(stream));
+    QMLP_API_END
+}
+
+int qmlp_tokens_grouped_linear(const qmlp_tensor* input, const qmlp_tensor* weight, const qmlp_tensor* offsets, const qmlp_tensor* bias,
+                               const qmlp_tensor* output, void* stream)
+{
+    QMLP_API_BEGIN
+    Tensor out = wrapToken(output);
+    Tokens::groupedLinear(wrapToken(input), wrapToken(weight), wrapToken(offsets), wrapToken(bias), out, static_cast<stream_t>(stream));
+    QMLP_API_END
+}
+
+int qmlp_tokens_grouped_linear_adjoint_memory(long long rows, int experts, int inputs, int outputs, size_t* bytes)
+{
+    QMLP_API_BEGIN
+    *bytes = Tokens::groupedLinearAdjointMemory(rows, experts, inputs, outputs);
+    QMLP_API_END
+}
+
+int qmlp_tokens_grouped_linear_adjoint(const qmlp_tensor* input, const qmlp_tensor* weight, const qmlp_tensor* offsets, const qmlp_tensor* adj_output,
+                                       const qmlp_tensor* adj_input, const qmlp_tensor* adj_weight, const qmlp_tensor* adj_bias, void* memory,
+                                       void* stream)
+{
+    QMLP_API_BEGIN
+    Tensor adjInput = wrapToken(adj_input), adjWeight = wrapToken(adj_weight), adjBias = wrapToken(adj_bias);
+    Tokens::groupedLinearAdjoint(wrapToken(input), wrapToken(weight), wrapToken(offsets), wrapToken(adj_output), adjInput, adjWeight, adjBias, memory,
+                                 static_cast<stream_t>(stream));
+    QMLP_API_END
+}
+
+int qmlp_tokens_precompile(int precision)
+{
+    QMLP_API_BEGIN
+    if (precision != QMLP_FLOAT && precision != QMLP_HALF && precision != QMLP_BFLOAT16) throw std::runtime_error("precision must be float, half or bfloat16");
+    Tokens::precompile(static_cast<Tensor::Precision>(precision));
     QMLP_API_END
 }
 

@@ -11,9 +11,9 @@ struct device_delete
 };
 } // namespace internal
 
-const int Tensor::BytesPerEntry[] = {4, 2, 8};
-const std::string Tensor::DatatypePerEntry[] = {"float", "half", "double"};
-const std::string Tensor::NamePerEntry[] = {"FLOAT", "HALF", "DOUBLE"};
+const int Tensor::BytesPerEntry[] = {4, 2, 8, 2, 4, 8};
+const std::string Tensor::DatatypePerEntry[] = {"float", "half", "double", "bfloat16", "int", "long long"};
+const std::string Tensor::NamePerEntry[] = {"FLOAT", "HALF", "DOUBLE", "BFLOAT16", "INT32", "INT64"};
 
 Tensor::Tensor(Precision precision, const std::vector<int32_t>& sizes)
     : hostsData_(true)

@@ -1,0 +1,687 @@
+#include <qmlp/tokens.h>
+
+#include <qmlp/errors.h>
+#include <qmlp/qmlp.h>
+
+#include "qmlp_hip.h"
+
+#include <algorithm>
+#include <array>
+#include <mutex>
+#include <unordered_map>
+
+QUICKMLP_NAMESPACE_BEGIN
+
+namespace {
+
+constexpr size_t ALIGNMENT = 256;
+
+// ------------------------------------------------------------------------------------------------ kernels
+const char* scalarName(Tensor::Precision p)
+{
+    switch (p) {
+        case Tensor::FLOAT: return "float";
+        case Tensor::HALF: return "_Float16";
+        case Tensor::BFLOAT16: return "__bf16";
+        case Tensor::INT32: return "int";
+        case Tensor::INT64: return "long long";
+        default: throw std::runtime_error("values must be float, half or bfloat16, indices 32- or 64-bit integers");
+    }
+}
+
+/** Entries of a 16-byte access. */
+int wide(Tensor::Precision p) { return 16 / Tensor::BytesPerEntry[p]; }
+
+/** The kernels stay loaded for the life of the process. File: below kernels/qmlp/kernels; name: with its template arguments. */
+KernelFunction& tokenKernel(const char* file, const std::string& name)
+{
+    static std::mutex mutex;
+    static std::unordered_map<std::string, KernelFunction> kernels;
+    std::lock_guard<std::mutex> lock(mutex);
+    auto it = kernels.find(name);
+    if (it == kernels.end()) {
+        auto loaded = QuickMLP::Instance().kernelLoader()->getKernel("qmlp::kernel::" + name, KernelLoader::MainFile(std::string("qmlp/kernels/") + file),
+                                                                     QuickMLP::Instance().getCompileFlags() | KernelLoader::CompileThrowOnError);
+        it = kernels.emplace(name, std::move(*loaded)).first;
+    }
+    return it->second;
+}
+void precompileKernel(const char* file, const std::string& name)
+{
+    QuickMLP::Instance().kernelLoader()->getKernel("qmlp::kernel::" + name, KernelLoader::MainFile(std::string("qmlp/kernels/") + file),
+                                                   QuickMLP::Instance().getCompileFlags() | KernelLoader::CompileThrowOnError | KernelLoader::CompileOnly);
+}
+
+/** Hands out a workspace piece by piece; without a base only its size is wanted. */
+struct Workspace
+{
+    char* base;
+    size_t bytes = 0;
+    template <typename T>
+    T* take(int64_t count)
+    {
+        T* p = base ? reinterpret_cast<T*>(base + bytes) : nullptr;
+        bytes += roundUp(static_cast<size_t>(std::max<int64_t>(count, 0)) * sizeof(T), ALIGNMENT);
+        return p;
+    }
+};
+
+// ------------------------------------------------------------------------------------------------ checks
+bool isValue(Tensor::Precision p) { return p == Tensor::FLOAT || p == Tensor::HALF || p == Tensor::BFLOAT16; }
+
+void checkStrides(const Tensor& t, const char* what)
+{
+    for (int d = 0; d < t.ndim(); ++d) {
+        CHECK_ERROR(t.size(d) >= 0, what, " has a negative size");
+        if (t.size(d) <= 1) continue;   // its stride is not used
+        CHECK_ERROR(t.stride(d) >= 0, what, " has a negative stride");
+    }
+}
+/** Values, whose last dimension is consecutive. */
+void checkValues(const Tensor& t, const char* what, int dims)
+{
+    CHECK_ERROR(t.defined(), what, " is undefined");
+    CHECK_ERROR(t.ndim() == dims, what, " must be a tensor with ", dims, " dimensions, but has ", t.ndim());
+    CHECK_ERROR(isValue(t.precision()), what, " must be of type float, half or bfloat16, but is ", Tensor::NamePerEntry[t.precision()]);
+    checkStrides(t, what);
+    CHECK_ERROR(t.size(dims - 1) <= 1 || t.numel() == 0 || t.stride(dims - 1) == 1, what, " must be consecutive along its last dimension");
+}
+void checkSizes(const Tensor& t, const char* what, std::initializer_list<int64_t> sizes)
+{
+    int d = 0;
+    for (const int64_t s : sizes) {
+        CHECK_ERROR(t.size(d) == s, what, " must have ", s, " entries at dimension ", d, ", but has ", t.size(d));
+        ++d;
+    }
+}
+void checkType(const Tensor& t, const char* what, Tensor::Precision p)
+{
+    CHECK_ERROR(t.precision() == p, what, " must be of type ", Tensor::NamePerEntry[p], ", but is ", Tensor::NamePerEntry[t.precision()]);
+}
+/** Something is written: no two entries may be one. */
+void checkOutput(const Tensor& t, const char* what)
+{
+    for (int d = 0; d + 1 < t.ndim(); ++d) {
+        int64_t inner = 1;
+        for (int k = d + 1; k < t.ndim(); ++k) inner += static_cast<int64_t>(t.size(k) - 1) * t.stride(k);
+        CHECK_ERROR(t.numel() == 0 || t.size(d) <= 1 || t.stride(d) >= inner, what, " has entries that share memory");
+    }
+}
+void checkContiguous(const Tensor& t, const char* what)
+{
+    int64_t stride = 1;
+    for (int d = t.ndim() - 1; d >= 0; --d) {
+        CHECK_ERROR(t.size(d) <= 1 || t.stride(d) == stride, what, " must be contiguous");
+        stride *= t.size(d);
+    }
+}
+void checkIndex(const Tensor& t, const char* what)
+{
+    CHECK_ERROR(t.defined() && t.ndim() == 1, what, " must be a tensor with 1 dimension");
+    CHECK_ERROR(t.precision() == Tensor::INT32 || t.precision() == Tensor::INT64, what, " must hold 32- or 64-bit integers, but is ",
+                Tensor::NamePerEntry[t.precision()]);
+    checkStrides(t, what);
+}
+void checkMemory(const void* memory, size_t bytes)
+{
+    CHECK_ERROR(bytes == 0 || memory != nullptr, "the call needs ", bytes, " bytes of memory");
+    CHECK_ERROR(reinterpret_cast<uintptr_t>(memory) % ALIGNMENT == 0, "memory must be aligned to ", ALIGNMENT, " bytes");
+}
+
+template <typename T>
+T* ptr(const Tensor& t) { return t.defined() ? static_cast<T*>(const_cast<void*>(t.rawPtr())) : nullptr; }
+/** The stride of a dimension; of one with a single entry it may be anything. */
+long long strideOf(const Tensor& t, int d) { return t.size(d) <= 1 ? 0 : t.stride(d); }
+
+/** Workgroups for so many pieces of work of their own, no more than 'most' (the kernels go on in steps of the grid). */
+unsigned workgroups(int64_t pieces, int64_t most) { return static_cast<unsigned>(std::max<int64_t>(1, std::min(pieces, most))); }
+
+// ------------------------------------------------------------------------------------------------ groups
+// as in kernels/row_groups.h
+constexpr int GROUP_SMALL_THREADS = 1024, GROUP_SMALL_ROWS = 8192, GROUP_SMALL_BITS = 8, GROUP_THREADS = 256, GROUP_TILE = 4096, GROUP_MAX_BITS = 13,
+              GROUP_SCAN_DIGITS = 64, GROUP_SCAN_THREADS = 1024;
+/** GroupSource of kernels/row_groups.h */
+struct GroupSource
+{
+    const void* index;
+    long long stride;
+    const unsigned* keys;
+    const int* order;
+    unsigned groups;
+};
+
+int bitsOf(unsigned v)
+{
+    int bits = 1;
+    while (v >> bits && bits < 32) ++bits;
+    return bits;
+}
+
+/** How many rows are sorted, and where what lies between the passes. */
+struct GroupPlan
+{
+    int64_t rows;
+    unsigned groups;
+    int passes, digitBits, maxDigits;
+    int64_t tiles;
+    unsigned *counts = nullptr, *totals = nullptr, *keys[2] = {};
+    int* order[2] = {};
+
+    /** \param keysKept whether the caller has a place for the keys in order */
+    GroupPlan(int64_t rows_, unsigned groups_, bool keysKept, Workspace& memory) : rows(rows_), groups(groups_)
+    {
+        const int bits = bitsOf(groups);
+        const bool small = rows <= GROUP_SMALL_ROWS;
+        passes = divUp(bits, GROUP_MAX_BITS);
+        digitBits = divUp(bits, passes);
+        maxDigits = static_cast<int>(std::min<int64_t>(1ll << digitBits, static_cast<int64_t>(groups) + 1));
+        tiles = divUp<int64_t>(rows, GROUP_TILE);
+        if (small) return;
+        counts = memory.take<unsigned>(tiles * maxDigits);
+        totals = memory.take<unsigned>(maxDigits);
+        // a pass writes where the one before did not; the last one where the caller wants it
+        for (int i = 0; i < std::min(passes - 1, 2); ++i) {
+            keys[i] = memory.take<unsigned>(rows);
+            order[i] = memory.take<int>(rows);
+        }
+        if (passes == 2 && !keysKept) keys[1] = memory.take<unsigned>(rows);
+    }
+};
+
+/** Sorts; keysOut (the groups in order) and offsets may be null. */
+void sortByGroup(const Tensor& index, GroupPlan& plan, int* order, unsigned* keysOut, int* offsets, stream_t stream)
+{
+    const std::string type = std::string("<") + scalarName(index.precision()) + ">";
+    const long long stride = strideOf(index, 0);
+    const int bits = bitsOf(plan.groups);
+    if (plan.rows <= GROUP_SMALL_ROWS) {
+        const size_t lds = plan.rows * 6 + 64 + (static_cast<size_t>(GROUP_SMALL_THREADS / 64 * 4) << std::min(bits, GROUP_SMALL_BITS)) + 4;
+        tokenKernel("row_groups.h", "GroupSmallKernel" + type)
+            .call(1, GROUP_SMALL_THREADS, static_cast<unsigned>(lds), stream, index.rawPtr(), stride, static_cast<int>(plan.rows), plan.groups, bits, order,
+                  keysOut, offsets);
+        return;
+    }
+    GroupSource source{index.rawPtr(), stride, nullptr, nullptr, plan.groups};
+    long long rows = plan.rows;
+    for (int pass = 0; pass < plan.passes; ++pass) {
+        const bool last = pass == plan.passes - 1;
+        const int shift = pass * plan.digitBits;
+        const int digitBits = std::min(plan.digitBits, bits - shift);
+        const int digits = static_cast<int>(std::min<int64_t>(1ll << digitBits, static_cast<int64_t>(plan.groups >> shift) + 1));
+        const unsigned mask = (1u << digitBits) - 1;
+        const unsigned tiles = static_cast<unsigned>(plan.tiles);
+        tokenKernel("row_groups.h", "GroupCountKernel" + type).call(tiles, GROUP_THREADS, digits * 4, stream, source, rows, shift, mask, digits, plan.counts);
+        tokenKernel("row_groups.h", "GroupScanKernel")
+            .call(static_cast<unsigned>(divUp(digits, GROUP_SCAN_DIGITS)), GROUP_SCAN_THREADS, 0, stream, plan.counts, static_cast<int>(tiles), digits, plan.totals);
+        int* to = last ? order : plan.order[pass % 2];
+        unsigned* toKeys = last ? (keysOut ? keysOut : plan.passes > 1 ? plan.keys[pass % 2] : nullptr) : plan.keys[pass % 2];
+        const unsigned lds = digits * 4 + digits * 2 * (GROUP_THREADS / 64);
+        tokenKernel("row_groups.h", "GroupScatterKernel" + type)
+            .call(tiles, GROUP_THREADS, lds, stream, source, rows, shift, digitBits, digits, static_cast<const unsigned*>(plan.counts),
+                  static_cast<const unsigned*>(plan.totals), to, toKeys, plan.passes == 1 ? offsets : nullptr);
+        source.keys = toKeys;
+        source.order = to;
+    }
+    if (offsets && plan.passes > 1)
+        tokenKernel("row_groups.h", "GroupOffsetsKernel")
+            .call(static_cast<unsigned>(divUp<int64_t>(static_cast<int64_t>(plan.groups) + 1, 256)), 256, 0, stream, source.keys, rows, plan.groups, offsets);
+}
+
+// ------------------------------------------------------------------------------------------------ embeddings
+// as in kernels/embedding.h
+constexpr int EMBEDDING_THREADS = 256, EMBEDDING_BLOCK_BITS = 5;
+struct EmbeddingBlocks
+{
+    static constexpr int SIZES = 6;
+    int sizes;
+    const float* sums[SIZES];
+};
+
+/** Lanes per row of C entries, at most 64. */
+int lanesPerRow(int C, int vec)
+{
+    int lanes = 8;
+    while (lanes < 64 && lanes * vec < C) lanes *= 2;
+    return lanes;
+}
+
+struct EmbeddingPlan
+{
+    Workspace memory;
+    unsigned *keys, *spans;
+    int* order;
+    EmbeddingBlocks blocks = {};
+    GroupPlan sort;
+    EmbeddingPlan(int64_t rows, int64_t vocabulary, int channels, void* base)
+        : memory{static_cast<char*>(base)}, keys(memory.take<unsigned>(rows)), spans(memory.take<unsigned>(2 * vocabulary)), order(memory.take<int>(rows)),
+          sort(rows, static_cast<unsigned>(vocabulary), true, memory)
+    {
+        for (int s = 0; s < EmbeddingBlocks::SIZES && rows >> (EMBEDDING_BLOCK_BITS * (s + 1)) > 0; ++s) {
+            blocks.sums[s] = memory.take<float>((rows >> (EMBEDDING_BLOCK_BITS * (s + 1))) * channels);
+            blocks.sizes = s + 1;
+        }
+    }
+};
+
+// ------------------------------------------------------------------------------------------------ layer norm
+// as in kernels/layer_norm.h
+constexpr int LAYER_NORM_SUM_COLUMNS = 32, LAYER_NORM_SUM_THREADS = 1024, LAYER_NORM_LONG_THREADS = 1024;
+
+/** Lanes that share a row, and how many entries each of them holds. */
+struct LayerNormShape
+{
+    int lanes, entries, vec;   // lanes = 0: no workgroup holds a row
+    int threads() const { return std::max(lanes, 256); }
+    int rows() const { return threads() / lanes; }   // of a workgroup at a time
+    std::string arguments() const { return std::to_string(vec) + ", " + std::to_string(lanes) + ", " + std::to_string(entries / vec); }
+};
+// 8 entries a lane for short rows, so that many lanes ask for memory; 64 lanes at first, whose sums need no LDS.
+constexpr std::array<std::array<int, 2>, 10> LAYER_NORM_SHAPES = {
+    {{8, 8}, {16, 8}, {32, 8}, {64, 8}, {64, 16}, {256, 8}, {256, 16}, {256, 32}, {1024, 16}, {1024, 32}}};
+
+LayerNormShape layerNormShape(int channels, Tensor::Precision p)
+{
+    if (channels < wide(p)) return {8, 1, 1};
+    for (const auto& s : LAYER_NORM_SHAPES)
+        if (s[0] * s[1] >= channels) return {s[0], s[1], wide(p)};
+    return {0, 0, 0};
+}
+std::string valueTypes(Tensor::Precision p, Tensor::Precision weights) { return std::string(scalarName(p)) + ", " + scalarName(weights); }
+
+/** Workgroups of the adjoint kernel: each leaves a row of sums. Two per compute unit where rows are held by wavefronts, four short of that. */
+unsigned layerNormAdjointWorkgroups(int64_t rows, const LayerNormShape& s)
+{
+    if (s.lanes == 0) return workgroups(rows, 256);   // slices of the rows
+    return workgroups(divUp<int64_t>(rows, s.rows()), s.lanes == 1024 ? 256 : 512);
+}
+
+// ------------------------------------------------------------------------------------------------ grouped linear layers
+struct GroupedTiles
+{
+    int i, j, wavesI, wavesJ;
+    int threads() const { return 64 * wavesI * wavesJ; }
+    unsigned lds() const { return 2 * 128 * (i + j); }
+    std::string arguments() const { return str(i, ", ", j, ", ", wavesI, ", ", wavesJ); }
+};
+constexpr GroupedTiles LARGE_TILES = {128, 128, 2, 2}, SMALL_TILES = {64, 64, 2, 2};
+
+GroupedTiles tilesFor(int64_t i, int64_t j) { return i <= 64 || j <= 64 ? SMALL_TILES : LARGE_TILES; }
+
+/** Places of tiles (kernels/grouped_linear.h): one more than rows / tileRows for each expert and for the rows behind them. */
+int64_t tilePlaces(int64_t rows, int64_t experts, int64_t tileRows) { return rows / tileRows + experts + 1; }
+
+/** Rows of a chunk of GroupedWeightsKernel: several chunks per expert where its tiles alone are too few for the chip. */
+int64_t weightsChunk(int64_t rows, int64_t experts, int64_t tiles)
+{
+    constexpr int64_t WORKGROUPS = 1024, SHORTEST = 512;
+    const int64_t chunks = divUp<int64_t>(WORKGROUPS, std::max<int64_t>(1, experts * tiles));   // per expert
+    if (chunks <= 1) return std::max<int64_t>(rows, 1);
+    return std::max(SHORTEST, roundUp<int64_t>(divUp<int64_t>(rows, experts * chunks), 64));
+}
+
+struct GroupedAdjointPlan
+{
+    GroupedTiles tiles;
+    int64_t tilesI, tilesJ, chunk, places;
+    Workspace memory;
+    float* partial = nullptr;
+    GroupedAdjointPlan(int64_t rows, int64_t experts, int64_t inputs, int64_t outputs, void* base) : memory{static_cast<char*>(base)}
+    {
+        tiles = tilesFor(outputs, inputs);
+        tilesI = divUp<int64_t>(outputs, tiles.i);
+        tilesJ = divUp<int64_t>(inputs, tiles.j);
+        chunk = weightsChunk(rows, experts, tilesI * tilesJ);
+        places = rows / chunk + experts;
+        if (chunk < rows) partial = memory.take<float>(places * (outputs * inputs + outputs));
+    }
+};
+
+void checkLaunch(int64_t groups, int threads)
+{
+    CHECK_ERROR(groups * threads < (1ll << 32), "the call is too large for one launch");
+}
+
+struct GroupedSizes
+{
+    int rows, experts, inputs, outputs;
+};
+GroupedSizes checkGrouped(const Tensor& input, const Tensor& weight, const Tensor& offsets)
+{
+    checkValues(input, "input", 2);
+    checkValues(weight, "weight", 3);
+    checkType(weight, "weight", input.precision());
+    CHECK_ERROR(offsets.defined() && offsets.ndim() == 1, "offsets must be a tensor with 1 dimension");
+    checkType(offsets, "offsets", Tensor::INT32);
+    CHECK_ERROR(offsets.size(0) <= 1 || offsets.stride(0) == 1, "offsets must be contiguous");
+    const GroupedSizes s{input.size(0), weight.size(0), input.size(1), weight.size(1)};
+    CHECK_ERROR(s.inputs > 0 && s.outputs > 0, "experts must have inputs and outputs");
+    checkSizes(weight, "weight", {s.experts, s.outputs, s.inputs});
+    checkSizes(offsets, "offsets", {s.experts + 1ll});
+    return s;
+}
+
+} // namespace
+
+// ------------------------------------------------------------------------------------------------ entry points
+size_t Tokens::groupMemory(int64_t rows, int groups)
+{
+    CHECK_ERROR(rows >= 0 && rows < (1ll << 31) && groups >= 0, "rows and groups must not be negative and fit into 32 bits");
+    Workspace memory{nullptr};
+    GroupPlan plan(rows, static_cast<unsigned>(groups), false, memory);
+    return memory.bytes;
+}
+
+void Tokens::group(const Tensor& index, int groups, Tensor& order, Tensor& offsets, void* memory, stream_t stream)
+{
+    checkIndex(index, "index");
+    CHECK_ERROR(groups >= 0, "the number of groups must not be negative");
+    for (const auto& [t, what, size] : {std::tuple<const Tensor&, const char*, int64_t>{order, "order", index.size(0)}, {offsets, "offsets", groups + 1ll}}) {
+        CHECK_ERROR(t.defined() && t.ndim() == 1, what, " must be a tensor with 1 dimension");
+        checkType(t, what, Tensor::INT32);
+        checkSizes(t, what, {size});
+        checkContiguous(t, what);
+    }
+    checkMemory(memory, groupMemory(index.size(0), groups));
+    Workspace workspace{static_cast<char*>(memory)};
+    GroupPlan plan(index.size(0), static_cast<unsigned>(groups), false, workspace);
+    sortByGroup(index, plan, ptr<int>(order), nullptr, ptr<int>(offsets), stream);
+}
+
+void Tokens::embedding(const Tensor& index, const Tensor& table, float scale, Tensor& output, stream_t stream)
+{
+    checkIndex(index, "index");
+    checkValues(table, "table", 2);
+    checkValues(output, "output", 2);
+    checkType(output, "output", table.precision());
+    checkSizes(output, "output", {index.size(0), table.size(1)});
+    checkOutput(output, "output");
+    if (output.numel() == 0) return;
+    const int C = table.size(1), vec = C < wide(table.precision()) ? 1 : wide(table.precision()), lanes = lanesPerRow(C, vec);
+    const long long rows = index.size(0), vocabulary = table.size(0);
+    tokenKernel("embedding.h", str("EmbeddingKernel<", scalarName(table.precision()), ", ", scalarName(index.precision()), ", ", vec, ", ", lanes, ">"))
+        .call(workgroups(divUp<int64_t>(rows, EMBEDDING_THREADS / lanes), 1 << 20), EMBEDDING_THREADS, 0, stream, index.rawPtr(), strideOf(index, 0),
+              static_cast<const void*>(ptr<void>(table)), strideOf(table, 0), scale, output.rawPtr(), strideOf(output, 0), rows, vocabulary, C);
+}
+
+size_t Tokens::embeddingAdjointMemory(int64_t rows, int64_t vocabulary, int channels)
+{
+    CHECK_ERROR(rows >= 0 && rows < (1ll << 31) && vocabulary >= 0 && vocabulary < (1ll << 31) && channels >= 0,
+                "rows, vocabulary and channels must not be negative and fit into 32 bits");
+    return EmbeddingPlan(rows, vocabulary, channels, nullptr).memory.bytes;
+}
+
+void Tokens::embeddingAdjoint(const Tensor& index, const Tensor& adjOutput, float scale, Tensor& adjTable, void* memory, stream_t stream)
+{
+    checkIndex(index, "index");
+    checkValues(adjTable, "adjTable", 2);
+    checkOutput(adjTable, "adjTable");
+    checkValues(adjOutput, "adjOutput", 2);
+    checkType(adjOutput, "adjOutput", adjTable.precision());
+    checkSizes(adjOutput, "adjOutput", {index.size(0), adjTable.size(1)});
+    const long long rows = index.size(0), vocabulary = adjTable.size(0);
+    const int C = adjTable.size(1);
+    checkMemory(memory, embeddingAdjointMemory(rows, vocabulary, C));
+    if (adjTable.numel() == 0) return;
+    const Tensor::Precision p = adjTable.precision();
+    const int vec = C < wide(p) ? 1 : wide(p), lanes = lanesPerRow(C, vec);
+    const std::string shape = str(vec, ", ", lanes);
+    EmbeddingPlan plan(rows, vocabulary, C, memory);
+    QMLP_HIP_CALL(qmlp_hip_memset_async(plan.spans, 0, sizeof(unsigned) * 2 * vocabulary, stream));
+    const void* dy = ptr<void>(adjOutput);
+    if (rows > 0) {
+        sortByGroup(index, plan.sort, plan.order, plan.keys, nullptr, stream);
+        tokenKernel("embedding.h", "EmbeddingSpansKernel")
+            .call(static_cast<unsigned>(divUp<int64_t>(rows, EMBEDDING_THREADS)), EMBEDDING_THREADS, 0, stream, static_cast<const unsigned*>(plan.keys), rows,
+                  static_cast<unsigned>(vocabulary), plan.spans);
+        for (int s = 0; s < plan.blocks.sizes; ++s) {
+            const int64_t blocks = rows >> (EMBEDDING_BLOCK_BITS * (s + 1));
+            tokenKernel("embedding.h", str("EmbeddingBlocksKernel<", scalarName(p), ", ", shape, s == 0 ? ", true>" : ", false>"))
+                .call(static_cast<unsigned>(divUp<int64_t>(blocks, EMBEDDING_THREADS / lanes)), EMBEDDING_THREADS, 0, stream,
+                      static_cast<const unsigned*>(plan.keys), static_cast<const int*>(plan.order), rows, static_cast<unsigned>(vocabulary),
+                      EMBEDDING_BLOCK_BITS * (s + 1), dy, strideOf(adjOutput, 0), s == 0 ? nullptr : plan.blocks.sums[s - 1],
+                      const_cast<float*>(plan.blocks.sums[s]), C);
+        }
+    }
+    tokenKernel("embedding.h", str("EmbeddingAdjointKernel<", scalarName(p), ", ", shape, ">"))
+        .call(workgroups(divUp<int64_t>(vocabulary, EMBEDDING_THREADS / lanes), 1 << 20), EMBEDDING_THREADS, 0, stream,
+              static_cast<const unsigned*>(plan.spans), static_cast<const int*>(plan.order), plan.blocks, dy, strideOf(adjOutput, 0), scale,
+              adjTable.rawPtr(), strideOf(adjTable, 0), vocabulary, C);
+}
+
+void Tokens::layerNorm(const Tensor& input, const Tensor& weight, const Tensor& bias, float epsilon, Tensor& output, Tensor& mean, Tensor& rstd,
+                       stream_t stream)
+{
+    checkValues(input, "input", 2);
+    const long long rows = input.size(0);
+    const int C = input.size(1);
+    const Tensor::Precision p = input.precision(), weights = weight.defined() ? weight.precision() : bias.defined() ? bias.precision() : p;
+    for (const auto& [t, what] : {std::pair<const Tensor&, const char*>{weight, "weight"}, {bias, "bias"}}) {
+        if (!t.defined()) continue;
+        checkValues(t, what, 1);
+        checkSizes(t, what, {C});
+        CHECK_ERROR(t.precision() == p || t.precision() == Tensor::FLOAT, what, " must be of the input's type or FLOAT");
+        CHECK_ERROR(t.precision() == weights, "weight and bias must be of one type");
+    }
+    checkValues(output, "output", 2);
+    checkType(output, "output", p);
+    checkSizes(output, "output", {rows, C});
+    checkOutput(output, "output");
+    for (const auto& [t, what] : {std::pair<const Tensor&, const char*>{mean, "mean"}, {rstd, "rstd"}}) {
+        if (!t.defined()) continue;
+        checkValues(t, what, 1);
+        checkType(t, what, Tensor::FLOAT);
+        checkSizes(t, what, {rows});
+    }
+    if (input.numel() == 0) return;
+    const LayerNormShape s = layerNormShape(C, p);
+    const std::string types = valueTypes(p, weights);
+    const void *x = input.rawPtr(), *w = ptr<void>(weight), *b = ptr<void>(bias);
+    const long long strideX = strideOf(input, 0), strideY = strideOf(output, 0);
+    const bool isLong = s.lanes == 0;
+    tokenKernel("layer_norm.h", isLong ? "LayerNormLongKernel<" + types + ">" : "LayerNormKernel<" + types + ", " + s.arguments() + ">")
+        .call(isLong ? workgroups(rows, 512) : workgroups(divUp<int64_t>(rows, s.rows()), s.lanes == 1024 ? 512 : 2048),
+              isLong ? LAYER_NORM_LONG_THREADS : s.threads(), 0, stream, x, strideX, w, b, epsilon, output.rawPtr(), strideY, ptr<float>(mean),
+              ptr<float>(rstd), rows, C);
+}
+
+size_t Tokens::layerNormAdjointMemory(int64_t rows, int channels)
+{
+    CHECK_ERROR(rows >= 0 && channels >= 0, "rows and channels must not be negative");
+    if (rows == 0) return 0;
+    // (for any precision)
+    size_t bytes = 0;
+    for (const Tensor::Precision p : {Tensor::FLOAT, Tensor::HALF})
+        bytes = std::max(bytes, sizeof(float) * 2 * channels * layerNormAdjointWorkgroups(rows, layerNormShape(channels, p)));
+    return roundUp(bytes, ALIGNMENT);
+}
+
+void Tokens::layerNormAdjoint(const Tensor& input, const Tensor& weight, const Tensor& mean, const Tensor& rstd, const Tensor& adjOutput, Tensor& adjInput,
+                              Tensor& adjWeight, Tensor& adjBias, void* memory, stream_t stream)
+{
+    checkValues(input, "input", 2);
+    const long long rows = input.size(0);
+    const int C = input.size(1);
+    const Tensor::Precision p = input.precision();
+    if (weight.defined()) {
+        checkValues(weight, "weight", 1);
+        checkSizes(weight, "weight", {C});
+        CHECK_ERROR(weight.precision() == p || weight.precision() == Tensor::FLOAT, "weight must be of the input's type or FLOAT");
+    }
+    for (const auto& [t, what] : {std::pair<const Tensor&, const char*>{mean, "mean"}, {rstd, "rstd"}}) {
+        checkValues(t, what, 1);
+        checkType(t, what, Tensor::FLOAT);
+        checkSizes(t, what, {rows});
+    }
+    checkValues(adjOutput, "adjOutput", 2);
+    checkType(adjOutput, "adjOutput", p);
+    checkSizes(adjOutput, "adjOutput", {rows, C});
+    if (adjInput.defined()) {
+        checkValues(adjInput, "adjInput", 2);
+        checkType(adjInput, "adjInput", p);
+        checkSizes(adjInput, "adjInput", {rows, C});
+        checkOutput(adjInput, "adjInput");
+    }
+    Tensor::Precision weights = weight.defined() ? weight.precision() : p;
+    for (const auto& [t, what] : {std::pair<const Tensor&, const char*>{adjWeight, "adjWeight"}, {adjBias, "adjBias"}}) {
+        if (!t.defined()) continue;
+        checkValues(t, what, 1);
+        checkSizes(t, what, {C});
+        CHECK_ERROR(t.precision() == p || t.precision() == Tensor::FLOAT, what, " must be of the input's type or FLOAT");
+        if (!weight.defined()) weights = t.precision();
+    }
+    for (const auto& [t, what] : {std::pair<const Tensor&, const char*>{adjWeight, "adjWeight"}, {adjBias, "adjBias"}})
+        if (t.defined()) checkType(t, what, weights);
+    const bool sums = adjWeight.defined() || adjBias.defined();
+    if (C == 0 || (!sums && !adjInput.defined())) return;
+    const size_t bytes = sums ? layerNormAdjointMemory(rows, C) : 0;
+    checkMemory(memory, bytes);
+    float* partial = sums ? static_cast<float*>(memory) : nullptr;
+    const LayerNormShape s = layerNormShape(C, p);
+    const std::string types = valueTypes(p, weights);
+    int count = 0;
+    if (rows > 0) {
+        const unsigned groups = layerNormAdjointWorkgroups(rows, s);
+        count = static_cast<int>(groups);
+        const void *x = input.rawPtr(), *w = ptr<void>(weight), *dy = adjOutput.rawPtr();
+        const float *m = ptr<float>(mean), *r = ptr<float>(rstd);
+        const long long strideX = strideOf(input, 0), strideDy = strideOf(adjOutput, 0), strideDx = adjInput.defined() ? strideOf(adjInput, 0) : 0;
+        void* dx = ptr<void>(adjInput);
+        if (s.lanes > 0) {
+            tokenKernel("layer_norm.h", "LayerNormAdjointKernel<" + types + ", " + s.arguments() + ">")
+                .call(groups, s.threads(), 0, stream, x, strideX, w, m, r, dy, strideDy, dx, strideDx, partial, rows, C);
+        } else {
+            if (dx)
+                tokenKernel("layer_norm.h", "LayerNormLongAdjointKernel<" + types + ">")
+                    .call(workgroups(rows, 512), LAYER_NORM_LONG_THREADS, 0, stream, x, strideX, w, m, r, dy, strideDy, dx, strideDx, rows, C);
+            if (sums)
+                tokenKernel("layer_norm.h", std::string("LayerNormLongSumsKernel<") + scalarName(p) + ">")
+                    .call(groups * static_cast<unsigned>(divUp(C, 256)), 256, 0, stream, x, strideX, m, r, dy, strideDy, partial, rows, C, count);
+        }
+    }
+    if (sums)
+        tokenKernel("layer_norm.h", std::string("LayerNormSumKernel<") + scalarName(weights) + ">")
+            .call(static_cast<unsigned>(divUp<int64_t>(2ll * C, LAYER_NORM_SUM_COLUMNS)), LAYER_NORM_SUM_THREADS, 0, stream, static_cast<const float*>(partial), count, C,
+                  ptr<void>(adjWeight), ptr<void>(adjBias));
+}
+
+void Tokens::groupedLinear(const Tensor& input, const Tensor& weight, const Tensor& offsets, const Tensor& bias, Tensor& output, stream_t stream)
+{
+    const GroupedSizes s = checkGrouped(input, weight, offsets);
+    const Tensor::Precision p = input.precision();
+    if (bias.defined()) {
+        checkValues(bias, "bias", 2);
+        checkType(bias, "bias", p);
+        checkSizes(bias, "bias", {s.experts, s.outputs});
+    }
+    checkValues(output, "output", 2);
+    checkType(output, "output", p);
+    checkSizes(output, "output", {s.rows, s.outputs});
+    checkOutput(output, "output");
+    if (s.rows == 0) return;
+    const GroupedTiles t = tilesFor(s.rows / std::max(s.experts, 1), s.outputs);
+    const int tilesJ = divUp(s.outputs, t.j);
+    const int64_t groups = tilePlaces(s.rows, s.experts, t.i) * tilesJ;
+    checkLaunch(groups, t.threads());
+    tokenKernel("grouped_linear.h", str("GroupedRowsKernel<", scalarName(p), ", true, ", t.arguments(), ">"))
+        .call(static_cast<unsigned>(groups), t.threads(), t.lds(), stream, input.rawPtr(), strideOf(input, 0), static_cast<const void*>(ptr<void>(weight)),
+              strideOf(weight, 0), strideOf(weight, 1), static_cast<const void*>(ptr<void>(bias)), bias.defined() ? strideOf(bias, 0) : 0ll,
+              static_cast<const int*>(ptr<int>(offsets)), s.experts, output.rawPtr(), strideOf(output, 0), s.rows, s.outputs, s.inputs, tilesJ);
+}
+
+size_t Tokens::groupedLinearAdjointMemory(int64_t rows, int experts, int inputs, int outputs)
+{
+    CHECK_ERROR(rows >= 0 && experts >= 0 && inputs >= 0 && outputs >= 0, "sizes must not be negative");
+    if (experts == 0) return 0;
+    return GroupedAdjointPlan(rows, experts, inputs, outputs, nullptr).memory.bytes;
+}
+
+void Tokens::groupedLinearAdjoint(const Tensor& input, const Tensor& weight, const Tensor& offsets, const Tensor& adjOutput, Tensor& adjInput,
+                                  Tensor& adjWeight, Tensor& adjBias, void* memory, stream_t stream)
+{
+    const GroupedSizes s = checkGrouped(input, weight, offsets);
+    const Tensor::Precision p = input.precision();
+    checkValues(adjOutput, "adjOutput", 2);
+    checkType(adjOutput, "adjOutput", p);
+    checkSizes(adjOutput, "adjOutput", {s.rows, s.outputs});
+    if (adjInput.defined()) {
+        checkValues(adjInput, "adjInput", 2);
+        checkType(adjInput, "adjInput", p);
+        checkSizes(adjInput, "adjInput", {s.rows, s.inputs});
+        checkOutput(adjInput, "adjInput");
+    }
+    if (adjWeight.defined()) {
+        checkValues(adjWeight, "adjWeight", 3);
+        checkType(adjWeight, "adjWeight", p);
+        checkSizes(adjWeight, "adjWeight", {s.experts, s.outputs, s.inputs});
+        checkContiguous(adjWeight, "adjWeight");
+    }
+    if (adjBias.defined()) {
+        checkValues(adjBias, "adjBias", 2);
+        checkType(adjBias, "adjBias", p);
+        checkSizes(adjBias, "adjBias", {s.experts, s.outputs});
+        checkContiguous(adjBias, "adjBias");
+    }
+    const int* off = ptr<int>(offsets);
+    const void *x = ptr<void>(input), *dy = ptr<void>(adjOutput);
+    if (adjInput.defined() && s.rows > 0) {
+        const GroupedTiles t = tilesFor(s.rows / std::max(s.experts, 1), s.inputs);
+        const int tilesJ = divUp(s.inputs, t.j);
+        const int64_t groups = tilePlaces(s.rows, s.experts, t.i) * tilesJ;
+        checkLaunch(groups, t.threads());
+        tokenKernel("grouped_linear.h", str("GroupedRowsKernel<", scalarName(p), ", false, ", t.arguments(), ">"))
+            .call(static_cast<unsigned>(groups), t.threads(), t.lds(), stream, dy, strideOf(adjOutput, 0), static_cast<const void*>(ptr<void>(weight)),
+                  strideOf(weight, 0), strideOf(weight, 1), static_cast<const void*>(nullptr), 0ll, off, s.experts, adjInput.rawPtr(),
+                  strideOf(adjInput, 0), s.rows, s.inputs, s.outputs, tilesJ);
+    }
+    if (s.experts == 0 || (!adjWeight.defined() && !adjBias.defined())) return;
+    checkMemory(memory, groupedLinearAdjointMemory(s.rows, s.experts, s.inputs, s.outputs));
+    GroupedAdjointPlan plan(s.rows, s.experts, s.inputs, s.outputs, memory);
+    const int64_t groups = plan.places * plan.tilesI * plan.tilesJ;
+    checkLaunch(groups, plan.tiles.threads());
+    const int chunk = static_cast<int>(plan.chunk);
+    tokenKernel("grouped_linear.h", str("GroupedWeightsKernel<", scalarName(p), ", ", plan.tiles.arguments(), ">"))
+        .call(static_cast<unsigned>(groups), plan.tiles.threads(), plan.tiles.lds(), stream, dy, strideOf(adjOutput, 0), x, strideOf(input, 0), off, s.experts,
+              ptr<void>(adjWeight), ptr<void>(adjBias), plan.partial, s.rows, s.outputs, s.inputs, static_cast<int>(plan.tilesI), static_cast<int>(plan.tilesJ), chunk);
+    if (plan.partial) {
+        const long long size = static_cast<long long>(s.inputs) * s.outputs;
+        const int64_t pieces = divUp<int64_t>(size + s.outputs, 256);
+        checkLaunch(pieces * s.experts, 256);
+        tokenKernel("grouped_linear.h", str("GroupedSumKernel<", scalarName(p), ">"))
+            .call(static_cast<unsigned>(pieces * s.experts), 256, 0, stream, static_cast<const float*>(plan.partial), off, ptr<void>(adjWeight),
+                  ptr<void>(adjBias), s.rows, size, s.outputs, chunk, static_cast<int>(pieces));
+    }
+}
+
+void Tokens::precompile(Tensor::Precision p)
+{
+    CHECK_ERROR(isValue(p), "precision must be float, half or bfloat16");
+    const std::string t = scalarName(p);
+    const std::vector<std::string> indices = {"int", "long long"};
+    for (const auto& i : indices)
+        for (const char* kernel : {"GroupSmallKernel", "GroupCountKernel", "GroupScatterKernel"}) precompileKernel("row_groups.h", str(kernel, "<", i, ">"));
+    for (const char* kernel : {"GroupScanKernel", "GroupOffsetsKernel"}) precompileKernel("row_groups.h", kernel);
+    precompileKernel("embedding.h", "EmbeddingSpansKernel");
+    for (const int vec : {1, wide(p)})
+        for (const int lanes : {8, 16, 32, 64}) {
+            if (vec == 1 && lanes > 8) continue;
+            const std::string shape = str(t, ", ", vec, ", ", lanes);
+            for (const auto& i : indices) precompileKernel("embedding.h", str("EmbeddingKernel<", t, ", ", i, ", ", vec, ", ", lanes, ">"));
+            precompileKernel("embedding.h", str("EmbeddingBlocksKernel<", shape, ", true>"));
+            precompileKernel("embedding.h", str("EmbeddingBlocksKernel<", shape, ", false>"));
+            precompileKernel("embedding.h", str("EmbeddingAdjointKernel<", shape, ">"));
+        }
+    std::vector<LayerNormShape> shapes = {{8, 1, 1}};
+    for (const auto& s : LAYER_NORM_SHAPES) shapes.push_back({s[0], s[1], wide(p)});
+    for (const LayerNormShape& s : shapes)
+        for (const char* kernel : {"LayerNormKernel", "LayerNormAdjointKernel"}) precompileKernel("layer_norm.h", str(kernel, "<", t, ", ", t, ", ", s.arguments(), ">"));
+    for (const char* kernel : {"LayerNormLongKernel", "LayerNormLongAdjointKernel"}) precompileKernel("layer_norm.h", str(kernel, "<", t, ", ", t, ">"));
+    for (const char* kernel : {"LayerNormLongSumsKernel", "LayerNormSumKernel"}) precompileKernel("layer_norm.h", str(kernel, "<", t, ">"));
+    for (const GroupedTiles& tiles : {LARGE_TILES, SMALL_TILES}) {
+        precompileKernel("grouped_linear.h", str("GroupedRowsKernel<", t, ", true, ", tiles.arguments(), ">"));
+        precompileKernel("grouped_linear.h", str("GroupedRowsKernel<", t, ", false, ", tiles.arguments(), ">"));
+        precompileKernel("grouped_linear.h", str("GroupedWeightsKernel<", t, ", ", tiles.arguments(), ">"));
+    }
+    precompileKernel("grouped_linear.h", str("GroupedSumKernel<", t, ">"));
+}
+
+QUICKMLP_NAMESPACE_END

@@ -7,11 +7,13 @@
 // replaces the one of the reference's binding (src_cpp/pytorch-bindings/src/bind_network.cpp:189-319).
 #include <torch/extension.h>
 #include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/Exceptions.h>
 #include <ATen/FuncTorchTLS.h>
 #include <ATen/TracerMode.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
 #include "qmlp_capi.h"
@@ -70,7 +72,7 @@ void setError(const Failure& f)
     throw std::logic_error("unreachable");
 }
 
-qmlp_tensor wrap(const at::Tensor& t)
+qmlp_tensor wrap(const at::Tensor& t, bool token = false)
 {
     qmlp_tensor d{};
     if (!t.defined()) return d;
@@ -80,7 +82,12 @@ qmlp_tensor wrap(const at::Tensor& t)
         case at::kFloat: d.precision = QMLP_FLOAT; break;
         case at::kHalf: d.precision = QMLP_HALF; break;
         case at::kDouble: d.precision = QMLP_DOUBLE; break;
-        default: throw py::type_error("unsupported dtype " + std::string(c10::toString(t.scalar_type())));
+        default:
+            // types that the operators on rows of tokens know besides
+            if (token && t.scalar_type() == at::kBFloat16) d.precision = QMLP_BFLOAT16;
+            else if (token && t.scalar_type() == at::kInt) d.precision = QMLP_INT32;
+            else if (token && t.scalar_type() == at::kLong) d.precision = QMLP_INT64;
+            else throw py::type_error("unsupported dtype " + std::string(c10::toString(t.scalar_type())));
     }
     d.data = t.data_ptr();
     d.ndim = static_cast<int32_t>(dim);
@@ -179,7 +186,7 @@ void refuseOtherModes(at::TensorList tensors)
     if (const auto& functorch = at::functorch::functorchTLSAccessor()) functorch->checkSupportsCppAutogradFunction();
     for (const auto& t : tensors) {
         if (!t.defined() || !t._fw_grad(0).defined()) continue;
-        PyErr_SetString(PyExc_NotImplementedError, "forward-mode AD is not implemented for networks and encodings");
+        PyErr_SetString(PyExc_NotImplementedError, "forward-mode AD is not implemented for networks, encodings and operators on tokens");
         throw py::error_already_set();
     }
 }
@@ -508,6 +515,254 @@ at::Tensor encodeForward(const Encoding_ptr& enc, const at::Tensor& input, const
     return output;
 }
 
+// ------------------------------------------------------------------------------------------------ rows of tokens
+qmlp_tensor wrapToken(const at::Tensor& t) { return wrap(t, true); }
+
+/** All tensors on the GPU of the first. */
+void checkDevices(std::initializer_list<const at::Tensor*> tensors)
+{
+    const at::Tensor& first = **tensors.begin();
+    for (const at::Tensor* t : tensors) {
+        if (!t->defined()) continue;
+        if (!t->is_cuda()) throw std::runtime_error("QuickMLP tensors must live on the GPU");
+        if (t->device() != first.device()) throw std::runtime_error("the tensors of a call must live on one GPU");
+    }
+}
+/** With entries of the last dimension side by side, as the kernels want them. */
+at::Tensor consecutive(const at::Tensor& t)
+{
+    return !t.defined() || t.dim() == 0 || t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous();
+}
+at::Tensor temporary(const at::Tensor& like, size_t bytes) { return bytes > 0 ? bytesOn(like, bytes) : at::Tensor(); }
+void* dataOf(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+at::Tensor emptyLike(const at::Tensor& t) { return at::empty(t.sizes(), t.options().requires_grad(false)); }
+
+/** Calls from Python: errors of the C ABI become exceptions, the tensors' GPU is current. */
+template <typename Call>
+auto guarded(const at::Tensor& on, Call call)
+{
+    try {
+        at::AutoDispatchBelowADInplaceOrView below;
+        const c10::OptionalDeviceGuard guard(on.device());
+        return call();
+    } catch (const Failure& f) {
+        raise(f);
+    }
+}
+
+bool wantsGradient(const at::Tensor& t) { return t.defined() && at::GradMode::is_enabled() && t.requires_grad(); }
+
+/**
+ * What the nodes below have in common. Their gradients are not differentiable themselves: where the caller asks for a graph of them, a
+ * second backward pass is refused.
+ */
+struct TokenNode : torch::autograd::Node
+{
+    std::vector<SavedVariable> saved;
+
+    void release_variables() override
+    {
+        std::lock_guard<std::mutex> lock(mutex_);   // (as generated nodes do: two threads may run backward on one graph)
+        for (auto& v : saved) v.reset_data();
+    }
+    virtual void adjoint(const at::Tensor& gradOutput, variable_list& grads) = 0;
+    variable_list apply(variable_list&& gradOutputs) override
+    {
+        std::lock_guard<std::mutex> lock(mutex_);
+        variable_list grads(num_outputs());
+        if (!gradOutputs[0].defined()) return grads;
+        try {
+            at::AutoDispatchBelowADInplaceOrView below;
+            const c10::OptionalDeviceGuard guard(gradOutputs[0].device());
+            adjoint(gradOutputs[0], grads);
+        } catch (...) {
+            raiseFromBackward();
+        }
+        if (at::GradMode::is_enabled()) {
+            for (auto& g : grads)
+                if (g.defined()) g = g.detach().set_requires_grad(true);
+            grads = (*std::make_shared<torch::autograd::DelayedError>("gradients of " + name() + " cannot be differentiated again", grads.size()))(
+                std::move(grads));
+        }
+        return grads;
+    }
+};
+
+/** \param edges the inputs that gradients go to; \param saved what the backward pass reads */
+template <typename Node>
+std::shared_ptr<Node> attach(const at::Tensor& output, at::TensorList edges, at::TensorList saved)
+{
+    auto node = std::shared_ptr<Node>(new Node(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(edges));
+    node->saved.reserve(saved.size());
+    for (const auto& t : saved) node->saved.emplace_back(t, false);
+    torch::autograd::set_history(output, node);
+    return node;
+}
+
+void refuseRecording()
+{
+    if (at::tracer::impl::is_dispatch_enabled()) throw std::runtime_error("operators on tokens cannot be recorded by torch.jit.trace");
+}
+
+py::tuple group(const at::Tensor& index, int64_t groups)
+{
+    refuseRecording();
+    checkDevices({&index});
+    if (groups < 0 || groups >= INT32_MAX) throw py::value_error("the number of groups must be at least 0 and less than 2^31 - 1");
+    return guarded(index, [&] {
+        const at::Tensor flat = index.reshape({-1});
+        const auto options = flat.options().dtype(at::kInt);
+        const at::Tensor order = at::empty({flat.size(0)}, options), offsets = at::empty({groups + 1}, options);
+        size_t bytes = 0;
+        check(qmlp_tokens_group_memory(flat.size(0), static_cast<int>(groups), &bytes));
+        const at::Tensor memory = temporary(flat, bytes);
+        const qmlp_tensor in = wrapToken(flat), ord = wrapToken(order), off = wrapToken(offsets);
+        check(qmlp_tokens_group(&in, static_cast<int>(groups), &ord, &off, dataOf(memory), currentStream(flat)));
+        return py::make_tuple(order, offsets);
+    });
+}
+
+struct EmbeddingBackward : TokenNode
+{
+    float scale = 1;
+    std::string name() const override { return "QmlpEmbeddingBackward"; }
+    std::vector<int64_t> tableSizes;
+    void adjoint(const at::Tensor& gradOutput, variable_list& grads) override
+    {
+        const at::Tensor index = saved[0].unpack().reshape({-1}), adjOutput = consecutive(gradOutput.reshape({index.size(0), tableSizes[1]}));
+        const at::Tensor adjTable = at::empty(tableSizes, adjOutput.options());
+        size_t bytes = 0;
+        check(qmlp_tokens_embedding_adjoint_memory(index.size(0), tableSizes[0], static_cast<int>(tableSizes[1]), &bytes));
+        const at::Tensor memory = temporary(adjOutput, bytes);
+        const qmlp_tensor in = wrapToken(index), dy = wrapToken(adjOutput), dt = wrapToken(adjTable);
+        check(qmlp_tokens_embedding_adjoint(&in, &dy, scale, &dt, dataOf(memory), currentStream(adjOutput)));
+        grads[0] = adjTable;
+    }
+};
+
+at::Tensor embedding(const at::Tensor& index, const at::Tensor& table, double scale)
+{
+    refuseRecording();
+    checkDevices({&table, &index});
+    refuseOtherModes({index, table});
+    if (table.dim() != 2) throw std::runtime_error("table must be a tensor with 2 dimensions (vocabulary, channels)");
+    const at::Tensor output = guarded(table, [&] {
+        const at::Tensor flat = index.reshape({-1}), rows = consecutive(table);
+        const at::Tensor out = at::empty({flat.size(0), table.size(1)}, table.options().requires_grad(false));
+        const qmlp_tensor in = wrapToken(flat), t = wrapToken(rows), o = wrapToken(out);
+        check(qmlp_tokens_embedding(&in, &t, static_cast<float>(scale), &o, currentStream(table)));
+        auto sizes = index.sizes().vec();
+        sizes.push_back(table.size(1));
+        return sizes.size() == 2 ? out : out.view(sizes);
+    });
+    if (wantsGradient(table)) {
+        auto node = attach<EmbeddingBackward>(output, {table}, {index});
+        node->scale = static_cast<float>(scale);
+        node->tableSizes = table.sizes().vec();
+    }
+    return output;
+}
+
+struct LayerNormBackward : TokenNode
+{
+    at::ScalarType weightType = at::kFloat;
+    std::string name() const override { return "QmlpLayerNormBackward"; }
+    void adjoint(const at::Tensor& gradOutput, variable_list& grads) override
+    {
+        const at::Tensor x = saved[0].unpack(), weight = saved[1].unpack(), mean = saved[2].unpack(), rstd = saved[3].unpack();
+        const int64_t channels = x.size(-1);
+        const at::Tensor rows = consecutive(x.reshape({mean.size(0), channels})), adjOutput = consecutive(gradOutput.reshape(rows.sizes()));
+        const bool sums = task_should_compute_output(1) || task_should_compute_output(2);
+        at::Tensor adjX, adjWeight, adjBias;
+        if (task_should_compute_output(0)) adjX = at::empty(rows.sizes(), rows.options());
+        if (task_should_compute_output(1)) adjWeight = at::empty({channels}, rows.options().dtype(weightType));
+        if (task_should_compute_output(2)) adjBias = at::empty({channels}, rows.options().dtype(weightType));
+        size_t bytes = 0;
+        if (sums) check(qmlp_tokens_layer_norm_adjoint_memory(rows.size(0), static_cast<int>(channels), &bytes));
+        const at::Tensor memory = temporary(rows, bytes);
+        const qmlp_tensor in = wrapToken(rows), w = wrapToken(weight), m = wrapToken(mean), r = wrapToken(rstd), dy = wrapToken(adjOutput),
+                          dx = wrapToken(adjX), dw = wrapToken(adjWeight), db = wrapToken(adjBias);
+        check(qmlp_tokens_layer_norm_adjoint(&in, &w, &m, &r, &dy, &dx, &dw, &db, dataOf(memory), currentStream(rows)));
+        if (adjX.defined()) grads[0] = adjX.view(x.sizes());
+        grads[1] = adjWeight;
+        grads[2] = adjBias;
+    }
+};
+
+at::Tensor layerNorm(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& bias, double epsilon)
+{
+    refuseRecording();
+    checkDevices({&x, &weight, &bias});
+    refuseOtherModes({x, weight, bias});
+    if (x.dim() < 1) throw std::runtime_error("input must have a dimension of channels");
+    const bool train = wantsGradient(x) || wantsGradient(weight) || wantsGradient(bias);
+    at::Tensor mean, rstd, w;
+    const at::Tensor output = guarded(x, [&] {
+        const int64_t channels = x.size(-1), count = channels > 0 ? x.numel() / channels : 0;
+        const at::Tensor rows = consecutive(x.dim() == 2 ? x : x.reshape({count, channels}));
+        const at::Tensor out = at::empty({rows.size(0), channels}, x.options().requires_grad(false));
+        w = consecutive(weight);
+        const at::Tensor b = consecutive(bias);
+        if (train) {
+            mean = at::empty({rows.size(0)}, out.options().dtype(at::kFloat));
+            rstd = at::empty({rows.size(0)}, out.options().dtype(at::kFloat));
+        }
+        const qmlp_tensor in = wrapToken(rows), wt = wrapToken(w), bt = wrapToken(b), o = wrapToken(out), m = wrapToken(mean), r = wrapToken(rstd);
+        check(qmlp_tokens_layer_norm(&in, &wt, &bt, static_cast<float>(epsilon), &o, &m, &r, currentStream(x)));
+        return x.dim() == 2 ? out : out.view(x.sizes());
+    });
+    if (train) {
+        auto node = attach<LayerNormBackward>(output, {x, weight, bias}, {x, w.defined() && !w.is_same(weight) ? w.detach() : weight, mean, rstd});
+        node->weightType = weight.defined() ? weight.scalar_type() : bias.defined() ? bias.scalar_type() : x.scalar_type();
+    }
+    return output;
+}
+
+struct GroupedLinearBackward : TokenNode
+{
+    std::string name() const override { return "QmlpGroupedLinearBackward"; }
+    void adjoint(const at::Tensor& gradOutput, variable_list& grads) override
+    {
+        const at::Tensor x = consecutive(saved[0].unpack()), weight = consecutive(saved[1].unpack()), offsets = saved[2].unpack(),
+                         adjOutput = consecutive(gradOutput);
+        at::Tensor adjX, adjWeight, adjBias;
+        if (task_should_compute_output(0)) adjX = emptyLike(x);
+        if (task_should_compute_output(1)) adjWeight = emptyLike(weight);
+        if (task_should_compute_output(2)) adjBias = at::empty({weight.size(0), weight.size(1)}, weight.options().requires_grad(false));
+        size_t bytes = 0;
+        if (adjWeight.defined() || adjBias.defined())
+            check(qmlp_tokens_grouped_linear_adjoint_memory(x.size(0), static_cast<int>(weight.size(0)), static_cast<int>(weight.size(2)),
+                                                            static_cast<int>(weight.size(1)), &bytes));
+        const at::Tensor memory = temporary(x, bytes);
+        const qmlp_tensor in = wrapToken(x), w = wrapToken(weight), off = wrapToken(offsets), dy = wrapToken(adjOutput), dx = wrapToken(adjX),
+                          dw = wrapToken(adjWeight), db = wrapToken(adjBias);
+        check(qmlp_tokens_grouped_linear_adjoint(&in, &w, &off, &dy, &dx, &dw, &db, dataOf(memory), currentStream(x)));
+        grads[0] = adjX;
+        grads[1] = adjWeight;
+        grads[2] = adjBias;
+    }
+};
+
+at::Tensor groupedLinear(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& offsets, const at::Tensor& bias)
+{
+    refuseRecording();
+    checkDevices({&x, &weight, &offsets, &bias});
+    refuseOtherModes({x, weight, offsets, bias});
+    if (x.dim() != 2) throw std::runtime_error("input must be a tensor with 2 dimensions (rows, inputs)");
+    if (weight.dim() != 3) throw std::runtime_error("weight must be a tensor with 3 dimensions (experts, outputs, inputs)");
+    const at::Tensor output = guarded(x, [&] {
+        const at::Tensor rows = consecutive(x), w = consecutive(weight), b = consecutive(bias), off = consecutive(offsets);
+        const at::Tensor out = at::empty({x.size(0), weight.size(1)}, x.options().requires_grad(false));
+        const qmlp_tensor in = wrapToken(rows), wt = wrapToken(w), of = wrapToken(off), bt = wrapToken(b), o = wrapToken(out);
+        check(qmlp_tokens_grouped_linear(&in, &wt, &of, &bt, &o, currentStream(x)));
+        return out;
+    });
+    if (wantsGradient(x) || wantsGradient(weight) || wantsGradient(bias))
+        attach<GroupedLinearBackward>(output, {x, weight, bias}, {x, weight, consecutive(offsets)});
+    return output;
+}
+
 at::Tensor tensorOrNone(const py::object& o) { return o.is_none() ? at::Tensor() : o.cast<at::Tensor>(); }
 py::object noneOr(const at::Tensor& t) { return t.defined() ? py::cast(t) : py::none(); }
 
@@ -592,4 +847,12 @@ PYBIND11_MODULE(_native, m)
                  return py::make_tuple(noneOr(g.first), noneOr(g.second));
              },
              "Gradients (input, parameter), the latter in floats; None where flags do not ask for them.");
+    m.def("group", group);
+    m.def("embedding", embedding);
+    m.def("layer_norm", [](const at::Tensor& x, const py::object& weight, const py::object& bias, double epsilon) {
+        return layerNorm(x, tensorOrNone(weight), tensorOrNone(bias), epsilon);
+    });
+    m.def("grouped_linear", [](const at::Tensor& x, const at::Tensor& weight, const at::Tensor& offsets, const py::object& bias) {
+        return groupedLinear(x, weight, offsets, tensorOrNone(bias));
+    });
 }

@@ -6,7 +6,9 @@ from ._version import __version__
 from .activation import FusedActivation
 from .encoding import FusedEncoding
 from .network import FusedNetwork, SimulatedNetwork, copy_torch_to_fused
+from . import tokens     # operators on rows of tokens: qmlp.tokens.layer_norm(x, weight, bias), ...
 from . import pullpush   # qmlp.pullpush.pullpush(mask, data), like the reference's module
+from .tokens import FusedEmbedding, FusedGroupedLinear, FusedLayerNorm
 from .classes import Activation, Encoding, Network, QuickMLP
 from ._lib import QmlpError, set_kernel_cache_dir, set_log_level
 
@@ -34,5 +36,5 @@ def load_library():
 
 __all__ = [
     "__version__", "load_library", "FusedActivation", "FusedEncoding", "FusedNetwork", "SimulatedNetwork",
-    "copy_torch_to_fused", "pullpush", "Activation", "Encoding", "Network", "QuickMLP", "QmlpError",
+    "FusedEmbedding", "FusedGroupedLinear", "FusedLayerNorm", "copy_torch_to_fused", "pullpush", "tokens", "Activation", "Encoding", "Network", "QuickMLP", "QmlpError",
     "set_kernel_cache_dir", "set_log_level"]

@@ -12,6 +12,7 @@ LIB_PATH = os.path.join(_HERE, "libqmlp.so")
 DEFAULT_CACHE_DIR = os.path.join(os.path.dirname(_HERE), ".kernel_cache")
 
 QMLP_FLOAT, QMLP_HALF, QMLP_DOUBLE = 0, 1, 2
+QMLP_BFLOAT16, QMLP_INT32, QMLP_INT64 = 3, 4, 5   # of the operators on rows of tokens alone
 QMLP_INFERENCE, QMLP_GRADIENTS = 0, 1
 GRADIENTS_INPUT, GRADIENTS_NETWORK_WEIGHTS, GRADIENTS_INPUT_ENCODINGS = 1, 2, 4
 
@@ -120,6 +121,18 @@ _SIGNATURES = {
     "qmlp_utils_pullpush_forward_in": [_TD, _TD, _TD, _vp, _vp],
     "qmlp_utils_pullpush_adjoint_in": [_TD, _TD, _TD, _TD, _TD, _ci, _vp, _ci, _vp, _vp],
     "qmlp_utils_pullpush_precompile": [_ci],
+    "qmlp_tokens_group_memory": [ctypes.c_longlong, _ci, _P(ctypes.c_size_t)],
+    "qmlp_tokens_group": [_TD, _ci, _TD, _TD, _vp, _vp],
+    "qmlp_tokens_embedding": [_TD, _TD, ctypes.c_float, _TD, _vp],
+    "qmlp_tokens_embedding_adjoint_memory": [ctypes.c_longlong, ctypes.c_longlong, _ci, _P(ctypes.c_size_t)],
+    "qmlp_tokens_embedding_adjoint": [_TD, _TD, ctypes.c_float, _TD, _vp, _vp],
+    "qmlp_tokens_layer_norm": [_TD, _TD, _TD, ctypes.c_float, _TD, _TD, _TD, _vp],
+    "qmlp_tokens_layer_norm_adjoint_memory": [ctypes.c_longlong, _ci, _P(ctypes.c_size_t)],
+    "qmlp_tokens_layer_norm_adjoint": [_TD, _TD, _TD, _TD, _TD, _TD, _TD, _TD, _vp, _vp],
+    "qmlp_tokens_grouped_linear": [_TD, _TD, _TD, _TD, _TD, _vp],
+    "qmlp_tokens_grouped_linear_adjoint_memory": [ctypes.c_longlong, _ci, _ci, _ci, _P(ctypes.c_size_t)],
+    "qmlp_tokens_grouped_linear_adjoint": [_TD, _TD, _TD, _TD, _TD, _TD, _TD, _vp, _vp],
+    "qmlp_tokens_precompile": [_ci],
 }
 for _name, _args in _SIGNATURES.items():
     _fn = getattr(lib, _name)
