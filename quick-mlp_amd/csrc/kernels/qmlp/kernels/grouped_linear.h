@@ -180,9 +180,7 @@ struct TileProduct
     static __device__ __forceinline__ int firstI() { return threadIdx.x / 64 / WJ * (NI * 32); }
     static __device__ __forceinline__ int firstJ() { return threadIdx.x / 64 % WJ * (NJ * 32); }
 
-    /** a, b: at the tile's first index and k = 0; ni, nj: indices that are there. sumA: also sums A over k. */
-    __device__ __forceinline__ void run(char* lds, const T* __restrict__ a, long long strideA, int ni, const T* __restrict__ b, long long strideB,
-                                        int nj, int K, bool sumA)
+    __device__ __forceinline__ void clear()
     {
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
@@ -190,8 +188,38 @@ struct TileProduct
 #pragma unroll
             for (int j = 0; j < NJ; ++j) sums[i][j] = f32x16{};
         }
-        const long long advanceA = A_ALONG_K ? TILE_K<T> : TILE_K<T> * strideA, advanceB = B_ALONG_K ? TILE_K<T> : TILE_K<T> * strideB;
+    }
+    /** Adds the products of tiles in LDS. */
+    __device__ __forceinline__ void multiplyTile(const T* ldsA, const T* ldsB, bool sumA)
+    {
         const int fromI = firstI(), fromJ = firstJ();
+#pragma unroll
+        for (int step = 0; step < TILE_K<T> / STEP_K<T>; ++step) {
+            typename Matrix<T>::Operand x[NI], w[NJ];
+#pragma unroll
+            for (int i = 0; i < NI; ++i) x[i] = TileA::operand(ldsA, fromI + i * 32, step);
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) w[j] = TileB::operand(ldsB, fromJ + j * 32, step);
+#pragma unroll
+            for (int i = 0; i < NI; ++i)
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) sums[i][j] = Matrix<T>::multiply(w[j], x[i], sums[i][j]);
+            if (sumA) {
+                typename Matrix<T>::Operand ones;
+#pragma unroll
+                for (int n = 0; n < static_cast<int>(sizeof(ones) / sizeof(T)); ++n) ones[n] = static_cast<T>(1);
+#pragma unroll
+                for (int i = 0; i < NI; ++i) sumsOfA[i] = Matrix<T>::multiply(ones, x[i], sumsOfA[i]);
+            }
+        }
+    }
+
+    /** a, b: at the tile's first index and k = 0; ni, nj: indices that are there. sumA: also sums A over k. */
+    __device__ __forceinline__ void run(char* lds, const T* __restrict__ a, long long strideA, int ni, const T* __restrict__ b, long long strideB,
+                                        int nj, int K, bool sumA)
+    {
+        clear();
+        const long long advanceA = A_ALONG_K ? TILE_K<T> : TILE_K<T> * strideA, advanceB = B_ALONG_K ? TILE_K<T> : TILE_K<T> * strideB;
         TileA tileA;
         TileB tileB;
         int buffer = 0;
@@ -210,25 +238,7 @@ struct TileProduct
                 tileA.read(a, strideA, ni, left);
                 tileB.read(b, strideB, nj, left);
             }
-#pragma unroll
-            for (int step = 0; step < TILE_K<T> / STEP_K<T>; ++step) {
-                typename Matrix<T>::Operand x[NI], w[NJ];
-#pragma unroll
-                for (int i = 0; i < NI; ++i) x[i] = TileA::operand(ldsA, fromI + i * 32, step);
-#pragma unroll
-                for (int j = 0; j < NJ; ++j) w[j] = TileB::operand(ldsB, fromJ + j * 32, step);
-#pragma unroll
-                for (int i = 0; i < NI; ++i)
-#pragma unroll
-                    for (int j = 0; j < NJ; ++j) sums[i][j] = Matrix<T>::multiply(w[j], x[i], sums[i][j]);
-                if (sumA) {
-                    typename Matrix<T>::Operand ones;
-#pragma unroll
-                    for (int n = 0; n < static_cast<int>(sizeof(ones) / sizeof(T)); ++n) ones[n] = static_cast<T>(1);
-#pragma unroll
-                    for (int i = 0; i < NI; ++i) sumsOfA[i] = Matrix<T>::multiply(ones, x[i], sumsOfA[i]);
-                }
-            }
+            multiplyTile(ldsA, ldsB, sumA);
             buffer ^= 1;
         }
     }
@@ -250,6 +260,120 @@ struct TileProduct
                     put(firstI() + i * 32 + lane % 32, firstJ() + j * 32 + n * 2 + lane / 32 * 4, v);
                 }
     }
+};
+
+/** A buffer descriptor for raw accesses of 'bytes' bytes at p; reads behind them give zeros. */
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ u32x4 bufferAt(const void* p, unsigned bytes)
+{
+    const unsigned long long a = reinterpret_cast<unsigned long long>(p);
+    return u32x4{static_cast<unsigned>(__builtin_amdgcn_readfirstlane(static_cast<int>(a))),
+                 static_cast<unsigned>(__builtin_amdgcn_readfirstlane(static_cast<int>(a >> 32))) & 0xffffu,
+                 static_cast<unsigned>(__builtin_amdgcn_readfirstlane(static_cast<int>(bytes))), 0x00020000u};
+}
+/**
+ * Every lane moves 16 bytes from its offset into the buffer to LDS, those of the wavefront side by side from 'lds' on. As a builtin the
+ * compiler would wait for it in front of every later read of LDS; this way it is waited for by waitForTiles() alone. (The wait states: a
+ * descriptor in scalar registers that vector instructions wrote may be read five later.)
+ */
+__device__ __forceinline__ void loadToLds(u32x4 buffer, unsigned offset, unsigned lds)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(buffer) : "memory");
+}
+/** All of the wavefront's loads to LDS have arrived, its reads of LDS are done, and so are those of the others. */
+__device__ __forceinline__ void waitForTiles()
+{
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+/**
+ * Moves the tiles of an operand of 16 bits straight from global memory to LDS. The address, the strides and the operand's sizes are
+ * multiples of 16 bytes, and rows do not overlap. Indices that are not there hold others' values, which no result depends on;
+ * k that are not there are zero.
+ */
+template <typename T, bool ALONG_K, int SIZE, int THREADS>
+struct DirectTile
+{
+    typedef Tile<T, ALONG_K, SIZE, THREADS> Layout;
+    static constexpr int PIECES = Layout::PIECES, EACH = Layout::EACH;
+    const T* p;
+    long long stride;
+    int indices;
+    unsigned offsets[EACH];
+    int columns[EACH];   // along k: the first k of a piece
+
+    __device__ __forceinline__ void begin(const T* p_, long long stride_, int indices_)
+    {
+        p = p_;
+        stride = stride_;
+        indices = indices_;
+#pragma unroll
+        for (int n = 0; n < EACH; ++n) {
+            const int piece = n * THREADS + threadIdx.x;
+            const int row = piece / PIECES;
+            // which piece belongs here is what Layout::place() says of the piece there: exchanging is its own inverse
+            const int column = Layout::place(row, piece % PIECES * WIDE<T>) - row * Layout::ROW;
+            columns[n] = column;
+            // (rows behind the last index are read from the last one; columns behind it lie in the next row, or behind the buffer)
+            offsets[n] = static_cast<unsigned>(((ALONG_K ? min(row, indices - 1) : row) * stride + column) * sizeof(T));
+        }
+    }
+    /** The tile of the 'ks' next values of k, to LDS from 'lds' on. */
+    __device__ __forceinline__ void load(unsigned lds, int ks)
+    {
+        const unsigned bytes = static_cast<unsigned>(((ALONG_K ? indices - 1 : ks - 1) * stride + (ALONG_K ? ks : indices)) * sizeof(T));
+        const u32x4 buffer = bufferAt(p, bytes);
+        const unsigned to = __builtin_amdgcn_readfirstlane(lds + threadIdx.x / 64 * 1024);
+        const bool whole = !ALONG_K || ks == TILE_K<T>;
+#pragma unroll
+        for (int n = 0; n < EACH; ++n) loadToLds(buffer, whole || columns[n] < ks ? offsets[n] : 0x80000000u, to + n * THREADS * 16);
+        p += ALONG_K ? TILE_K<T> : TILE_K<T> * stride;
+    }
+};
+
+/** TileProduct whose tiles go to LDS without registers in between, the next ones while the present ones are multiplied. */
+template <typename T, bool A_ALONG_K, bool B_ALONG_K, int TI, int TJ, int WI, int WJ>
+struct DirectProduct : TileProduct<T, A_ALONG_K, B_ALONG_K, TI, TJ, WI, WJ>
+{
+    typedef TileProduct<T, A_ALONG_K, B_ALONG_K, TI, TJ, WI, WJ> Base;
+
+    __device__ __forceinline__ void run(char* lds, const T* __restrict__ a, long long strideA, int ni, const T* __restrict__ b, long long strideB,
+                                        int nj, int K, bool sumA)
+    {
+        this->clear();
+        if (K <= 0) return;
+        DirectTile<T, A_ALONG_K, TI, Base::THREADS> tileA;
+        DirectTile<T, B_ALONG_K, TJ, Base::THREADS> tileB;
+        tileA.begin(a, strideA, ni);
+        tileB.begin(b, strideB, nj);
+        constexpr unsigned BYTES_A = Base::TileA::BYTES, BYTES = BYTES_A + Base::TileB::BYTES;
+        const unsigned at = static_cast<unsigned>(reinterpret_cast<unsigned long long>((__attribute__((address_space(3))) char*)lds));
+        unsigned buffer = 0;
+        tileA.load(at, min(K, TILE_K<T>));
+        tileB.load(at + BYTES_A, min(K, TILE_K<T>));
+        for (int k = 0; k < K; k += TILE_K<T>) {
+            waitForTiles();
+            const int left = min(K - k - TILE_K<T>, TILE_K<T>);
+            if (left > 0) {
+                tileA.load(at + (buffer ^ BYTES), left);
+                tileB.load(at + (buffer ^ BYTES) + BYTES_A, left);
+            }
+            this->multiplyTile(reinterpret_cast<const T*>(lds + buffer), reinterpret_cast<const T*>(lds + buffer + BYTES_A), sumA);
+            buffer ^= BYTES;
+        }
+    }
+};
+
+/** The product of tiles of any address and size, or of those that can go straight to LDS. */
+template <bool DIRECT, typename T, bool A_ALONG_K, bool B_ALONG_K, int TI, int TJ, int WI, int WJ>
+struct ProductOf
+{
+    typedef TileProduct<T, A_ALONG_K, B_ALONG_K, TI, TJ, WI, WJ> Type;
+};
+template <typename T, bool A_ALONG_K, bool B_ALONG_K, int TI, int TJ, int WI, int WJ>
+struct ProductOf<true, T, A_ALONG_K, B_ALONG_K, TI, TJ, WI, WJ>
+{
+    typedef DirectProduct<T, A_ALONG_K, B_ALONG_K, TI, TJ, WI, WJ> Type;
 };
 
 /** Up to four consecutive values, as many as are left before 'end'. */
@@ -306,22 +430,42 @@ __device__ __forceinline__ ExpertTile expertTile(const int* __restrict__ offsets
     return t;
 }
 
+/**
+ * Which of 'places' x 'tiles' a workgroup takes. Workgroups go to the dies in turn, each with an L2 of its own: a die takes consecutive
+ * ones of an order that goes through the tiles for GROUP_PLACES places at a time, so that those at work on it share both operands.
+ */
+constexpr int GROUP_PLACES = 4;
+struct Work
+{
+    int place, tile;
+};
+__device__ __forceinline__ Work workOf(unsigned id, unsigned places, unsigned tiles)
+{
+    const unsigned total = places * tiles, each = total / DIES, rest = total % DIES;
+    const unsigned die = id % DIES;
+    const unsigned n = die * each + min(die, rest) + id / DIES;
+    const unsigned group = n / (GROUP_PLACES * tiles), within = n - group * (GROUP_PLACES * tiles);
+    const unsigned count = min(static_cast<unsigned>(GROUP_PLACES), places - group * GROUP_PLACES);
+    return {static_cast<int>(group * GROUP_PLACES + within % count), static_cast<int>(within / count)};
+}
+
 // ------------------------------------------------------------------------------------------------ kernels
 /**
  * Rows times the experts' matrices: y[r][j] = sum over k of x[r][k] B(j, k) + bias[e][j]. B_ALONG_K: weights[e][j][k] (the layer),
  * otherwise weights[e][k][j] (its adjoint). Workgroups: places of tiles x tiles of J.
  */
-template <typename T, bool B_ALONG_K, int TI, int TJ, int WI, int WJ>
+template <typename T, bool DIRECT, bool B_ALONG_K, int TI, int TJ, int WI, int WJ>
 __global__ void __launch_bounds__(64 * WI * WJ)
 GroupedRowsKernel(const T* __restrict__ x, long long strideX, const T* __restrict__ weights, long long strideExpert, long long strideWeights,
                   const T* __restrict__ bias, long long strideBias, const int* __restrict__ offsets, int experts, T* __restrict__ y, long long strideY,
-                  int rows, int J, int K, int tilesJ)
+                  int rows, int J, int K, int places, int tilesJ)
 {
-    typedef TileProduct<T, true, B_ALONG_K, TI, TJ, WI, WJ> Product;
+    typedef typename ProductOf<DIRECT, T, true, B_ALONG_K, TI, TJ, WI, WJ>::Type Product;
     extern __shared__ __attribute__((aligned(16))) char groupedLds[];
-    const ExpertTile at = expertTile(offsets, experts, rows, TI, blockIdx.x / tilesJ);
+    const Work work = workOf(blockIdx.x, places, tilesJ);
+    const ExpertTile at = expertTile(offsets, experts, rows, TI, work.place);
     if (at.to <= at.from) return;
-    const int j0 = blockIdx.x % tilesJ * TJ;
+    const int j0 = work.tile * TJ;
     const int ni = at.to - at.from, nj = min(J - j0, TJ);
     Product product;
     const bool none = at.expert >= experts;
@@ -343,25 +487,26 @@ GroupedRowsKernel(const T* __restrict__ x, long long strideX, const T* __restric
  * adjY (null: not wanted). Workgroups: places of 'chunk' rows x tiles of I x tiles of J. An expert with more rows than a chunk has
  * its sums per chunk in partial[place], I x J and I floats, for GroupedSumKernel.
  */
-template <typename T, int TI, int TJ, int WI, int WJ>
+template <typename T, bool DIRECT, int TI, int TJ, int WI, int WJ>
 __global__ void __launch_bounds__(64 * WI * WJ)
 GroupedWeightsKernel(const T* __restrict__ adjY, long long strideAdjY, const T* __restrict__ x, long long strideX, const int* __restrict__ offsets,
-                     int experts, T* __restrict__ adjWeights, T* __restrict__ adjBias, float* __restrict__ partial, int rows, int I, int J, int tilesI,
-                     int tilesJ, int chunk)
+                     int experts, T* __restrict__ adjWeights, T* __restrict__ adjBias, float* __restrict__ partial, int rows, int I, int J, int places,
+                     int tilesI, int tilesJ, int chunk)
 {
-    typedef TileProduct<T, false, false, TI, TJ, WI, WJ> Product;
+    typedef typename ProductOf<DIRECT, T, false, false, TI, TJ, WI, WJ>::Type Product;
     extern __shared__ __attribute__((aligned(16))) char groupedLds[];
-    const int tile = blockIdx.x % (tilesI * tilesJ);
-    const ExpertTile at = expertTile(offsets, experts, rows, chunk, blockIdx.x / (tilesI * tilesJ));
+    const Work work = workOf(blockIdx.x % (tilesI * tilesJ), tilesI, tilesJ);   // (tiles of one place: rows of tiles for its places)
+    const int place = blockIdx.x / (tilesI * tilesJ);
+    const ExpertTile at = expertTile(offsets, experts, rows, chunk, place);
     if (at.expert >= experts || (at.to <= at.from && at.index != 0)) return;   // (the first place of an expert without rows writes zeros)
-    const int i0 = tile / tilesJ * TI, j0 = tile % tilesJ * TJ;
+    const int i0 = work.place * TI, j0 = work.tile * TJ;
     const int ni = min(I - i0, TI), nj = min(J - j0, TJ);
     const bool whole = at.expertRows <= chunk;
     const bool sumA = adjBias && j0 == 0;
     Product product;
     product.run(groupedLds, adjY + at.from * strideAdjY + i0, strideAdjY, ni, x + at.from * strideX + j0, strideX, nj, max(0, at.to - at.from), sumA);
     const long long size = static_cast<long long>(I) * J;
-    float* sums = whole ? nullptr : partial + (blockIdx.x / (tilesI * tilesJ)) * (size + I);
+    float* sums = whole ? nullptr : partial + place * (size + I);
     T* out = adjWeights + at.expert * size;
     if (adjWeights || !whole)
         product.results([&](int i, int j, float (&v)[4]) {

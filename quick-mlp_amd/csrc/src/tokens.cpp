@@ -130,8 +130,8 @@ void checkMemory(const void* memory, size_t bytes)
 
 template <typename T>
 T* ptr(const Tensor& t) { return t.defined() ? static_cast<T*>(const_cast<void*>(t.rawPtr())) : nullptr; }
-/** The stride of a dimension; of one with a single entry it may be anything. */
-long long strideOf(const Tensor& t, int d) { return t.size(d) <= 1 ? 0 : t.stride(d); }
+/** The stride of a dimension; of one with a single entry it may be anything and is taken to be that of rows side by side. */
+long long strideOf(const Tensor& t, int d) { return t.size(d) <= 1 ? t.size(t.ndim() - 1) : t.stride(d); }
 
 /** Workgroups for so many pieces of work of their own, no more than 'most' (the kernels go on in steps of the grid). */
 unsigned workgroups(int64_t pieces, int64_t most) { return static_cast<unsigned>(std::max<int64_t>(1, std::min(pieces, most))); }
@@ -303,9 +303,26 @@ struct GroupedTiles
     unsigned lds() const { return 2 * 128 * (i + j); }
     std::string arguments() const { return str(i, ", ", j, ", ", wavesI, ", ", wavesJ); }
 };
-constexpr GroupedTiles LARGE_TILES = {128, 128, 2, 2}, SMALL_TILES = {64, 64, 2, 2};
+constexpr GroupedTiles HUGE_TILES = {256, 256, 2, 4}, LARGE_TILES = {128, 128, 2, 2}, SMALL_TILES = {64, 64, 2, 2};
 
-GroupedTiles tilesFor(int64_t i, int64_t j) { return i <= 64 || j <= 64 ? SMALL_TILES : LARGE_TILES; }
+GroupedTiles tilesFor(int64_t i, int64_t j, bool direct)
+{
+    if (i <= 64 || j <= 64) return SMALL_TILES;
+    return direct && i > 128 && j > 128 ? HUGE_TILES : LARGE_TILES;
+}
+
+/** Whether tiles of the operand can go straight from global memory to LDS (DirectTile). */
+bool isDirect(const Tensor& t)
+{
+    if (t.bytesPerEntry() != 2 || reinterpret_cast<uintptr_t>(t.rawPtr()) % 16 != 0) return false;
+    const int n = t.ndim();
+    if (t.size(n - 1) % 8 != 0) return false;
+    for (int d = 0; d + 1 < n; ++d)
+        if (t.size(d) > 1 && t.stride(d) % 8 != 0) return false;
+    // rows that do not overlap, 256 of which have 32-bit offsets
+    return t.size(n - 2) <= 1 || (t.stride(n - 2) >= t.size(n - 1) && t.stride(n - 2) < (1 << 21));
+}
+const char* boolName(bool b) { return b ? "true" : "false"; }
 
 /** Places of tiles (kernels/grouped_linear.h): one more than rows / tileRows for each expert and for the rows behind them. */
 int64_t tilePlaces(int64_t rows, int64_t experts, int64_t tileRows) { return rows / tileRows + experts + 1; }
@@ -325,9 +342,9 @@ struct GroupedAdjointPlan
     int64_t tilesI, tilesJ, chunk, places;
     Workspace memory;
     float* partial = nullptr;
-    GroupedAdjointPlan(int64_t rows, int64_t experts, int64_t inputs, int64_t outputs, void* base) : memory{static_cast<char*>(base)}
+    GroupedAdjointPlan(int64_t rows, int64_t experts, int64_t inputs, int64_t outputs, bool direct, void* base) : memory{static_cast<char*>(base)}
     {
-        tiles = tilesFor(outputs, inputs);
+        tiles = tilesFor(outputs, inputs, direct);
         tilesI = divUp<int64_t>(outputs, tiles.i);
         tilesJ = divUp<int64_t>(inputs, tiles.j);
         chunk = weightsChunk(rows, experts, tilesI * tilesJ);
@@ -358,6 +375,22 @@ GroupedSizes checkGrouped(const Tensor& input, const Tensor& weight, const Tenso
     checkSizes(weight, "weight", {s.experts, s.outputs, s.inputs});
     checkSizes(offsets, "offsets", {s.experts + 1ll});
     return s;
+}
+
+/** GroupedRowsKernel: y (rows, J) from x (rows, K) and the weights along K (the layer) or across it (its adjoint). */
+void launchRows(bool alongK, const Tensor& x, const Tensor& weight, const Tensor& offsets, const Tensor& bias, const Tensor& y, const GroupedSizes& s,
+                int J, int K, stream_t stream)
+{
+    const bool direct = isDirect(x) && isDirect(weight);
+    const GroupedTiles t = tilesFor(s.rows / std::max(s.experts, 1), J, direct);
+    const int tilesJ = divUp(J, t.j);
+    const int64_t places = tilePlaces(s.rows, s.experts, t.i);
+    checkLaunch(places * tilesJ, t.threads());
+    tokenKernel("grouped_linear.h", str("GroupedRowsKernel<", scalarName(x.precision()), ", ", boolName(direct), ", ", boolName(alongK), ", ", t.arguments(), ">"))
+        .call(static_cast<unsigned>(places * tilesJ), t.threads(), t.lds(), stream, x.rawPtr(), strideOf(x, 0), static_cast<const void*>(ptr<void>(weight)),
+              strideOf(weight, 0), strideOf(weight, 1), static_cast<const void*>(ptr<void>(bias)), bias.defined() ? strideOf(bias, 0) : 0ll,
+              static_cast<const int*>(ptr<int>(offsets)), s.experts, static_cast<void*>(ptr<void>(y)), strideOf(y, 0), s.rows, J, K, static_cast<int>(places),
+              tilesJ);
 }
 
 } // namespace
@@ -578,21 +611,16 @@ void Tokens::groupedLinear(const Tensor& input, const Tensor& weight, const Tens
     checkSizes(output, "output", {s.rows, s.outputs});
     checkOutput(output, "output");
     if (s.rows == 0) return;
-    const GroupedTiles t = tilesFor(s.rows / std::max(s.experts, 1), s.outputs);
-    const int tilesJ = divUp(s.outputs, t.j);
-    const int64_t groups = tilePlaces(s.rows, s.experts, t.i) * tilesJ;
-    checkLaunch(groups, t.threads());
-    tokenKernel("grouped_linear.h", str("GroupedRowsKernel<", scalarName(p), ", true, ", t.arguments(), ">"))
-        .call(static_cast<unsigned>(groups), t.threads(), t.lds(), stream, input.rawPtr(), strideOf(input, 0), static_cast<const void*>(ptr<void>(weight)),
-              strideOf(weight, 0), strideOf(weight, 1), static_cast<const void*>(ptr<void>(bias)), bias.defined() ? strideOf(bias, 0) : 0ll,
-              static_cast<const int*>(ptr<int>(offsets)), s.experts, output.rawPtr(), strideOf(output, 0), s.rows, s.outputs, s.inputs, tilesJ);
+    launchRows(true, input, weight, offsets, bias, output, s, s.outputs, s.inputs, stream);
 }
 
 size_t Tokens::groupedLinearAdjointMemory(int64_t rows, int experts, int inputs, int outputs)
 {
     CHECK_ERROR(rows >= 0 && experts >= 0 && inputs >= 0 && outputs >= 0, "sizes must not be negative");
     if (experts == 0) return 0;
-    return GroupedAdjointPlan(rows, experts, inputs, outputs, nullptr).memory.bytes;
+    // (for any type and alignment)
+    return std::max(GroupedAdjointPlan(rows, experts, inputs, outputs, true, nullptr).memory.bytes,
+                    GroupedAdjointPlan(rows, experts, inputs, outputs, false, nullptr).memory.bytes);
 }
 
 void Tokens::groupedLinearAdjoint(const Tensor& input, const Tensor& weight, const Tensor& offsets, const Tensor& adjOutput, Tensor& adjInput,
@@ -623,25 +651,18 @@ void Tokens::groupedLinearAdjoint(const Tensor& input, const Tensor& weight, con
     }
     const int* off = ptr<int>(offsets);
     const void *x = ptr<void>(input), *dy = ptr<void>(adjOutput);
-    if (adjInput.defined() && s.rows > 0) {
-        const GroupedTiles t = tilesFor(s.rows / std::max(s.experts, 1), s.inputs);
-        const int tilesJ = divUp(s.inputs, t.j);
-        const int64_t groups = tilePlaces(s.rows, s.experts, t.i) * tilesJ;
-        checkLaunch(groups, t.threads());
-        tokenKernel("grouped_linear.h", str("GroupedRowsKernel<", scalarName(p), ", false, ", t.arguments(), ">"))
-            .call(static_cast<unsigned>(groups), t.threads(), t.lds(), stream, dy, strideOf(adjOutput, 0), static_cast<const void*>(ptr<void>(weight)),
-                  strideOf(weight, 0), strideOf(weight, 1), static_cast<const void*>(nullptr), 0ll, off, s.experts, adjInput.rawPtr(),
-                  strideOf(adjInput, 0), s.rows, s.inputs, s.outputs, tilesJ);
-    }
+    if (adjInput.defined() && s.rows > 0) launchRows(false, adjOutput, weight, offsets, {}, adjInput, s, s.inputs, s.outputs, stream);
     if (s.experts == 0 || (!adjWeight.defined() && !adjBias.defined())) return;
     checkMemory(memory, groupedLinearAdjointMemory(s.rows, s.experts, s.inputs, s.outputs));
-    GroupedAdjointPlan plan(s.rows, s.experts, s.inputs, s.outputs, memory);
+    const bool direct = isDirect(input) && isDirect(adjOutput);
+    GroupedAdjointPlan plan(s.rows, s.experts, s.inputs, s.outputs, direct, memory);
     const int64_t groups = plan.places * plan.tilesI * plan.tilesJ;
     checkLaunch(groups, plan.tiles.threads());
     const int chunk = static_cast<int>(plan.chunk);
-    tokenKernel("grouped_linear.h", str("GroupedWeightsKernel<", scalarName(p), ", ", plan.tiles.arguments(), ">"))
+    tokenKernel("grouped_linear.h", str("GroupedWeightsKernel<", scalarName(p), ", ", boolName(direct), ", ", plan.tiles.arguments(), ">"))
         .call(static_cast<unsigned>(groups), plan.tiles.threads(), plan.tiles.lds(), stream, dy, strideOf(adjOutput, 0), x, strideOf(input, 0), off, s.experts,
-              ptr<void>(adjWeight), ptr<void>(adjBias), plan.partial, s.rows, s.outputs, s.inputs, static_cast<int>(plan.tilesI), static_cast<int>(plan.tilesJ), chunk);
+              ptr<void>(adjWeight), ptr<void>(adjBias), plan.partial, s.rows, s.outputs, s.inputs,
+              static_cast<int>(plan.places), static_cast<int>(plan.tilesI), static_cast<int>(plan.tilesJ), chunk);
     if (plan.partial) {
         const long long size = static_cast<long long>(s.inputs) * s.outputs;
         const int64_t pieces = divUp<int64_t>(size + s.outputs, 256);
@@ -676,11 +697,13 @@ void Tokens::precompile(Tensor::Precision p)
         for (const char* kernel : {"LayerNormKernel", "LayerNormAdjointKernel"}) precompileKernel("layer_norm.h", str(kernel, "<", t, ", ", t, ", ", s.arguments(), ">"));
     for (const char* kernel : {"LayerNormLongKernel", "LayerNormLongAdjointKernel"}) precompileKernel("layer_norm.h", str(kernel, "<", t, ", ", t, ">"));
     for (const char* kernel : {"LayerNormLongSumsKernel", "LayerNormSumKernel"}) precompileKernel("layer_norm.h", str(kernel, "<", t, ">"));
-    for (const GroupedTiles& tiles : {LARGE_TILES, SMALL_TILES}) {
-        precompileKernel("grouped_linear.h", str("GroupedRowsKernel<", t, ", true, ", tiles.arguments(), ">"));
-        precompileKernel("grouped_linear.h", str("GroupedRowsKernel<", t, ", false, ", tiles.arguments(), ">"));
-        precompileKernel("grouped_linear.h", str("GroupedWeightsKernel<", t, ", ", tiles.arguments(), ">"));
-    }
+    for (const bool direct : {false, true})
+        for (const GroupedTiles& tiles : {HUGE_TILES, LARGE_TILES, SMALL_TILES}) {
+            if (direct ? p == Tensor::FLOAT : tiles.i > 128) continue;
+            const std::string types = str(t, ", ", boolName(direct));
+            for (const char* along : {", true, ", ", false, "}) precompileKernel("grouped_linear.h", str("GroupedRowsKernel<", types, along, tiles.arguments(), ">"));
+            precompileKernel("grouped_linear.h", str("GroupedWeightsKernel<", types, ", ", tiles.arguments(), ">"));
+        }
     precompileKernel("grouped_linear.h", str("GroupedSumKernel<", t, ">"));
 }
 

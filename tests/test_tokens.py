@@ -315,7 +315,7 @@ COUNTS = {
 
 @gpu
 @pytest.mark.parametrize("counts", list(COUNTS))
-@pytest.mark.parametrize("inputs,outputs", [(1, 1), (3, 5), (16, 32), (64, 64), (77, 130), (200, 33), (256, 512)])
+@pytest.mark.parametrize("inputs,outputs", [(1, 1), (3, 5), (16, 32), (64, 64), (64, 56), (77, 130), (200, 33), (256, 512)])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_grouped_linear_and_its_gradients(counts, inputs, outputs, dtype):
     say("grouped linear", counts, inputs, outputs, dtype)
