@@ -175,7 +175,7 @@ struct TileProduct
     static constexpr int LDS_BYTES = 2 * (TileA::BYTES + TileB::BYTES);
 
     f32x16 sums[NI][NJ];
-    f32x16 sumsOfA[NI];   // over k alone
+    float sumsOfA[NI];   // over k alone, of index l % 32; lanes l and l ^ 32 have half of the k each
 
     static __device__ __forceinline__ int firstI() { return threadIdx.x / 64 / WJ * (NI * 32); }
     static __device__ __forceinline__ int firstJ() { return threadIdx.x / 64 % WJ * (NJ * 32); }
@@ -184,33 +184,44 @@ struct TileProduct
     {
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
-            sumsOfA[i] = f32x16{};
+            sumsOfA[i] = 0;
 #pragma unroll
             for (int j = 0; j < NJ; ++j) sums[i][j] = f32x16{};
         }
     }
-    /** Adds the products of tiles in LDS. */
-    __device__ __forceinline__ void multiplyTile(const T* ldsA, const T* ldsB, bool sumA)
+    /** What a wavefront multiplies in one step of a tile's k. */
+    struct Operands
     {
-        const int fromI = firstI(), fromJ = firstJ();
+        typename Matrix<T>::Operand a[NI], b[NJ];
+    };
+    static constexpr int STEPS = TILE_K<T> / STEP_K<T>;
+    static __device__ __forceinline__ void readStep(Operands& o, const T* ldsA, const T* ldsB, int step)
+    {
 #pragma unroll
-        for (int step = 0; step < TILE_K<T> / STEP_K<T>; ++step) {
-            typename Matrix<T>::Operand x[NI], w[NJ];
+        for (int j = 0; j < NJ; ++j) o.b[j] = TileB::operand(ldsB, firstJ() + j * 32, step);
 #pragma unroll
-            for (int i = 0; i < NI; ++i) x[i] = TileA::operand(ldsA, fromI + i * 32, step);
+        for (int i = 0; i < NI; ++i) o.a[i] = TileA::operand(ldsA, firstI() + i * 32, step);
+    }
+    __device__ __forceinline__ void multiplyStep(const Operands& o, bool sumA)
+    {
 #pragma unroll
-            for (int j = 0; j < NJ; ++j) w[j] = TileB::operand(ldsB, fromJ + j * 32, step);
+        for (int i = 0; i < NI; ++i)
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) sums[i][j] = Matrix<T>::multiply(o.b[j], o.a[i], sums[i][j]);
+        if (sumA)
 #pragma unroll
             for (int i = 0; i < NI; ++i)
 #pragma unroll
-                for (int j = 0; j < NJ; ++j) sums[i][j] = Matrix<T>::multiply(w[j], x[i], sums[i][j]);
-            if (sumA) {
-                typename Matrix<T>::Operand ones;
+                for (int n = 0; n < WIDE<T>; ++n) sumsOfA[i] += static_cast<float>(o.a[i][n]);
+    }
+    /** Adds the products of tiles in LDS. */
+    __device__ __forceinline__ void multiplyTile(const T* ldsA, const T* ldsB, bool sumA)
+    {
 #pragma unroll
-                for (int n = 0; n < static_cast<int>(sizeof(ones) / sizeof(T)); ++n) ones[n] = static_cast<T>(1);
-#pragma unroll
-                for (int i = 0; i < NI; ++i) sumsOfA[i] = Matrix<T>::multiply(ones, x[i], sumsOfA[i]);
-            }
+        for (int step = 0; step < STEPS; ++step) {
+            Operands o;
+            readStep(o, ldsA, ldsB, step);
+            multiplyStep(o, sumA);
         }
     }
 
@@ -262,6 +273,58 @@ struct TileProduct
     }
 };
 
+/**
+ * Writes a tile of results, converted to T, as whole rows: through LDS, which by then holds no operands any more. From registers a
+ * lane would write 8 bytes of a row each time. bias: of the tile's first j, or null. All threads take part.
+ */
+template <typename Product, typename T>
+__device__ __forceinline__ void storeTile(const Product& product, char* lds, const T* __restrict__ bias, T* __restrict__ to, long long stride, int ni, int nj)
+{
+    constexpr int NI = Product::NI, NJ = Product::NJ, ROW = NJ * 32, PIECE = WIDE<T>, PIECES = ROW / PIECE;   // of a wavefront's own part
+    const int lane = threadIdx.x % 64;
+    const int fromI = Product::firstI(), fromJ = Product::firstJ();
+    T* const part = reinterpret_cast<T*>(lds) + threadIdx.x / 64 * (NI * 32 * ROW);
+    float b[NJ][16] = {};
+    if (bias)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int n = 0; n < 16; ++n) {
+                const int at = fromJ + j * 32 + n / 4 * 8 + lane / 32 * 4 + n % 4;
+                b[j][n] = static_cast<float>(bias[min(at, nj - 1)]);   // (the columns behind are not written)
+            }
+    __syncthreads();   // the last tiles have been read
+    // (a row's pieces in an order that depends on the row, for the banks)
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int n = 0; n < 16; n += 4) {
+                const int row = i * 32 + lane % 32, column = j * 32 + n * 2 + lane / 32 * 4;
+                float v[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] = product.sums[i][j][n + k] + b[j][n + k];
+                T* at = part + row * ROW + ((column / PIECE ^ (row & (PIECES < 8 ? PIECES - 1 : 7))) * PIECE + column % PIECE);
+                storeFloats(static_cast<T*>(__builtin_assume_aligned(at, 4 * sizeof(T))), v);
+            }
+    waveLdsSync();
+#pragma unroll 4
+    for (int n = 0; n < NI * 32 * PIECES / 64; ++n) {
+        const int row = (n * 64 + lane) / PIECES, piece = (n * 64 + lane) % PIECES;
+        T raw[PIECE];
+        __builtin_memcpy(raw, __builtin_assume_aligned(part + row * ROW + (piece ^ (row & (PIECES < 8 ? PIECES - 1 : 7))) * PIECE, 16), 16);
+        const int i = fromI + row, j = fromJ + piece * PIECE;
+        if (i >= ni || j >= nj) continue;
+        T* out = to + i * stride + j;
+        if (j + PIECE <= nj) __builtin_memcpy(out, raw, 16);
+        else
+#pragma unroll
+            for (int k = 0; k < PIECE; ++k)
+                if (j + k < nj) out[k] = raw[k];
+    }
+}
+
 /** A buffer descriptor for raw accesses of 'bytes' bytes at p; reads behind them give zeros. */
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ u32x4 bufferAt(const void* p, unsigned bytes)
@@ -280,10 +343,11 @@ __device__ __forceinline__ void loadToLds(u32x4 buffer, unsigned offset, unsigne
 {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(buffer) : "memory");
 }
-/** All of the wavefront's loads to LDS have arrived, its reads of LDS are done, and so are those of the others. */
+/** All but the last 'pending' of the wavefront's loads to LDS have arrived, its reads of LDS are done, and so are those of the others. */
+template <int PENDING>
 __device__ __forceinline__ void waitForTiles()
 {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(PENDING) : "memory");
 }
 
 /**
@@ -331,7 +395,11 @@ struct DirectTile
     }
 };
 
-/** TileProduct whose tiles go to LDS without registers in between, the next ones while the present ones are multiplied. */
+/**
+ * TileProduct whose tiles go to LDS without registers in between, two tiles ahead of the matrix cores. Operands are read from LDS
+ * a step ahead, also from one tile to the next: the barrier between two tiles stands before the last step of the first, whose
+ * operands every wavefront has by then.
+ */
 template <typename T, bool A_ALONG_K, bool B_ALONG_K, int TI, int TJ, int WI, int WJ>
 struct DirectProduct : TileProduct<T, A_ALONG_K, B_ALONG_K, TI, TJ, WI, WJ>
 {
@@ -342,24 +410,50 @@ struct DirectProduct : TileProduct<T, A_ALONG_K, B_ALONG_K, TI, TJ, WI, WJ>
     {
         this->clear();
         if (K <= 0) return;
-        DirectTile<T, A_ALONG_K, TI, Base::THREADS> tileA;
-        DirectTile<T, B_ALONG_K, TJ, Base::THREADS> tileB;
+        typedef DirectTile<T, A_ALONG_K, TI, Base::THREADS> LoadsA;
+        typedef DirectTile<T, B_ALONG_K, TJ, Base::THREADS> LoadsB;
+        LoadsA tileA;
+        LoadsB tileB;
         tileA.begin(a, strideA, ni);
         tileB.begin(b, strideB, nj);
         constexpr unsigned BYTES_A = Base::TileA::BYTES, BYTES = BYTES_A + Base::TileB::BYTES;
         const unsigned at = static_cast<unsigned>(reinterpret_cast<unsigned long long>((__attribute__((address_space(3))) char*)lds));
+        auto load = [&](unsigned buffer, int ks) {
+            tileA.load(at + buffer, ks);
+            tileB.load(at + buffer + BYTES_A, ks);
+        };
+        typename Base::Operands now, next;
+        auto read = [&](typename Base::Operands& o, unsigned buffer, int step) {
+            Base::readStep(o, reinterpret_cast<const T*>(lds + buffer), reinterpret_cast<const T*>(lds + buffer + BYTES_A), step);
+            __builtin_amdgcn_sched_barrier(0);   // the compiler would move the reads to where they are used
+        };
+        int left = K - TILE_K<T>;   // behind the tiles asked for
+        load(0, min(K, TILE_K<T>));
+        if (left > 0) {
+            load(BYTES, min(left, TILE_K<T>));
+            waitForTiles<LoadsA::EACH + LoadsB::EACH>();
+        } else
+            waitForTiles<0>();
+        left -= TILE_K<T>;
+        read(now, 0, 0);
         unsigned buffer = 0;
-        tileA.load(at, min(K, TILE_K<T>));
-        tileB.load(at + BYTES_A, min(K, TILE_K<T>));
         for (int k = 0; k < K; k += TILE_K<T>) {
-            waitForTiles();
-            const int left = min(K - k - TILE_K<T>, TILE_K<T>);
-            if (left > 0) {
-                tileA.load(at + (buffer ^ BYTES), left);
-                tileB.load(at + (buffer ^ BYTES) + BYTES_A, left);
+#pragma unroll
+            for (int step = 0; step + 1 < Base::STEPS; ++step) {
+                read(next, buffer, step + 1);
+                this->multiplyStep(now, sumA);
+                __builtin_amdgcn_sched_barrier(0);
+                now = next;
             }
-            this->multiplyTile(reinterpret_cast<const T*>(lds + buffer), reinterpret_cast<const T*>(lds + buffer + BYTES_A), sumA);
-            buffer ^= BYTES;
+            if (k + TILE_K<T> < K) {
+                waitForTiles<0>();
+                if (left > 0) load(buffer, min(left, TILE_K<T>));
+                left -= TILE_K<T>;
+                buffer ^= BYTES;
+                read(next, buffer, 0);
+            }
+            this->multiplyStep(now, sumA);
+            now = next;
         }
     }
 };
@@ -431,21 +525,21 @@ __device__ __forceinline__ ExpertTile expertTile(const int* __restrict__ offsets
 }
 
 /**
- * Which of 'places' x 'tiles' a workgroup takes. Workgroups go to the dies in turn, each with an L2 of its own: a die takes consecutive
- * ones of an order that goes through the tiles for GROUP_PLACES places at a time, so that those at work on it share both operands.
+ * Which of 'places' x 'tiles' a workgroup takes. Workgroups go to the dies in turn, each with an L2 of its own. In an order that goes
+ * through the tiles for GROUP_PLACES places at a time, 32 consecutive ones are the work of one die (a workgroup for each of its
+ * compute units), so that they share both operands; the next 32 are the next die's, so that all have as much to do.
  */
-constexpr int GROUP_PLACES = 4;
+constexpr unsigned GROUP_PLACES = 4, DIE_UNITS = 32;
 struct Work
 {
     int place, tile;
 };
 __device__ __forceinline__ Work workOf(unsigned id, unsigned places, unsigned tiles)
 {
-    const unsigned total = places * tiles, each = total / DIES, rest = total % DIES;
-    const unsigned die = id % DIES;
-    const unsigned n = die * each + min(die, rest) + id / DIES;
+    const unsigned total = places * tiles, round = DIES * DIE_UNITS;
+    const unsigned n = id < total / round * round ? id / round * round + id % DIES * DIE_UNITS + id % round / DIES : id;
     const unsigned group = n / (GROUP_PLACES * tiles), within = n - group * (GROUP_PLACES * tiles);
-    const unsigned count = min(static_cast<unsigned>(GROUP_PLACES), places - group * GROUP_PLACES);
+    const unsigned count = min(GROUP_PLACES, places - group * GROUP_PLACES);
     return {static_cast<int>(group * GROUP_PLACES + within % count), static_cast<int>(within / count)};
 }
 
@@ -471,15 +565,7 @@ GroupedRowsKernel(const T* __restrict__ x, long long strideX, const T* __restric
     const bool none = at.expert >= experts;
     const T* w = weights + (none ? 0 : at.expert) * strideExpert;
     product.run(groupedLds, x + at.from * strideX, strideX, ni, w + (B_ALONG_K ? j0 * strideWeights : j0), strideWeights, nj, none ? 0 : K, false);
-    const T* b = bias && !none ? bias + at.expert * strideBias + j0 : nullptr;
-    product.results([&](int i, int j, float (&v)[4]) {
-        if (i >= ni || j >= nj) return;
-        if (b)
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if (j + k < nj) v[k] += static_cast<float>(b[j + k]);
-        storeUpToFour(y + (at.from + i) * strideY + j0 + j, v, nj - j);
-    });
+    storeTile(product, groupedLds, bias && !none ? bias + at.expert * strideBias + j0 : nullptr, y + at.from * strideY + j0, strideY, ni, nj);
 }
 
 /**
@@ -502,26 +588,25 @@ GroupedWeightsKernel(const T* __restrict__ adjY, long long strideAdjY, const T* 
     const int i0 = work.place * TI, j0 = work.tile * TJ;
     const int ni = min(I - i0, TI), nj = min(J - j0, TJ);
     const bool whole = at.expertRows <= chunk;
-    const bool sumA = adjBias && j0 == 0;
+    const bool sumA = adjBias && j0 == 0 && Product::firstJ() == 0;   // the wavefronts of the first columns
     Product product;
     product.run(groupedLds, adjY + at.from * strideAdjY + i0, strideAdjY, ni, x + at.from * strideX + j0, strideX, nj, max(0, at.to - at.from), sumA);
     const long long size = static_cast<long long>(I) * J;
     float* sums = whole ? nullptr : partial + place * (size + I);
-    T* out = adjWeights + at.expert * size;
-    if (adjWeights || !whole)
+    if (!whole)
         product.results([&](int i, int j, float (&v)[4]) {
-            if (i >= ni || j >= nj) return;
-            const long long to = static_cast<long long>(i0 + i) * J + j0 + j;
-            if (whole) storeUpToFour(out + to, v, nj - j);
-            else storeUpToFour(sums + to, v, nj - j);
+            if (i < ni && j < nj) storeUpToFour(sums + static_cast<long long>(i0 + i) * J + j0 + j, v, nj - j);
         });
-    if (sumA && Product::firstJ() == 0 && threadIdx.x % 64 < 32)
+    else if (adjWeights)
+        storeTile(product, groupedLds, static_cast<const T*>(nullptr), adjWeights + at.expert * size + static_cast<long long>(i0) * J + j0, J, ni, nj);
+    if (sumA)
 #pragma unroll
         for (int n = 0; n < Product::NI; ++n) {
             const int i = Product::firstI() + n * 32 + threadIdx.x % 32;
-            if (i >= ni) continue;
-            if (whole) adjBias[static_cast<long long>(at.expert) * I + i0 + i] = static_cast<T>(product.sumsOfA[n][0]);
-            else sums[size + i0 + i] = product.sumsOfA[n][0];
+            const float sum = product.sumsOfA[n] + __shfl_xor(product.sumsOfA[n], 32);
+            if (threadIdx.x % 64 >= 32 || i >= ni) continue;
+            if (whole) adjBias[static_cast<long long>(at.expert) * I + i0 + i] = static_cast<T>(sum);
+            else sums[size + i0 + i] = sum;
         }
 }
 
