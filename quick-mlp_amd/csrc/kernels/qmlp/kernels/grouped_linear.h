@@ -98,7 +98,7 @@ struct Tile
     /** Place of an entry of the tile. */
     static __device__ __forceinline__ int place(int row, int column)
     {
-        if constexpr (ALONG_K) return row * ROW + ((column / PIECE ^ (row & 7)) * PIECE + column % PIECE);
+        if constexpr (ALONG_K) return row * ROW + ((column / PIECE ^ (row >> 1 & 7)) * PIECE + column % PIECE);   // 16 rows of a piece: all 64 banks
         else if constexpr (sizeof(T) == 2) {
             // 32 entries (64 bytes) are read of each of four consecutive rows
             constexpr int UNITS = ROW / 32;
@@ -202,12 +202,17 @@ struct TileProduct
 #pragma unroll
         for (int i = 0; i < NI; ++i) o.a[i] = TileA::operand(ldsA, firstI() + i * 32, step);
     }
-    __device__ __forceinline__ void multiplyStep(const Operands& o, bool sumA)
+    /** between(n): what is to be done beside the n-th product. */
+    template <typename Between>
+    __device__ __forceinline__ void multiplyStep(const Operands& o, bool sumA, Between between)
     {
 #pragma unroll
         for (int i = 0; i < NI; ++i)
 #pragma unroll
-            for (int j = 0; j < NJ; ++j) sums[i][j] = Matrix<T>::multiply(o.b[j], o.a[i], sums[i][j]);
+            for (int j = 0; j < NJ; ++j) {
+                sums[i][j] = Matrix<T>::multiply(o.b[j], o.a[i], sums[i][j]);
+                between(i * NJ + j);
+            }
         if (sumA)
 #pragma unroll
             for (int i = 0; i < NI; ++i)
@@ -221,7 +226,7 @@ struct TileProduct
         for (int step = 0; step < STEPS; ++step) {
             Operands o;
             readStep(o, ldsA, ldsB, step);
-            multiplyStep(o, sumA);
+            multiplyStep(o, sumA, [](int) {});
         }
     }
 
@@ -382,16 +387,20 @@ struct DirectTile
             offsets[n] = static_cast<unsigned>(((ALONG_K ? min(row, indices - 1) : row) * stride + column) * sizeof(T));
         }
     }
-    /** The tile of the 'ks' next values of k, to LDS from 'lds' on. */
-    __device__ __forceinline__ void load(unsigned lds, int ks)
+    u32x4 buffer;
+    unsigned to;
+    int ks;
+    /** Turns to the tile of the 'ks' next values of k, which goes to LDS from 'lds' on with the calls of load(0) to load(EACH - 1). */
+    __device__ __forceinline__ void next(unsigned lds, int ks_)
     {
-        const unsigned bytes = static_cast<unsigned>(((ALONG_K ? indices - 1 : ks - 1) * stride + (ALONG_K ? ks : indices)) * sizeof(T));
-        const u32x4 buffer = bufferAt(p, bytes);
-        const unsigned to = __builtin_amdgcn_readfirstlane(lds + threadIdx.x / 64 * 1024);
-        const bool whole = !ALONG_K || ks == TILE_K<T>;
-#pragma unroll
-        for (int n = 0; n < EACH; ++n) loadToLds(buffer, whole || columns[n] < ks ? offsets[n] : 0x80000000u, to + n * THREADS * 16);
+        ks = ks_;
+        buffer = bufferAt(p, static_cast<unsigned>(((ALONG_K ? indices - 1 : ks - 1) * stride + (ALONG_K ? ks : indices)) * sizeof(T)));
+        to = __builtin_amdgcn_readfirstlane(lds + threadIdx.x / 64 * 1024);
         p += ALONG_K ? TILE_K<T> : TILE_K<T> * stride;
+    }
+    __device__ __forceinline__ void load(int n) const
+    {
+        loadToLds(buffer, !ALONG_K || columns[n] < ks ? offsets[n] : 0x80000000u, to + n * THREADS * 16);
     }
 };
 
@@ -418,42 +427,56 @@ struct DirectProduct : TileProduct<T, A_ALONG_K, B_ALONG_K, TI, TJ, WI, WJ>
         tileB.begin(b, strideB, nj);
         constexpr unsigned BYTES_A = Base::TileA::BYTES, BYTES = BYTES_A + Base::TileB::BYTES;
         const unsigned at = static_cast<unsigned>(reinterpret_cast<unsigned long long>((__attribute__((address_space(3))) char*)lds));
-        auto load = [&](unsigned buffer, int ks) {
-            tileA.load(at + buffer, ks);
-            tileB.load(at + buffer + BYTES_A, ks);
+        constexpr int LOADS = LoadsA::EACH + LoadsB::EACH, PRODUCTS = Base::NI * Base::NJ;
+        auto next = [&](unsigned buffer, int ks) {
+            tileA.next(at + buffer, ks);
+            tileB.next(at + buffer + BYTES_A, ks);
         };
-        typename Base::Operands now, next;
+        auto load = [&](int from, int to) {
+#pragma unroll
+            for (int n = from; n < to; ++n) {
+                if (n < LoadsA::EACH) tileA.load(n);
+                else tileB.load(n - LoadsA::EACH);
+            }
+        };
+        static_assert(Base::STEPS % 2 == 0, "the operands of a tile's first step are the first ones");
+        typename Base::Operands operands[2];   // of a step and of the one behind it
         auto read = [&](typename Base::Operands& o, unsigned buffer, int step) {
             Base::readStep(o, reinterpret_cast<const T*>(lds + buffer), reinterpret_cast<const T*>(lds + buffer + BYTES_A), step);
             __builtin_amdgcn_sched_barrier(0);   // the compiler would move the reads to where they are used
         };
         int left = K - TILE_K<T>;   // behind the tiles asked for
-        load(0, min(K, TILE_K<T>));
+        next(0, min(K, TILE_K<T>));
+        load(0, LOADS);
         if (left > 0) {
-            load(BYTES, min(left, TILE_K<T>));
-            waitForTiles<LoadsA::EACH + LoadsB::EACH>();
+            next(BYTES, min(left, TILE_K<T>));
+            load(0, LOADS);
+            waitForTiles<LOADS>();
         } else
             waitForTiles<0>();
         left -= TILE_K<T>;
-        read(now, 0, 0);
+        read(operands[0], 0, 0);
         unsigned buffer = 0;
         for (int k = 0; k < K; k += TILE_K<T>) {
 #pragma unroll
             for (int step = 0; step + 1 < Base::STEPS; ++step) {
-                read(next, buffer, step + 1);
-                this->multiplyStep(now, sumA);
+                read(operands[(step + 1) % 2], buffer, step + 1);
+                this->multiplyStep(operands[step % 2], sumA, [](int) {});
                 __builtin_amdgcn_sched_barrier(0);
-                now = next;
             }
-            if (k + TILE_K<T> < K) {
-                waitForTiles<0>();
-                if (left > 0) load(buffer, min(left, TILE_K<T>));
+            const bool more = left > 0, last = k + TILE_K<T> >= K;
+            if (!last) {
+                if (more) next(buffer, min(left, TILE_K<T>));
                 left -= TILE_K<T>;
                 buffer ^= BYTES;
-                read(next, buffer, 0);
+                waitForTiles<0>();
             }
-            this->multiplyStep(now, sumA);
-            now = next;
+            // Behind the barrier the matrix cores go on at once; what else there is to do stands between the products.
+            this->multiplyStep(operands[1], sumA, [&](int n) {
+                if (n == 0 && !last) read(operands[0], buffer, 0);
+                if (more) load(n * LOADS / PRODUCTS, (n + 1) * LOADS / PRODUCTS);
+                __builtin_amdgcn_sched_barrier(0);
+            });
         }
     }
 };
