@@ -13,7 +13,7 @@
 QUICKMLP_KERNEL_NAMESPACE_BEGIN
 
 constexpr int EMBEDDING_THREADS = 256;
-constexpr int EMBEDDING_BLOCK_BITS = 5;   // 32 places per block, 32 blocks per block of the next size
+constexpr int EMBEDDING_BLOCK_BITS = 6;   // 64 places per block, 64 blocks per block of the next size
 
 /** G lanes per row, PIECES of VEC entries each at a time. */
 template <typename T, typename I, int VEC, int G>
@@ -40,41 +40,54 @@ EmbeddingKernel(const I* __restrict__ index, long long strideIndex, const T* __r
     }
 }
 
-/** Entries of the sorted order that begin (end) a token's terms: spans[token] and spans[vocabulary + token]. */
-__global__ void __launch_bounds__(EMBEDDING_THREADS)
-EmbeddingSpansKernel(const unsigned* __restrict__ keys, long long rows, unsigned vocabulary, unsigned* __restrict__ spans)
+/** Adds COUNT terms; term(n, values) has the n-th one. */
+template <int VEC, int COUNT, typename Term>
+__device__ __forceinline__ void addTerms(float (&sum)[VEC], Term term)
 {
-    const long long i = static_cast<long long>(blockIdx.x) * EMBEDDING_THREADS + threadIdx.x;
-    if (i >= rows) return;
-    const unsigned key = keys[i];
-    if (key >= vocabulary) return;
-    if (i == 0 || keys[i - 1] != key) spans[key] = static_cast<unsigned>(i);
-    if (i == rows - 1 || keys[i + 1] != key) spans[vocabulary + key] = static_cast<unsigned>(i + 1);
+    float terms[COUNT][VEC];   // all of them asked for before the first is added
+#pragma unroll
+    for (int n = 0; n < COUNT; ++n) term(n, terms[n]);
+#pragma unroll
+    for (int n = 0; n < COUNT; ++n)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) sum[k] += terms[n][k];
+}
+/** Adds 'count' consecutive terms, eight of them in flight. */
+template <int VEC, typename Term>
+__device__ __forceinline__ void addRange(float (&sum)[VEC], int count, Term term)
+{
+    int n = 0;
+    for (; n + 8 <= count; n += 8) addTerms<VEC, 8>(sum, [&](int k, float (&v)[VEC]) { term(n + k, v); });
+    if (n + 4 <= count) {
+        addTerms<VEC, 4>(sum, [&](int k, float (&v)[VEC]) { term(n + k, v); });
+        n += 4;
+    }
+    for (; n < count; ++n) addTerms<VEC, 1>(sum, [&](int k, float (&v)[VEC]) { term(n + k, v); });
 }
 
 /**
  * The sums of the blocks of one size that hold one token only: sums[block][C], G lanes per block. FIRST: blocks of places, whose
- * terms are rows of dy through the order; otherwise blocks of blocks, whose terms are the sums of those. 1 << bits places per block.
+ * terms are rows of dy through the order, and the spans of all tokens (null: they are known); otherwise blocks of blocks, whose terms
+ * are the sums of those. 1 << bits places per block.
  */
 template <typename T, int VEC, int G, bool FIRST>
 __global__ void __launch_bounds__(EMBEDDING_THREADS)
 EmbeddingBlocksKernel(const unsigned* __restrict__ keys, const int* __restrict__ order, long long rows, unsigned vocabulary, int bits,
-                      const T* __restrict__ adjY, long long strideAdjY, const float* __restrict__ smaller, float* __restrict__ sums, int C)
+                      const T* __restrict__ adjY, long long strideAdjY, const float* __restrict__ smaller, float* __restrict__ sums, int C,
+                      unsigned* __restrict__ spans)
 {
     const long long block = static_cast<long long>(blockIdx.x) * (EMBEDDING_THREADS / G) + threadIdx.x / G;
     const long long from = block << bits, to = (block + 1) << bits;
+    if (FIRST && spans)
+        for (long long i = from + threadIdx.x % G; i < min(to, rows); i += G) markSpans(keys, i, rows, vocabulary, spans);
     if (to > rows || keys[from] != keys[to - 1] || keys[from] >= vocabulary) return;
     for (int c = threadIdx.x % G * VEC; c < C; c += G * VEC) {
         const int at = VEC == 1 ? c : min(c, C - VEC);
         float sum[VEC] = {};
-#pragma unroll 8
-        for (int i = 0; i < (1 << EMBEDDING_BLOCK_BITS); ++i) {
-            float term[VEC];
-            if constexpr (FIRST) loadFloats(adjY + order[from + i] * strideAdjY + at, term);
-            else loadFloats(smaller + ((block << EMBEDDING_BLOCK_BITS) + i) * C + at, term);
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) sum[k] += term[k];
-        }
+        addRange(sum, 1 << EMBEDDING_BLOCK_BITS, [&](int i, float (&v)[VEC]) {
+            if constexpr (FIRST) loadFloats(adjY + order[from + i] * strideAdjY + at, v);
+            else loadFloats(smaller + ((block << EMBEDDING_BLOCK_BITS) + i) * C + at, v);
+        });
         storeFloats(sums + block * C + at, sum);
     }
 }
@@ -90,40 +103,44 @@ struct EmbeddingBlocks
 /** G lanes per row of the table. */
 template <typename T, int VEC, int G>
 __global__ void __launch_bounds__(EMBEDDING_THREADS)
-EmbeddingAdjointKernel(const unsigned* __restrict__ spans, const int* __restrict__ order, EmbeddingBlocks blocks, const T* __restrict__ adjY,
-                       long long strideAdjY, float scale, T* __restrict__ adjTable, long long strideTable, long long vocabulary, int C)
+EmbeddingAdjointKernel(const unsigned* __restrict__ keys, const unsigned* __restrict__ spans, const int* __restrict__ order, long long rows,
+                       EmbeddingBlocks blocks, const T* __restrict__ adjY, long long strideAdjY, float scale, T* __restrict__ adjTable,
+                       long long strideTable, long long vocabulary, int C)
 {
     constexpr int ROWS = EMBEDDING_THREADS / G;
     const int lane = threadIdx.x % G;
     for (long long v = static_cast<long long>(blockIdx.x) * ROWS + threadIdx.x / G; v < vocabulary; v += static_cast<long long>(gridDim.x) * ROWS) {
-        const long long from = spans[v], to = spans[vocabulary + v];
+        unsigned span[2] = {spans[v], spans[vocabulary + v]};
+        if constexpr (G >= 64) {   // one row for the whole wavefront
+            span[0] = __builtin_amdgcn_readfirstlane(span[0]);
+            span[1] = __builtin_amdgcn_readfirstlane(span[1]);
+        }
+        const long long from = span[0];
+        const bool any = from < rows && keys[from] == v;   // otherwise no token names the row, and nothing was written there
+        const long long to = any ? static_cast<long long>(span[1]) : from;
         for (int c = lane * VEC; c < C; c += G * VEC) {
             const int at = VEC == 1 ? c : min(c, C - VEC);
             float sum[VEC] = {};
-            auto add = [&](auto* p) {
-                float term[VEC];
-                loadFloats(p + at, term);
-#pragma unroll
-                for (int k = 0; k < VEC; ++k) sum[k] += term[k];
-            };
-            // the largest whole block that begins here, one after the other
+            // places up to the first block, blocks up to the first larger block, ..., and down again
             long long i = from;
-            while (i < to) {
-                int size = 0;
-                while (size < blocks.sizes) {
-                    const long long places = 1ll << (EMBEDDING_BLOCK_BITS * (size + 1));
-                    if ((i & (places - 1)) != 0 || i + places > to) break;
-                    ++size;
+            auto add = [&](int size, long long end) {
+                const int bits = EMBEDDING_BLOCK_BITS * size;
+                const long long first = i >> bits;
+                const int count = static_cast<int>((end - i) >> bits);
+                if (size == 0) addRange(sum, count, [&](int n, float (&term)[VEC]) { loadFloats(adjY + order[first + n] * strideAdjY + at, term); });
+                else {
+                    const float* p = blocks.sums[size - 1] + first * C + at;
+                    addRange(sum, count, [&](int n, float (&term)[VEC]) { loadFloats(p + static_cast<long long>(n) * C, term); });
                 }
-                if (size == 0) {
-                    add(adjY + order[i] * strideAdjY);
-                    ++i;
-                } else {
-                    const int bits = EMBEDDING_BLOCK_BITS * size;
-                    add(blocks.sums[size - 1] + (i >> bits) * C);
-                    i += 1ll << bits;
-                }
+                i = end;
+            };
+            int size = 0;
+            for (; size < blocks.sizes; ++size) {
+                const long long places = 1ll << (EMBEDDING_BLOCK_BITS * (size + 1)), next = (i + places - 1) & -places;
+                if (next + places > to) break;   // no larger block in here
+                add(size, next);
             }
+            for (; size >= 0; --size) add(size, to >> (EMBEDDING_BLOCK_BITS * size) << (EMBEDDING_BLOCK_BITS * size));
 #pragma unroll
             for (int k = 0; k < VEC; ++k) sum[k] *= scale;
             storeFloats(adjTable + v * strideTable + at, sum);

@@ -14,7 +14,7 @@ QUICKMLP_KERNEL_NAMESPACE_BEGIN
 
 constexpr int GROUP_SMALL_THREADS = 1024, GROUP_SMALL_ITEMS = 8, GROUP_SMALL_BITS = 8;
 constexpr int GROUP_SMALL_ROWS = GROUP_SMALL_THREADS * GROUP_SMALL_ITEMS;
-constexpr int GROUP_THREADS = 256, GROUP_ITEMS = 16, GROUP_TILE = GROUP_THREADS * GROUP_ITEMS;
+constexpr int GROUP_THREADS = 1024;   // tiles of as many rows, or ITEMS times as many
 constexpr int GROUP_MAX_BITS = 13;
 constexpr int GROUP_SCAN_DIGITS = 64, GROUP_SCAN_SLICES = 16;
 
@@ -91,13 +91,25 @@ __device__ __forceinline__ unsigned lowerBound(const unsigned* keys, unsigned n,
 }
 
 /**
- * All of up to GROUP_SMALL_ROWS rows by one workgroup. bits: of the number 'groups'. keys (the groups in order) and offsets (groups + 1
- * of them) may be null. LDS: GROUP_SMALL_ROWS keys and rows, the counters of the wavefronts.
+ * Where the entries of a group among the sorted keys begin and end: spans[group] and spans[groups + group], from the entry at i. Groups
+ * without entries have no spans: whatever lies there, a reader finds that no key at the beginning it names is the group's.
+ */
+__device__ __forceinline__ void markSpans(const unsigned* keys, long long i, long long rows, unsigned groups, unsigned* __restrict__ spans)
+{
+    const unsigned key = keys[i];
+    if (key >= groups) return;
+    if (i == 0 || keys[i - 1] != key) spans[key] = static_cast<unsigned>(i);
+    if (i == rows - 1 || keys[i + 1] != key) spans[groups + key] = static_cast<unsigned>(i + 1);
+}
+
+/**
+ * All of up to GROUP_SMALL_ROWS rows by one workgroup. bits: of the number 'groups'. keys (the groups in order), offsets (groups + 1
+ * of them) and spans (see markSpans()) may be null. LDS: GROUP_SMALL_ROWS keys and rows, the counters of the wavefronts.
  */
 template <typename I>
 __global__ void __launch_bounds__(GROUP_SMALL_THREADS)
 GroupSmallKernel(const I* __restrict__ index, long long stride, int rows, unsigned groups, int bits, int* __restrict__ order,
-                 unsigned* __restrict__ keys, int* __restrict__ offsets)
+                 unsigned* __restrict__ keys, int* __restrict__ offsets, unsigned* __restrict__ spans)
 {
     constexpr int WAVES = GROUP_SMALL_THREADS / 64;
     extern __shared__ unsigned groupLds[];
@@ -162,6 +174,7 @@ GroupSmallKernel(const I* __restrict__ index, long long stride, int rows, unsign
         if (i < items && p < rows) {
             order[p] = row[i];
             if (keys) keys[p] = key[i];
+            if (spans) markSpans(keysLds, p, rows, groups, spans);
         }
     }
     if (offsets)   // (keysLds: as the last pass left them)
@@ -182,22 +195,22 @@ struct GroupSource
 };
 
 /** Rows per digit of every tile: counts[tile][digit]; digits: as many as there are, their bits in 'mask'. LDS: a counter per digit. */
-template <typename I>
+template <typename I, int ITEMS>
 __global__ void __launch_bounds__(GROUP_THREADS)
 GroupCountKernel(GroupSource<I> source, long long rows, int shift, unsigned mask, int digits, unsigned* __restrict__ counts)
 {
     extern __shared__ unsigned groupLds[];
     for (int d = threadIdx.x; d < digits; d += GROUP_THREADS) groupLds[d] = 0;
     __syncthreads();
-    const long long first = static_cast<long long>(blockIdx.x) * GROUP_TILE;
-    unsigned key[GROUP_ITEMS];
+    const long long first = static_cast<long long>(blockIdx.x) * (GROUP_THREADS * ITEMS);
+    unsigned key[ITEMS];
 #pragma unroll
-    for (int i = 0; i < GROUP_ITEMS; ++i) {
+    for (int i = 0; i < ITEMS; ++i) {
         const long long r = first + i * GROUP_THREADS + threadIdx.x;
         if (r < rows) key[i] = source.key(r);
     }
 #pragma unroll
-    for (int i = 0; i < GROUP_ITEMS; ++i)
+    for (int i = 0; i < ITEMS; ++i)
         if (first + i * GROUP_THREADS + threadIdx.x < rows) atomicAdd(groupLds + ((key[i] >> shift) & mask), 1u);
     __syncthreads();
     unsigned* out = counts + static_cast<long long>(blockIdx.x) * digits;
@@ -234,7 +247,7 @@ GroupScanKernel(unsigned* __restrict__ counts, int tiles, int digits, unsigned* 
  * Writes the rows of a tile to their places. keysOut, offsets: may be null; offsets for a sort of one pass only, whose digits are
  * the groups. LDS: a start per digit, the counters of the wavefronts.
  */
-template <typename I>
+template <typename I, int ITEMS>
 __global__ void __launch_bounds__(GROUP_THREADS)
 GroupScatterKernel(GroupSource<I> source, long long rows, int shift, int digitBits, int digits, const unsigned* __restrict__ counts,
                    const unsigned* __restrict__ totals, int* __restrict__ orderOut, unsigned* __restrict__ keysOut, int* __restrict__ offsets)
@@ -252,12 +265,12 @@ GroupScatterKernel(GroupSource<I> source, long long rows, int shift, int digitBi
         for (int w = 0; w < WAVES; ++w) counters[w * digits + d] = 0;
     }
     // a wavefront takes consecutive rows, 64 at a time
-    const long long first = static_cast<long long>(blockIdx.x) * GROUP_TILE + wave * (64 * GROUP_ITEMS) + threadIdx.x % 64;
-    unsigned key[GROUP_ITEMS];
-    int row[GROUP_ITEMS];
-    unsigned short place[GROUP_ITEMS];
+    const long long first = static_cast<long long>(blockIdx.x) * (GROUP_THREADS * ITEMS) + wave * (64 * ITEMS) + threadIdx.x % 64;
+    unsigned key[ITEMS];
+    int row[ITEMS];
+    unsigned short place[ITEMS];
 #pragma unroll
-    for (int i = 0; i < GROUP_ITEMS; ++i)
+    for (int i = 0; i < ITEMS; ++i)
         if (first + i * 64 < rows) {
             key[i] = source.key(first + i * 64);
             row[i] = source.row(first + i * 64);
@@ -267,7 +280,7 @@ GroupScatterKernel(GroupSource<I> source, long long rows, int shift, int digitBi
     if (offsets && blockIdx.x == 0)
         for (unsigned g = threadIdx.x; g <= source.groups; g += GROUP_THREADS) offsets[g] = static_cast<int>(starts[g]);
 #pragma unroll
-    for (int i = 0; i < GROUP_ITEMS; ++i) {
+    for (int i = 0; i < ITEMS; ++i) {
         const bool has = first + i * 64 < rows;
         const unsigned d = has ? (key[i] >> shift) & mask : 0;
         const unsigned long long same = lanesLike(d, digitBits, __ballot(has));
@@ -281,7 +294,7 @@ GroupScatterKernel(GroupSource<I> source, long long rows, int shift, int digitBi
     __syncthreads();
     const unsigned* before = counts + static_cast<long long>(blockIdx.x) * digits;
 #pragma unroll
-    for (int i = 0; i < GROUP_ITEMS; ++i) {
+    for (int i = 0; i < ITEMS; ++i) {
         if (first + i * 64 >= rows) continue;
         const unsigned d = (key[i] >> shift) & mask;
         unsigned p = starts[d] + before[d] + place[i];

@@ -138,7 +138,7 @@ unsigned workgroups(int64_t pieces, int64_t most) { return static_cast<unsigned>
 
 // ------------------------------------------------------------------------------------------------ groups
 // as in kernels/row_groups.h
-constexpr int GROUP_SMALL_THREADS = 1024, GROUP_SMALL_ROWS = 8192, GROUP_SMALL_BITS = 8, GROUP_THREADS = 256, GROUP_TILE = 4096, GROUP_MAX_BITS = 13,
+constexpr int GROUP_SMALL_THREADS = 1024, GROUP_SMALL_ROWS = 8192, GROUP_SMALL_BITS = 8, GROUP_THREADS = 1024, GROUP_MAX_BITS = 13,
               GROUP_SCAN_DIGITS = 64, GROUP_SCAN_THREADS = 1024;
 /** GroupSource of kernels/row_groups.h */
 struct GroupSource
@@ -162,7 +162,7 @@ struct GroupPlan
 {
     int64_t rows;
     unsigned groups;
-    int passes, digitBits, maxDigits;
+    int passes, digitBits, maxDigits, items;
     int64_t tiles;
     unsigned *counts = nullptr, *totals = nullptr, *keys[2] = {};
     int* order[2] = {};
@@ -175,7 +175,10 @@ struct GroupPlan
         passes = divUp(bits, GROUP_MAX_BITS);
         digitBits = divUp(bits, passes);
         maxDigits = static_cast<int>(std::min<int64_t>(1ll << digitBits, static_cast<int64_t>(groups) + 1));
-        tiles = divUp<int64_t>(rows, GROUP_TILE);
+        // a workgroup for every compute unit: tiles of one row per thread, of four where there are as many anyway (2^20 rows of 4096
+        // groups: XX us, with one XX)
+        items = rows <= 256 * GROUP_THREADS ? 1 : 4;
+        tiles = divUp<int64_t>(rows, GROUP_THREADS * items);
         if (small) return;
         counts = memory.take<unsigned>(tiles * maxDigits);
         totals = memory.take<unsigned>(maxDigits);
@@ -188,8 +191,8 @@ struct GroupPlan
     }
 };
 
-/** Sorts; keysOut (the groups in order) and offsets may be null. */
-void sortByGroup(const Tensor& index, GroupPlan& plan, int* order, unsigned* keysOut, int* offsets, stream_t stream)
+/** Sorts; keysOut (the groups in order) and offsets may be null. spans, if not null, are written for small batches: true. */
+bool sortByGroup(const Tensor& index, GroupPlan& plan, int* order, unsigned* keysOut, int* offsets, unsigned* spans, stream_t stream)
 {
     const std::string type = std::string("<") + scalarName(index.precision()) + ">";
     const long long stride = strideOf(index, 0);
@@ -198,9 +201,10 @@ void sortByGroup(const Tensor& index, GroupPlan& plan, int* order, unsigned* key
         const size_t lds = plan.rows * 6 + 64 + (static_cast<size_t>(GROUP_SMALL_THREADS / 64 * 4) << std::min(bits, GROUP_SMALL_BITS)) + 4;
         tokenKernel("row_groups.h", "GroupSmallKernel" + type)
             .call(1, GROUP_SMALL_THREADS, static_cast<unsigned>(lds), stream, index.rawPtr(), stride, static_cast<int>(plan.rows), plan.groups, bits, order,
-                  keysOut, offsets);
-        return;
+                  keysOut, offsets, spans);
+        return spans != nullptr;
     }
+    const std::string types = str("<", scalarName(index.precision()), ", ", plan.items, ">");
     GroupSource source{index.rawPtr(), stride, nullptr, nullptr, plan.groups};
     long long rows = plan.rows;
     for (int pass = 0; pass < plan.passes; ++pass) {
@@ -210,13 +214,13 @@ void sortByGroup(const Tensor& index, GroupPlan& plan, int* order, unsigned* key
         const int digits = static_cast<int>(std::min<int64_t>(1ll << digitBits, static_cast<int64_t>(plan.groups >> shift) + 1));
         const unsigned mask = (1u << digitBits) - 1;
         const unsigned tiles = static_cast<unsigned>(plan.tiles);
-        tokenKernel("row_groups.h", "GroupCountKernel" + type).call(tiles, GROUP_THREADS, digits * 4, stream, source, rows, shift, mask, digits, plan.counts);
+        tokenKernel("row_groups.h", "GroupCountKernel" + types).call(tiles, GROUP_THREADS, digits * 4, stream, source, rows, shift, mask, digits, plan.counts);
         tokenKernel("row_groups.h", "GroupScanKernel")
             .call(static_cast<unsigned>(divUp(digits, GROUP_SCAN_DIGITS)), GROUP_SCAN_THREADS, 0, stream, plan.counts, static_cast<int>(tiles), digits, plan.totals);
         int* to = last ? order : plan.order[pass % 2];
         unsigned* toKeys = last ? (keysOut ? keysOut : plan.passes > 1 ? plan.keys[pass % 2] : nullptr) : plan.keys[pass % 2];
         const unsigned lds = digits * 4 + digits * 2 * (GROUP_THREADS / 64);
-        tokenKernel("row_groups.h", "GroupScatterKernel" + type)
+        tokenKernel("row_groups.h", "GroupScatterKernel" + types)
             .call(tiles, GROUP_THREADS, lds, stream, source, rows, shift, digitBits, digits, static_cast<const unsigned*>(plan.counts),
                   static_cast<const unsigned*>(plan.totals), to, toKeys, plan.passes == 1 ? offsets : nullptr);
         source.keys = toKeys;
@@ -225,11 +229,12 @@ void sortByGroup(const Tensor& index, GroupPlan& plan, int* order, unsigned* key
     if (offsets && plan.passes > 1)
         tokenKernel("row_groups.h", "GroupOffsetsKernel")
             .call(static_cast<unsigned>(divUp<int64_t>(static_cast<int64_t>(plan.groups) + 1, 256)), 256, 0, stream, source.keys, rows, plan.groups, offsets);
+    return false;
 }
 
 // ------------------------------------------------------------------------------------------------ embeddings
 // as in kernels/embedding.h
-constexpr int EMBEDDING_THREADS = 256, EMBEDDING_BLOCK_BITS = 5;
+constexpr int EMBEDDING_THREADS = 256, EMBEDDING_BLOCK_BITS = 6;
 struct EmbeddingBlocks
 {
     static constexpr int SIZES = 6;
@@ -237,11 +242,11 @@ struct EmbeddingBlocks
     const float* sums[SIZES];
 };
 
-/** Lanes per row of C entries, at most 64. */
+/** Lanes per row of C entries. */
 int lanesPerRow(int C, int vec)
 {
     int lanes = 8;
-    while (lanes < 64 && lanes * vec < C) lanes *= 2;
+    while (lanes < EMBEDDING_THREADS && lanes * vec < C) lanes *= 2;
     return lanes;
 }
 
@@ -256,7 +261,8 @@ struct EmbeddingPlan
         : memory{static_cast<char*>(base)}, keys(memory.take<unsigned>(rows)), spans(memory.take<unsigned>(2 * vocabulary)), order(memory.take<int>(rows)),
           sort(rows, static_cast<unsigned>(vocabulary), true, memory)
     {
-        for (int s = 0; s < EmbeddingBlocks::SIZES && rows >> (EMBEDDING_BLOCK_BITS * (s + 1)) > 0; ++s) {
+        // (blocks of places whenever there is one, larger blocks where a row could have many of the smaller ones to add)
+        for (int s = 0; s < EmbeddingBlocks::SIZES && rows >> (EMBEDDING_BLOCK_BITS * (s + 1)) >= (s == 0 ? 1 : 4); ++s) {
             blocks.sums[s] = memory.take<float>((rows >> (EMBEDDING_BLOCK_BITS * (s + 1))) * channels);
             blocks.sizes = s + 1;
         }
@@ -417,7 +423,7 @@ void Tokens::group(const Tensor& index, int groups, Tensor& order, Tensor& offse
     checkMemory(memory, groupMemory(index.size(0), groups));
     Workspace workspace{static_cast<char*>(memory)};
     GroupPlan plan(index.size(0), static_cast<unsigned>(groups), false, workspace);
-    sortByGroup(index, plan, ptr<int>(order), nullptr, ptr<int>(offsets), stream);
+    sortByGroup(index, plan, ptr<int>(order), nullptr, ptr<int>(offsets), nullptr, stream);
 }
 
 void Tokens::embedding(const Tensor& index, const Tensor& table, float scale, Tensor& output, stream_t stream)
@@ -459,25 +465,22 @@ void Tokens::embeddingAdjoint(const Tensor& index, const Tensor& adjOutput, floa
     const int vec = C < wide(p) ? 1 : wide(p), lanes = lanesPerRow(C, vec);
     const std::string shape = str(vec, ", ", lanes);
     EmbeddingPlan plan(rows, vocabulary, C, memory);
-    QMLP_HIP_CALL(qmlp_hip_memset_async(plan.spans, 0, sizeof(unsigned) * 2 * vocabulary, stream));
     const void* dy = ptr<void>(adjOutput);
     if (rows > 0) {
-        sortByGroup(index, plan.sort, plan.order, plan.keys, nullptr, stream);
-        tokenKernel("embedding.h", "EmbeddingSpansKernel")
-            .call(static_cast<unsigned>(divUp<int64_t>(rows, EMBEDDING_THREADS)), EMBEDDING_THREADS, 0, stream, static_cast<const unsigned*>(plan.keys), rows,
-                  static_cast<unsigned>(vocabulary), plan.spans);
+        const bool marked = sortByGroup(index, plan.sort, plan.order, plan.keys, nullptr, plan.spans, stream);
         for (int s = 0; s < plan.blocks.sizes; ++s) {
-            const int64_t blocks = rows >> (EMBEDDING_BLOCK_BITS * (s + 1));
+            // (the first kernel looks at every place for the spans)
+            const int64_t blocks = s == 0 && !marked ? divUp<int64_t>(rows, 1 << EMBEDDING_BLOCK_BITS) : rows >> (EMBEDDING_BLOCK_BITS * (s + 1));
             tokenKernel("embedding.h", str("EmbeddingBlocksKernel<", scalarName(p), ", ", shape, s == 0 ? ", true>" : ", false>"))
                 .call(static_cast<unsigned>(divUp<int64_t>(blocks, EMBEDDING_THREADS / lanes)), EMBEDDING_THREADS, 0, stream,
                       static_cast<const unsigned*>(plan.keys), static_cast<const int*>(plan.order), rows, static_cast<unsigned>(vocabulary),
                       EMBEDDING_BLOCK_BITS * (s + 1), dy, strideOf(adjOutput, 0), s == 0 ? nullptr : plan.blocks.sums[s - 1],
-                      const_cast<float*>(plan.blocks.sums[s]), C);
+                      const_cast<float*>(plan.blocks.sums[s]), C, marked ? nullptr : plan.spans);
         }
     }
     tokenKernel("embedding.h", str("EmbeddingAdjointKernel<", scalarName(p), ", ", shape, ">"))
         .call(workgroups(divUp<int64_t>(vocabulary, EMBEDDING_THREADS / lanes), 1 << 20), EMBEDDING_THREADS, 0, stream,
-              static_cast<const unsigned*>(plan.spans), static_cast<const int*>(plan.order), plan.blocks, dy, strideOf(adjOutput, 0), scale,
+              static_cast<const unsigned*>(plan.keys), static_cast<const unsigned*>(plan.spans), static_cast<const int*>(plan.order), rows, plan.blocks, dy, strideOf(adjOutput, 0), scale,
               adjTable.rawPtr(), strideOf(adjTable, 0), vocabulary, C);
 }
 
@@ -679,11 +682,14 @@ void Tokens::precompile(Tensor::Precision p)
     const std::string t = scalarName(p);
     const std::vector<std::string> indices = {"int", "long long"};
     for (const auto& i : indices)
-        for (const char* kernel : {"GroupSmallKernel", "GroupCountKernel", "GroupScatterKernel"}) precompileKernel("row_groups.h", str(kernel, "<", i, ">"));
+    {
+        precompileKernel("row_groups.h", str("GroupSmallKernel<", i, ">"));
+        for (const int items : {1, 4})
+            for (const char* kernel : {"GroupCountKernel", "GroupScatterKernel"}) precompileKernel("row_groups.h", str(kernel, "<", i, ", ", items, ">"));
+    }
     for (const char* kernel : {"GroupScanKernel", "GroupOffsetsKernel"}) precompileKernel("row_groups.h", kernel);
-    precompileKernel("embedding.h", "EmbeddingSpansKernel");
     for (const int vec : {1, wide(p)})
-        for (const int lanes : {8, 16, 32, 64}) {
+        for (const int lanes : {8, 16, 32, 64, 128, 256}) {
             if (vec == 1 && lanes > 8) continue;
             const std::string shape = str(t, ", ", vec, ", ", lanes);
             for (const auto& i : indices) precompileKernel("embedding.h", str("EmbeddingKernel<", t, ", ", i, ", ", vec, ", ", lanes, ">"));
