@@ -15,54 +15,59 @@ QUICKMLP_KERNEL_NAMESPACE_BEGIN
 constexpr int EMBEDDING_THREADS = 256;
 constexpr int EMBEDDING_BLOCK_BITS = 6;   // 64 places per block, 64 blocks per block of the next size
 
-/** G lanes per row, PIECES of VEC entries each at a time. */
-template <typename T, typename I, int VEC, int G>
+/** G lanes per row, AT_ONCE consecutive rows at a time: their indices and then their pieces are in flight together. */
+template <typename T, typename I, int VEC, int G, int AT_ONCE>
 __global__ void __launch_bounds__(EMBEDDING_THREADS)
 EmbeddingKernel(const I* __restrict__ index, long long strideIndex, const T* __restrict__ table, long long strideTable, float scale,
                 T* __restrict__ y, long long strideY, long long rows, long long vocabulary, int C)
 {
-    constexpr int ROWS = EMBEDDING_THREADS / G;
+    constexpr int ROWS = EMBEDDING_THREADS / G * AT_ONCE;
     const int lane = threadIdx.x % G;
-    for (long long row = static_cast<long long>(blockIdx.x) * ROWS + threadIdx.x / G; row < rows; row += static_cast<long long>(gridDim.x) * ROWS) {
-        const long long v = index[row * strideIndex];
-        const bool valid = v >= 0 && v < vocabulary;
-        const T* from = table + (valid ? v : 0) * strideTable;
-        T* to = y + row * strideY;
-#pragma unroll 4
+    for (long long row = static_cast<long long>(blockIdx.x) * ROWS + threadIdx.x / G * AT_ONCE; row < rows; row += static_cast<long long>(gridDim.x) * ROWS) {
+        long long v[AT_ONCE];
+#pragma unroll
+        for (int n = 0; n < AT_ONCE; ++n) v[n] = index[min(row + n, rows - 1) * strideIndex];
         for (int c = lane * VEC; c < C; c += G * VEC) {
             const int at = VEC == 1 ? c : min(c, C - VEC);   // the last piece ends with the row
-            float values[VEC] = {};
-            if (valid) loadFloats(from + at, values);
+            Raw<T, VEC> raw[AT_ONCE];
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) values[k] = valid ? values[k] * scale : 0;
-            storeFloats(to + at, values);
+            for (int n = 0; n < AT_ONCE; ++n)
+                if (v[n] >= 0 && v[n] < vocabulary) raw[n].load(table + v[n] * strideTable + at);
+#pragma unroll
+            for (int n = 0; n < AT_ONCE; ++n) {
+                const bool valid = v[n] >= 0 && v[n] < vocabulary;
+                float values[VEC];
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) values[k] = valid ? static_cast<float>(raw[n].v[k]) * scale : 0;
+                if (row + n < rows) storeFloats(y + (row + n) * strideY + at, values);
+            }
         }
     }
 }
 
-/** Adds COUNT terms; term(n, values) has the n-th one. */
-template <int VEC, int COUNT, typename Term>
-__device__ __forceinline__ void addTerms(float (&sum)[VEC], Term term)
+/** Adds COUNT terms of T; at(n) is where the n-th one is. All of them are asked for before the first is added. */
+template <typename T, int VEC, int COUNT, typename At>
+__device__ __forceinline__ void addTerms(float (&sum)[VEC], At at)
 {
-    float terms[COUNT][VEC];   // all of them asked for before the first is added
+    Raw<T, VEC> terms[COUNT];
 #pragma unroll
-    for (int n = 0; n < COUNT; ++n) term(n, terms[n]);
+    for (int n = 0; n < COUNT; ++n) terms[n].load(at(n));
 #pragma unroll
     for (int n = 0; n < COUNT; ++n)
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) sum[k] += terms[n][k];
+        for (int k = 0; k < VEC; ++k) sum[k] += static_cast<float>(terms[n].v[k]);
 }
 /** Adds 'count' consecutive terms, eight of them in flight. */
-template <int VEC, typename Term>
-__device__ __forceinline__ void addRange(float (&sum)[VEC], int count, Term term)
+template <typename T, int VEC, typename At>
+__device__ __forceinline__ void addRange(float (&sum)[VEC], int count, At at)
 {
     int n = 0;
-    for (; n + 8 <= count; n += 8) addTerms<VEC, 8>(sum, [&](int k, float (&v)[VEC]) { term(n + k, v); });
+    for (; n + 8 <= count; n += 8) addTerms<T, VEC, 8>(sum, [&](int k) { return at(n + k); });
     if (n + 4 <= count) {
-        addTerms<VEC, 4>(sum, [&](int k, float (&v)[VEC]) { term(n + k, v); });
+        addTerms<T, VEC, 4>(sum, [&](int k) { return at(n + k); });
         n += 4;
     }
-    for (; n < count; ++n) addTerms<VEC, 1>(sum, [&](int k, float (&v)[VEC]) { term(n + k, v); });
+    for (; n < count; ++n) addTerms<T, VEC, 1>(sum, [&](int k) { return at(n + k); });
 }
 
 /**
@@ -81,14 +86,22 @@ EmbeddingBlocksKernel(const unsigned* __restrict__ keys, const int* __restrict__
     if (FIRST && spans)
         for (long long i = from + threadIdx.x % G; i < min(to, rows); i += G) markSpans(keys, i, rows, vocabulary, spans);
     if (to > rows || keys[from] != keys[to - 1] || keys[from] >= vocabulary) return;
-    for (int c = threadIdx.x % G * VEC; c < C; c += G * VEC) {
-        const int at = VEC == 1 ? c : min(c, C - VEC);
+    // All lanes go through the loop, those behind the last column with its address: a place of the order is a lane's register,
+    // which the others read.
+    for (int column = 0; column < C; column += G * VEC) {
+        const int c = column + threadIdx.x % G * VEC, at = min(c, C - VEC);
         float sum[VEC] = {};
-        addRange(sum, 1 << EMBEDDING_BLOCK_BITS, [&](int i, float (&v)[VEC]) {
-            if constexpr (FIRST) loadFloats(adjY + order[from + i] * strideAdjY + at, v);
-            else loadFloats(smaller + ((block << EMBEDDING_BLOCK_BITS) + i) * C + at, v);
-        });
-        storeFloats(sums + block * C + at, sum);
+        if constexpr (FIRST && G >= 64) {
+            static_assert(EMBEDDING_BLOCK_BITS == 6, "a place for each lane of a wavefront");
+            const int own = order[from + threadIdx.x % 64];
+#pragma unroll
+            for (int n = 0; n < 64; n += 16)
+                addTerms<T, VEC, 16>(sum, [&](int k) { return adjY + __builtin_amdgcn_readlane(own, n + k) * strideAdjY + at; });
+        } else if constexpr (FIRST)
+            addRange<T>(sum, 1 << EMBEDDING_BLOCK_BITS, [&](int i) { return adjY + order[from + i] * strideAdjY + at; });
+        else
+            addRange<float>(sum, 1 << EMBEDDING_BLOCK_BITS, [&](int i) { return smaller + ((block << EMBEDDING_BLOCK_BITS) + i) * C + at; });
+        if (c < C) storeFloats(sums + block * C + at, sum);
     }
 }
 
@@ -100,50 +113,69 @@ struct EmbeddingBlocks
     const float* sums[SIZES];
 };
 
-/** G lanes per row of the table. */
+constexpr int EMBEDDING_MOST_ROWS = 64;
+/**
+ * The gradient of 'each' (up to EMBEDDING_MOST_ROWS) consecutive rows of the table per workgroup, G lanes per row. Their spans are
+ * looked up together first, with the only term of those that have one.
+ */
 template <typename T, int VEC, int G>
 __global__ void __launch_bounds__(EMBEDDING_THREADS)
 EmbeddingAdjointKernel(const unsigned* __restrict__ keys, const unsigned* __restrict__ spans, const int* __restrict__ order, long long rows,
                        EmbeddingBlocks blocks, const T* __restrict__ adjY, long long strideAdjY, float scale, T* __restrict__ adjTable,
-                       long long strideTable, long long vocabulary, int C)
+                       long long strideTable, long long vocabulary, int C, int each)
 {
-    constexpr int ROWS = EMBEDDING_THREADS / G;
+    __shared__ unsigned begin[EMBEDDING_MOST_ROWS], end[EMBEDDING_MOST_ROWS];
+    __shared__ int only[EMBEDDING_MOST_ROWS];
+    const long long firstRow = static_cast<long long>(blockIdx.x) * each;
+    const int count = static_cast<int>(min(static_cast<long long>(each), vocabulary - firstRow));
+    if (static_cast<int>(threadIdx.x) < count) {
+        const long long v = firstRow + threadIdx.x;
+        const unsigned from = spans[v], to = spans[vocabulary + v];
+        const bool any = from < rows && keys[from] == v;   // otherwise no token names the row, and nothing was written there
+        begin[threadIdx.x] = any ? from : 0;
+        end[threadIdx.x] = any ? to : 0;
+        only[threadIdx.x] = any ? order[from] : 0;
+    }
+    __syncthreads();
     const int lane = threadIdx.x % G;
-    for (long long v = static_cast<long long>(blockIdx.x) * ROWS + threadIdx.x / G; v < vocabulary; v += static_cast<long long>(gridDim.x) * ROWS) {
-        unsigned span[2] = {spans[v], spans[vocabulary + v]};
+    for (int r = threadIdx.x / G; r < count; r += EMBEDDING_THREADS / G) {
+        unsigned span[2] = {begin[r], end[r]};
+        int single = only[r];
         if constexpr (G >= 64) {   // one row for the whole wavefront
             span[0] = __builtin_amdgcn_readfirstlane(span[0]);
             span[1] = __builtin_amdgcn_readfirstlane(span[1]);
+            single = __builtin_amdgcn_readfirstlane(single);
         }
-        const long long from = span[0];
-        const bool any = from < rows && keys[from] == v;   // otherwise no token names the row, and nothing was written there
-        const long long to = any ? static_cast<long long>(span[1]) : from;
+        const long long from = span[0], to = span[1];
         for (int c = lane * VEC; c < C; c += G * VEC) {
             const int at = VEC == 1 ? c : min(c, C - VEC);
             float sum[VEC] = {};
-            // places up to the first block, blocks up to the first larger block, ..., and down again
-            long long i = from;
-            auto add = [&](int size, long long end) {
-                const int bits = EMBEDDING_BLOCK_BITS * size;
-                const long long first = i >> bits;
-                const int count = static_cast<int>((end - i) >> bits);
-                if (size == 0) addRange(sum, count, [&](int n, float (&term)[VEC]) { loadFloats(adjY + order[first + n] * strideAdjY + at, term); });
-                else {
-                    const float* p = blocks.sums[size - 1] + first * C + at;
-                    addRange(sum, count, [&](int n, float (&term)[VEC]) { loadFloats(p + static_cast<long long>(n) * C, term); });
+            if (to - from == 1) addTerms<T, VEC, 1>(sum, [&](int) { return adjY + single * strideAdjY + at; });
+            else if (to > from) {
+                // places up to the first block, blocks up to the first larger block, ..., and down again
+                long long i = from;
+                auto add = [&](int size, long long last) {
+                    const int bits = EMBEDDING_BLOCK_BITS * size;
+                    const long long first = i >> bits;
+                    const int terms = static_cast<int>((last - i) >> bits);
+                    if (size == 0) addRange<T>(sum, terms, [&](int n) { return adjY + order[first + n] * strideAdjY + at; });
+                    else {
+                        const float* p = blocks.sums[size - 1] + first * C + at;
+                        addRange<float>(sum, terms, [&](int n) { return p + static_cast<long long>(n) * C; });
+                    }
+                    i = last;
+                };
+                int size = 0;
+                for (; size < blocks.sizes; ++size) {
+                    const long long places = 1ll << (EMBEDDING_BLOCK_BITS * (size + 1)), next = (i + places - 1) & -places;
+                    if (next + places > to) break;   // no larger block in here
+                    add(size, next);
                 }
-                i = end;
-            };
-            int size = 0;
-            for (; size < blocks.sizes; ++size) {
-                const long long places = 1ll << (EMBEDDING_BLOCK_BITS * (size + 1)), next = (i + places - 1) & -places;
-                if (next + places > to) break;   // no larger block in here
-                add(size, next);
+                for (; size >= 0; --size) add(size, to >> (EMBEDDING_BLOCK_BITS * size) << (EMBEDDING_BLOCK_BITS * size));
             }
-            for (; size >= 0; --size) add(size, to >> (EMBEDDING_BLOCK_BITS * size) << (EMBEDDING_BLOCK_BITS * size));
 #pragma unroll
             for (int k = 0; k < VEC; ++k) sum[k] *= scale;
-            storeFloats(adjTable + v * strideTable + at, sum);
+            storeFloats(adjTable + (firstRow + r) * strideTable + at, sum);
         }
     }
 }

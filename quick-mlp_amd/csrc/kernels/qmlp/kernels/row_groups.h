@@ -2,8 +2,9 @@
 // Rows in the order of the group that they belong to: a stable counting sort by one or more digits of the group's number.
 //
 // The sort reads an index per row and writes a place per row; what bounds it is the latency of its launches, not its bytes
-// (2^20 rows: 8 MB). So a digit has up to 13 bits, which makes one pass of up to 8191 groups, and a batch that fits the
-// registers of a workgroup is sorted by one workgroup in one launch.
+// (2^20 rows: 8 MB). So a digit has as many values as the LDS has
+// counters for, which makes one pass of up to 4399 groups, and a batch that fits the registers of a workgroup is sorted by one
+// workgroup in one launch.
 //
 // The place of a row among those of its digit is found by ballots: of the lanes of a wavefront with the same digit, those
 // with lower numbers come first; wavefronts and tiles follow in the order of their rows. No atomic decides an order.
@@ -15,8 +16,9 @@ QUICKMLP_KERNEL_NAMESPACE_BEGIN
 constexpr int GROUP_SMALL_THREADS = 1024, GROUP_SMALL_ITEMS = 8, GROUP_SMALL_BITS = 8;
 constexpr int GROUP_SMALL_ROWS = GROUP_SMALL_THREADS * GROUP_SMALL_ITEMS;
 constexpr int GROUP_THREADS = 1024;   // tiles of as many rows, or ITEMS times as many
-constexpr int GROUP_MAX_BITS = 13;
+constexpr int GROUP_MOST_DIGITS = 4400;   // 36 bytes of LDS each
 constexpr int GROUP_SCAN_DIGITS = 64, GROUP_SCAN_SLICES = 16;
+constexpr int GROUP_FEW_TILES = 64;   // that many, the workgroups of the last kernel add up the tiles before theirs themselves
 
 /** The group of a row; 'groups' for rows whose index names none. */
 template <typename I>
@@ -244,7 +246,8 @@ GroupScanKernel(unsigned* __restrict__ counts, int tiles, int digits, unsigned* 
 }
 
 /**
- * Writes the rows of a tile to their places. keysOut, offsets: may be null; offsets for a sort of one pass only, whose digits are
+ * Writes the rows of a tile to their places. counts: as GroupScanKernel leaves them, with totals; without totals (up to
+ * GROUP_FEW_TILES tiles) as GroupCountKernel does. keysOut, offsets: may be null; offsets for a sort of one pass only, whose digits are
  * the groups. LDS: a start per digit, the counters of the wavefronts.
  */
 template <typename I, int ITEMS>
@@ -259,8 +262,27 @@ GroupScatterKernel(GroupSource<I> source, long long rows, int shift, int digitBi
     unsigned short* const counters = reinterpret_cast<unsigned short*>(groupLds + digits);   // [wavefront][digit]
     __shared__ unsigned sums[WAVES];
     const int wave = threadIdx.x / 64;
-    for (int d = threadIdx.x; d < digits; d += GROUP_THREADS) {
-        starts[d] = totals[d];
+    constexpr int OWN = (GROUP_MOST_DIGITS + GROUP_THREADS - 1) / GROUP_THREADS;
+    unsigned before[OWN];   // rows of the thread's digits in the tiles before
+#pragma unroll
+    for (int n = 0; n < OWN; ++n) {
+        const int d = n * GROUP_THREADS + threadIdx.x;
+        if (d >= digits) break;
+        if (totals) {
+            starts[d] = totals[d];
+            before[n] = counts[static_cast<long long>(blockIdx.x) * digits + d];
+        } else {
+            unsigned all = 0, those = 0;
+            const int tiles = gridDim.x;
+#pragma unroll 16
+            for (int t = 0; t < tiles; ++t) {
+                const unsigned here = counts[t * digits + d];
+                all += here;
+                those += t < static_cast<int>(blockIdx.x) ? here : 0;
+            }
+            starts[d] = all;
+            before[n] = those;
+        }
 #pragma unroll
         for (int w = 0; w < WAVES; ++w) counters[w * digits + d] = 0;
     }
@@ -278,26 +300,30 @@ GroupScatterKernel(GroupSource<I> source, long long rows, int shift, int digitBi
     __syncthreads();
     scanInLds<GROUP_THREADS>(starts, digits, sums);
     if (offsets && blockIdx.x == 0)
-        for (unsigned g = threadIdx.x; g <= source.groups; g += GROUP_THREADS) offsets[g] = static_cast<int>(starts[g]);
+        for (unsigned g = threadIdx.x; g <= source.groups; g += GROUP_THREADS) offsets[g] = static_cast<int>(starts[g]);   // (nothing is before the first tile)
+#pragma unroll
+    for (int n = 0; n < OWN; ++n) {
+        const int d = n * GROUP_THREADS + threadIdx.x;
+        if (d < digits) starts[d] += before[n];
+    }
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
         const bool has = first + i * 64 < rows;
         const unsigned d = has ? (key[i] >> shift) & mask : 0;
         const unsigned long long same = lanesLike(d, digitBits, __ballot(has));
         unsigned short* const counter = counters + wave * digits + d;
-        const unsigned before = has ? *counter : 0;
-        place[i] = static_cast<unsigned short>(before + lanesBelow(same));
+        const unsigned own = has ? *counter : 0;
+        place[i] = static_cast<unsigned short>(own + lanesBelow(same));
         waveLdsSync();
-        if (has && lanesBelow(same) == 0) *counter = static_cast<unsigned short>(before + __popcll(same));
+        if (has && lanesBelow(same) == 0) *counter = static_cast<unsigned short>(own + __popcll(same));
         waveLdsSync();
     }
     __syncthreads();
-    const unsigned* before = counts + static_cast<long long>(blockIdx.x) * digits;
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
         if (first + i * 64 >= rows) continue;
         const unsigned d = (key[i] >> shift) & mask;
-        unsigned p = starts[d] + before[d] + place[i];
+        unsigned p = starts[d] + place[i];
 #pragma unroll
         for (int w = 0; w < WAVES - 1; ++w)
             if (w < wave) p += counters[w * digits + d];

@@ -12,6 +12,14 @@ typedef __bf16 bf16;
 template <typename T>
 constexpr int WIDE = 16 / static_cast<int>(sizeof(T));
 
+/** N consecutive entries as they are in memory, for values that wait in registers: half of the registers of floats. */
+template <typename T, int N>
+struct Raw
+{
+    T v[N];
+    __device__ __forceinline__ void load(const T* __restrict__ p) { __builtin_memcpy(v, p, sizeof(v)); }
+};
+
 /**
  * N consecutive entries as floats. The address needs the alignment of one entry only: the hardware takes wide accesses at any
  * address, so rows of odd lengths are moved 16 bytes at a time as well.

@@ -138,7 +138,7 @@ unsigned workgroups(int64_t pieces, int64_t most) { return static_cast<unsigned>
 
 // ------------------------------------------------------------------------------------------------ groups
 // as in kernels/row_groups.h
-constexpr int GROUP_SMALL_THREADS = 1024, GROUP_SMALL_ROWS = 8192, GROUP_SMALL_BITS = 8, GROUP_THREADS = 1024, GROUP_MAX_BITS = 13,
+constexpr int GROUP_SMALL_THREADS = 1024, GROUP_SMALL_ROWS = 8192, GROUP_SMALL_BITS = 8, GROUP_THREADS = 1024, GROUP_FEW_TILES = 64, GROUP_MOST_DIGITS = 4400, GROUP_PASS_BITS = 12,
               GROUP_SCAN_DIGITS = 64, GROUP_SCAN_THREADS = 1024;
 /** GroupSource of kernels/row_groups.h */
 struct GroupSource
@@ -172,7 +172,7 @@ struct GroupPlan
     {
         const int bits = bitsOf(groups);
         const bool small = rows <= GROUP_SMALL_ROWS;
-        passes = divUp(bits, GROUP_MAX_BITS);
+        passes = groups < GROUP_MOST_DIGITS ? 1 : divUp(bits, GROUP_PASS_BITS);
         digitBits = divUp(bits, passes);
         maxDigits = static_cast<int>(std::min<int64_t>(1ll << digitBits, static_cast<int64_t>(groups) + 1));
         // a workgroup for every compute unit: tiles of one row per thread, of four where there are as many anyway (2^20 rows of 4096
@@ -215,14 +215,17 @@ bool sortByGroup(const Tensor& index, GroupPlan& plan, int* order, unsigned* key
         const unsigned mask = (1u << digitBits) - 1;
         const unsigned tiles = static_cast<unsigned>(plan.tiles);
         tokenKernel("row_groups.h", "GroupCountKernel" + types).call(tiles, GROUP_THREADS, digits * 4, stream, source, rows, shift, mask, digits, plan.counts);
-        tokenKernel("row_groups.h", "GroupScanKernel")
-            .call(static_cast<unsigned>(divUp(digits, GROUP_SCAN_DIGITS)), GROUP_SCAN_THREADS, 0, stream, plan.counts, static_cast<int>(tiles), digits, plan.totals);
+        const bool few = tiles <= GROUP_FEW_TILES;
+        if (!few)
+            tokenKernel("row_groups.h", "GroupScanKernel")
+                .call(static_cast<unsigned>(divUp(digits, GROUP_SCAN_DIGITS)), GROUP_SCAN_THREADS, 0, stream, plan.counts, static_cast<int>(tiles), digits,
+                      plan.totals);
         int* to = last ? order : plan.order[pass % 2];
         unsigned* toKeys = last ? (keysOut ? keysOut : plan.passes > 1 ? plan.keys[pass % 2] : nullptr) : plan.keys[pass % 2];
         const unsigned lds = digits * 4 + digits * 2 * (GROUP_THREADS / 64);
         tokenKernel("row_groups.h", "GroupScatterKernel" + types)
             .call(tiles, GROUP_THREADS, lds, stream, source, rows, shift, digitBits, digits, static_cast<const unsigned*>(plan.counts),
-                  static_cast<const unsigned*>(plan.totals), to, toKeys, plan.passes == 1 ? offsets : nullptr);
+                  few ? nullptr : static_cast<const unsigned*>(plan.totals), to, toKeys, plan.passes == 1 ? offsets : nullptr);
         source.keys = toKeys;
         source.order = to;
     }
@@ -234,7 +237,7 @@ bool sortByGroup(const Tensor& index, GroupPlan& plan, int* order, unsigned* key
 
 // ------------------------------------------------------------------------------------------------ embeddings
 // as in kernels/embedding.h
-constexpr int EMBEDDING_THREADS = 256, EMBEDDING_BLOCK_BITS = 6;
+constexpr int EMBEDDING_THREADS = 256, EMBEDDING_BLOCK_BITS = 6, EMBEDDING_MOST_ROWS = 64;
 struct EmbeddingBlocks
 {
     static constexpr int SIZES = 6;
@@ -248,6 +251,15 @@ int lanesPerRow(int C, int vec)
     int lanes = 8;
     while (lanes < EMBEDDING_THREADS && lanes * vec < C) lanes *= 2;
     return lanes;
+}
+
+/** Four rows at a time where that leaves four workgroups for every compute unit. */
+int embeddingRowsAtOnce(int64_t rows, int lanes) { return rows >= 4 * 4 * 256 * (EMBEDDING_THREADS / lanes) ? 4 : 1; }
+/** Rows of the table per workgroup of the adjoint kernel: as many as its lanes take at a time, and more where there are many workgroups. */
+int embeddingAdjointRows(int64_t vocabulary, int lanes)
+{
+    const int64_t atATime = EMBEDDING_THREADS / lanes;
+    return static_cast<int>(std::min<int64_t>(EMBEDDING_MOST_ROWS, roundUp(std::max<int64_t>(1, vocabulary / 2048), atATime)));
 }
 
 struct EmbeddingPlan
@@ -437,8 +449,9 @@ void Tokens::embedding(const Tensor& index, const Tensor& table, float scale, Te
     if (output.numel() == 0) return;
     const int C = table.size(1), vec = C < wide(table.precision()) ? 1 : wide(table.precision()), lanes = lanesPerRow(C, vec);
     const long long rows = index.size(0), vocabulary = table.size(0);
-    tokenKernel("embedding.h", str("EmbeddingKernel<", scalarName(table.precision()), ", ", scalarName(index.precision()), ", ", vec, ", ", lanes, ">"))
-        .call(workgroups(divUp<int64_t>(rows, EMBEDDING_THREADS / lanes), 1 << 20), EMBEDDING_THREADS, 0, stream, index.rawPtr(), strideOf(index, 0),
+    const int atOnce = embeddingRowsAtOnce(rows, lanes), each = EMBEDDING_THREADS / lanes * atOnce;
+    tokenKernel("embedding.h", str("EmbeddingKernel<", scalarName(table.precision()), ", ", scalarName(index.precision()), ", ", vec, ", ", lanes, ", ", atOnce, ">"))
+        .call(workgroups(divUp<int64_t>(rows, each), 1 << 20), EMBEDDING_THREADS, 0, stream, index.rawPtr(), strideOf(index, 0),
               static_cast<const void*>(ptr<void>(table)), strideOf(table, 0), scale, output.rawPtr(), strideOf(output, 0), rows, vocabulary, C);
 }
 
@@ -478,10 +491,10 @@ void Tokens::embeddingAdjoint(const Tensor& index, const Tensor& adjOutput, floa
                       const_cast<float*>(plan.blocks.sums[s]), C, marked ? nullptr : plan.spans);
         }
     }
+    const int each = embeddingAdjointRows(vocabulary, lanes);
     tokenKernel("embedding.h", str("EmbeddingAdjointKernel<", scalarName(p), ", ", shape, ">"))
-        .call(workgroups(divUp<int64_t>(vocabulary, EMBEDDING_THREADS / lanes), 1 << 20), EMBEDDING_THREADS, 0, stream,
-              static_cast<const unsigned*>(plan.keys), static_cast<const unsigned*>(plan.spans), static_cast<const int*>(plan.order), rows, plan.blocks, dy, strideOf(adjOutput, 0), scale,
-              adjTable.rawPtr(), strideOf(adjTable, 0), vocabulary, C);
+        .call(static_cast<unsigned>(divUp<int64_t>(vocabulary, each)), EMBEDDING_THREADS, 0, stream, static_cast<const unsigned*>(plan.keys), static_cast<const unsigned*>(plan.spans), static_cast<const int*>(plan.order), rows, plan.blocks, dy, strideOf(adjOutput, 0), scale,
+              adjTable.rawPtr(), strideOf(adjTable, 0), vocabulary, C, each);
 }
 
 void Tokens::layerNorm(const Tensor& input, const Tensor& weight, const Tensor& bias, float epsilon, Tensor& output, Tensor& mean, Tensor& rstd,
@@ -692,7 +705,8 @@ void Tokens::precompile(Tensor::Precision p)
         for (const int lanes : {8, 16, 32, 64, 128, 256}) {
             if (vec == 1 && lanes > 8) continue;
             const std::string shape = str(t, ", ", vec, ", ", lanes);
-            for (const auto& i : indices) precompileKernel("embedding.h", str("EmbeddingKernel<", t, ", ", i, ", ", vec, ", ", lanes, ">"));
+            for (const auto& i : indices)
+                for (const int atOnce : {1, 4}) precompileKernel("embedding.h", str("EmbeddingKernel<", t, ", ", i, ", ", vec, ", ", lanes, ", ", atOnce, ">"));
             precompileKernel("embedding.h", str("EmbeddingBlocksKernel<", shape, ", true>"));
             precompileKernel("embedding.h", str("EmbeddingBlocksKernel<", shape, ", false>"));
             precompileKernel("embedding.h", str("EmbeddingAdjointKernel<", shape, ">"));

@@ -43,8 +43,8 @@ def say(*what):
 
 # ------------------------------------------------------------------------------------------------ groups
 @gpu
-@pytest.mark.parametrize("groups", [0, 1, 2, 8, 255, 256, 4096, 9000, 70000])
-@pytest.mark.parametrize("rows", [0, 1, 63, 64, 65, 1000, 8192, 8193, 50001])
+@pytest.mark.parametrize("groups", [0, 1, 2, 8, 255, 256, 4096, 4399, 4400, 8191, 9000, 70000])
+@pytest.mark.parametrize("rows", [0, 1, 63, 64, 65, 1000, 8192, 8193, 70001, 300007])
 @pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
 def test_groups_are_a_stable_sort(rows, groups, dtype):
     say("group", rows, groups, dtype)
