@@ -50,6 +50,27 @@ __device__ __forceinline__ void loadPieces(const RowPieces<VEC, G>& at, const T*
     }
 }
 
+/** A lane's pieces of a row, as they are in memory. */
+template <typename T, int VEC, int G, int CHUNKS>
+struct RawPieces
+{
+    Raw<T, VEC> raw[CHUNKS];
+    __device__ __forceinline__ void load(const RowPieces<VEC, G>& at, const T* __restrict__ p)
+    {
+#pragma unroll
+        for (int j = 0; j < CHUNKS; ++j)
+            if (at.has(j)) raw[j].load(p + at.start(j));
+    }
+    /** As floats; 0 where the lane has none. */
+    __device__ __forceinline__ void floats(const RowPieces<VEC, G>& at, float (&v)[CHUNKS][VEC]) const
+    {
+#pragma unroll
+        for (int j = 0; j < CHUNKS; ++j)
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) v[j][k] = at.has(j) ? static_cast<float>(raw[j].v[k]) : 0;
+    }
+};
+
 /**
  * One row per G lanes. weight, bias: may be null (1 and 0); mean, rstd: may be null (not kept for an adjoint).
  * G * VEC * CHUNKS >= C >= VEC.
@@ -65,9 +86,14 @@ LayerNormKernel(const T* __restrict__ x, long long strideX, const W* __restrict_
     float w[CHUNKS][VEC], b[CHUNKS][VEC];
     loadPieces(at, weight, 1.0f, w);
     loadPieces(at, bias, 0.0f, b);
-    for (long long row = static_cast<long long>(blockIdx.x) * ROWS + threadIdx.x / G; row < rows; row += static_cast<long long>(gridDim.x) * ROWS) {
+    const long long step = static_cast<long long>(gridDim.x) * ROWS;
+    long long row = static_cast<long long>(blockIdx.x) * ROWS + threadIdx.x / G;
+    RawPieces<T, VEC, G, CHUNKS> coming;   // the next row is asked for before the present one is worked on
+    if (row < rows) coming.load(at, x + row * strideX);
+    for (; row < rows; row += step) {
         float v[CHUNKS][VEC];
-        loadPieces(at, x + row * strideX, 0.0f, v);
+        coming.floats(at, v);
+        if (row + step < rows) coming.load(at, x + (row + step) * strideX);
         float sum[1] = {0};
 #pragma unroll
         for (int j = 0; j < CHUNKS; ++j)
@@ -114,11 +140,23 @@ LayerNormAdjointKernel(const T* __restrict__ x, long long strideX, const W* __re
     float w[CHUNKS][VEC], sumW[CHUNKS][VEC] = {}, sumB[CHUNKS][VEC] = {};
     loadPieces(at, weight, 1.0f, w);
     const float scale = 1.0f / C;
-    for (long long row = static_cast<long long>(blockIdx.x) * ROWS + threadIdx.x / G; row < rows; row += static_cast<long long>(gridDim.x) * ROWS) {
-        const float m = mean[row], r = rstd[row];
+    const long long step = static_cast<long long>(gridDim.x) * ROWS;
+    long long row = static_cast<long long>(blockIdx.x) * ROWS + threadIdx.x / G;
+    RawPieces<T, VEC, G, CHUNKS> comingX, comingD;   // of the next row
+    float comingMean = 0, comingRstd = 0;
+    auto ask = [&](long long r) {
+        comingX.load(at, x + r * strideX);
+        comingD.load(at, adjY + r * strideAdjY);
+        comingMean = mean[r];
+        comingRstd = rstd[r];
+    };
+    if (row < rows) ask(row);
+    for (; row < rows; row += step) {
+        const float m = comingMean, r = comingRstd;
         float n[CHUNKS][VEC], d[CHUNKS][VEC];
-        loadPieces(at, x + row * strideX, 0.0f, n);
-        loadPieces(at, adjY + row * strideAdjY, 0.0f, d);
+        comingX.floats(at, n);
+        comingD.floats(at, d);
+        if (row + step < rows) ask(row + step);
         float sums[2] = {0, 0};
 #pragma unroll
         for (int j = 0; j < CHUNKS; ++j)

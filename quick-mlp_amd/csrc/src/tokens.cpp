@@ -32,17 +32,31 @@ const char* scalarName(Tensor::Precision p)
 /** Entries of a 16-byte access. */
 int wide(Tensor::Precision p) { return 16 / Tensor::BytesPerEntry[p]; }
 
-/** The kernels stay loaded for the life of the process. File: below kernels/qmlp/kernels; name: with its template arguments. */
-KernelFunction& tokenKernel(const char* file, const std::string& name)
+enum KernelId { GROUP_SMALL, GROUP_COUNT, GROUP_SCAN, GROUP_SCATTER, GROUP_OFFSETS, EMBEDDING, EMBEDDING_BLOCKS, EMBEDDING_ADJOINT, LAYER_NORM,
+                LAYER_NORM_ADJOINT, LAYER_NORM_SUM, LAYER_NORM_LONG, LAYER_NORM_LONG_ADJOINT, LAYER_NORM_LONG_SUMS, GROUPED_ROWS, GROUPED_WEIGHTS,
+                GROUPED_SUM };
+/** One number for a kernel and its template arguments, each below 2^11: to build its name takes as long as to launch it. */
+template <typename... Args>
+uint64_t kernelKey(KernelId id, Args... args)
+{
+    static_assert(sizeof...(args) <= 5, "64 bits");
+    uint64_t key = id;
+    ((key = key << 11 | static_cast<uint64_t>(args)), ...);
+    return key;
+}
+/** The kernels stay loaded for the life of the process. File: below kernels/qmlp/kernels; name(): with its template arguments. */
+template <typename Name>
+KernelFunction& tokenKernel(const char* file, uint64_t key, Name name)
 {
     static std::mutex mutex;
-    static std::unordered_map<std::string, KernelFunction> kernels;
+    static std::unordered_map<uint64_t, KernelFunction> kernels;
     std::lock_guard<std::mutex> lock(mutex);
-    auto it = kernels.find(name);
+    auto it = kernels.find(key);
     if (it == kernels.end()) {
-        auto loaded = QuickMLP::Instance().kernelLoader()->getKernel("qmlp::kernel::" + name, KernelLoader::MainFile(std::string("qmlp/kernels/") + file),
+        auto loaded = QuickMLP::Instance().kernelLoader()->getKernel("qmlp::kernel::" + std::string(name()),
+                                                                     KernelLoader::MainFile(std::string("qmlp/kernels/") + file),
                                                                      QuickMLP::Instance().getCompileFlags() | KernelLoader::CompileThrowOnError);
-        it = kernels.emplace(name, std::move(*loaded)).first;
+        it = kernels.emplace(key, std::move(*loaded)).first;
     }
     return it->second;
 }
@@ -194,17 +208,17 @@ struct GroupPlan
 /** Sorts; keysOut (the groups in order) and offsets may be null. spans, if not null, are written for small batches: true. */
 bool sortByGroup(const Tensor& index, GroupPlan& plan, int* order, unsigned* keysOut, int* offsets, unsigned* spans, stream_t stream)
 {
-    const std::string type = std::string("<") + scalarName(index.precision()) + ">";
+    const Tensor::Precision type = index.precision();
     const long long stride = strideOf(index, 0);
     const int bits = bitsOf(plan.groups);
     if (plan.rows <= GROUP_SMALL_ROWS) {
         const size_t lds = plan.rows * 6 + 64 + (static_cast<size_t>(GROUP_SMALL_THREADS / 64 * 4) << std::min(bits, GROUP_SMALL_BITS)) + 4;
-        tokenKernel("row_groups.h", "GroupSmallKernel" + type)
+        tokenKernel("row_groups.h", kernelKey(GROUP_SMALL, type), [&] { return str("GroupSmallKernel<", scalarName(type), ">"); })
             .call(1, GROUP_SMALL_THREADS, static_cast<unsigned>(lds), stream, index.rawPtr(), stride, static_cast<int>(plan.rows), plan.groups, bits, order,
                   keysOut, offsets, spans);
         return spans != nullptr;
     }
-    const std::string types = str("<", scalarName(index.precision()), ", ", plan.items, ">");
+    auto arguments = [&] { return str("<", scalarName(type), ", ", plan.items, ">"); };
     GroupSource source{index.rawPtr(), stride, nullptr, nullptr, plan.groups};
     long long rows = plan.rows;
     for (int pass = 0; pass < plan.passes; ++pass) {
@@ -214,23 +228,24 @@ bool sortByGroup(const Tensor& index, GroupPlan& plan, int* order, unsigned* key
         const int digits = static_cast<int>(std::min<int64_t>(1ll << digitBits, static_cast<int64_t>(plan.groups >> shift) + 1));
         const unsigned mask = (1u << digitBits) - 1;
         const unsigned tiles = static_cast<unsigned>(plan.tiles);
-        tokenKernel("row_groups.h", "GroupCountKernel" + types).call(tiles, GROUP_THREADS, digits * 4, stream, source, rows, shift, mask, digits, plan.counts);
+        tokenKernel("row_groups.h", kernelKey(GROUP_COUNT, type, plan.items), [&] { return "GroupCountKernel" + arguments(); })
+            .call(tiles, GROUP_THREADS, digits * 4, stream, source, rows, shift, mask, digits, plan.counts);
         const bool few = tiles <= GROUP_FEW_TILES;
         if (!few)
-            tokenKernel("row_groups.h", "GroupScanKernel")
+            tokenKernel("row_groups.h", kernelKey(GROUP_SCAN), [] { return "GroupScanKernel"; })
                 .call(static_cast<unsigned>(divUp(digits, GROUP_SCAN_DIGITS)), GROUP_SCAN_THREADS, 0, stream, plan.counts, static_cast<int>(tiles), digits,
                       plan.totals);
         int* to = last ? order : plan.order[pass % 2];
         unsigned* toKeys = last ? (keysOut ? keysOut : plan.passes > 1 ? plan.keys[pass % 2] : nullptr) : plan.keys[pass % 2];
         const unsigned lds = digits * 4 + digits * 2 * (GROUP_THREADS / 64);
-        tokenKernel("row_groups.h", "GroupScatterKernel" + types)
+        tokenKernel("row_groups.h", kernelKey(GROUP_SCATTER, type, plan.items), [&] { return "GroupScatterKernel" + arguments(); })
             .call(tiles, GROUP_THREADS, lds, stream, source, rows, shift, digitBits, digits, static_cast<const unsigned*>(plan.counts),
                   few ? nullptr : static_cast<const unsigned*>(plan.totals), to, toKeys, plan.passes == 1 ? offsets : nullptr);
         source.keys = toKeys;
         source.order = to;
     }
     if (offsets && plan.passes > 1)
-        tokenKernel("row_groups.h", "GroupOffsetsKernel")
+        tokenKernel("row_groups.h", kernelKey(GROUP_OFFSETS), [] { return "GroupOffsetsKernel"; })
             .call(static_cast<unsigned>(divUp<int64_t>(static_cast<int64_t>(plan.groups) + 1, 256)), 256, 0, stream, source.keys, rows, plan.groups, offsets);
     return false;
 }
@@ -294,8 +309,9 @@ struct LayerNormShape
     std::string arguments() const { return std::to_string(vec) + ", " + std::to_string(lanes) + ", " + std::to_string(entries / vec); }
 };
 // 8 entries a lane for short rows, so that many lanes ask for memory; 64 lanes at first, whose sums need no LDS.
-constexpr std::array<std::array<int, 2>, 10> LAYER_NORM_SHAPES = {
-    {{8, 8}, {16, 8}, {32, 8}, {64, 8}, {64, 16}, {256, 8}, {256, 16}, {256, 32}, {1024, 16}, {1024, 32}}};
+// (32 entries a lane do not fit the registers: the adjoint kernel holds seven values for each, two of them of the next row)
+constexpr std::array<std::array<int, 2>, 9> LAYER_NORM_SHAPES = {
+    {{8, 8}, {16, 8}, {32, 8}, {64, 8}, {64, 16}, {256, 8}, {256, 16}, {512, 16}, {1024, 16}}};
 
 LayerNormShape layerNormShape(int channels, Tensor::Precision p)
 {
@@ -404,7 +420,8 @@ void launchRows(bool alongK, const Tensor& x, const Tensor& weight, const Tensor
     const int tilesJ = divUp(J, t.j);
     const int64_t places = tilePlaces(s.rows, s.experts, t.i);
     checkLaunch(places * tilesJ, t.threads());
-    tokenKernel("grouped_linear.h", str("GroupedRowsKernel<", scalarName(x.precision()), ", ", boolName(direct), ", ", boolName(alongK), ", ", t.arguments(), ">"))
+    tokenKernel("grouped_linear.h", kernelKey(GROUPED_ROWS, x.precision() * 4 + direct * 2 + alongK, t.i, t.j, t.wavesI, t.wavesJ),
+                [&] { return str("GroupedRowsKernel<", scalarName(x.precision()), ", ", boolName(direct), ", ", boolName(alongK), ", ", t.arguments(), ">"); })
         .call(static_cast<unsigned>(places * tilesJ), t.threads(), t.lds(), stream, x.rawPtr(), strideOf(x, 0), static_cast<const void*>(ptr<void>(weight)),
               strideOf(weight, 0), strideOf(weight, 1), static_cast<const void*>(ptr<void>(bias)), bias.defined() ? strideOf(bias, 0) : 0ll,
               static_cast<const int*>(ptr<int>(offsets)), s.experts, static_cast<void*>(ptr<void>(y)), strideOf(y, 0), s.rows, J, K, static_cast<int>(places),
@@ -450,7 +467,9 @@ void Tokens::embedding(const Tensor& index, const Tensor& table, float scale, Te
     const int C = table.size(1), vec = C < wide(table.precision()) ? 1 : wide(table.precision()), lanes = lanesPerRow(C, vec);
     const long long rows = index.size(0), vocabulary = table.size(0);
     const int atOnce = embeddingRowsAtOnce(rows, lanes), each = EMBEDDING_THREADS / lanes * atOnce;
-    tokenKernel("embedding.h", str("EmbeddingKernel<", scalarName(table.precision()), ", ", scalarName(index.precision()), ", ", vec, ", ", lanes, ", ", atOnce, ">"))
+    const Tensor::Precision p = table.precision(), i = index.precision();
+    tokenKernel("embedding.h", kernelKey(EMBEDDING, p, i, vec, lanes, atOnce),
+                [&] { return str("EmbeddingKernel<", scalarName(p), ", ", scalarName(i), ", ", vec, ", ", lanes, ", ", atOnce, ">"); })
         .call(workgroups(divUp<int64_t>(rows, each), 1 << 20), EMBEDDING_THREADS, 0, stream, index.rawPtr(), strideOf(index, 0),
               static_cast<const void*>(ptr<void>(table)), strideOf(table, 0), scale, output.rawPtr(), strideOf(output, 0), rows, vocabulary, C);
 }
@@ -476,7 +495,7 @@ void Tokens::embeddingAdjoint(const Tensor& index, const Tensor& adjOutput, floa
     if (adjTable.numel() == 0) return;
     const Tensor::Precision p = adjTable.precision();
     const int vec = C < wide(p) ? 1 : wide(p), lanes = lanesPerRow(C, vec);
-    const std::string shape = str(vec, ", ", lanes);
+    auto arguments = [&] { return str("<", scalarName(p), ", ", vec, ", ", lanes); };
     EmbeddingPlan plan(rows, vocabulary, C, memory);
     const void* dy = ptr<void>(adjOutput);
     if (rows > 0) {
@@ -484,7 +503,8 @@ void Tokens::embeddingAdjoint(const Tensor& index, const Tensor& adjOutput, floa
         for (int s = 0; s < plan.blocks.sizes; ++s) {
             // (the first kernel looks at every place for the spans)
             const int64_t blocks = s == 0 && !marked ? divUp<int64_t>(rows, 1 << EMBEDDING_BLOCK_BITS) : rows >> (EMBEDDING_BLOCK_BITS * (s + 1));
-            tokenKernel("embedding.h", str("EmbeddingBlocksKernel<", scalarName(p), ", ", shape, s == 0 ? ", true>" : ", false>"))
+            tokenKernel("embedding.h", kernelKey(EMBEDDING_BLOCKS, p, vec, lanes, s == 0),
+                        [&] { return "EmbeddingBlocksKernel" + arguments() + (s == 0 ? ", true>" : ", false>"); })
                 .call(static_cast<unsigned>(divUp<int64_t>(blocks, EMBEDDING_THREADS / lanes)), EMBEDDING_THREADS, 0, stream,
                       static_cast<const unsigned*>(plan.keys), static_cast<const int*>(plan.order), rows, static_cast<unsigned>(vocabulary),
                       EMBEDDING_BLOCK_BITS * (s + 1), dy, strideOf(adjOutput, 0), s == 0 ? nullptr : plan.blocks.sums[s - 1],
@@ -492,7 +512,7 @@ void Tokens::embeddingAdjoint(const Tensor& index, const Tensor& adjOutput, floa
         }
     }
     const int each = embeddingAdjointRows(vocabulary, lanes);
-    tokenKernel("embedding.h", str("EmbeddingAdjointKernel<", scalarName(p), ", ", shape, ">"))
+    tokenKernel("embedding.h", kernelKey(EMBEDDING_ADJOINT, p, vec, lanes), [&] { return "EmbeddingAdjointKernel" + arguments() + ">"; })
         .call(static_cast<unsigned>(divUp<int64_t>(vocabulary, each)), EMBEDDING_THREADS, 0, stream, static_cast<const unsigned*>(plan.keys), static_cast<const unsigned*>(plan.spans), static_cast<const int*>(plan.order), rows, plan.blocks, dy, strideOf(adjOutput, 0), scale,
               adjTable.rawPtr(), strideOf(adjTable, 0), vocabulary, C, each);
 }
@@ -523,11 +543,12 @@ void Tokens::layerNorm(const Tensor& input, const Tensor& weight, const Tensor& 
     }
     if (input.numel() == 0) return;
     const LayerNormShape s = layerNormShape(C, p);
-    const std::string types = valueTypes(p, weights);
+    auto types = [&] { return "<" + valueTypes(p, weights); };
     const void *x = input.rawPtr(), *w = ptr<void>(weight), *b = ptr<void>(bias);
     const long long strideX = strideOf(input, 0), strideY = strideOf(output, 0);
     const bool isLong = s.lanes == 0;
-    tokenKernel("layer_norm.h", isLong ? "LayerNormLongKernel<" + types + ">" : "LayerNormKernel<" + types + ", " + s.arguments() + ">")
+    tokenKernel("layer_norm.h", isLong ? kernelKey(LAYER_NORM_LONG, p, weights) : kernelKey(LAYER_NORM, p, weights, s.vec, s.lanes, s.entries),
+                [&] { return isLong ? "LayerNormLongKernel" + types() + ">" : "LayerNormKernel" + types() + ", " + s.arguments() + ">"; })
         .call(isLong ? workgroups(rows, 512) : workgroups(divUp<int64_t>(rows, s.rows()), s.lanes == 1024 ? 512 : 2048),
               isLong ? LAYER_NORM_LONG_THREADS : s.threads(), 0, stream, x, strideX, w, b, epsilon, output.rawPtr(), strideY, ptr<float>(mean),
               ptr<float>(rstd), rows, C);
@@ -586,7 +607,7 @@ void Tokens::layerNormAdjoint(const Tensor& input, const Tensor& weight, const T
     checkMemory(memory, bytes);
     float* partial = sums ? static_cast<float*>(memory) : nullptr;
     const LayerNormShape s = layerNormShape(C, p);
-    const std::string types = valueTypes(p, weights);
+    auto types = [&] { return "<" + valueTypes(p, weights); };
     int count = 0;
     if (rows > 0) {
         const unsigned groups = layerNormAdjointWorkgroups(rows, s);
@@ -596,19 +617,20 @@ void Tokens::layerNormAdjoint(const Tensor& input, const Tensor& weight, const T
         const long long strideX = strideOf(input, 0), strideDy = strideOf(adjOutput, 0), strideDx = adjInput.defined() ? strideOf(adjInput, 0) : 0;
         void* dx = ptr<void>(adjInput);
         if (s.lanes > 0) {
-            tokenKernel("layer_norm.h", "LayerNormAdjointKernel<" + types + ", " + s.arguments() + ">")
+            tokenKernel("layer_norm.h", kernelKey(LAYER_NORM_ADJOINT, p, weights, s.vec, s.lanes, s.entries),
+                        [&] { return "LayerNormAdjointKernel" + types() + ", " + s.arguments() + ">"; })
                 .call(groups, s.threads(), 0, stream, x, strideX, w, m, r, dy, strideDy, dx, strideDx, partial, rows, C);
         } else {
             if (dx)
-                tokenKernel("layer_norm.h", "LayerNormLongAdjointKernel<" + types + ">")
+                tokenKernel("layer_norm.h", kernelKey(LAYER_NORM_LONG_ADJOINT, p, weights), [&] { return "LayerNormLongAdjointKernel" + types() + ">"; })
                     .call(workgroups(rows, 512), LAYER_NORM_LONG_THREADS, 0, stream, x, strideX, w, m, r, dy, strideDy, dx, strideDx, rows, C);
             if (sums)
-                tokenKernel("layer_norm.h", std::string("LayerNormLongSumsKernel<") + scalarName(p) + ">")
+                tokenKernel("layer_norm.h", kernelKey(LAYER_NORM_LONG_SUMS, p), [&] { return str("LayerNormLongSumsKernel<", scalarName(p), ">"); })
                     .call(groups * static_cast<unsigned>(divUp(C, 256)), 256, 0, stream, x, strideX, m, r, dy, strideDy, partial, rows, C, count);
         }
     }
     if (sums)
-        tokenKernel("layer_norm.h", std::string("LayerNormSumKernel<") + scalarName(weights) + ">")
+        tokenKernel("layer_norm.h", kernelKey(LAYER_NORM_SUM, weights), [&] { return str("LayerNormSumKernel<", scalarName(weights), ">"); })
             .call(static_cast<unsigned>(divUp<int64_t>(2ll * C, LAYER_NORM_SUM_COLUMNS)), LAYER_NORM_SUM_THREADS, 0, stream, static_cast<const float*>(partial), count, C,
                   ptr<void>(adjWeight), ptr<void>(adjBias));
 }
@@ -675,7 +697,8 @@ void Tokens::groupedLinearAdjoint(const Tensor& input, const Tensor& weight, con
     const int64_t groups = plan.places * plan.tilesI * plan.tilesJ;
     checkLaunch(groups, plan.tiles.threads());
     const int chunk = static_cast<int>(plan.chunk);
-    tokenKernel("grouped_linear.h", str("GroupedWeightsKernel<", scalarName(p), ", ", boolName(direct), ", ", plan.tiles.arguments(), ">"))
+    tokenKernel("grouped_linear.h", kernelKey(GROUPED_WEIGHTS, p * 2 + direct, plan.tiles.i, plan.tiles.j, plan.tiles.wavesI, plan.tiles.wavesJ),
+                [&] { return str("GroupedWeightsKernel<", scalarName(p), ", ", boolName(direct), ", ", plan.tiles.arguments(), ">"); })
         .call(static_cast<unsigned>(groups), plan.tiles.threads(), plan.tiles.lds(), stream, dy, strideOf(adjOutput, 0), x, strideOf(input, 0), off, s.experts,
               ptr<void>(adjWeight), ptr<void>(adjBias), plan.partial, s.rows, s.outputs, s.inputs,
               static_cast<int>(plan.places), static_cast<int>(plan.tilesI), static_cast<int>(plan.tilesJ), chunk);
@@ -683,7 +706,7 @@ void Tokens::groupedLinearAdjoint(const Tensor& input, const Tensor& weight, con
         const long long size = static_cast<long long>(s.inputs) * s.outputs;
         const int64_t pieces = divUp<int64_t>(size + s.outputs, 256);
         checkLaunch(pieces * s.experts, 256);
-        tokenKernel("grouped_linear.h", str("GroupedSumKernel<", scalarName(p), ">"))
+        tokenKernel("grouped_linear.h", kernelKey(GROUPED_SUM, p), [&] { return str("GroupedSumKernel<", scalarName(p), ">"); })
             .call(static_cast<unsigned>(pieces * s.experts), 256, 0, stream, static_cast<const float*>(plan.partial), off, ptr<void>(adjWeight),
                   ptr<void>(adjBias), s.rows, size, s.outputs, chunk, static_cast<int>(pieces));
     }
