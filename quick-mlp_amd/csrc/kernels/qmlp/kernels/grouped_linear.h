@@ -11,7 +11,7 @@
 // How many rows an expert has is known on the device only. The rows of the experts are cut into tiles that begin where the
 // expert does, and the places of the tiles follow without a scan: expert e has the places from e + floor(offsets[e] / TI) on,
 // of which it has always enough, as floor(b / T) - floor(a / T) + 1 >= ceil((b - a) / T). A workgroup finds the expert of its
-// place by a search of 64 steps at a time, and has nothing to do where the expert has fewer tiles than places.
+// place among the offsets, 64 or all of them at a time, and has nothing to do where the expert has fewer tiles than places.
 //
 // Offsets are limited to the rows there are wherever they are read: no access depends on their values.
 
@@ -236,26 +236,28 @@ struct TileProduct
     {
         clear();
         const long long advanceA = A_ALONG_K ? TILE_K<T> : TILE_K<T> * strideA, advanceB = B_ALONG_K ? TILE_K<T> : TILE_K<T> * strideB;
-        TileA tileA;
-        TileB tileB;
-        int buffer = 0;
-        tileA.read(a, strideA, ni, min(K, TILE_K<T>));
-        tileB.read(b, strideB, nj, min(K, TILE_K<T>));
-        for (int k = 0; k < K; k += TILE_K<T>) {
-            T* const ldsA = reinterpret_cast<T*>(lds + buffer * (TileA::BYTES + TileB::BYTES));
-            T* const ldsB = reinterpret_cast<T*>(lds + buffer * (TileA::BYTES + TileB::BYTES) + TileA::BYTES);
-            tileA.write(ldsA);
-            tileB.write(ldsB);
+        TileA tileA[2];   // two tiles in flight: one is less than the latency of the memory where a workgroup has its compute unit to itself
+        TileB tileB[2];
+        auto read = [&](int n, int left) {
+            tileA[n].read(a, strideA, ni, min(left, TILE_K<T>));
+            tileB[n].read(b, strideB, nj, min(left, TILE_K<T>));
+            a += advanceA;
+            b += advanceB;
+        };
+        auto step = [&](int n, int left) {   // left: from this tile on
+            T* const ldsA = reinterpret_cast<T*>(lds + n * (TileA::BYTES + TileB::BYTES));
+            T* const ldsB = reinterpret_cast<T*>(lds + n * (TileA::BYTES + TileB::BYTES) + TileA::BYTES);
+            tileA[n].write(ldsA);
+            tileB[n].write(ldsB);
             __syncthreads();   // (and the other buffer's readers of the step before are done)
-            if (k + TILE_K<T> < K) {
-                a += advanceA;
-                b += advanceB;
-                const int left = min(K - k - TILE_K<T>, TILE_K<T>);
-                tileA.read(a, strideA, ni, left);
-                tileB.read(b, strideB, nj, left);
-            }
+            if (left > 2 * TILE_K<T>) read(n, left - 2 * TILE_K<T>);
             multiplyTile(ldsA, ldsB, sumA);
-            buffer ^= 1;
+        };
+        if (K > 0) read(0, K);
+        if (K > TILE_K<T>) read(1, K - TILE_K<T>);
+        for (int k = 0; k < K; k += 2 * TILE_K<T>) {
+            step(0, K - k);
+            if (K - k > TILE_K<T>) step(1, K - k - TILE_K<T>);
         }
     }
 
@@ -523,16 +525,24 @@ struct ExpertTile
 __device__ __forceinline__ ExpertTile expertTile(const int* __restrict__ offsets, int experts, int rows, int tileRows, int place)
 {
     // the last e of 0 .. experts with e + floor(begin / tileRows) <= place; the first one has that
-    int from = 0, count = experts + 1;
-    while (count > 1) {
-        const int step = (count + 63) / 64;
-        const int e = from + min(static_cast<int>(threadIdx.x % 64) * step, count - 1);
-        const unsigned long long votes = __ballot(e + expertBegin(offsets, e, rows) / tileRows <= place);
-        // (the first lane votes yes: e = from; where the offsets are in order, so do the lanes up to the one looked for)
-        const int lane = max(0, 63 - __clzll(votes));
-        const int chosen = min(lane * step, count - 1);
-        from += chosen;
-        count = min(step, count - chosen);
+    auto reached = [&](int e) { return __ballot(e <= experts && e + expertBegin(offsets, min(e, experts), rows) / tileRows <= place); };
+    const int lane = threadIdx.x % 64;
+    int from = 0;
+    if (experts < 8 * 64) {   // all of them at once
+        int count = 0;
+#pragma unroll
+        for (int n = 0; n < 8; ++n) count += __popcll(reached(n * 64 + lane));
+        from = min(max(count - 1, 0), experts);
+    } else {
+        int count = experts + 1;
+        while (count > 1) {
+            const int step = (count + 63) / 64;
+            // (the first lane has reached its own; where the offsets are in order, so have the lanes up to the one looked for)
+            const int last = max(0, 63 - __clzll(reached(from + min(lane * step, count - 1))));
+            const int chosen = min(last * step, count - 1);
+            from += chosen;
+            count = min(step, count - chosen);
+        }
     }
     from = __builtin_amdgcn_readfirstlane(from);
     const int begin = expertBegin(offsets, from, rows), end = from < experts ? expertBegin(offsets, from + 1, rows) : rows;

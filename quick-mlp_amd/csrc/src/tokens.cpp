@@ -334,15 +334,33 @@ struct GroupedTiles
 {
     int i, j, wavesI, wavesJ;
     int threads() const { return 64 * wavesI * wavesJ; }
-    unsigned lds() const { return 2 * 128 * (i + j); }
+    /** Two tiles of each operand (one, where that is all there is of K), later the results. */
+    unsigned lds(int64_t K, int entry) const { return static_cast<unsigned>(std::max((K * entry <= 128 ? 1 : 2) * 128 * (i + j), i * j * entry)); }
     std::string arguments() const { return str(i, ", ", j, ", ", wavesI, ", ", wavesJ); }
 };
-constexpr GroupedTiles HUGE_TILES = {256, 256, 2, 4}, LARGE_TILES = {128, 128, 2, 2}, SMALL_TILES = {64, 64, 2, 2};
+constexpr GroupedTiles HUGE_TILES = {256, 256, 2, 4}, TALL_TILES = {256, 64, 4, 1}, LARGE_TILES = {128, 128, 2, 2}, SMALL_TILES = {64, 64, 2, 2};
+const std::array<GroupedTiles, 4> GROUPED_TILES = {HUGE_TILES, TALL_TILES, LARGE_TILES, SMALL_TILES};
+// Fewer tiles than that leave compute units without work: smaller ones, then.
+constexpr int64_t ENOUGH_HUGE = 192, ENOUGH_TILES = 256;
 
-GroupedTiles tilesFor(int64_t i, int64_t j, bool direct)
+/** Tiles of GroupedRowsKernel for (rows, J). */
+GroupedTiles rowsTiles(int64_t rows, int64_t experts, int64_t J, bool direct)
 {
-    if (i <= 64 || j <= 64) return SMALL_TILES;
-    return direct && i > 128 && j > 128 ? HUGE_TILES : LARGE_TILES;
+    const int64_t each = rows / std::max<int64_t>(experts, 1);
+    auto count = [&](const GroupedTiles& t) { return (rows / t.i + experts) * divUp<int64_t>(J, t.j); };
+    if (direct && each > 128 && J > 128 && count(HUGE_TILES) >= ENOUGH_HUGE) return HUGE_TILES;
+    if (each >= 128 && J <= 64 && count(TALL_TILES) >= ENOUGH_TILES) return TALL_TILES;
+    if (each > 64 && J > 64 && count(LARGE_TILES) >= ENOUGH_TILES) return LARGE_TILES;
+    return SMALL_TILES;
+}
+/** Tiles of GroupedWeightsKernel for experts of (I, J); an expert's rows may be shared out, in chunks that are worth it. */
+GroupedTiles weightsTiles(int64_t rows, int64_t experts, int64_t I, int64_t J, bool direct)
+{
+    const int64_t each = divUp(rows, experts);
+    auto count = [&](const GroupedTiles& t, int64_t chunk) { return experts * divUp<int64_t>(I, t.i) * divUp<int64_t>(J, t.j) * std::max<int64_t>(1, each / chunk); };
+    if (direct && I > 128 && J > 128 && count(HUGE_TILES, 512) >= ENOUGH_HUGE) return HUGE_TILES;
+    if (I > 64 && J > 64 && count(LARGE_TILES, 256) >= ENOUGH_TILES) return LARGE_TILES;
+    return SMALL_TILES;
 }
 
 /** Whether tiles of the operand can go straight from global memory to LDS (DirectTile). */
@@ -362,12 +380,11 @@ const char* boolName(bool b) { return b ? "true" : "false"; }
 int64_t tilePlaces(int64_t rows, int64_t experts, int64_t tileRows) { return rows / tileRows + experts + 1; }
 
 /** Rows of a chunk of GroupedWeightsKernel: several chunks per expert where its tiles alone are too few for the chip. */
-int64_t weightsChunk(int64_t rows, int64_t experts, int64_t tiles)
+int64_t weightsChunk(int64_t rows, int64_t experts, int64_t tiles, int tile)
 {
-    constexpr int64_t WORKGROUPS = 1024, SHORTEST = 512;
-    const int64_t chunks = divUp<int64_t>(WORKGROUPS, std::max<int64_t>(1, experts * tiles));   // per expert
+    const int64_t chunks = divUp<int64_t>(512, std::max<int64_t>(1, experts * tiles));   // per expert
     if (chunks <= 1) return std::max<int64_t>(rows, 1);
-    return std::max(SHORTEST, roundUp<int64_t>(divUp<int64_t>(rows, experts * chunks), 64));
+    return std::max<int64_t>(2 * tile, roundUp<int64_t>(divUp<int64_t>(rows, experts * chunks), 64));
 }
 
 struct GroupedAdjointPlan
@@ -378,10 +395,10 @@ struct GroupedAdjointPlan
     float* partial = nullptr;
     GroupedAdjointPlan(int64_t rows, int64_t experts, int64_t inputs, int64_t outputs, bool direct, void* base) : memory{static_cast<char*>(base)}
     {
-        tiles = tilesFor(outputs, inputs, direct);
+        tiles = weightsTiles(rows, experts, outputs, inputs, direct);
         tilesI = divUp<int64_t>(outputs, tiles.i);
         tilesJ = divUp<int64_t>(inputs, tiles.j);
-        chunk = weightsChunk(rows, experts, tilesI * tilesJ);
+        chunk = weightsChunk(rows, experts, tilesI * tilesJ, tiles.i);
         places = rows / chunk + experts;
         if (chunk < rows) partial = memory.take<float>(places * (outputs * inputs + outputs));
     }
@@ -416,13 +433,13 @@ void launchRows(bool alongK, const Tensor& x, const Tensor& weight, const Tensor
                 int J, int K, stream_t stream)
 {
     const bool direct = isDirect(x) && isDirect(weight);
-    const GroupedTiles t = tilesFor(s.rows / std::max(s.experts, 1), J, direct);
+    const GroupedTiles t = rowsTiles(s.rows, s.experts, J, direct);
     const int tilesJ = divUp(J, t.j);
     const int64_t places = tilePlaces(s.rows, s.experts, t.i);
     checkLaunch(places * tilesJ, t.threads());
     tokenKernel("grouped_linear.h", kernelKey(GROUPED_ROWS, x.precision() * 4 + direct * 2 + alongK, t.i, t.j, t.wavesI, t.wavesJ),
                 [&] { return str("GroupedRowsKernel<", scalarName(x.precision()), ", ", boolName(direct), ", ", boolName(alongK), ", ", t.arguments(), ">"); })
-        .call(static_cast<unsigned>(places * tilesJ), t.threads(), t.lds(), stream, x.rawPtr(), strideOf(x, 0), static_cast<const void*>(ptr<void>(weight)),
+        .call(static_cast<unsigned>(places * tilesJ), t.threads(), t.lds(K, x.bytesPerEntry()), stream, x.rawPtr(), strideOf(x, 0), static_cast<const void*>(ptr<void>(weight)),
               strideOf(weight, 0), strideOf(weight, 1), static_cast<const void*>(ptr<void>(bias)), bias.defined() ? strideOf(bias, 0) : 0ll,
               static_cast<const int*>(ptr<int>(offsets)), s.experts, static_cast<void*>(ptr<void>(y)), strideOf(y, 0), s.rows, J, K, static_cast<int>(places),
               tilesJ);
@@ -699,7 +716,7 @@ void Tokens::groupedLinearAdjoint(const Tensor& input, const Tensor& weight, con
     const int chunk = static_cast<int>(plan.chunk);
     tokenKernel("grouped_linear.h", kernelKey(GROUPED_WEIGHTS, p * 2 + direct, plan.tiles.i, plan.tiles.j, plan.tiles.wavesI, plan.tiles.wavesJ),
                 [&] { return str("GroupedWeightsKernel<", scalarName(p), ", ", boolName(direct), ", ", plan.tiles.arguments(), ">"); })
-        .call(static_cast<unsigned>(groups), plan.tiles.threads(), plan.tiles.lds(), stream, dy, strideOf(adjOutput, 0), x, strideOf(input, 0), off, s.experts,
+        .call(static_cast<unsigned>(groups), plan.tiles.threads(), plan.tiles.lds(s.rows, input.bytesPerEntry()), stream, dy, strideOf(adjOutput, 0), x, strideOf(input, 0), off, s.experts,
               ptr<void>(adjWeight), ptr<void>(adjBias), plan.partial, s.rows, s.outputs, s.inputs,
               static_cast<int>(plan.places), static_cast<int>(plan.tilesI), static_cast<int>(plan.tilesJ), chunk);
     if (plan.partial) {
@@ -741,11 +758,11 @@ void Tokens::precompile(Tensor::Precision p)
     for (const char* kernel : {"LayerNormLongKernel", "LayerNormLongAdjointKernel"}) precompileKernel("layer_norm.h", str(kernel, "<", t, ", ", t, ">"));
     for (const char* kernel : {"LayerNormLongSumsKernel", "LayerNormSumKernel"}) precompileKernel("layer_norm.h", str(kernel, "<", t, ">"));
     for (const bool direct : {false, true})
-        for (const GroupedTiles& tiles : {HUGE_TILES, LARGE_TILES, SMALL_TILES}) {
-            if (direct ? p == Tensor::FLOAT : tiles.i > 128) continue;
+        for (const GroupedTiles& tiles : GROUPED_TILES) {
+            if (direct ? p == Tensor::FLOAT : tiles.i == HUGE_TILES.i && tiles.j == HUGE_TILES.j) continue;
             const std::string types = str(t, ", ", boolName(direct));
             for (const char* along : {", true, ", ", false, "}) precompileKernel("grouped_linear.h", str("GroupedRowsKernel<", types, along, tiles.arguments(), ">"));
-            precompileKernel("grouped_linear.h", str("GroupedWeightsKernel<", types, ", ", tiles.arguments(), ">"));
+            if (tiles.i == tiles.j) precompileKernel("grouped_linear.h", str("GroupedWeightsKernel<", types, ", ", tiles.arguments(), ">"));
         }
     precompileKernel("grouped_linear.h", str("GroupedSumKernel<", t, ">"));
 }
