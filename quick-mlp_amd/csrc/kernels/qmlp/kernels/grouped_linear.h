@@ -20,6 +20,7 @@
 QUICKMLP_KERNEL_NAMESPACE_BEGIN
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
@@ -78,10 +79,9 @@ template <typename T>
 constexpr int STEP_K = 2 * WIDE<T>;
 
 /**
- * A tile of an operand: SIZE of its indices by TILE_K. ALONG_K: rows of 128 bytes, one for each index; otherwise one row for each k.
- * It goes from global memory through the registers of all THREADS, 16 bytes at a time, whatever the alignment.
- * Pieces of a row lie in an order that depends on the row, so that the lanes that read the same piece of different rows find
- * them in different banks.
+ * A tile of an operand in LDS: SIZE of its indices by TILE_K. ALONG_K: rows of 128 bytes, one for each index; otherwise one row for
+ * each k. THREADS move it 16 bytes at a time, in EACH turns. Pieces of a row lie in an order that depends on the row, so that the
+ * lanes that read the same piece of different rows find them in different banks.
  */
 template <typename T, bool ALONG_K, int SIZE, int THREADS>
 struct Tile
@@ -93,8 +93,6 @@ struct Tile
     static constexpr int BYTES = SIZE * 128;
     static_assert(SIZE * 8 % THREADS == 0, "every thread moves the same number of pieces");
 
-    T raw[EACH][PIECE];
-
     /** Place of an entry of the tile. */
     static __device__ __forceinline__ int place(int row, int column)
     {
@@ -105,38 +103,6 @@ struct Tile
             return row * ROW + (((column / 32) ^ (row & (UNITS < 4 ? UNITS - 1 : 3))) * 32 + column % 32);
         } else
             return row * ROW + column;
-    }
-
-    /**
-     * Reads the tile whose first index and k are at 'p': 'indices' and 'ks' of them are there (no more than the tile's), the
-     * others are zero. stride: between rows.
-     */
-    __device__ __forceinline__ void read(const T* __restrict__ p, long long stride, int indices, int ks)
-    {
-        const int rows = ALONG_K ? indices : ks, columns = ALONG_K ? ks : indices;
-#pragma unroll
-        for (int n = 0; n < EACH; ++n) {
-            const int piece = n * THREADS + threadIdx.x;
-            const int row = piece / PIECES, column = piece % PIECES * PIECE;
-#pragma unroll
-            for (int k = 0; k < PIECE; ++k) raw[n][k] = static_cast<T>(0);
-            if (row >= rows) continue;
-            const T* from = p + row * stride + column;
-            if (column + PIECE <= columns) __builtin_memcpy(raw[n], from, 16);
-            else {
-#pragma unroll
-                for (int k = 0; k < PIECE; ++k)
-                    if (column + k < columns) raw[n][k] = from[k];
-            }
-        }
-    }
-    __device__ __forceinline__ void write(T* lds) const
-    {
-#pragma unroll
-        for (int n = 0; n < EACH; ++n) {
-            const int piece = n * THREADS + threadIdx.x;
-            __builtin_memcpy(__builtin_assume_aligned(lds + place(piece / PIECES, piece % PIECES * PIECE), 16), raw[n], 16);
-        }
     }
 
     /** The operand of the matrix cores for 32 indices from i on and the given step of the tile's k. */
@@ -161,18 +127,205 @@ struct Tile
     }
 };
 
+/** An operand of a tile of results: at its first index and k = 0. */
+template <typename T>
+struct Source
+{
+    const T* p;
+    long long stride;   // between rows
+    int indices;        // that the tile of results has of it
+    int rows;           // of the matrix from p on
+};
+
+/**
+ * Moves the tiles of an operand of any address and size through registers; its rows are less than 2^21 entries apart. Indices that are not there hold anything, which no result
+ * depends on; k that are not there are zero.
+ */
+template <typename T, bool ALONG_K, int SIZE, int THREADS>
+struct RegisterTile
+{
+    typedef Tile<T, ALONG_K, SIZE, THREADS> Layout;
+    static constexpr int PIECE = Layout::PIECE, PIECES = Layout::PIECES, EACH = Layout::EACH;
+    // A thread's pieces lie in one column of pieces, 'TURN' rows apart.
+    static constexpr int TURN = THREADS / PIECES;
+    static_assert(THREADS % PIECES == 0, "a column of pieces per thread");
+    const T* p;    // the next tile
+    const T* at;   // the tile that is being read
+    long long stride;
+    unsigned first, turn;   // bytes from a tile to the thread's first piece, and from one to its next
+    int indices, ks, safe, nextSafe;
+    u32x4 raw[EACH];
+
+    static __device__ __forceinline__ int row() { return threadIdx.x / PIECES; }
+    static __device__ __forceinline__ int column() { return threadIdx.x % PIECES * PIECE; }
+    __device__ __forceinline__ void begin(const Source<T>& s)
+    {
+        stride = s.stride;
+        indices = s.indices;
+        p = s.p;
+        first = static_cast<unsigned>((row() * stride + column()) * sizeof(T));
+        turn = static_cast<unsigned>(TURN * stride * sizeof(T));
+        // rows whose last piece may be read as a whole: behind it begins the next row
+        nextSafe = s.stride >= PIECE ? s.rows - 1 : 0;
+    }
+    /** Turns to the tile of the 'ks' next values of k, which the calls of load(0) to load(EACH - 1) read. */
+    __device__ __forceinline__ void next(unsigned, int ks_)
+    {
+        ks = ks_;
+        at = p;
+        safe = nextSafe;
+        p += ALONG_K ? TILE_K<T> : TILE_K<T> * stride;
+        if (!ALONG_K) nextSafe -= TILE_K<T>;
+    }
+    /** (One load or none into registers that are zero before: anything more would make the compiler wait for it here.) */
+    __device__ __forceinline__ void load(int n)
+    {
+        const int rows = ALONG_K ? indices : ks, columns = ALONG_K ? ks : indices;
+        // pieces that end with their row or before it, and others that something lies behind
+        const int upTo = column() + PIECE <= columns ? rows : column() < columns ? min(rows, safe) : 0;
+        raw[n] = u32x4{0, 0, 0, 0};
+        if (row() < upTo - n * TURN) __builtin_memcpy(&raw[n], piece(n), 16);
+    }
+    __device__ __forceinline__ const T* piece(int n) const
+    {
+        return reinterpret_cast<const T*>(reinterpret_cast<const char*>(at) + (first + n * turn));
+    }
+    /** Writes the tile, with what load() left to do: pieces that end behind the last column. */
+    __device__ __forceinline__ void write(T* lds)
+    {
+        const int rows = ALONG_K ? indices : ks, columns = ALONG_K ? ks : indices;
+        if (columns < Layout::ROW && column() < columns && column() + PIECE > columns) {
+            constexpr int WORD = 4 / static_cast<int>(sizeof(T));   // entries of 32 bits
+#pragma unroll
+            for (int n = 0; n < EACH; ++n) {
+                if (row() + n * TURN >= rows) continue;
+                if (row() + n * TURN >= safe) {
+                    const T* from = piece(n);
+#pragma unroll
+                    for (int k = 0; k < PIECE; ++k)
+                        if (column() + k < columns) {
+                            if constexpr (sizeof(T) == 2) raw[n][k / 2] |= static_cast<unsigned>(__builtin_bit_cast(unsigned short, from[k])) << (k % 2 * 16);
+                            else raw[n][k] = __builtin_bit_cast(unsigned, from[k]);
+                        }
+                } else
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const int left = columns - column() - k * WORD;
+                        raw[n][k] = left >= WORD ? raw[n][k] : left > 0 ? raw[n][k] & 0xffffu : 0u;
+                    }
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < EACH; ++n)
+            __builtin_memcpy(__builtin_assume_aligned(lds + Layout::place(row() + n * TURN, column()), 16), &raw[n], 16);
+    }
+};
+
+/** A buffer descriptor for raw accesses of 'bytes' bytes at p; reads behind them give zeros. */
+__device__ __forceinline__ u32x4 bufferAt(const void* p, unsigned bytes)
+{
+    const unsigned long long a = reinterpret_cast<unsigned long long>(p);
+    return u32x4{static_cast<unsigned>(__builtin_amdgcn_readfirstlane(static_cast<int>(a))),
+                 static_cast<unsigned>(__builtin_amdgcn_readfirstlane(static_cast<int>(a >> 32))) & 0xffffu,
+                 static_cast<unsigned>(__builtin_amdgcn_readfirstlane(static_cast<int>(bytes))), 0x00020000u};
+}
+/**
+ * Every lane moves 16 bytes from its offset into the buffer to LDS, those of the wavefront side by side from 'lds' on. As a builtin the
+ * compiler would wait for it in front of every later read of LDS; this way it is waited for by waitForTiles() alone. (The wait states: a
+ * descriptor in scalar registers that vector instructions wrote may be read five later.)
+ */
+__device__ __forceinline__ void loadToLds(u32x4 buffer, unsigned offset, unsigned lds)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(buffer) : "memory");
+}
+/** The wavefront's writes to and reads of LDS are done, and so are those of the others. */
+__device__ __forceinline__ void waitForLds()
+{
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+/** All but the last 'pending' of the wavefront's loads to LDS have arrived, its reads of LDS are done, and so are those of the others. */
+template <int PENDING>
+__device__ __forceinline__ void waitForTiles()
+{
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(PENDING) : "memory");
+}
+
+/**
+ * Moves the tiles of an operand of 16 bits straight from global memory to LDS. The address, the strides and the operand's sizes are
+ * multiples of 16 bytes, and rows do not overlap. Indices that are not there hold others' values, which no result depends on;
+ * k that are not there are zero.
+ */
+template <typename T, bool ALONG_K, int SIZE, int THREADS>
+struct DirectTile
+{
+    typedef Tile<T, ALONG_K, SIZE, THREADS> Layout;
+    static constexpr int PIECES = Layout::PIECES, EACH = Layout::EACH;
+    const T* p;
+    long long stride;
+    int indices;
+    unsigned offsets[EACH];
+    int columns[EACH];   // along k: the first k of a piece
+
+    __device__ __forceinline__ void begin(const Source<T>& s)
+    {
+        p = s.p;
+        stride = s.stride;
+        indices = s.indices;
+#pragma unroll
+        for (int n = 0; n < EACH; ++n) {
+            const int piece = n * THREADS + threadIdx.x;
+            const int row = piece / PIECES;
+            // which piece belongs here is what Layout::place() says of the piece there: exchanging is its own inverse
+            const int column = Layout::place(row, piece % PIECES * WIDE<T>) - row * Layout::ROW;
+            columns[n] = column;
+            // (rows behind the last index are read from the last one; columns behind it lie in the next row, or behind the buffer)
+            offsets[n] = static_cast<unsigned>(((ALONG_K ? min(row, indices - 1) : row) * stride + column) * sizeof(T));
+        }
+    }
+    u32x4 buffer;
+    unsigned to;
+    int ks;
+    /** Turns to the tile of the 'ks' next values of k, which goes to LDS from 'lds' on with the calls of load(0) to load(EACH - 1). */
+    __device__ __forceinline__ void next(unsigned lds, int ks_)
+    {
+        ks = ks_;
+        buffer = bufferAt(p, static_cast<unsigned>(((ALONG_K ? indices - 1 : ks - 1) * stride + (ALONG_K ? ks : indices)) * sizeof(T)));
+        to = __builtin_amdgcn_readfirstlane(lds + threadIdx.x / 64 * 1024);
+        p += ALONG_K ? TILE_K<T> : TILE_K<T> * stride;
+    }
+    __device__ __forceinline__ void load(int n) const
+    {
+        loadToLds(buffer, !ALONG_K || columns[n] < ks ? offsets[n] : 0x80000000u, to + n * THREADS * 16);
+    }
+};
+
+/** How tiles are moved. */
+template <bool DIRECT, typename T, bool ALONG_K, int SIZE, int THREADS>
+struct Loads
+{
+    typedef RegisterTile<T, ALONG_K, SIZE, THREADS> Type;
+};
+template <typename T, bool ALONG_K, int SIZE, int THREADS>
+struct Loads<true, T, ALONG_K, SIZE, THREADS>
+{
+    typedef DirectTile<T, ALONG_K, SIZE, THREADS> Type;
+};
+
 /**
  * The sums of a tile of TI x TJ by WI x WJ wavefronts. In an accumulator, lane l holds C(i, j) of i = l % 32 and
  * j = 8 (n / 4) + 4 (l / 32) + n % 4 for n = 0 .. 15: four consecutive j at a time.
+ *
+ * Tiles are asked for two ahead of the matrix cores, DIRECT ones straight to LDS. Operands are read from LDS a step ahead, also from
+ * one tile to the next: the barrier between two tiles stands before the last step of the first, whose operands every wavefront has by
+ * then.
  */
-template <typename T, bool A_ALONG_K, bool B_ALONG_K, int TI, int TJ, int WI, int WJ>
+template <bool DIRECT, typename T, bool A_ALONG_K, bool B_ALONG_K, int TI, int TJ, int WI, int WJ>
 struct TileProduct
 {
     static constexpr int THREADS = 64 * WI * WJ;
     static constexpr int NI = TI / WI / 32, NJ = TJ / WJ / 32;
     typedef Tile<T, A_ALONG_K, TI, THREADS> TileA;
     typedef Tile<T, B_ALONG_K, TJ, THREADS> TileB;
-    static constexpr int LDS_BYTES = 2 * (TileA::BYTES + TileB::BYTES);
 
     f32x16 sums[NI][NJ];
     float sumsOfA[NI];   // over k alone, of index l % 32; lanes l and l ^ 32 have half of the k each
@@ -180,15 +333,6 @@ struct TileProduct
     static __device__ __forceinline__ int firstI() { return threadIdx.x / 64 / WJ * (NI * 32); }
     static __device__ __forceinline__ int firstJ() { return threadIdx.x / 64 % WJ * (NJ * 32); }
 
-    __device__ __forceinline__ void clear()
-    {
-#pragma unroll
-        for (int i = 0; i < NI; ++i) {
-            sumsOfA[i] = 0;
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) sums[i][j] = f32x16{};
-        }
-    }
     /** What a wavefront multiplies in one step of a tile's k. */
     struct Operands
     {
@@ -219,45 +363,92 @@ struct TileProduct
 #pragma unroll
                 for (int n = 0; n < WIDE<T>; ++n) sumsOfA[i] += static_cast<float>(o.a[i][n]);
     }
-    /** Adds the products of tiles in LDS. */
-    __device__ __forceinline__ void multiplyTile(const T* ldsA, const T* ldsB, bool sumA)
+
+    /** sumA: also sums A over k. */
+    __device__ __forceinline__ void run(char* lds, const Source<T>& a, const Source<T>& b, int K, bool sumA)
     {
 #pragma unroll
-        for (int step = 0; step < STEPS; ++step) {
-            Operands o;
-            readStep(o, ldsA, ldsB, step);
-            multiplyStep(o, sumA, [](int) {});
+        for (int i = 0; i < NI; ++i) {
+            sumsOfA[i] = 0;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) sums[i][j] = f32x16{};
         }
-    }
-
-    /** a, b: at the tile's first index and k = 0; ni, nj: indices that are there. sumA: also sums A over k. */
-    __device__ __forceinline__ void run(char* lds, const T* __restrict__ a, long long strideA, int ni, const T* __restrict__ b, long long strideB,
-                                        int nj, int K, bool sumA)
-    {
-        clear();
-        const long long advanceA = A_ALONG_K ? TILE_K<T> : TILE_K<T> * strideA, advanceB = B_ALONG_K ? TILE_K<T> : TILE_K<T> * strideB;
-        TileA tileA[2];   // two tiles in flight: one is less than the latency of the memory where a workgroup has its compute unit to itself
-        TileB tileB[2];
-        auto read = [&](int n, int left) {
-            tileA[n].read(a, strideA, ni, min(left, TILE_K<T>));
-            tileB[n].read(b, strideB, nj, min(left, TILE_K<T>));
-            a += advanceA;
-            b += advanceB;
+        if (K <= 0) return;
+        typedef typename Loads<DIRECT, T, A_ALONG_K, TI, THREADS>::Type LoadsA;
+        typedef typename Loads<DIRECT, T, B_ALONG_K, TJ, THREADS>::Type LoadsB;
+        LoadsA tileA;
+        LoadsB tileB;
+        tileA.begin(a);
+        tileB.begin(b);
+        constexpr unsigned BYTES_A = TileA::BYTES, BYTES = BYTES_A + TileB::BYTES;
+        constexpr int LOADS = LoadsA::EACH + LoadsB::EACH, PRODUCTS = NI * NJ;
+        const unsigned at = static_cast<unsigned>(reinterpret_cast<unsigned long long>((__attribute__((address_space(3))) char*)lds));
+        int ahead = K;   // values of k that have not been asked for
+        auto ask = [&](unsigned buffer) {
+            const int ks = min(ahead, TILE_K<T>);   // (none left: 0)
+            ahead -= ks;
+            tileA.next(at + buffer, ks);
+            tileB.next(at + buffer + BYTES_A, ks);
         };
-        auto step = [&](int n, int left) {   // left: from this tile on
-            T* const ldsA = reinterpret_cast<T*>(lds + n * (TileA::BYTES + TileB::BYTES));
-            T* const ldsB = reinterpret_cast<T*>(lds + n * (TileA::BYTES + TileB::BYTES) + TileA::BYTES);
-            tileA[n].write(ldsA);
-            tileB[n].write(ldsB);
-            __syncthreads();   // (and the other buffer's readers of the step before are done)
-            if (left > 2 * TILE_K<T>) read(n, left - 2 * TILE_K<T>);
-            multiplyTile(ldsA, ldsB, sumA);
+        auto load = [&](int from, int to) {
+#pragma unroll
+            for (int n = from; n < to; ++n) {
+                if (n < LoadsA::EACH) tileA.load(n);
+                else tileB.load(n - LoadsA::EACH);
+            }
         };
-        if (K > 0) read(0, K);
-        if (K > TILE_K<T>) read(1, K - TILE_K<T>);
-        for (int k = 0; k < K; k += 2 * TILE_K<T>) {
-            step(0, K - k);
-            if (K - k > TILE_K<T>) step(1, K - k - TILE_K<T>);
+        auto write = [&](unsigned buffer) {
+            if constexpr (!DIRECT) {
+                tileA.write(reinterpret_cast<T*>(lds + buffer));
+                tileB.write(reinterpret_cast<T*>(lds + buffer + BYTES_A));
+            }
+        };
+        static_assert(STEPS % 2 == 0, "the operands of a tile's first step are the first ones");
+        Operands operands[2];   // of a step and of the one behind it
+        auto read = [&](Operands& o, unsigned buffer, int step) {
+            readStep(o, reinterpret_cast<const T*>(lds + buffer), reinterpret_cast<const T*>(lds + buffer + BYTES_A), step);
+            __builtin_amdgcn_sched_barrier(0);   // the compiler would move the reads to where they are used
+        };
+        ask(0);
+        load(0, LOADS);
+        write(0);
+        if constexpr (DIRECT) {
+            if (ahead > 0) {
+                ask(BYTES);
+                load(0, LOADS);
+                waitForTiles<LOADS>();
+            } else
+                waitForTiles<0>();
+        } else {
+            ask(BYTES);
+            load(0, LOADS);
+            waitForLds();
+        }
+        read(operands[0], 0, 0);
+        unsigned buffer = 0;
+        for (int k = 0; k < K; k += TILE_K<T>) {
+#pragma unroll
+            for (int step = 0; step + 1 < STEPS; ++step) {
+                read(operands[(step + 1) % 2], buffer, step + 1);
+                multiplyStep(operands[step % 2], sumA, [](int) {});
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            // Through registers a tile of no k is asked for and written where there is none: with branches around the loads the compiler
+            // would wait for each before the next.
+            const bool more = !DIRECT || ahead > 0, last = k + TILE_K<T> >= K;
+            if (!DIRECT || !last) {
+                write(buffer ^ BYTES);   // (the next tile; the barrier before saw the last readers of the one there)
+                if (more) ask(buffer);
+                buffer ^= BYTES;
+                if constexpr (DIRECT) waitForTiles<0>();
+                else waitForLds();
+            }
+            // Behind the barrier the matrix cores go on at once; what else there is to do stands between the products.
+            multiplyStep(operands[1], sumA, [&](int n) {
+                if (n == 0 && !last) read(operands[0], buffer, 0);
+                if (more) load(n * LOADS / PRODUCTS, (n + 1) * LOADS / PRODUCTS);
+                __builtin_amdgcn_sched_barrier(0);
+            });
         }
     }
 
@@ -331,169 +522,6 @@ __device__ __forceinline__ void storeTile(const Product& product, char* lds, con
                 if (j + k < nj) out[k] = raw[k];
     }
 }
-
-/** A buffer descriptor for raw accesses of 'bytes' bytes at p; reads behind them give zeros. */
-typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-__device__ __forceinline__ u32x4 bufferAt(const void* p, unsigned bytes)
-{
-    const unsigned long long a = reinterpret_cast<unsigned long long>(p);
-    return u32x4{static_cast<unsigned>(__builtin_amdgcn_readfirstlane(static_cast<int>(a))),
-                 static_cast<unsigned>(__builtin_amdgcn_readfirstlane(static_cast<int>(a >> 32))) & 0xffffu,
-                 static_cast<unsigned>(__builtin_amdgcn_readfirstlane(static_cast<int>(bytes))), 0x00020000u};
-}
-/**
- * Every lane moves 16 bytes from its offset into the buffer to LDS, those of the wavefront side by side from 'lds' on. As a builtin the
- * compiler would wait for it in front of every later read of LDS; this way it is waited for by waitForTiles() alone. (The wait states: a
- * descriptor in scalar registers that vector instructions wrote may be read five later.)
- */
-__device__ __forceinline__ void loadToLds(u32x4 buffer, unsigned offset, unsigned lds)
-{
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(buffer) : "memory");
-}
-/** All but the last 'pending' of the wavefront's loads to LDS have arrived, its reads of LDS are done, and so are those of the others. */
-template <int PENDING>
-__device__ __forceinline__ void waitForTiles()
-{
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(PENDING) : "memory");
-}
-
-/**
- * Moves the tiles of an operand of 16 bits straight from global memory to LDS. The address, the strides and the operand's sizes are
- * multiples of 16 bytes, and rows do not overlap. Indices that are not there hold others' values, which no result depends on;
- * k that are not there are zero.
- */
-template <typename T, bool ALONG_K, int SIZE, int THREADS>
-struct DirectTile
-{
-    typedef Tile<T, ALONG_K, SIZE, THREADS> Layout;
-    static constexpr int PIECES = Layout::PIECES, EACH = Layout::EACH;
-    const T* p;
-    long long stride;
-    int indices;
-    unsigned offsets[EACH];
-    int columns[EACH];   // along k: the first k of a piece
-
-    __device__ __forceinline__ void begin(const T* p_, long long stride_, int indices_)
-    {
-        p = p_;
-        stride = stride_;
-        indices = indices_;
-#pragma unroll
-        for (int n = 0; n < EACH; ++n) {
-            const int piece = n * THREADS + threadIdx.x;
-            const int row = piece / PIECES;
-            // which piece belongs here is what Layout::place() says of the piece there: exchanging is its own inverse
-            const int column = Layout::place(row, piece % PIECES * WIDE<T>) - row * Layout::ROW;
-            columns[n] = column;
-            // (rows behind the last index are read from the last one; columns behind it lie in the next row, or behind the buffer)
-            offsets[n] = static_cast<unsigned>(((ALONG_K ? min(row, indices - 1) : row) * stride + column) * sizeof(T));
-        }
-    }
-    u32x4 buffer;
-    unsigned to;
-    int ks;
-    /** Turns to the tile of the 'ks' next values of k, which goes to LDS from 'lds' on with the calls of load(0) to load(EACH - 1). */
-    __device__ __forceinline__ void next(unsigned lds, int ks_)
-    {
-        ks = ks_;
-        buffer = bufferAt(p, static_cast<unsigned>(((ALONG_K ? indices - 1 : ks - 1) * stride + (ALONG_K ? ks : indices)) * sizeof(T)));
-        to = __builtin_amdgcn_readfirstlane(lds + threadIdx.x / 64 * 1024);
-        p += ALONG_K ? TILE_K<T> : TILE_K<T> * stride;
-    }
-    __device__ __forceinline__ void load(int n) const
-    {
-        loadToLds(buffer, !ALONG_K || columns[n] < ks ? offsets[n] : 0x80000000u, to + n * THREADS * 16);
-    }
-};
-
-/**
- * TileProduct whose tiles go to LDS without registers in between, two tiles ahead of the matrix cores. Operands are read from LDS
- * a step ahead, also from one tile to the next: the barrier between two tiles stands before the last step of the first, whose
- * operands every wavefront has by then.
- */
-template <typename T, bool A_ALONG_K, bool B_ALONG_K, int TI, int TJ, int WI, int WJ>
-struct DirectProduct : TileProduct<T, A_ALONG_K, B_ALONG_K, TI, TJ, WI, WJ>
-{
-    typedef TileProduct<T, A_ALONG_K, B_ALONG_K, TI, TJ, WI, WJ> Base;
-
-    __device__ __forceinline__ void run(char* lds, const T* __restrict__ a, long long strideA, int ni, const T* __restrict__ b, long long strideB,
-                                        int nj, int K, bool sumA)
-    {
-        this->clear();
-        if (K <= 0) return;
-        typedef DirectTile<T, A_ALONG_K, TI, Base::THREADS> LoadsA;
-        typedef DirectTile<T, B_ALONG_K, TJ, Base::THREADS> LoadsB;
-        LoadsA tileA;
-        LoadsB tileB;
-        tileA.begin(a, strideA, ni);
-        tileB.begin(b, strideB, nj);
-        constexpr unsigned BYTES_A = Base::TileA::BYTES, BYTES = BYTES_A + Base::TileB::BYTES;
-        const unsigned at = static_cast<unsigned>(reinterpret_cast<unsigned long long>((__attribute__((address_space(3))) char*)lds));
-        constexpr int LOADS = LoadsA::EACH + LoadsB::EACH, PRODUCTS = Base::NI * Base::NJ;
-        auto next = [&](unsigned buffer, int ks) {
-            tileA.next(at + buffer, ks);
-            tileB.next(at + buffer + BYTES_A, ks);
-        };
-        auto load = [&](int from, int to) {
-#pragma unroll
-            for (int n = from; n < to; ++n) {
-                if (n < LoadsA::EACH) tileA.load(n);
-                else tileB.load(n - LoadsA::EACH);
-            }
-        };
-        static_assert(Base::STEPS % 2 == 0, "the operands of a tile's first step are the first ones");
-        typename Base::Operands operands[2];   // of a step and of the one behind it
-        auto read = [&](typename Base::Operands& o, unsigned buffer, int step) {
-            Base::readStep(o, reinterpret_cast<const T*>(lds + buffer), reinterpret_cast<const T*>(lds + buffer + BYTES_A), step);
-            __builtin_amdgcn_sched_barrier(0);   // the compiler would move the reads to where they are used
-        };
-        int left = K - TILE_K<T>;   // behind the tiles asked for
-        next(0, min(K, TILE_K<T>));
-        load(0, LOADS);
-        if (left > 0) {
-            next(BYTES, min(left, TILE_K<T>));
-            load(0, LOADS);
-            waitForTiles<LOADS>();
-        } else
-            waitForTiles<0>();
-        left -= TILE_K<T>;
-        read(operands[0], 0, 0);
-        unsigned buffer = 0;
-        for (int k = 0; k < K; k += TILE_K<T>) {
-#pragma unroll
-            for (int step = 0; step + 1 < Base::STEPS; ++step) {
-                read(operands[(step + 1) % 2], buffer, step + 1);
-                this->multiplyStep(operands[step % 2], sumA, [](int) {});
-                __builtin_amdgcn_sched_barrier(0);
-            }
-            const bool more = left > 0, last = k + TILE_K<T> >= K;
-            if (!last) {
-                if (more) next(buffer, min(left, TILE_K<T>));
-                left -= TILE_K<T>;
-                buffer ^= BYTES;
-                waitForTiles<0>();
-            }
-            // Behind the barrier the matrix cores go on at once; what else there is to do stands between the products.
-            this->multiplyStep(operands[1], sumA, [&](int n) {
-                if (n == 0 && !last) read(operands[0], buffer, 0);
-                if (more) load(n * LOADS / PRODUCTS, (n + 1) * LOADS / PRODUCTS);
-                __builtin_amdgcn_sched_barrier(0);
-            });
-        }
-    }
-};
-
-/** The product of tiles of any address and size, or of those that can go straight to LDS. */
-template <bool DIRECT, typename T, bool A_ALONG_K, bool B_ALONG_K, int TI, int TJ, int WI, int WJ>
-struct ProductOf
-{
-    typedef TileProduct<T, A_ALONG_K, B_ALONG_K, TI, TJ, WI, WJ> Type;
-};
-template <typename T, bool A_ALONG_K, bool B_ALONG_K, int TI, int TJ, int WI, int WJ>
-struct ProductOf<true, T, A_ALONG_K, B_ALONG_K, TI, TJ, WI, WJ>
-{
-    typedef DirectProduct<T, A_ALONG_K, B_ALONG_K, TI, TJ, WI, WJ> Type;
-};
 
 /** Up to four consecutive values, as many as are left before 'end'. */
 template <typename T>
@@ -587,7 +615,7 @@ GroupedRowsKernel(const T* __restrict__ x, long long strideX, const T* __restric
                   const T* __restrict__ bias, long long strideBias, const int* __restrict__ offsets, int experts, T* __restrict__ y, long long strideY,
                   int rows, int J, int K, int places, int tilesJ)
 {
-    typedef typename ProductOf<DIRECT, T, true, B_ALONG_K, TI, TJ, WI, WJ>::Type Product;
+    typedef TileProduct<DIRECT, T, true, B_ALONG_K, TI, TJ, WI, WJ> Product;
     extern __shared__ __attribute__((aligned(16))) char groupedLds[];
     const Work work = workOf(blockIdx.x, places, tilesJ);
     const ExpertTile at = expertTile(offsets, experts, rows, TI, work.place);
@@ -597,7 +625,9 @@ GroupedRowsKernel(const T* __restrict__ x, long long strideX, const T* __restric
     Product product;
     const bool none = at.expert >= experts;
     const T* w = weights + (none ? 0 : at.expert) * strideExpert;
-    product.run(groupedLds, x + at.from * strideX, strideX, ni, w + (B_ALONG_K ? j0 * strideWeights : j0), strideWeights, nj, none ? 0 : K, false);
+    const Source<T> a = {x + at.from * strideX, strideX, ni, rows - at.from};
+    const Source<T> b = {w + (B_ALONG_K ? j0 * strideWeights : j0), strideWeights, nj, B_ALONG_K ? J - j0 : K};
+    product.run(groupedLds, a, b, none ? 0 : K, false);
     storeTile(product, groupedLds, bias && !none ? bias + at.expert * strideBias + j0 : nullptr, y + at.from * strideY + j0, strideY, ni, nj);
 }
 
@@ -612,7 +642,7 @@ GroupedWeightsKernel(const T* __restrict__ adjY, long long strideAdjY, const T* 
                      int experts, T* __restrict__ adjWeights, T* __restrict__ adjBias, float* __restrict__ partial, int rows, int I, int J, int places,
                      int tilesI, int tilesJ, int chunk)
 {
-    typedef typename ProductOf<DIRECT, T, false, false, TI, TJ, WI, WJ>::Type Product;
+    typedef TileProduct<DIRECT, T, false, false, TI, TJ, WI, WJ> Product;
     extern __shared__ __attribute__((aligned(16))) char groupedLds[];
     const Work work = workOf(blockIdx.x % (tilesI * tilesJ), tilesI, tilesJ);   // (tiles of one place: rows of tiles for its places)
     const int place = blockIdx.x / (tilesI * tilesJ);
@@ -623,7 +653,8 @@ GroupedWeightsKernel(const T* __restrict__ adjY, long long strideAdjY, const T* 
     const bool whole = at.expertRows <= chunk;
     const bool sumA = adjBias && j0 == 0 && Product::firstJ() == 0;   // the wavefronts of the first columns
     Product product;
-    product.run(groupedLds, adjY + at.from * strideAdjY + i0, strideAdjY, ni, x + at.from * strideX + j0, strideX, nj, max(0, at.to - at.from), sumA);
+    const Source<T> a = {adjY + at.from * strideAdjY + i0, strideAdjY, ni, rows - at.from}, b = {x + at.from * strideX + j0, strideX, nj, rows - at.from};
+    product.run(groupedLds, a, b, max(0, at.to - at.from), sumA);
     const long long size = static_cast<long long>(I) * J;
     float* sums = whole ? nullptr : partial + place * (size + I);
     if (!whole)

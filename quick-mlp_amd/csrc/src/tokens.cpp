@@ -338,29 +338,37 @@ struct GroupedTiles
     unsigned lds(int64_t K, int entry) const { return static_cast<unsigned>(std::max((K * entry <= 128 ? 1 : 2) * 128 * (i + j), i * j * entry)); }
     std::string arguments() const { return str(i, ", ", j, ", ", wavesI, ", ", wavesJ); }
 };
-constexpr GroupedTiles HUGE_TILES = {256, 256, 2, 4}, TALL_TILES = {256, 64, 4, 1}, LARGE_TILES = {128, 128, 2, 2}, SMALL_TILES = {64, 64, 2, 2};
-const std::array<GroupedTiles, 4> GROUPED_TILES = {HUGE_TILES, TALL_TILES, LARGE_TILES, SMALL_TILES};
-// Fewer tiles than that leave compute units without work: smaller ones, then.
-constexpr int64_t ENOUGH_HUGE = 192, ENOUGH_TILES = 256;
+constexpr GroupedTiles HUGE_TILES = {256, 256, 2, 4}, LARGE_TILES = {128, 128, 2, 2}, SMALL_TILES = {64, 64, 2, 2};
+const std::array<GroupedTiles, 3> GROUPED_TILES = {HUGE_TILES, LARGE_TILES, SMALL_TILES};
 
-/** Tiles of GroupedRowsKernel for (rows, J). */
-GroupedTiles rowsTiles(int64_t rows, int64_t experts, int64_t J, bool direct)
+/**
+ * The tiles for 'rows' of 'each' rows per expert and J results of K terms each, for values of 16 bits. A huge tile takes a compute unit
+ * for itself, so that its first loads and its last stores stand alone: it pays where sums are long or where there are many of them, and
+ * small ones pay where larger ones would leave compute units without work. us, huge | large | small, bfloat16, 16 or 17 experts:
+ * 32768 rows, K 2048, J 4096: 610 | 670 | 958; 54272, 2240, 256: 79 | 94 | 140; 54272, 256, 2240: 142 | 139 | 192; 16384, 1024, 1024: 65 | 51 | 64;
+ * 4096, 1024, 1024: 34 | 22 | 25; 16384, 4096, 64: 91 | 47 | 38; through registers 32768, 2047, 4095: 840 | 996 | 1467.
+ * Single precision is bound by the matrix cores with small tiles as well (16384 rows, 4 experts, 1024, 1024: - | 342 | 322).
+ */
+GroupedTiles rowsTiles(Tensor::Precision p, int64_t rows, int64_t experts, int64_t J, int64_t K)
 {
+    if (p == Tensor::FLOAT) return SMALL_TILES;
     const int64_t each = rows / std::max<int64_t>(experts, 1);
     auto count = [&](const GroupedTiles& t) { return (rows / t.i + experts) * divUp<int64_t>(J, t.j); };
-    if (direct && each > 128 && J > 128 && count(HUGE_TILES) >= ENOUGH_HUGE) return HUGE_TILES;
-    if (each >= 128 && J <= 64 && count(TALL_TILES) >= ENOUGH_TILES) return TALL_TILES;
-    if (each > 64 && J > 64 && count(LARGE_TILES) >= ENOUGH_TILES) return LARGE_TILES;
-    return SMALL_TILES;
+    if (each > 128 && J > 128 && ((K >= 1536 && count(HUGE_TILES) >= 192) || (K >= 512 && count(HUGE_TILES) >= 768))) return HUGE_TILES;
+    return each > 64 && J > 64 && count(LARGE_TILES) >= 256 ? LARGE_TILES : SMALL_TILES;
 }
-/** Tiles of GroupedWeightsKernel for experts of (I, J); an expert's rows may be shared out, in chunks that are worth it. */
-GroupedTiles weightsTiles(int64_t rows, int64_t experts, int64_t I, int64_t J, bool direct)
+/**
+ * The tiles of the weights' gradients, experts x (I, J), whose terms, an expert's rows, may be shared out in chunks. us, huge | large | small, as above:
+ * 32768 rows, I 4096, J 2048: 542 | 641 | 1001; 16384, 1024, 1024: 127 | 48 | 65; through registers, where the huge tile's registers do not
+ * suffice, 32768, 4095, 2047: 1095 | 982 | 1488; float, 16384 rows of 4 experts, 1024, 1024: - | 317 | 324; 16384 of 16, 1024, 64: - | 57 | 37.
+ */
+GroupedTiles weightsTiles(Tensor::Precision p, int64_t rows, int64_t experts, int64_t I, int64_t J, bool direct)
 {
+    if (p == Tensor::FLOAT) return SMALL_TILES;
     const int64_t each = divUp(rows, experts);
     auto count = [&](const GroupedTiles& t, int64_t chunk) { return experts * divUp<int64_t>(I, t.i) * divUp<int64_t>(J, t.j) * std::max<int64_t>(1, each / chunk); };
-    if (direct && I > 128 && J > 128 && count(HUGE_TILES, 512) >= ENOUGH_HUGE) return HUGE_TILES;
-    if (I > 64 && J > 64 && count(LARGE_TILES, 256) >= ENOUGH_TILES) return LARGE_TILES;
-    return SMALL_TILES;
+    if (direct && I > 128 && J > 128 && each >= 512 && count(HUGE_TILES, 2048) >= 512) return HUGE_TILES;
+    return I > 64 && J > 64 && count(LARGE_TILES, 256) >= 256 ? LARGE_TILES : SMALL_TILES;
 }
 
 /** Whether tiles of the operand can go straight from global memory to LDS (DirectTile). */
@@ -393,9 +401,9 @@ struct GroupedAdjointPlan
     int64_t tilesI, tilesJ, chunk, places;
     Workspace memory;
     float* partial = nullptr;
-    GroupedAdjointPlan(int64_t rows, int64_t experts, int64_t inputs, int64_t outputs, bool direct, void* base) : memory{static_cast<char*>(base)}
+    GroupedAdjointPlan(Tensor::Precision p, int64_t rows, int64_t experts, int64_t inputs, int64_t outputs, bool direct, void* base) : memory{static_cast<char*>(base)}
     {
-        tiles = weightsTiles(rows, experts, outputs, inputs, direct);
+        tiles = weightsTiles(p, rows, experts, outputs, inputs, direct);
         tilesI = divUp<int64_t>(outputs, tiles.i);
         tilesJ = divUp<int64_t>(inputs, tiles.j);
         chunk = weightsChunk(rows, experts, tilesI * tilesJ, tiles.i);
@@ -403,6 +411,13 @@ struct GroupedAdjointPlan
         if (chunk < rows) partial = memory.take<float>(places * (outputs * inputs + outputs));
     }
 };
+
+/** Rows of an operand of the experts' products have 32-bit offsets within a tile. */
+void checkRows(const Tensor& t, const char* what)
+{
+    const int d = t.ndim() - 2;
+    CHECK_ERROR(t.size(d) <= 1 || t.stride(d) < (1 << 21), "rows of ", what, " must be less than 2^21 entries apart");
+}
 
 void checkLaunch(int64_t groups, int threads)
 {
@@ -418,6 +433,8 @@ GroupedSizes checkGrouped(const Tensor& input, const Tensor& weight, const Tenso
     checkValues(input, "input", 2);
     checkValues(weight, "weight", 3);
     checkType(weight, "weight", input.precision());
+    checkRows(input, "input");
+    checkRows(weight, "weight");
     CHECK_ERROR(offsets.defined() && offsets.ndim() == 1, "offsets must be a tensor with 1 dimension");
     checkType(offsets, "offsets", Tensor::INT32);
     CHECK_ERROR(offsets.size(0) <= 1 || offsets.stride(0) == 1, "offsets must be contiguous");
@@ -433,7 +450,7 @@ void launchRows(bool alongK, const Tensor& x, const Tensor& weight, const Tensor
                 int J, int K, stream_t stream)
 {
     const bool direct = isDirect(x) && isDirect(weight);
-    const GroupedTiles t = rowsTiles(s.rows, s.experts, J, direct);
+    const GroupedTiles t = rowsTiles(x.precision(), s.rows, s.experts, J, K);
     const int tilesJ = divUp(J, t.j);
     const int64_t places = tilePlaces(s.rows, s.experts, t.i);
     checkLaunch(places * tilesJ, t.threads());
@@ -674,8 +691,10 @@ size_t Tokens::groupedLinearAdjointMemory(int64_t rows, int experts, int inputs,
     CHECK_ERROR(rows >= 0 && experts >= 0 && inputs >= 0 && outputs >= 0, "sizes must not be negative");
     if (experts == 0) return 0;
     // (for any type and alignment)
-    return std::max(GroupedAdjointPlan(rows, experts, inputs, outputs, true, nullptr).memory.bytes,
-                    GroupedAdjointPlan(rows, experts, inputs, outputs, false, nullptr).memory.bytes);
+    size_t bytes = 0;
+    for (const Tensor::Precision p : {Tensor::FLOAT, Tensor::HALF})
+        for (const bool direct : {false, true}) bytes = std::max(bytes, GroupedAdjointPlan(p, rows, experts, inputs, outputs, direct, nullptr).memory.bytes);
+    return bytes;
 }
 
 void Tokens::groupedLinearAdjoint(const Tensor& input, const Tensor& weight, const Tensor& offsets, const Tensor& adjOutput, Tensor& adjInput,
@@ -686,6 +705,7 @@ void Tokens::groupedLinearAdjoint(const Tensor& input, const Tensor& weight, con
     checkValues(adjOutput, "adjOutput", 2);
     checkType(adjOutput, "adjOutput", p);
     checkSizes(adjOutput, "adjOutput", {s.rows, s.outputs});
+    checkRows(adjOutput, "adjOutput");
     if (adjInput.defined()) {
         checkValues(adjInput, "adjInput", 2);
         checkType(adjInput, "adjInput", p);
@@ -710,7 +730,7 @@ void Tokens::groupedLinearAdjoint(const Tensor& input, const Tensor& weight, con
     if (s.experts == 0 || (!adjWeight.defined() && !adjBias.defined())) return;
     checkMemory(memory, groupedLinearAdjointMemory(s.rows, s.experts, s.inputs, s.outputs));
     const bool direct = isDirect(input) && isDirect(adjOutput);
-    GroupedAdjointPlan plan(s.rows, s.experts, s.inputs, s.outputs, direct, memory);
+    GroupedAdjointPlan plan(p, s.rows, s.experts, s.inputs, s.outputs, direct, memory);
     const int64_t groups = plan.places * plan.tilesI * plan.tilesJ;
     checkLaunch(groups, plan.tiles.threads());
     const int chunk = static_cast<int>(plan.chunk);
@@ -759,10 +779,10 @@ void Tokens::precompile(Tensor::Precision p)
     for (const char* kernel : {"LayerNormLongSumsKernel", "LayerNormSumKernel"}) precompileKernel("layer_norm.h", str(kernel, "<", t, ">"));
     for (const bool direct : {false, true})
         for (const GroupedTiles& tiles : GROUPED_TILES) {
-            if (direct ? p == Tensor::FLOAT : tiles.i == HUGE_TILES.i && tiles.j == HUGE_TILES.j) continue;
+            if (p == Tensor::FLOAT && (direct || tiles.i != SMALL_TILES.i)) continue;
             const std::string types = str(t, ", ", boolName(direct));
             for (const char* along : {", true, ", ", false, "}) precompileKernel("grouped_linear.h", str("GroupedRowsKernel<", types, along, tiles.arguments(), ">"));
-            if (tiles.i == tiles.j) precompileKernel("grouped_linear.h", str("GroupedWeightsKernel<", types, ", ", tiles.arguments(), ">"));
+            if (direct || tiles.i != HUGE_TILES.i) precompileKernel("grouped_linear.h", str("GroupedWeightsKernel<", types, ", ", tiles.arguments(), ">"));
         }
     precompileKernel("grouped_linear.h", str("GroupedSumKernel<", t, ">"));
 }

@@ -533,6 +533,11 @@ at::Tensor consecutive(const at::Tensor& t)
 {
     return !t.defined() || t.dim() == 0 || t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous();
 }
+/** And rows no further apart than the kernels of the experts' products reach. */
+at::Tensor near(const at::Tensor& t)
+{
+    return t.dim() >= 2 && t.size(-2) > 1 && t.stride(-2) >= (1 << 21) ? t.contiguous() : consecutive(t);
+}
 at::Tensor temporary(const at::Tensor& like, size_t bytes) { return bytes > 0 ? bytesOn(like, bytes) : at::Tensor(); }
 void* dataOf(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 at::Tensor emptyLike(const at::Tensor& t) { return at::empty(t.sizes(), t.options().requires_grad(false)); }
@@ -724,8 +729,7 @@ struct GroupedLinearBackward : TokenNode
     std::string name() const override { return "QmlpGroupedLinearBackward"; }
     void adjoint(const at::Tensor& gradOutput, variable_list& grads) override
     {
-        const at::Tensor x = consecutive(saved[0].unpack()), weight = consecutive(saved[1].unpack()), offsets = saved[2].unpack(),
-                         adjOutput = consecutive(gradOutput);
+        const at::Tensor x = near(saved[0].unpack()), weight = near(saved[1].unpack()), offsets = saved[2].unpack(), adjOutput = near(gradOutput);
         at::Tensor adjX, adjWeight, adjBias;
         if (task_should_compute_output(0)) adjX = emptyLike(x);
         if (task_should_compute_output(1)) adjWeight = emptyLike(weight);
@@ -752,7 +756,7 @@ at::Tensor groupedLinear(const at::Tensor& x, const at::Tensor& weight, const at
     if (x.dim() != 2) throw std::runtime_error("input must be a tensor with 2 dimensions (rows, inputs)");
     if (weight.dim() != 3) throw std::runtime_error("weight must be a tensor with 3 dimensions (experts, outputs, inputs)");
     const at::Tensor output = guarded(x, [&] {
-        const at::Tensor rows = consecutive(x), w = consecutive(weight), b = consecutive(bias), off = consecutive(offsets);
+        const at::Tensor rows = near(x), w = near(weight), b = consecutive(bias), off = consecutive(offsets);
         const at::Tensor out = at::empty({x.size(0), weight.size(1)}, x.options().requires_grad(false));
         const qmlp_tensor in = wrapToken(rows), wt = wrapToken(w), of = wrapToken(off), bt = wrapToken(b), o = wrapToken(out);
         check(qmlp_tokens_grouped_linear(&in, &wt, &of, &bt, &o, currentStream(x)));
