@@ -294,8 +294,9 @@ int qmlp_tokens_layer_norm_adjoint(const qmlp_tensor* input, const qmlp_tensor* 
 /* output[r] = weight[e] input[r] + bias[e] for offsets[e] <= r < offsets[e + 1]: input (rows, inputs), weight (experts, outputs, inputs),
  * offsets (experts + 1, INT32, device memory, not decreasing, from 0 on), bias (experts, outputs; optional), output (rows, outputs).
  * Rows behind the last expert's get zeros. Rows of input and of a matrix are less than 2^21 entries apart. */
+int qmlp_tokens_grouped_linear_memory(long long rows, int experts, int inputs, int outputs, size_t* bytes);
 int qmlp_tokens_grouped_linear(const qmlp_tensor* input, const qmlp_tensor* weight, const qmlp_tensor* offsets, const qmlp_tensor* bias,
-                               const qmlp_tensor* output, void* stream);
+                               const qmlp_tensor* output, void* memory, void* stream);
 /* The gradients (each optional; adj_weight and adj_bias contiguous). */
 int qmlp_tokens_grouped_linear_adjoint_memory(long long rows, int experts, int inputs, int outputs, size_t* bytes);
 int qmlp_tokens_grouped_linear_adjoint(const qmlp_tensor* input, const qmlp_tensor* weight, const qmlp_tensor* offsets,

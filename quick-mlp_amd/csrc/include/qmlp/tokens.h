@@ -59,13 +59,15 @@ public:
     static void layerNormAdjoint(const Tensor& input, const Tensor& weight, const Tensor& mean, const Tensor& rstd, const Tensor& adjOutput,
                                  Tensor& adjInput, Tensor& adjWeight, Tensor& adjBias, void* memory, stream_t stream);
 
+    /** Bytes of 'memory' for groupedLinear(). */
+    static size_t groupedLinearMemory(int64_t rows, int experts, int inputs, int outputs);
     /**
      * The linear layer of every expert on its rows: output[r] = weight[e] input[r] + bias[e] for offsets[e] <= r < offsets[e + 1].
      * \param input (rows, inputs) \param weight (experts, outputs, inputs), of the input's type \param offsets (experts + 1) INT32, in device
      * memory, not decreasing, from 0 on; rows behind the last expert's get zeros \param bias (experts, outputs) or undefined
      * \param output (rows, outputs)
      */
-    static void groupedLinear(const Tensor& input, const Tensor& weight, const Tensor& offsets, const Tensor& bias, Tensor& output,
+    static void groupedLinear(const Tensor& input, const Tensor& weight, const Tensor& offsets, const Tensor& bias, Tensor& output, void* memory,
                               stream_t stream);
     /** Bytes of 'memory' for groupedLinearAdjoint(). */
     static size_t groupedLinearAdjointMemory(int64_t rows, int experts, int inputs, int outputs);

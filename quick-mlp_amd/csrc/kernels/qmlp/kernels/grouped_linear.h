@@ -607,17 +607,19 @@ __device__ __forceinline__ Work workOf(unsigned id, unsigned places, unsigned ti
 // ------------------------------------------------------------------------------------------------ kernels
 /**
  * Rows times the experts' matrices: y[r][j] = sum over k of x[r][k] B(j, k) + bias[e][j]. B_ALONG_K: weights[e][j][k] (the layer),
- * otherwise weights[e][k][j] (its adjoint). Workgroups: places of tiles x tiles of J.
+ * otherwise weights[e][k][j] (its adjoint). Workgroups: places of tiles x tiles of J, times slices of 'slice' of the K where those are too
+ * few: then every slice leaves its floats in partial[slice][r][j], for GroupedJoinKernel.
  */
 template <typename T, bool DIRECT, bool B_ALONG_K, int TI, int TJ, int WI, int WJ>
 __global__ void __launch_bounds__(64 * WI * WJ)
 GroupedRowsKernel(const T* __restrict__ x, long long strideX, const T* __restrict__ weights, long long strideExpert, long long strideWeights,
                   const T* __restrict__ bias, long long strideBias, const int* __restrict__ offsets, int experts, T* __restrict__ y, long long strideY,
-                  int rows, int J, int K, int places, int tilesJ)
+                  int rows, int J, int K, int places, int tilesJ, int slices, int slice, float* __restrict__ partial)
 {
     typedef TileProduct<DIRECT, T, true, B_ALONG_K, TI, TJ, WI, WJ> Product;
     extern __shared__ __attribute__((aligned(16))) char groupedLds[];
-    const Work work = workOf(blockIdx.x, places, tilesJ);
+    const Work work = workOf(blockIdx.x / slices, places, tilesJ);
+    const int s = blockIdx.x % slices, k0 = s * slice;
     const ExpertTile at = expertTile(offsets, experts, rows, TI, work.place);
     if (at.to <= at.from) return;
     const int j0 = work.tile * TJ;
@@ -625,10 +627,22 @@ GroupedRowsKernel(const T* __restrict__ x, long long strideX, const T* __restric
     Product product;
     const bool none = at.expert >= experts;
     const T* w = weights + (none ? 0 : at.expert) * strideExpert;
-    const Source<T> a = {x + at.from * strideX, strideX, ni, rows - at.from};
-    const Source<T> b = {w + (B_ALONG_K ? j0 * strideWeights : j0), strideWeights, nj, B_ALONG_K ? J - j0 : K};
-    product.run(groupedLds, a, b, none ? 0 : K, false);
-    storeTile(product, groupedLds, bias && !none ? bias + at.expert * strideBias + j0 : nullptr, y + at.from * strideY + j0, strideY, ni, nj);
+    const Source<T> a = {x + at.from * strideX + k0, strideX, ni, rows - at.from};
+    const Source<T> b = {w + (B_ALONG_K ? j0 * strideWeights + k0 : k0 * strideWeights + j0), strideWeights, nj, B_ALONG_K ? J - j0 : K - k0};
+    product.run(groupedLds, a, b, none ? 0 : min(slice, K - k0), false);
+    const T* const biases = bias && !none && s == 0 ? bias + at.expert * strideBias + j0 : nullptr;
+    if (!partial) {
+        storeTile(product, groupedLds, biases, y + at.from * strideY + j0, strideY, ni, nj);
+        return;
+    }
+    float* const out = partial + (static_cast<long long>(s) * rows + at.from) * J + j0;
+    product.results([&](int i, int j, float (&v)[4]) {
+        if (i >= ni || j >= nj) return;
+        if (biases)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] += static_cast<float>(biases[min(j + k, nj - 1)]);
+        storeUpToFour(out + static_cast<long long>(i) * J + j, v, nj - j);
+    });
 }
 
 /**
@@ -672,6 +686,20 @@ GroupedWeightsKernel(const T* __restrict__ adjY, long long strideAdjY, const T* 
             if (whole) adjBias[static_cast<long long>(at.expert) * I + i0 + i] = static_cast<T>(sum);
             else sums[size + i0 + i] = sum;
         }
+}
+
+/** y = the sum over the slices of GroupedRowsKernel. */
+template <typename T>
+__global__ void __launch_bounds__(256)
+GroupedJoinKernel(const float* __restrict__ partial, int slices, T* __restrict__ y, long long strideY, int rows, int J)
+{
+    const long long size = static_cast<long long>(rows) * J;
+    for (long long at = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; at < size; at += static_cast<long long>(gridDim.x) * 256) {
+        float sum = 0;
+#pragma unroll 4
+        for (int s = 0; s < slices; ++s) sum += partial[s * size + at];
+        y[at / J * strideY + at % J] = static_cast<T>(sum);
+    }
 }
 
 /** Adds up the sums per chunk of the experts that have several. Workgroups: experts x pieces of 256 of their size + I sums. */

@@ -755,12 +755,19 @@ int qmlp_tokens_layer_norm_adjoint(const qmlp_tensor* input, const qmlp_tensor* 
     QMLP_API_END
 }
 
+int qmlp_tokens_grouped_linear_memory(long long rows, int experts, int inputs, int outputs, size_t* bytes)
+{
+    QMLP_API_BEGIN
+    *bytes = Tokens::groupedLinearMemory(rows, experts, inputs, outputs);
+    QMLP_API_END
+}
+
 int qmlp_tokens_grouped_linear(const qmlp_tensor* input, const qmlp_tensor* weight, const qmlp_tensor* offsets, const qmlp_tensor* bias,
-                               const qmlp_tensor* output, void* stream)
+                               const qmlp_tensor* output, void* memory, void* stream)
 {
     QMLP_API_BEGIN
     Tensor out = wrapToken(output);
-    Tokens::groupedLinear(wrapToken(input), wrapToken(weight), wrapToken(offsets), wrapToken(bias), out, static_cast<stream_t>(stream));
+    Tokens::groupedLinear(wrapToken(input), wrapToken(weight), wrapToken(offsets), wrapToken(bias), out, memory, static_cast<stream_t>(stream));
     QMLP_API_END
 }
 

@@ -34,7 +34,7 @@ int wide(Tensor::Precision p) { return 16 / Tensor::BytesPerEntry[p]; }
 
 enum KernelId { GROUP_SMALL, GROUP_COUNT, GROUP_SCAN, GROUP_SCATTER, GROUP_OFFSETS, EMBEDDING, EMBEDDING_BLOCKS, EMBEDDING_ADJOINT, LAYER_NORM,
                 LAYER_NORM_ADJOINT, LAYER_NORM_SUM, LAYER_NORM_LONG, LAYER_NORM_LONG_ADJOINT, LAYER_NORM_LONG_SUMS, GROUPED_ROWS, GROUPED_WEIGHTS,
-                GROUPED_SUM };
+                GROUPED_SUM, GROUPED_JOIN };
 /** One number for a kernel and its template arguments, each below 2^11: to build its name takes as long as to launch it. */
 template <typename... Args>
 uint64_t kernelKey(KernelId id, Args... args)
@@ -445,21 +445,54 @@ GroupedSizes checkGrouped(const Tensor& input, const Tensor& weight, const Tenso
     return s;
 }
 
-/** GroupedRowsKernel: y (rows, J) from x (rows, K) and the weights along K (the layer) or across it (its adjoint). */
-void launchRows(bool alongK, const Tensor& x, const Tensor& weight, const Tensor& offsets, const Tensor& bias, const Tensor& y, const GroupedSizes& s,
-                int J, int K, stream_t stream)
+/** How GroupedRowsKernel makes (rows, J) of sums of K terms. */
+struct RowsPlan
 {
+    GroupedTiles tiles;
+    int64_t tilesJ, places;
+    int slices = 1, slice;
+    size_t bytes = 0;   // of memory for the slices
+    RowsPlan(Tensor::Precision p, int64_t rows, int64_t experts, int64_t J, int64_t K)
+        : tiles(rowsTiles(p, rows, experts, J, K)), tilesJ(divUp<int64_t>(J, tiles.j)), places(tilePlaces(rows, experts, tiles.i)), slice(static_cast<int>(K))
+    {
+        // Few tiles of long sums: a tile goes through 16 tiles of K or more (about 1 us each) alone on its compute unit. Slices of four at
+        // least, and a second launch that adds them up.
+        const int64_t tileK = 128 / Tensor::BytesPerEntry[p], steps = divUp(K, tileK);
+        const int64_t count = (rows / tiles.i + std::min(experts, rows)) * tilesJ;
+        if (steps < 16 || count >= 256 || count == 0) return;
+        const int64_t wanted = std::min<int64_t>({divUp<int64_t>(512, count), steps / 4, 32});
+        slice = static_cast<int>(divUp(steps, wanted) * tileK);
+        slices = static_cast<int>(divUp<int64_t>(K, slice));
+        if (slices > 1) bytes = roundUp<size_t>(sizeof(float) * slices * rows * J, ALIGNMENT);
+    }
+};
+/** Memory for any type. */
+size_t rowsMemory(int64_t rows, int64_t experts, int64_t J, int64_t K)
+{
+    return std::max(RowsPlan(Tensor::FLOAT, rows, experts, J, K).bytes, RowsPlan(Tensor::HALF, rows, experts, J, K).bytes);
+}
+
+/** y (rows, J) from x (rows, K) and the weights along K (the layer) or across it (its adjoint). */
+void launchRows(bool alongK, const Tensor& x, const Tensor& weight, const Tensor& offsets, const Tensor& bias, const Tensor& y, const GroupedSizes& s,
+                int J, int K, void* memory, stream_t stream)
+{
+    const Tensor::Precision p = x.precision();
     const bool direct = isDirect(x) && isDirect(weight);
-    const GroupedTiles t = rowsTiles(x.precision(), s.rows, s.experts, J, K);
-    const int tilesJ = divUp(J, t.j);
-    const int64_t places = tilePlaces(s.rows, s.experts, t.i);
-    checkLaunch(places * tilesJ, t.threads());
-    tokenKernel("grouped_linear.h", kernelKey(GROUPED_ROWS, x.precision() * 4 + direct * 2 + alongK, t.i, t.j, t.wavesI, t.wavesJ),
-                [&] { return str("GroupedRowsKernel<", scalarName(x.precision()), ", ", boolName(direct), ", ", boolName(alongK), ", ", t.arguments(), ">"); })
-        .call(static_cast<unsigned>(places * tilesJ), t.threads(), t.lds(K, x.bytesPerEntry()), stream, x.rawPtr(), strideOf(x, 0), static_cast<const void*>(ptr<void>(weight)),
-              strideOf(weight, 0), strideOf(weight, 1), static_cast<const void*>(ptr<void>(bias)), bias.defined() ? strideOf(bias, 0) : 0ll,
-              static_cast<const int*>(ptr<int>(offsets)), s.experts, static_cast<void*>(ptr<void>(y)), strideOf(y, 0), s.rows, J, K, static_cast<int>(places),
-              tilesJ);
+    const RowsPlan plan(p, s.rows, s.experts, J, K);
+    const GroupedTiles& t = plan.tiles;
+    const int64_t groups = plan.places * plan.tilesJ * plan.slices;
+    checkLaunch(groups, t.threads());
+    float* partial = plan.slices > 1 ? static_cast<float*>(memory) : nullptr;
+    tokenKernel("grouped_linear.h", kernelKey(GROUPED_ROWS, p * 4 + direct * 2 + alongK, t.i, t.j, t.wavesI, t.wavesJ),
+                [&] { return str("GroupedRowsKernel<", scalarName(p), ", ", boolName(direct), ", ", boolName(alongK), ", ", t.arguments(), ">"); })
+        .call(static_cast<unsigned>(groups), t.threads(), t.lds(plan.slice, x.bytesPerEntry()), stream, x.rawPtr(), strideOf(x, 0),
+              static_cast<const void*>(ptr<void>(weight)), strideOf(weight, 0), strideOf(weight, 1), static_cast<const void*>(ptr<void>(bias)),
+              bias.defined() ? strideOf(bias, 0) : 0ll, static_cast<const int*>(ptr<int>(offsets)), s.experts, static_cast<void*>(ptr<void>(y)),
+              strideOf(y, 0), s.rows, J, K, static_cast<int>(plan.places), static_cast<int>(plan.tilesJ), plan.slices, plan.slice, partial);
+    if (partial)
+        tokenKernel("grouped_linear.h", kernelKey(GROUPED_JOIN, p), [&] { return str("GroupedJoinKernel<", scalarName(p), ">"); })
+            .call(workgroups(divUp<int64_t>(static_cast<int64_t>(s.rows) * J, 256), 4096), 256, 0, stream, static_cast<const float*>(partial), plan.slices,
+                  static_cast<void*>(ptr<void>(y)), strideOf(y, 0), s.rows, J);
 }
 
 } // namespace
@@ -669,7 +702,14 @@ void Tokens::layerNormAdjoint(const Tensor& input, const Tensor& weight, const T
                   ptr<void>(adjWeight), ptr<void>(adjBias));
 }
 
-void Tokens::groupedLinear(const Tensor& input, const Tensor& weight, const Tensor& offsets, const Tensor& bias, Tensor& output, stream_t stream)
+size_t Tokens::groupedLinearMemory(int64_t rows, int experts, int inputs, int outputs)
+{
+    CHECK_ERROR(rows >= 0 && experts >= 0 && inputs >= 0 && outputs >= 0, "sizes must not be negative");
+    return rowsMemory(rows, experts, outputs, inputs);
+}
+
+void Tokens::groupedLinear(const Tensor& input, const Tensor& weight, const Tensor& offsets, const Tensor& bias, Tensor& output, void* memory,
+                           stream_t stream)
 {
     const GroupedSizes s = checkGrouped(input, weight, offsets);
     const Tensor::Precision p = input.precision();
@@ -683,15 +723,16 @@ void Tokens::groupedLinear(const Tensor& input, const Tensor& weight, const Tens
     checkSizes(output, "output", {s.rows, s.outputs});
     checkOutput(output, "output");
     if (s.rows == 0) return;
-    launchRows(true, input, weight, offsets, bias, output, s, s.outputs, s.inputs, stream);
+    checkMemory(memory, groupedLinearMemory(s.rows, s.experts, s.inputs, s.outputs));
+    launchRows(true, input, weight, offsets, bias, output, s, s.outputs, s.inputs, memory, stream);
 }
 
 size_t Tokens::groupedLinearAdjointMemory(int64_t rows, int experts, int inputs, int outputs)
 {
     CHECK_ERROR(rows >= 0 && experts >= 0 && inputs >= 0 && outputs >= 0, "sizes must not be negative");
-    if (experts == 0) return 0;
-    // (for any type and alignment)
-    size_t bytes = 0;
+    // (for any type and alignment; the input's gradients are done before the weights' begin)
+    size_t bytes = rowsMemory(rows, experts, inputs, outputs);
+    if (experts == 0) return bytes;
     for (const Tensor::Precision p : {Tensor::FLOAT, Tensor::HALF})
         for (const bool direct : {false, true}) bytes = std::max(bytes, GroupedAdjointPlan(p, rows, experts, inputs, outputs, direct, nullptr).memory.bytes);
     return bytes;
@@ -726,9 +767,11 @@ void Tokens::groupedLinearAdjoint(const Tensor& input, const Tensor& weight, con
     }
     const int* off = ptr<int>(offsets);
     const void *x = ptr<void>(input), *dy = ptr<void>(adjOutput);
-    if (adjInput.defined() && s.rows > 0) launchRows(false, adjOutput, weight, offsets, {}, adjInput, s, s.inputs, s.outputs, stream);
-    if (s.experts == 0 || (!adjWeight.defined() && !adjBias.defined())) return;
+    const bool inputs = adjInput.defined() && s.rows > 0, weights = s.experts > 0 && (adjWeight.defined() || adjBias.defined());
+    if (!inputs && !weights) return;
     checkMemory(memory, groupedLinearAdjointMemory(s.rows, s.experts, s.inputs, s.outputs));
+    if (inputs) launchRows(false, adjOutput, weight, offsets, {}, adjInput, s, s.inputs, s.outputs, memory, stream);
+    if (!weights) return;
     const bool direct = isDirect(input) && isDirect(adjOutput);
     GroupedAdjointPlan plan(p, s.rows, s.experts, s.inputs, s.outputs, direct, memory);
     const int64_t groups = plan.places * plan.tilesI * plan.tilesJ;
@@ -784,7 +827,7 @@ void Tokens::precompile(Tensor::Precision p)
             for (const char* along : {", true, ", ", false, "}) precompileKernel("grouped_linear.h", str("GroupedRowsKernel<", types, along, tiles.arguments(), ">"));
             if (direct || tiles.i != HUGE_TILES.i) precompileKernel("grouped_linear.h", str("GroupedWeightsKernel<", types, ", ", tiles.arguments(), ">"));
         }
-    precompileKernel("grouped_linear.h", str("GroupedSumKernel<", t, ">"));
+    for (const char* kernel : {"GroupedSumKernel", "GroupedJoinKernel"}) precompileKernel("grouped_linear.h", str(kernel, "<", t, ">"));
 }
 
 QUICKMLP_NAMESPACE_END

@@ -735,9 +735,8 @@ struct GroupedLinearBackward : TokenNode
         if (task_should_compute_output(1)) adjWeight = emptyLike(weight);
         if (task_should_compute_output(2)) adjBias = at::empty({weight.size(0), weight.size(1)}, weight.options().requires_grad(false));
         size_t bytes = 0;
-        if (adjWeight.defined() || adjBias.defined())
-            check(qmlp_tokens_grouped_linear_adjoint_memory(x.size(0), static_cast<int>(weight.size(0)), static_cast<int>(weight.size(2)),
-                                                            static_cast<int>(weight.size(1)), &bytes));
+        check(qmlp_tokens_grouped_linear_adjoint_memory(x.size(0), static_cast<int>(weight.size(0)), static_cast<int>(weight.size(2)),
+                                                        static_cast<int>(weight.size(1)), &bytes));
         const at::Tensor memory = temporary(x, bytes);
         const qmlp_tensor in = wrapToken(x), w = wrapToken(weight), off = wrapToken(offsets), dy = wrapToken(adjOutput), dx = wrapToken(adjX),
                           dw = wrapToken(adjWeight), db = wrapToken(adjBias);
@@ -759,7 +758,10 @@ at::Tensor groupedLinear(const at::Tensor& x, const at::Tensor& weight, const at
         const at::Tensor rows = near(x), w = near(weight), b = consecutive(bias), off = consecutive(offsets);
         const at::Tensor out = at::empty({x.size(0), weight.size(1)}, x.options().requires_grad(false));
         const qmlp_tensor in = wrapToken(rows), wt = wrapToken(w), of = wrapToken(off), bt = wrapToken(b), o = wrapToken(out);
-        check(qmlp_tokens_grouped_linear(&in, &wt, &of, &bt, &o, currentStream(x)));
+        size_t bytes = 0;
+        check(qmlp_tokens_grouped_linear_memory(in.sizes[0], wt.sizes[0], wt.sizes[2], wt.sizes[1], &bytes));
+        const at::Tensor memory = temporary(rows, bytes);
+        check(qmlp_tokens_grouped_linear(&in, &wt, &of, &bt, &o, dataOf(memory), currentStream(x)));
         return out;
     });
     if (wantsGradient(x) || wantsGradient(weight) || wantsGradient(bias))

@@ -129,7 +129,8 @@ _SIGNATURES = {
     "qmlp_tokens_layer_norm": [_TD, _TD, _TD, ctypes.c_float, _TD, _TD, _TD, _vp],
     "qmlp_tokens_layer_norm_adjoint_memory": [ctypes.c_longlong, _ci, _P(ctypes.c_size_t)],
     "qmlp_tokens_layer_norm_adjoint": [_TD, _TD, _TD, _TD, _TD, _TD, _TD, _TD, _vp, _vp],
-    "qmlp_tokens_grouped_linear": [_TD, _TD, _TD, _TD, _TD, _vp],
+    "qmlp_tokens_grouped_linear_memory": [ctypes.c_longlong, _ci, _ci, _ci, _P(ctypes.c_size_t)],
+    "qmlp_tokens_grouped_linear": [_TD, _TD, _TD, _TD, _TD, _vp, _vp],
     "qmlp_tokens_grouped_linear_adjoint_memory": [ctypes.c_longlong, _ci, _ci, _ci, _P(ctypes.c_size_t)],
     "qmlp_tokens_grouped_linear_adjoint": [_TD, _TD, _TD, _TD, _TD, _TD, _TD, _vp, _vp],
     "qmlp_tokens_precompile": [_ci],

@@ -314,6 +314,26 @@ COUNTS = {
 
 
 @gpu
+@pytest.mark.parametrize("inputs,outputs", [(2000, 40), (40, 2000), (1023, 1100)])
+@pytest.mark.parametrize("counts", [[1], [3, 0, 9], [70, 0, 0, 31]])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_long_sums_of_few_rows(inputs, outputs, counts, dtype):
+    """Sums that are shared out over workgroups and joined."""
+    say("long sums", inputs, outputs, counts, dtype)
+    g = generator(inputs)
+    rows = sum(counts) + 2
+    x, weight = normal(g, rows, inputs, dtype=dtype).requires_grad_(), normal(g, len(counts), outputs, inputs, dtype=dtype).requires_grad_()
+    bias = normal(g, len(counts), outputs, dtype=dtype).requires_grad_()
+    grad = normal(g, rows, outputs, dtype=dtype)
+    y = tokens.grouped_linear(x, weight, offsets_of(counts), bias)
+    gradients = torch.autograd.grad(y, (x, weight, bias), grad)
+    exact = grouped_reference(x.detach(), weight.detach(), counts, bias.detach(), grad)
+    for value, (expected, error), what in zip((y.detach(), *gradients), exact, ("y", "x", "weight", "bias")):
+        near(value, expected, error, what)
+    assert torch.equal(y, tokens.grouped_linear(x, weight, offsets_of(counts), bias))
+
+
+@gpu
 @pytest.mark.parametrize("counts", list(COUNTS))
 @pytest.mark.parametrize("inputs,outputs", [(1, 1), (3, 5), (16, 32), (64, 64), (64, 56), (77, 130), (200, 33), (256, 512)])
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -582,9 +602,9 @@ def test_c_interface_refuses_before_any_launch():
     refused(lib.qmlp_tokens_group(descriptor(I, 4), -1, descriptor(I, 4), descriptor(I, 4), None, None), "must not be negative")
     refused(lib.qmlp_tokens_group(descriptor(I, 4), 3, descriptor(I, 4), descriptor(I, 3), None, None), "must have 4 entries")
     w, off = descriptor(F, 3, 5, 6), descriptor(I, 4)
-    refused(lib.qmlp_tokens_grouped_linear(x, w, off, none, y, None), "must have 5 entries")
-    refused(lib.qmlp_tokens_grouped_linear(x, descriptor(H, 3, 5, 6), off, none, y, None), "must be of type FLOAT")
-    refused(lib.qmlp_tokens_grouped_linear(x, w, descriptor(F, 4), none, y, None), "must be of type INT32")
+    refused(lib.qmlp_tokens_grouped_linear(x, w, off, none, y, None, None), "must have 5 entries")
+    refused(lib.qmlp_tokens_grouped_linear(x, descriptor(H, 3, 5, 6), off, none, y, None, None), "must be of type FLOAT")
+    refused(lib.qmlp_tokens_grouped_linear(x, w, descriptor(F, 4), none, y, None, None), "must be of type INT32")
     dy = descriptor(F, 4, 5)
     refused(lib.qmlp_tokens_grouped_linear_adjoint(x, w, off, dy, none, descriptor(F, 3, 5, 6, strides=(60, 12, 1)), none, None, None), "contiguous")
     for call in (lambda b: lib.qmlp_tokens_group_memory(-1, 4, b), lambda b: lib.qmlp_tokens_group_memory(1 << 31, 4, b),
@@ -619,3 +639,4 @@ def test_memory_sizes_grow_with_the_work():
     assert of(lib.qmlp_tokens_layer_norm_adjoint_memory, 0, 64) == 0
     assert of(lib.qmlp_tokens_layer_norm_adjoint_memory, 1, 64) >= 2 * 64 * 4
     assert of(lib.qmlp_tokens_grouped_linear_adjoint_memory, 0, 4, 64, 64) == 0
+    assert of(lib.qmlp_tokens_grouped_linear_memory, 4096, 4, 64, 64) == 0 and of(lib.qmlp_tokens_grouped_linear_memory, 4, 4, 4096, 64) > 0
