@@ -338,8 +338,8 @@ struct GroupedTiles
     unsigned lds(int64_t K, int entry) const { return static_cast<unsigned>(std::max((K * entry <= 128 ? 1 : 2) * 128 * (i + j), i * j * entry)); }
     std::string arguments() const { return str(i, ", ", j, ", ", wavesI, ", ", wavesJ); }
 };
-constexpr GroupedTiles HUGE_TILES = {256, 256, 2, 4}, LARGE_TILES = {128, 128, 2, 2}, SMALL_TILES = {64, 64, 2, 2};
-const std::array<GroupedTiles, 3> GROUPED_TILES = {HUGE_TILES, LARGE_TILES, SMALL_TILES};
+constexpr GroupedTiles HUGE_TILES = {256, 256, 2, 4}, LARGE_TILES = {128, 128, 2, 2}, SMALL_TILES = {64, 64, 2, 2}, FEW_TILES = {32, 64, 1, 2};
+const std::array<GroupedTiles, 4> GROUPED_TILES = {HUGE_TILES, LARGE_TILES, SMALL_TILES, FEW_TILES};
 
 /**
  * The tiles for 'rows' of 'each' rows per expert and J results of K terms each, for values of 16 bits. A huge tile takes a compute unit
@@ -348,11 +348,13 @@ const std::array<GroupedTiles, 3> GROUPED_TILES = {HUGE_TILES, LARGE_TILES, SMAL
  * 32768 rows, K 2048, J 4096: 610 | 670 | 958; 54272, 2240, 256: 79 | 94 | 140; 54272, 256, 2240: 142 | 139 | 192; 16384, 1024, 1024: 65 | 51 | 64;
  * 4096, 1024, 1024: 34 | 22 | 25; 16384, 4096, 64: 91 | 47 | 38; through registers 32768, 2047, 4095: 840 | 996 | 1467.
  * Single precision is bound by the matrix cores with small tiles as well (16384 rows, 4 experts, 1024, 1024: - | 342 | 322).
+ * Where an expert has few rows, the weights are what is read: small | few: 24 rows of 64 experts, K 1024, J 4096: 53 | 44.
  */
 GroupedTiles rowsTiles(Tensor::Precision p, int64_t rows, int64_t experts, int64_t J, int64_t K)
 {
-    if (p == Tensor::FLOAT) return SMALL_TILES;
     const int64_t each = rows / std::max<int64_t>(experts, 1);
+    if (each <= 24) return FEW_TILES;
+    if (p == Tensor::FLOAT) return SMALL_TILES;
     auto count = [&](const GroupedTiles& t) { return (rows / t.i + experts) * divUp<int64_t>(J, t.j); };
     if (each > 128 && J > 128 && ((K >= 1536 && count(HUGE_TILES) >= 192) || (K >= 512 && count(HUGE_TILES) >= 768))) return HUGE_TILES;
     return each > 64 && J > 64 && count(LARGE_TILES) >= 256 ? LARGE_TILES : SMALL_TILES;
@@ -455,12 +457,13 @@ struct RowsPlan
     RowsPlan(Tensor::Precision p, int64_t rows, int64_t experts, int64_t J, int64_t K)
         : tiles(rowsTiles(p, rows, experts, J, K)), tilesJ(divUp<int64_t>(J, tiles.j)), places(tilePlaces(rows, experts, tiles.i)), slice(static_cast<int>(K))
     {
-        // Few tiles of long sums: a tile goes through 16 tiles of K or more (about 1 us each) alone on its compute unit. Slices of four at
-        // least, and a second launch that adds them up.
+        // Few tiles of long sums: a tile goes through 16 tiles of K or more (about 1 us each) alone on its compute unit, or, where there are few
+        // rows, too little of the weights is on its way. Slices of four at least, and a second launch that adds them up.
+        const bool few = tiles.i == FEW_TILES.i;
         const int64_t tileK = 128 / Tensor::BytesPerEntry[p], steps = divUp(K, tileK);
         const int64_t count = (rows / tiles.i + std::min(experts, rows)) * tilesJ;
-        if (steps < 16 || count >= 256 || count == 0) return;
-        const int64_t wanted = std::min<int64_t>({divUp<int64_t>(512, count), steps / 4, 32});
+        if (steps < 16 || count >= (few ? 768 : 256) || count == 0) return;
+        const int64_t wanted = std::min<int64_t>({divUp<int64_t>(few ? 1536 : 512, count), steps / 4, 32});
         slice = static_cast<int>(divUp(steps, wanted) * tileK);
         slices = static_cast<int>(divUp<int64_t>(K, slice));
         if (slices > 1) bytes = roundUp<size_t>(sizeof(float) * slices * rows * J, ALIGNMENT);
@@ -822,10 +825,10 @@ void Tokens::precompile(Tensor::Precision p)
     for (const char* kernel : {"LayerNormLongSumsKernel", "LayerNormSumKernel"}) precompileKernel("layer_norm.h", str(kernel, "<", t, ">"));
     for (const bool direct : {false, true})
         for (const GroupedTiles& tiles : GROUPED_TILES) {
-            if (p == Tensor::FLOAT && (direct || tiles.i != SMALL_TILES.i)) continue;
+            if (p == Tensor::FLOAT && (direct || tiles.i > SMALL_TILES.i)) continue;
             const std::string types = str(t, ", ", boolName(direct));
             for (const char* along : {", true, ", ", false, "}) precompileKernel("grouped_linear.h", str("GroupedRowsKernel<", types, along, tiles.arguments(), ">"));
-            if (direct || tiles.i != HUGE_TILES.i) precompileKernel("grouped_linear.h", str("GroupedWeightsKernel<", types, ", ", tiles.arguments(), ">"));
+            if (tiles.i != FEW_TILES.i && (direct || tiles.i != HUGE_TILES.i)) precompileKernel("grouped_linear.h", str("GroupedWeightsKernel<", types, ", ", tiles.arguments(), ">"));
         }
     for (const char* kernel : {"GroupedSumKernel", "GroupedJoinKernel"}) precompileKernel("grouped_linear.h", str(kernel, "<", t, ">"));
 }
