@@ -57,17 +57,33 @@ __device__ __forceinline__ void addTerms(float (&sum)[VEC], At at)
 #pragma unroll
         for (int k = 0; k < VEC; ++k) sum[k] += static_cast<float>(terms[n].v[k]);
 }
-/** Adds 'count' consecutive terms, eight of them in flight. */
-template <typename T, int VEC, typename At>
+/** Adds 'count' consecutive terms, as many of them in flight as go into REGISTERS. */
+template <typename T, int VEC, int REGISTERS, typename At>
 __device__ __forceinline__ void addRange(float (&sum)[VEC], int count, At at)
 {
+    constexpr int MOST = REGISTERS * 4 / (VEC * static_cast<int>(sizeof(T))), BATCH = MOST < 16 ? MOST : 16;
+    static_assert(BATCH >= 4, "batches, batches of 4, and single terms");
     int n = 0;
-    for (; n + 8 <= count; n += 8) addTerms<T, VEC, 8>(sum, [&](int k) { return at(n + k); });
-    if (n + 4 <= count) {
-        addTerms<T, VEC, 4>(sum, [&](int k) { return at(n + k); });
-        n += 4;
-    }
+    for (; n + BATCH <= count; n += BATCH) addTerms<T, VEC, BATCH>(sum, [&](int k) { return at(n + k); });
+    if constexpr (BATCH > 4)
+        for (; n + 4 <= count; n += 4) addTerms<T, VEC, 4>(sum, [&](int k) { return at(n + k); });
     for (; n < count; ++n) addTerms<T, VEC, 1>(sum, [&](int k) { return at(n + k); });
+}
+
+/**
+ * Adds the rows of dy at 'count' consecutive places of the order, which are looked up 64 at a time. WAVE: all lanes of the wavefront call it with
+ * the same place and count; a place is a lane's register then, which the others read.
+ */
+template <typename T, int VEC, int REGISTERS, bool WAVE>
+__device__ __forceinline__ void addPlaces(float (&sum)[VEC], const int* __restrict__ order, int count, const T* __restrict__ adjY, long long stride)
+{
+    if constexpr (WAVE)
+        for (int n = 0; n < count; n += 64) {
+            const int own = order[n + min(static_cast<int>(threadIdx.x % 64), count - n - 1)];
+            addRange<T, VEC, REGISTERS>(sum, min(64, count - n), [&](int k) { return adjY + __builtin_amdgcn_readlane(own, k) * stride; });
+        }
+    else
+        addRange<T, VEC, REGISTERS>(sum, count, [&](int n) { return adjY + order[n] * stride; });
 }
 
 /**
@@ -86,21 +102,12 @@ EmbeddingBlocksKernel(const unsigned* __restrict__ keys, const int* __restrict__
     if (FIRST && spans)
         for (long long i = from + threadIdx.x % G; i < min(to, rows); i += G) markSpans(keys, i, rows, vocabulary, spans);
     if (to > rows || keys[from] != keys[to - 1] || keys[from] >= vocabulary) return;
-    // All lanes go through the loop, those behind the last column with its address: a place of the order is a lane's register,
-    // which the others read.
+    // (all lanes go through the loop, those behind the last column with its address)
     for (int column = 0; column < C; column += G * VEC) {
         const int c = column + threadIdx.x % G * VEC, at = min(c, C - VEC);
         float sum[VEC] = {};
-        if constexpr (FIRST && G >= 64) {
-            static_assert(EMBEDDING_BLOCK_BITS == 6, "a place for each lane of a wavefront");
-            const int own = order[from + threadIdx.x % 64];
-#pragma unroll
-            for (int n = 0; n < 64; n += 16)
-                addTerms<T, VEC, 16>(sum, [&](int k) { return adjY + __builtin_amdgcn_readlane(own, n + k) * strideAdjY + at; });
-        } else if constexpr (FIRST)
-            addRange<T>(sum, 1 << EMBEDDING_BLOCK_BITS, [&](int i) { return adjY + order[from + i] * strideAdjY + at; });
-        else
-            addRange<float>(sum, 1 << EMBEDDING_BLOCK_BITS, [&](int i) { return smaller + ((block << EMBEDDING_BLOCK_BITS) + i) * C + at; });
+        if constexpr (FIRST) addPlaces<T, VEC, 64, (G >= 64)>(sum, order + from, 1 << EMBEDDING_BLOCK_BITS, adjY + at, strideAdjY);
+        else addRange<float, VEC, 64>(sum, 1 << EMBEDDING_BLOCK_BITS, [&](int i) { return smaller + ((block << EMBEDDING_BLOCK_BITS) + i) * C + at; });
         if (c < C) storeFloats(sums + block * C + at, sum);
     }
 }
@@ -115,21 +122,23 @@ struct EmbeddingBlocks
 
 constexpr int EMBEDDING_MOST_ROWS = 64;
 /**
- * The gradient of 'each' (up to EMBEDDING_MOST_ROWS) consecutive rows of the table per workgroup, G lanes per row. Their spans are
- * looked up together first, with the only term of those that have one.
+ * The gradient of up to 'each' (EMBEDDING_MOST_ROWS at most) rows of the table per workgroup, G lanes per row. Their spans are
+ * looked up together first, with the only term of those that have one. The rows of a workgroup are those of its number and as many as
+ * there are workgroups apart: frequent tokens often have neighbouring numbers (65536 tokens of a vocabulary of 65536 x 1024 bfloat16 in the
+ * order of their frequency: 54 us, 236 with consecutive rows), and workgroups that write consecutive rows write all channels of the
+ * memory at a time (tokens that name no row: 25 us, 42 with consecutive rows per workgroup).
  */
 template <typename T, int VEC, int G>
 __global__ void __launch_bounds__(EMBEDDING_THREADS)
 EmbeddingAdjointKernel(const unsigned* __restrict__ keys, const unsigned* __restrict__ spans, const int* __restrict__ order, long long rows,
                        EmbeddingBlocks blocks, const T* __restrict__ adjY, long long strideAdjY, float scale, T* __restrict__ adjTable,
-                       long long strideTable, long long vocabulary, int C, int each)
+                       long long strideTable, long long vocabulary, int C)
 {
     __shared__ unsigned begin[EMBEDDING_MOST_ROWS], end[EMBEDDING_MOST_ROWS];
     __shared__ int only[EMBEDDING_MOST_ROWS];
-    const long long firstRow = static_cast<long long>(blockIdx.x) * each;
-    const int count = static_cast<int>(min(static_cast<long long>(each), vocabulary - firstRow));
+    const int count = static_cast<int>((vocabulary - blockIdx.x + gridDim.x - 1) / gridDim.x);
     if (static_cast<int>(threadIdx.x) < count) {
-        const long long v = firstRow + threadIdx.x;
+        const long long v = blockIdx.x + static_cast<long long>(threadIdx.x) * gridDim.x;
         const unsigned from = spans[v], to = spans[vocabulary + v];
         const bool any = from < rows && keys[from] == v;   // otherwise no token names the row, and nothing was written there
         begin[threadIdx.x] = any ? from : 0;
@@ -147,8 +156,8 @@ EmbeddingAdjointKernel(const unsigned* __restrict__ keys, const unsigned* __rest
             single = __builtin_amdgcn_readfirstlane(single);
         }
         const long long from = span[0], to = span[1];
-        for (int c = lane * VEC; c < C; c += G * VEC) {
-            const int at = VEC == 1 ? c : min(c, C - VEC);
+        for (int column = 0; column < C; column += G * VEC) {   // (all lanes, as above)
+            const int c = column + lane * VEC, at = min(c, C - VEC);
             float sum[VEC] = {};
             if (to - from == 1) addTerms<T, VEC, 1>(sum, [&](int) { return adjY + single * strideAdjY + at; });
             else if (to > from) {
@@ -158,10 +167,10 @@ EmbeddingAdjointKernel(const unsigned* __restrict__ keys, const unsigned* __rest
                     const int bits = EMBEDDING_BLOCK_BITS * size;
                     const long long first = i >> bits;
                     const int terms = static_cast<int>((last - i) >> bits);
-                    if (size == 0) addRange<T>(sum, terms, [&](int n) { return adjY + order[first + n] * strideAdjY + at; });
+                    if (size == 0) addPlaces<T, VEC, 32, (G >= 64)>(sum, order + first, terms, adjY + at, strideAdjY);
                     else {
                         const float* p = blocks.sums[size - 1] + first * C + at;
-                        addRange<float>(sum, terms, [&](int n) { return p + static_cast<long long>(n) * C; });
+                        addRange<float, VEC, 32>(sum, terms, [&](int n) { return p + static_cast<long long>(n) * C; });
                     }
                     i = last;
                 };
@@ -175,7 +184,7 @@ EmbeddingAdjointKernel(const unsigned* __restrict__ keys, const unsigned* __rest
             }
 #pragma unroll
             for (int k = 0; k < VEC; ++k) sum[k] *= scale;
-            storeFloats(adjTable + (firstRow + r) * strideTable + at, sum);
+            if (c < C) storeFloats(adjTable + (blockIdx.x + static_cast<long long>(r) * gridDim.x) * strideTable + at, sum);
         }
     }
 }

@@ -229,15 +229,27 @@ GroupScanKernel(unsigned* __restrict__ counts, int tiles, int digits, unsigned* 
     const int each = (tiles + GROUP_SCAN_SLICES - 1) / GROUP_SCAN_SLICES;
     const int from = min(slice * each, tiles), to = d < digits ? min(from + each, tiles) : from;
     unsigned sum = 0;
+    constexpr int KEPT = 16;   // that many per slice are read once
+    unsigned kept[KEPT];
+    unsigned* const own = counts + static_cast<long long>(from) * digits + d;
+#pragma unroll
+    for (int n = 0; n < KEPT; ++n) kept[n] = from + n < to ? own[static_cast<long long>(n) * digits] : 0;
+#pragma unroll
+    for (int n = 0; n < KEPT; ++n) sum += kept[n];
 #pragma unroll 8
-    for (int t = from; t < to; ++t) sum += counts[static_cast<long long>(t) * digits + d];
+    for (int t = from + KEPT; t < to; ++t) sum += counts[static_cast<long long>(t) * digits + d];
     sums[slice][column] = sum;
     __syncthreads();
     unsigned before = 0;
     for (int s = 0; s < slice; ++s) before += sums[s][column];
     if (d < digits && slice == GROUP_SCAN_SLICES - 1) totals[d] = before + sum;
+#pragma unroll
+    for (int n = 0; n < KEPT; ++n) {
+        if (from + n < to) own[static_cast<long long>(n) * digits] = before;
+        before += kept[n];
+    }
 #pragma unroll 8
-    for (int t = from; t < to; ++t) {
+    for (int t = from + KEPT; t < to; ++t) {
         unsigned* const at = counts + static_cast<long long>(t) * digits + d;
         const unsigned v = *at;
         *at = before;
@@ -262,6 +274,10 @@ GroupScatterKernel(GroupSource<I> source, long long rows, int shift, int digitBi
     unsigned short* const counters = reinterpret_cast<unsigned short*>(groupLds + digits);   // [wavefront][digit]
     __shared__ unsigned sums[WAVES];
     const int wave = threadIdx.x / 64;
+    // Workgroups go to the dies in turn; a die takes consecutive tiles, whose rows of a group come one after the other, so that the lines it
+    // writes parts of are its own for the most part.
+    const unsigned die = blockIdx.x % DIES;
+    const int tile = static_cast<int>(die * (gridDim.x / DIES) + min(die, gridDim.x % DIES) + blockIdx.x / DIES);
     constexpr int OWN = (GROUP_MOST_DIGITS + GROUP_THREADS - 1) / GROUP_THREADS;
     unsigned before[OWN];   // rows of the thread's digits in the tiles before
 #pragma unroll
@@ -270,7 +286,7 @@ GroupScatterKernel(GroupSource<I> source, long long rows, int shift, int digitBi
         if (d >= digits) break;
         if (totals) {
             starts[d] = totals[d];
-            before[n] = counts[static_cast<long long>(blockIdx.x) * digits + d];
+            before[n] = counts[static_cast<long long>(tile) * digits + d];
         } else {
             unsigned all = 0, those = 0;
             const int tiles = gridDim.x;
@@ -278,16 +294,15 @@ GroupScatterKernel(GroupSource<I> source, long long rows, int shift, int digitBi
             for (int t = 0; t < tiles; ++t) {
                 const unsigned here = counts[t * digits + d];
                 all += here;
-                those += t < static_cast<int>(blockIdx.x) ? here : 0;
+                those += t < tile ? here : 0;
             }
             starts[d] = all;
             before[n] = those;
         }
-#pragma unroll
-        for (int w = 0; w < WAVES; ++w) counters[w * digits + d] = 0;
     }
+    for (int i = threadIdx.x; i < (digits * WAVES + 1) / 2; i += GROUP_THREADS) reinterpret_cast<unsigned*>(counters)[i] = 0;
     // a wavefront takes consecutive rows, 64 at a time
-    const long long first = static_cast<long long>(blockIdx.x) * (GROUP_THREADS * ITEMS) + wave * (64 * ITEMS) + threadIdx.x % 64;
+    const long long first = static_cast<long long>(tile) * (GROUP_THREADS * ITEMS) + wave * (64 * ITEMS) + threadIdx.x % 64;
     unsigned key[ITEMS];
     int row[ITEMS];
     unsigned short place[ITEMS];
@@ -299,7 +314,7 @@ GroupScatterKernel(GroupSource<I> source, long long rows, int shift, int digitBi
         }
     __syncthreads();
     scanInLds<GROUP_THREADS>(starts, digits, sums);
-    if (offsets && blockIdx.x == 0)
+    if (offsets && tile == 0)
         for (unsigned g = threadIdx.x; g <= source.groups; g += GROUP_THREADS) offsets[g] = static_cast<int>(starts[g]);   // (nothing is before the first tile)
 #pragma unroll
     for (int n = 0; n < OWN; ++n) {

@@ -584,7 +584,7 @@ void Tokens::embeddingAdjoint(const Tensor& index, const Tensor& adjOutput, floa
     const int each = embeddingAdjointRows(vocabulary, lanes);
     tokenKernel("embedding.h", kernelKey(EMBEDDING_ADJOINT, p, vec, lanes), [&] { return "EmbeddingAdjointKernel" + arguments() + ">"; })
         .call(static_cast<unsigned>(divUp<int64_t>(vocabulary, each)), EMBEDDING_THREADS, 0, stream, static_cast<const unsigned*>(plan.keys), static_cast<const unsigned*>(plan.spans), static_cast<const int*>(plan.order), rows, plan.blocks, dy, strideOf(adjOutput, 0), scale,
-              adjTable.rawPtr(), strideOf(adjTable, 0), vocabulary, C, each);
+              adjTable.rawPtr(), strideOf(adjTable, 0), vocabulary, C);
 }
 
 void Tokens::layerNorm(const Tensor& input, const Tensor& weight, const Tensor& bias, float epsilon, Tensor& output, Tensor& mean, Tensor& rstd,
