@@ -37,8 +37,8 @@ class Experts(torch.nn.Module):
         order, offsets = tokens.group(experts.flatten(), self.first.weight.shape[0])
         places = torch.empty_like(order)
         places[order.long()] = torch.arange(len(order), dtype=order.dtype, device=order.device)
-        rows = tokens.embedding(order // self.chosen, normal)
-        rows = self.second(self.activation(self.first(rows, offsets)), offsets)
+        rows = tokens.embedding(order // self.chosen, normal.half())
+        rows = self.second(self.activation(self.first(rows, offsets)), offsets)   # in 16 bits, as the activation works
         back = tokens.embedding(places.view(len(x), self.chosen), rows)
         return x + (back * weights[..., None]).sum(1)
 
@@ -60,7 +60,7 @@ class ObjectFields(torch.nn.Module):
     def forward(self, objects, positions):
         """The fields of the objects (B) at their positions (B, P, 3): (B, P)."""
         codes = self.experts(self.codes(objects))
-        inputs = torch.cat([positions, codes[:, None, :].expand(-1, positions.shape[1], -1)], 2)
+        inputs = torch.cat([2 * positions - 1, codes[:, None, :].expand(-1, positions.shape[1], -1)], 2)
         return self.decoder(inputs.reshape(-1, inputs.shape[2])).view(positions.shape[:2])
 
 
@@ -69,7 +69,7 @@ def train(steps=300, objects=500, batch=256, points=64, seed=0):
     torch.manual_seed(seed)
     centres, radii = torch.rand(objects, 3, device="cuda"), 0.1 + 0.3 * torch.rand(objects, device="cuda")
     model = ObjectFields(objects)
-    optimizer = torch.optim.Adam(model.parameters(), lr=5e-3)
+    optimizer = torch.optim.Adam(model.parameters(), lr=1e-2)
     losses = []
     for _ in range(steps):
         index = torch.randint(0, objects, (batch,), device="cuda")

@@ -236,7 +236,7 @@ __device__ __forceinline__ u32x4 bufferAt(const void* p, unsigned bytes)
  */
 __device__ __forceinline__ void loadToLds(u32x4 buffer, unsigned offset, unsigned lds)
 {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(buffer) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(buffer) : "memory", "m0");
 }
 /** The wavefront's writes to and reads of LDS are done, and so are those of the others. */
 __device__ __forceinline__ void waitForLds()

@@ -189,8 +189,7 @@ struct GroupPlan
         passes = groups < GROUP_MOST_DIGITS ? 1 : divUp(bits, GROUP_PASS_BITS);
         digitBits = divUp(bits, passes);
         maxDigits = static_cast<int>(std::min<int64_t>(1ll << digitBits, static_cast<int64_t>(groups) + 1));
-        // a workgroup for every compute unit: tiles of one row per thread, of four where there are as many anyway (2^20 rows of 4096
-        // groups: XX us, with one XX)
+        // a workgroup for every compute unit: tiles of one row per thread, of four where there are as many anyway
         items = rows <= 256 * GROUP_THREADS ? 1 : 4;
         tiles = divUp<int64_t>(rows, GROUP_THREADS * items);
         if (small) return;
@@ -334,8 +333,11 @@ struct GroupedTiles
 {
     int i, j, wavesI, wavesJ;
     int threads() const { return 64 * wavesI * wavesJ; }
-    /** Two tiles of each operand (one, where that is all there is of K), later the results. */
-    unsigned lds(int64_t K, int entry) const { return static_cast<unsigned>(std::max((K * entry <= 128 ? 1 : 2) * 128 * (i + j), i * j * entry)); }
+    /** Two tiles of each operand (one, where that is all there is of K; through registers a second one is written all the same), later the results. */
+    unsigned lds(int64_t K, int entry, bool direct) const
+    {
+        return static_cast<unsigned>(std::max((direct && K * entry <= 128 ? 1 : 2) * 128 * (i + j), i * j * entry));
+    }
     std::string arguments() const { return str(i, ", ", j, ", ", wavesI, ", ", wavesJ); }
 };
 constexpr GroupedTiles HUGE_TILES = {256, 256, 2, 4}, LARGE_TILES = {128, 128, 2, 2}, SMALL_TILES = {64, 64, 2, 2}, FEW_TILES = {32, 64, 1, 2};
@@ -488,7 +490,7 @@ void launchRows(bool alongK, const Tensor& x, const Tensor& weight, const Tensor
     float* partial = plan.slices > 1 ? static_cast<float*>(memory) : nullptr;
     tokenKernel("grouped_linear.h", kernelKey(GROUPED_ROWS, p * 4 + direct * 2 + alongK, t.i, t.j, t.wavesI, t.wavesJ),
                 [&] { return str("GroupedRowsKernel<", scalarName(p), ", ", boolName(direct), ", ", boolName(alongK), ", ", t.arguments(), ">"); })
-        .call(static_cast<unsigned>(groups), t.threads(), t.lds(plan.slice, x.bytesPerEntry()), stream, x.rawPtr(), strideOf(x, 0),
+        .call(static_cast<unsigned>(groups), t.threads(), t.lds(plan.slice, x.bytesPerEntry(), direct), stream, x.rawPtr(), strideOf(x, 0),
               static_cast<const void*>(ptr<void>(weight)), strideOf(weight, 0), strideOf(weight, 1), static_cast<const void*>(ptr<void>(bias)),
               bias.defined() ? strideOf(bias, 0) : 0ll, static_cast<const int*>(ptr<int>(offsets)), s.experts, static_cast<void*>(ptr<void>(y)),
               strideOf(y, 0), s.rows, J, K, static_cast<int>(plan.places), static_cast<int>(plan.tilesJ), plan.slices, plan.slice, partial);
@@ -782,7 +784,7 @@ void Tokens::groupedLinearAdjoint(const Tensor& input, const Tensor& weight, con
     const int chunk = static_cast<int>(plan.chunk);
     tokenKernel("grouped_linear.h", kernelKey(GROUPED_WEIGHTS, p * 2 + direct, plan.tiles.i, plan.tiles.j, plan.tiles.wavesI, plan.tiles.wavesJ),
                 [&] { return str("GroupedWeightsKernel<", scalarName(p), ", ", boolName(direct), ", ", plan.tiles.arguments(), ">"); })
-        .call(static_cast<unsigned>(groups), plan.tiles.threads(), plan.tiles.lds(s.rows, input.bytesPerEntry()), stream, dy, strideOf(adjOutput, 0), x, strideOf(input, 0), off, s.experts,
+        .call(static_cast<unsigned>(groups), plan.tiles.threads(), plan.tiles.lds(s.rows, input.bytesPerEntry(), direct), stream, dy, strideOf(adjOutput, 0), x, strideOf(input, 0), off, s.experts,
               ptr<void>(adjWeight), ptr<void>(adjBias), plan.partial, s.rows, s.outputs, s.inputs,
               static_cast<int>(plan.places), static_cast<int>(plan.tilesI), static_cast<int>(plan.tilesJ), chunk);
     if (plan.partial) {

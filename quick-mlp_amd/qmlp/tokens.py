@@ -98,7 +98,8 @@ class FusedLayerNorm(torch.nn.Module):
 
 
 class FusedGroupedLinear(torch.nn.Module):
-    """A linear layer per expert, and :func:`grouped_linear` with them."""
+    """A linear layer per expert, and :func:`grouped_linear` with them, in the type of the rows: as with :class:`qmlp.FusedNetwork` the
+    parameters may be float32 for the optimizer while the layers are evaluated in 16 bits."""
 
     def __init__(self, experts: int, inputs: int, outputs: int, bias: bool = True, dtype=torch.float32, device="cuda"):
         super().__init__()
@@ -107,7 +108,8 @@ class FusedGroupedLinear(torch.nn.Module):
         self.bias = torch.nn.Parameter(torch.zeros(experts, outputs, dtype=dtype, device=device)) if bias else None
 
     def forward(self, x: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
-        return grouped_linear(x, self.weight, offsets, self.bias)
+        bias = self.bias.to(x.dtype) if self.bias is not None else None
+        return grouped_linear(x, self.weight.to(x.dtype), offsets, bias)
 
     def extra_repr(self):
         experts, outputs, inputs = self.weight.shape
