@@ -669,15 +669,27 @@ at::Tensor embedding(const at::Tensor& index, const at::Tensor& table, double sc
     return output;
 }
 
+/** A row of a contiguous matrix that may be undefined. */
+qmlp_tensor rowOf(const at::Tensor& t, int row)
+{
+    qmlp_tensor d = wrapToken(t);
+    if (!t.defined()) return d;
+    d.data = static_cast<char*>(d.data) + row * t.stride(0) * t.element_size();
+    d.ndim = 1;
+    d.sizes[0] = d.sizes[1];
+    d.strides[0] = 1;
+    return d;
+}
+
 struct LayerNormBackward : TokenNode
 {
     at::ScalarType weightType = at::kFloat;
     std::string name() const override { return "QmlpLayerNormBackward"; }
     void adjoint(const at::Tensor& gradOutput, variable_list& grads) override
     {
-        const at::Tensor x = saved[0].unpack(), weight = saved[1].unpack(), mean = saved[2].unpack(), rstd = saved[3].unpack();
+        const at::Tensor x = saved[0].unpack(), weight = saved[1].unpack(), statistics = saved[2].unpack();
         const int64_t channels = x.size(-1);
-        const at::Tensor rows = consecutive(x.reshape({mean.size(0), channels})), adjOutput = consecutive(gradOutput.reshape(rows.sizes()));
+        const at::Tensor rows = consecutive(x.reshape({statistics.size(1), channels})), adjOutput = consecutive(gradOutput.reshape(rows.sizes()));
         const bool sums = task_should_compute_output(1) || task_should_compute_output(2);
         at::Tensor adjX, adjWeight, adjBias;
         if (task_should_compute_output(0)) adjX = at::empty(rows.sizes(), rows.options());
@@ -686,7 +698,7 @@ struct LayerNormBackward : TokenNode
         size_t bytes = 0;
         if (sums) check(qmlp_tokens_layer_norm_adjoint_memory(rows.size(0), static_cast<int>(channels), &bytes));
         const at::Tensor memory = temporary(rows, bytes);
-        const qmlp_tensor in = wrapToken(rows), w = wrapToken(weight), m = wrapToken(mean), r = wrapToken(rstd), dy = wrapToken(adjOutput),
+        const qmlp_tensor in = wrapToken(rows), w = wrapToken(weight), m = rowOf(statistics, 0), r = rowOf(statistics, 1), dy = wrapToken(adjOutput),
                           dx = wrapToken(adjX), dw = wrapToken(adjWeight), db = wrapToken(adjBias);
         check(qmlp_tokens_layer_norm_adjoint(&in, &w, &m, &r, &dy, &dx, &dw, &db, dataOf(memory), currentStream(rows)));
         if (adjX.defined()) grads[0] = adjX.view(x.sizes());
@@ -702,23 +714,20 @@ at::Tensor layerNorm(const at::Tensor& x, const at::Tensor& weight, const at::Te
     refuseOtherModes({x, weight, bias});
     if (x.dim() < 1) throw std::runtime_error("input must have a dimension of channels");
     const bool train = wantsGradient(x) || wantsGradient(weight) || wantsGradient(bias);
-    at::Tensor mean, rstd, w;
+    at::Tensor statistics, w;   // mean and 1 / sqrt(variance + epsilon) of every row
     const at::Tensor output = guarded(x, [&] {
         const int64_t channels = x.size(-1), count = channels > 0 ? x.numel() / channels : 0;
         const at::Tensor rows = consecutive(x.dim() == 2 ? x : x.reshape({count, channels}));
         const at::Tensor out = at::empty({rows.size(0), channels}, x.options().requires_grad(false));
         w = consecutive(weight);
         const at::Tensor b = consecutive(bias);
-        if (train) {
-            mean = at::empty({rows.size(0)}, out.options().dtype(at::kFloat));
-            rstd = at::empty({rows.size(0)}, out.options().dtype(at::kFloat));
-        }
-        const qmlp_tensor in = wrapToken(rows), wt = wrapToken(w), bt = wrapToken(b), o = wrapToken(out), m = wrapToken(mean), r = wrapToken(rstd);
+        if (train) statistics = at::empty({2, rows.size(0)}, out.options().dtype(at::kFloat));
+        const qmlp_tensor in = wrapToken(rows), wt = wrapToken(w), bt = wrapToken(b), o = wrapToken(out), m = rowOf(statistics, 0), r = rowOf(statistics, 1);
         check(qmlp_tokens_layer_norm(&in, &wt, &bt, static_cast<float>(epsilon), &o, &m, &r, currentStream(x)));
         return x.dim() == 2 ? out : out.view(x.sizes());
     });
     if (train) {
-        auto node = attach<LayerNormBackward>(output, {x, weight, bias}, {x, w.defined() && !w.is_same(weight) ? w.detach() : weight, mean, rstd});
+        auto node = attach<LayerNormBackward>(output, {x, weight, bias}, {x, w.defined() && !w.is_same(weight) ? w.detach() : weight, statistics});
         node->weightType = weight.defined() ? weight.scalar_type() : bias.defined() ? bias.scalar_type() : x.scalar_type();
     }
     return output;

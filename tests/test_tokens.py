@@ -4,6 +4,7 @@ Tolerances follow from the operators: sums of n terms are held in 32 bits, which
 magnitudes (in any order, with a bit to spare for the matrix cores' own rounding), and a result is rounded once to its type.
 """
 import ctypes
+import os
 
 import numpy as np
 import pytest
@@ -14,6 +15,13 @@ from qmlp import _lib
 from qmlp import tokens
 
 gpu = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def no_warming(request):
+    """(a pass without a GPU that fills the kernel cache: these kernels do not depend on the test)"""
+    if os.environ.get("QMLP_WARM_CACHE") and "gpu" in request.keywords:
+        pytest.skip("kernels are compiled by qmlp.tokens.precompile")
 
 DTYPES = [torch.float32, torch.float16, torch.bfloat16]
 ROUNDING = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
