@@ -11,9 +11,15 @@
 // How many rows an expert has is known on the device only. The rows of the experts are cut into tiles that begin where the
 // expert does, and the places of the tiles follow without a scan: expert e has the places from e + floor(offsets[e] / TI) on,
 // of which it has always enough, as floor(b / T) - floor(a / T) + 1 >= ceil((b - a) / T). A workgroup finds the expert of its
-// place among the offsets, 64 or all of them at a time, and has nothing to do where the expert has fewer tiles than places.
+// place among the offsets, 64 at a time, and has nothing to do where the expert has fewer tiles than places.
 //
 // Offsets are limited to the rows there are wherever they are read: no access depends on their values.
+//
+// What bounds them: the matrix cores where experts have many rows, and there the power that is left for the clock (fewer cycles
+// for the same tiles came with a lower clock, 2.02 to 1.82 GHz, in the same time); the weights' bytes where experts have few rows;
+// the latency of a tile's first bytes in between. Measured, us for y, dx and dW + db: 32768 rows of 16 experts, 2048 -> 4096, bfloat16 620, 610,
+// 577 (890 to 950 TFLOP/s; a large product of the same card reaches 1390); 2^17 rows of 512 experts, 64 -> 64, half 16.3, 15.0, 13.5; 5003 rows
+// of 12 experts, 333 -> 200, float 21, 22, 23 + 5; y of 24 rows of 64 experts, 1024 -> 4096, bfloat16 33 (the weights: 4.8 TB/s).
 
 #include <qmlp/kernels/token_types.h>
 
@@ -552,28 +558,18 @@ struct ExpertTile
 /** What the given place has; to <= from: nothing. */
 __device__ __forceinline__ ExpertTile expertTile(const int* __restrict__ offsets, int experts, int rows, int tileRows, int place)
 {
-    // the last e of 0 .. experts with e + floor(begin / tileRows) <= place; the first one has that
-    auto reached = [&](int e) { return __ballot(e <= experts && e + expertBegin(offsets, min(e, experts), rows) / tileRows <= place); };
+    // the last e of 0 .. experts with e + floor(begin / tileRows) <= place, which the first one has: 64 of those behind it at a time
     const int lane = threadIdx.x % 64;
-    int from = 0;
-    if (experts < 8 * 64) {   // all of them at once
-        int count = 0;
-#pragma unroll
-        for (int n = 0; n < 8; ++n) count += __popcll(reached(n * 64 + lane));
-        from = min(max(count - 1, 0), experts);
-    } else {
-        int count = experts + 1;
-        while (count > 1) {
-            const int step = (count + 63) / 64;
-            // (the first lane has reached its own; where the offsets are in order, so have the lanes up to the one looked for)
-            const int last = max(0, 63 - __clzll(reached(from + min(lane * step, count - 1))));
-            const int chosen = min(last * step, count - 1);
-            from += chosen;
-            count = min(step, count - chosen);
-        }
+    int from = 0, begin = 0, end = rows;   // of expert 'from'; the end while it is the last one
+    for (int count = experts; count > 0;) {
+        const int step = (count + 63) / 64, ahead = (lane + 1) * step, e = from + min(ahead, count);
+        const int begins = expertBegin(offsets, e, rows);
+        const int reached = __popcll(__ballot(ahead <= count && e + static_cast<int>(static_cast<unsigned>(begins) / tileRows) <= place));
+        if (reached > 0) begin = __builtin_amdgcn_readlane(begins, reached - 1);
+        if (reached < 64 && (reached + 1) * step <= count) end = __builtin_amdgcn_readlane(begins, reached);
+        from += reached * step;
+        count = min(step - 1, count - reached * step);
     }
-    from = __builtin_amdgcn_readfirstlane(from);
-    const int begin = expertBegin(offsets, from, rows), end = from < experts ? expertBegin(offsets, from + 1, rows) : rows;
     ExpertTile t;
     t.expert = from;
     t.index = place - (from + begin / tileRows);

@@ -350,7 +350,8 @@ const std::array<GroupedTiles, 4> GROUPED_TILES = {HUGE_TILES, LARGE_TILES, SMAL
  * 32768 rows, K 2048, J 4096: 610 | 670 | 958; 54272, 2240, 256: 79 | 94 | 140; 54272, 256, 2240: 142 | 139 | 192; 16384, 1024, 1024: 65 | 51 | 64;
  * 4096, 1024, 1024: 34 | 22 | 25; 16384, 4096, 64: 91 | 47 | 38; through registers 32768, 2047, 4095: 840 | 996 | 1467.
  * Single precision is bound by the matrix cores with small tiles as well (16384 rows, 4 experts, 1024, 1024: - | 342 | 322).
- * Where an expert has few rows, the weights are what is read: small | few: 24 rows of 64 experts, K 1024, J 4096: 53 | 44.
+ * Where an expert has few rows, the weights are what is read: small | few: 24 rows of 64 experts, K 1024, J 4096: 53 | 44
+ * (33 with its K shared out, RowsPlan).
  */
 GroupedTiles rowsTiles(Tensor::Precision p, int64_t rows, int64_t experts, int64_t J, int64_t K)
 {

@@ -366,6 +366,42 @@ def test_grouped_linear_and_its_gradients(counts, inputs, outputs, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("experts", [63, 64, 65, 128, 511, 512, 513, 4095, 4096, 4097, 5000])
+def test_numbers_of_experts(experts):
+    """A workgroup looks for its expert 64 at a time: numbers around the powers of 64, experts without rows among them."""
+    say("numbers of experts", experts)
+    g = generator(experts)
+    counts = [(11 * e + experts) % 5 * (e % 3 != 1) + 70 * (e in (0, 63, 64, experts - 1)) for e in range(experts)]
+    rows = sum(counts) + 3
+    x, weight = normal(g, rows, 16, dtype=torch.float16).requires_grad_(), normal(g, experts, 8, 16, dtype=torch.float16).requires_grad_()
+    grad = normal(g, rows, 8, dtype=torch.float16)
+    y = tokens.grouped_linear(x, weight, offsets_of(counts))
+    gradients = torch.autograd.grad(y, (x, weight), grad)
+    exact = grouped_reference(x.detach(), weight.detach(), counts, None, grad)
+    for value, (expected, error), what in zip((y.detach(), *gradients), exact, ("y", "x", "weight")):
+        near(value, expected, error, what)
+
+
+@gpu
+@pytest.mark.parametrize("stride", [(1 << 21) - 8, 1 << 21, (1 << 21) + 8, (1 << 22) + 1])
+def test_grouped_linear_of_rows_far_apart(stride):
+    """256 rows of a tile are reached with 32-bit offsets where they lie less than 2^21 entries apart; others are copied first."""
+    say("rows far apart", stride)
+    g = generator(stride)
+    counts = [5, 0, 11]
+    memory = torch.zeros(17 * stride + 64, dtype=torch.bfloat16, device="cuda")
+    x = memory.as_strided((17, 48), (stride, 1))
+    x.copy_(normal(g, 17, 48, dtype=torch.bfloat16))
+    x.requires_grad_()
+    weight, grad = normal(g, 3, 24, 48, dtype=torch.bfloat16).requires_grad_(), normal(g, 17, 24, dtype=torch.bfloat16)
+    y = tokens.grouped_linear(x, weight, offsets_of(counts))
+    gradients = torch.autograd.grad(y, (x, weight), grad)
+    exact = grouped_reference(x.detach(), weight.detach(), counts, None, grad)
+    for value, (expected, error), what in zip((y.detach(), *gradients), exact, ("y", "x", "weight")):
+        near(value, expected, error, what)
+
+
+@gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_grouped_linear_of_other_strides(dtype):
     """Rows and matrices that lie apart, begin at odd addresses, or are one and the same; gradients of a shared matrix."""
