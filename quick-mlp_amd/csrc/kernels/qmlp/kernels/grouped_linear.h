@@ -257,7 +257,7 @@ __device__ __forceinline__ void waitForTiles()
 }
 
 /**
- * Moves the tiles of an operand of 16 bits straight from global memory to LDS. The address, the strides and the operand's sizes are
+ * Moves the tiles of an operand straight from global memory to LDS. The address, the strides and the operand's sizes are
  * multiples of 16 bytes, and rows do not overlap. Indices that are not there hold others' values, which no result depends on;
  * k that are not there are zero.
  */

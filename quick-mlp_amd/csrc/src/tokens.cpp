@@ -349,7 +349,7 @@ const std::array<GroupedTiles, 4> GROUPED_TILES = {HUGE_TILES, LARGE_TILES, SMAL
  * small ones pay where larger ones would leave compute units without work. us, huge | large | small, bfloat16, 16 or 17 experts:
  * 32768 rows, K 2048, J 4096: 610 | 670 | 958; 54272, 2240, 256: 79 | 94 | 140; 54272, 256, 2240: 142 | 139 | 192; 16384, 1024, 1024: 65 | 51 | 64;
  * 4096, 1024, 1024: 34 | 22 | 25; 16384, 4096, 64: 91 | 47 | 38; through registers 32768, 2047, 4095: 840 | 996 | 1467.
- * Single precision is bound by the matrix cores with small tiles as well (16384 rows, 4 experts, 1024, 1024: - | 342 | 322).
+ * Single precision is bound by the matrix cores with small tiles as well (16384 rows, 4 experts, 1024, 1024: - | 365 | 343).
  * Where an expert has few rows, the weights are what is read: small | few: 24 rows of 64 experts, K 1024, J 4096: 53 | 44
  * (33 with its K shared out, RowsPlan).
  */
@@ -365,13 +365,15 @@ GroupedTiles rowsTiles(Tensor::Precision p, int64_t rows, int64_t experts, int64
 /**
  * The tiles of the weights' gradients, experts x (I, J), whose terms, an expert's rows, may be shared out in chunks. us, huge | large | small, as above:
  * 32768 rows, I 4096, J 2048: 542 | 641 | 1001; 16384, 1024, 1024: 127 | 48 | 65; through registers, where the huge tile's registers do not
- * suffice, 32768, 4095, 2047: 1095 | 982 | 1488; float, 16384 rows of 4 experts, 1024, 1024: - | 317 | 324; 16384 of 16, 1024, 64: - | 57 | 37.
+ * suffice, 32768, 4095, 2047: 1095 | 982 | 1488; float, 16384 rows of 4
+ * experts, 1024, 1024: - | 302 | 337 (through registers - | 317 | 324); 32768 of 16, 512, 2048: - | 554 | 615; 20000 of 12, 192, 320: - | 46 | 40;
+ * 16384 of 16, 64, 1024: - | 44 | 28.
  */
 GroupedTiles weightsTiles(Tensor::Precision p, int64_t rows, int64_t experts, int64_t I, int64_t J, bool direct)
 {
-    if (p == Tensor::FLOAT) return SMALL_TILES;
     const int64_t each = divUp(rows, experts);
     auto count = [&](const GroupedTiles& t, int64_t chunk) { return experts * divUp<int64_t>(I, t.i) * divUp<int64_t>(J, t.j) * std::max<int64_t>(1, each / chunk); };
+    if (p == Tensor::FLOAT) return direct && I > 64 && J > 64 && count(LARGE_TILES, 2048) >= 256 ? LARGE_TILES : SMALL_TILES;
     if (direct && I > 128 && J > 128 && each >= 512 && count(HUGE_TILES, 2048) >= 512) return HUGE_TILES;
     return I > 64 && J > 64 && count(LARGE_TILES, 256) >= 256 ? LARGE_TILES : SMALL_TILES;
 }
@@ -379,11 +381,11 @@ GroupedTiles weightsTiles(Tensor::Precision p, int64_t rows, int64_t experts, in
 /** Whether tiles of the operand can go straight from global memory to LDS (DirectTile). */
 bool isDirect(const Tensor& t)
 {
-    if (t.bytesPerEntry() != 2 || reinterpret_cast<uintptr_t>(t.rawPtr()) % 16 != 0) return false;
-    const int n = t.ndim();
-    if (t.size(n - 1) % 8 != 0) return false;
+    if (reinterpret_cast<uintptr_t>(t.rawPtr()) % 16 != 0) return false;
+    const int n = t.ndim(), piece = 16 / static_cast<int>(t.bytesPerEntry());
+    if (t.size(n - 1) % piece != 0) return false;
     for (int d = 0; d + 1 < n; ++d)
-        if (t.size(d) > 1 && t.stride(d) % 8 != 0) return false;
+        if (t.size(d) > 1 && t.stride(d) % piece != 0) return false;
     // rows that do not overlap, 256 of which have 32-bit offsets
     return t.size(n - 2) <= 1 || (t.stride(n - 2) >= t.size(n - 1) && t.stride(n - 2) < (1 << 21));
 }
@@ -828,10 +830,12 @@ void Tokens::precompile(Tensor::Precision p)
     for (const char* kernel : {"LayerNormLongSumsKernel", "LayerNormSumKernel"}) precompileKernel("layer_norm.h", str(kernel, "<", t, ">"));
     for (const bool direct : {false, true})
         for (const GroupedTiles& tiles : GROUPED_TILES) {
-            if (p == Tensor::FLOAT && (direct || tiles.i > SMALL_TILES.i)) continue;
+            const bool few = tiles.i == FEW_TILES.i, huge = tiles.i == HUGE_TILES.i, single = p == Tensor::FLOAT;
+            if (single && (huge || (tiles.i == LARGE_TILES.i && !direct))) continue;
             const std::string types = str(t, ", ", boolName(direct));
-            for (const char* along : {", true, ", ", false, "}) precompileKernel("grouped_linear.h", str("GroupedRowsKernel<", types, along, tiles.arguments(), ">"));
-            if (tiles.i != FEW_TILES.i && (direct || tiles.i != HUGE_TILES.i)) precompileKernel("grouped_linear.h", str("GroupedWeightsKernel<", types, ", ", tiles.arguments(), ">"));
+            for (const char* along : {", true, ", ", false, "})
+                if (!single || tiles.i <= SMALL_TILES.i) precompileKernel("grouped_linear.h", str("GroupedRowsKernel<", types, along, tiles.arguments(), ">"));
+            if (!few && (direct || !huge)) precompileKernel("grouped_linear.h", str("GroupedWeightsKernel<", types, ", ", tiles.arguments(), ">"));
         }
     for (const char* kernel : {"GroupedSumKernel", "GroupedJoinKernel"}) precompileKernel("grouped_linear.h", str(kernel, "<", t, ">"));
 }

@@ -383,6 +383,26 @@ def test_numbers_of_experts(experts):
 
 
 @gpu
+@pytest.mark.parametrize("inputs,outputs", [(520, 264), (521, 263), (96, 136)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_many_rows_of_many_experts(inputs, outputs, dtype):
+    """Enough work for the largest tiles, with and without alignment; experts whose rows end anywhere in one."""
+    say("many rows of many experts", inputs, outputs, dtype)
+    g = generator(outputs)
+    counts = [450 + (37 * e) % 140 for e in range(260)]
+    counts[7], counts[100], counts[259] = 0, 1, 3000
+    rows = sum(counts) + 5
+    x, weight = normal(g, rows, inputs, dtype=dtype).requires_grad_(), normal(g, 260, outputs, inputs, dtype=dtype).requires_grad_()
+    bias = normal(g, 260, outputs, dtype=dtype).requires_grad_()
+    grad = normal(g, rows, outputs, dtype=dtype)
+    y = tokens.grouped_linear(x, weight, offsets_of(counts), bias)
+    gradients = torch.autograd.grad(y, (x, weight, bias), grad)
+    exact = grouped_reference(x.detach(), weight.detach(), counts, bias.detach(), grad)
+    for value, (expected, error), what in zip((y.detach(), *gradients), exact, ("y", "x", "weight", "bias")):
+        near(value, expected, error, what)
+
+
+@gpu
 @pytest.mark.parametrize("stride", [(1 << 21) - 8, 1 << 21, (1 << 21) + 8, (1 << 22) + 1])
 def test_grouped_linear_of_rows_far_apart(stride):
     """256 rows of a tile are reached with 32-bit offsets where they lie less than 2^21 entries apart; others are copied first."""
