@@ -350,8 +350,9 @@ const std::array<GroupedTiles, 4> GROUPED_TILES = {HUGE_TILES, LARGE_TILES, SMAL
  * 32768 rows, K 2048, J 4096: 610 | 670 | 958; 54272, 2240, 256: 79 | 94 | 140; 54272, 256, 2240: 142 | 139 | 192; 16384, 1024, 1024: 65 | 51 | 64;
  * 4096, 1024, 1024: 34 | 22 | 25; 16384, 4096, 64: 91 | 47 | 38; through registers 32768, 2047, 4095: 840 | 996 | 1467.
  * Single precision is bound by the matrix cores with small tiles as well (16384 rows, 4 experts, 1024, 1024: - | 365 | 343).
- * Where an expert has few rows, the weights are what is read: small | few: 24 rows of 64 experts, K 1024, J 4096: 53 | 44
- * (33 with its K shared out, RowsPlan).
+ * Where an expert has few rows, the weights are what is read, and half of a small tile would be empty. small | few, y and dx of 64 experts,
+ * 1024 -> 4096, behind a training step's writes: 24 rows 69, 71 | 64, 48; 768 rows 141, 127 | 140, 115; 1536 rows 144, 123 | 140, 107; 2048 rows
+ * 140, 133 | 161, 162.
  */
 GroupedTiles rowsTiles(Tensor::Precision p, int64_t rows, int64_t experts, int64_t J, int64_t K)
 {
@@ -365,9 +366,8 @@ GroupedTiles rowsTiles(Tensor::Precision p, int64_t rows, int64_t experts, int64
 /**
  * The tiles of the weights' gradients, experts x (I, J), whose terms, an expert's rows, may be shared out in chunks. us, huge | large | small, as above:
  * 32768 rows, I 4096, J 2048: 542 | 641 | 1001; 16384, 1024, 1024: 127 | 48 | 65; through registers, where the huge tile's registers do not
- * suffice, 32768, 4095, 2047: 1095 | 982 | 1488; float, 16384 rows of 4
- * experts, 1024, 1024: - | 302 | 337 (through registers - | 317 | 324); 32768 of 16, 512, 2048: - | 554 | 615; 20000 of 12, 192, 320: - | 46 | 40;
- * 16384 of 16, 64, 1024: - | 44 | 28.
+ * suffice, 32768, 4095, 2047: 1095 | 982 | 1488; float, 16384 rows of 4 experts, 1024, 1024: - | 302 | 337 (through
+ * registers - | 317 | 324); 32768 of 16, 512, 2048: - | 554 | 615; 20000 of 12, 192, 320: - | 46 | 40; 16384 of 16, 64, 1024: - | 44 | 28.
  */
 GroupedTiles weightsTiles(Tensor::Precision p, int64_t rows, int64_t experts, int64_t I, int64_t J, bool direct)
 {
