@@ -43,7 +43,7 @@ EmbeddingKernel(const I* __restrict__ index, long long strideIndex, const T* __r
                 float values[VEC];
 #pragma unroll
                 for (int k = 0; k < VEC; ++k) values[k] = valid ? static_cast<float>(raw[n].v[k]) * scale : 0;
-                if (row + n < rows) storeFloats(y + (row + n) * strideY + at, values);
+                if (row + n < rows) streamFloats(y + (row + n) * strideY + at, values);
             }
         }
     }
@@ -188,7 +188,7 @@ EmbeddingAdjointKernel(const unsigned* __restrict__ keys, const unsigned* __rest
             }
 #pragma unroll
             for (int k = 0; k < VEC; ++k) sum[k] *= scale;
-            if (c < C) storeFloats(adjTable + (blockIdx.x + static_cast<long long>(r) * gridDim.x) * strideTable + at, sum);
+            if (c < C) streamFloats(adjTable + (blockIdx.x + static_cast<long long>(r) * gridDim.x) * strideTable + at, sum);
         }
     }
 }

@@ -26,7 +26,6 @@
 QUICKMLP_KERNEL_NAMESPACE_BEGIN
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
@@ -516,16 +515,19 @@ __device__ __forceinline__ void storeTile(const Product& product, char* lds, con
 #pragma unroll 4
     for (int n = 0; n < NI * 32 * PIECES / 64; ++n) {
         const int row = (n * 64 + lane) / PIECES, piece = (n * 64 + lane) % PIECES;
-        T raw[PIECE];
-        __builtin_memcpy(raw, __builtin_assume_aligned(part + row * ROW + (piece ^ (row & (PIECES < 8 ? PIECES - 1 : 7))) * PIECE, 16), 16);
+        u32x4 raw;
+        __builtin_memcpy(&raw, __builtin_assume_aligned(part + row * ROW + (piece ^ (row & (PIECES < 8 ? PIECES - 1 : 7))) * PIECE, 16), 16);
         const int i = fromI + row, j = fromJ + piece * PIECE;
         if (i >= ni || j >= nj) continue;
         T* out = to + i * stride + j;
-        if (j + PIECE <= nj) __builtin_memcpy(out, raw, 16);
-        else
+        if (j + PIECE <= nj) streamPiece(out, raw);
+        else {
+            T entries[PIECE];
+            __builtin_memcpy(entries, &raw, 16);
 #pragma unroll
             for (int k = 0; k < PIECE; ++k)
-                if (j + k < nj) out[k] = raw[k];
+                if (j + k < nj) out[k] = entries[k];
+        }
     }
 }
 

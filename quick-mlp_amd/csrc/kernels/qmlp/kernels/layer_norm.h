@@ -118,7 +118,7 @@ LayerNormKernel(const T* __restrict__ x, long long strideX, const W* __restrict_
         for (int j = 0; j < CHUNKS; ++j) {
 #pragma unroll
             for (int k = 0; k < VEC; ++k) v[j][k] = v[j][k] * r * w[j][k] + b[j][k];
-            if (at.has(j)) storeFloats(y + row * strideY + at.start(j), v[j]);
+            if (at.has(j)) streamFloats(y + row * strideY + at.start(j), v[j]);
         }
         if (at.lane == 0) {
             if (mean) mean[row] = m;
@@ -180,7 +180,7 @@ LayerNormAdjointKernel(const T* __restrict__ x, long long strideX, const W* __re
             for (int j = 0; j < CHUNKS; ++j) {
 #pragma unroll
                 for (int k = 0; k < VEC; ++k) d[j][k] = r * (d[j][k] - a - n[j][k] * c);
-                if (at.has(j)) storeFloats(adjX + row * strideAdjX + at.start(j), d[j]);
+                if (at.has(j)) streamFloats(adjX + row * strideAdjX + at.start(j), d[j]);
             }
         }
     }

@@ -48,6 +48,31 @@ __device__ __forceinline__ void storeFloats(T* __restrict__ p, const float (&v)[
     }
 }
 
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+/**
+ * 16 bytes of a result, at any address that T may have. They are marked as not to be kept: the kernel that reads them comes later, and lines that
+ * the L2 would hold until then are in the way of this one's reads and are still to be written when it ends. us without | with the mark: 2^17
+ * rows of 512 experts, 64 -> 64, half 17, 16 | 12, 11; 32768 rows of 16 experts, 2048 -> 4096, bfloat16, train 1700 | 1590; 99480 rows
+ * of 44 experts, 16 -> 2096, half 182 | 135; layer norm of 32768 x 4096 bfloat16, adjoint 153 | 141; table of 65536 x 1024 bfloat16 65 | 60.
+ */
+template <typename T>
+__device__ __forceinline__ void streamPiece(T* __restrict__ p, u32x4 piece)
+{
+    typedef u32x4 Loose __attribute__((aligned(2)));   // of the smallest T
+    __builtin_nontemporal_store(piece, reinterpret_cast<Loose*>(p));
+}
+/** As storeFloats(), for results. */
+template <int N, typename T>
+__device__ __forceinline__ void streamFloats(T* __restrict__ p, const float (&v)[N])
+{
+    if constexpr (N * sizeof(T) == 16) {
+        u32x4 piece;
+        storeFloats(reinterpret_cast<T*>(&piece), v);
+        streamPiece(p, piece);
+    } else
+        storeFloats(p, v);
+}
+
 /** Sum over the G (a power of two up to 64) consecutive lanes that a lane belongs to, in all of them. */
 template <int G>
 __device__ __forceinline__ float sumOfLanes(float v)
