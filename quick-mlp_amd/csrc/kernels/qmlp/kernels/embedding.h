@@ -8,9 +8,9 @@
 // of frequent tokens are shared out: blocks of consecutive places of the sorted order that hold one token only are summed in
 // advance, blocks of such blocks likewise, so that no row has more than a few blocks of each size left to add.
 //
-// Measured, 65536 tokens, most of them rare, of a vocabulary of 65536 x 1024 bfloat16: lookup 40 us, of which 134 MB are writes; gradient
-// 20 + 5 us for the blocks (24 us of sorting before) and 66 us for the table, 134 MB again and the rare tokens' rows. 20011 codes of
-// 1000 x 64 floats: 3.7 us, and 8 + 1 + 15 us.
+// Measured, 65536 tokens, most of them rare, of a vocabulary of 65536 x 1024 bfloat16: lookup 39 us, of which 134 MB are writes; gradient
+// 17 + 4 us for the blocks (22 us of sorting before) and 60 us for the table, 134 MB again and the rare tokens' rows. 20011 codes of
+// 1000 x 64 floats: 3.4 us, and 8 + 1 + 15 us.
 
 #include <qmlp/kernels/row_groups.h>
 

@@ -346,7 +346,8 @@ const std::array<GroupedTiles, 4> GROUPED_TILES = {HUGE_TILES, LARGE_TILES, SMAL
 /**
  * The tiles for 'rows' of 'each' rows per expert and J results of K terms each, for values of 16 bits. A huge tile takes a compute unit
  * for itself, so that its first loads and its last stores stand alone: it pays where sums are long or where there are many of them, and
- * small ones pay where larger ones would leave compute units without work. us, huge | large | small, bfloat16, 16 or 17 experts:
+ * small ones pay where larger ones would leave compute units without work. us, huge | large | small, bfloat16, 16 or 17 experts (before
+ * results were stored past the L2, which took some 6 % off each of them and 15 % where K is short):
  * 32768 rows, K 2048, J 4096: 610 | 670 | 958; 54272, 2240, 256: 79 | 94 | 140; 54272, 256, 2240: 142 | 139 | 192; 16384, 1024, 1024: 65 | 51 | 64;
  * 4096, 1024, 1024: 34 | 22 | 25; 16384, 4096, 64: 91 | 47 | 38; through registers 32768, 2047, 4095: 840 | 996 | 1467.
  * Single precision is bound by the matrix cores with small tiles as well (16384 rows, 4 experts, 1024, 1024: - | 365 | 343).
