@@ -570,16 +570,21 @@ struct TokenNode : torch::autograd::Node
         std::lock_guard<std::mutex> lock(mutex_);   // (as generated nodes do: two threads may run backward on one graph)
         for (auto& v : saved) v.reset_data();
     }
-    virtual void adjoint(const at::Tensor& gradOutput, variable_list& grads) = 0;
+    /** \param tensors the saved ones */
+    virtual void adjoint(const at::Tensor& gradOutput, const variable_list& tensors, variable_list& grads) = 0;
     variable_list apply(variable_list&& gradOutputs) override
     {
         std::lock_guard<std::mutex> lock(mutex_);
         variable_list grads(num_outputs());
         if (!gradOutputs[0].defined()) return grads;
+        // Before any guard: hooks of saved tensors run here, and those of a checkpoint record its part of the forward pass once more.
+        variable_list tensors;
+        tensors.reserve(saved.size());
+        for (auto& v : saved) tensors.push_back(v.unpack());
         try {
             at::AutoDispatchBelowADInplaceOrView below;
             const c10::OptionalDeviceGuard guard(gradOutputs[0].device());
-            adjoint(gradOutputs[0], grads);
+            adjoint(gradOutputs[0], tensors, grads);
         } catch (...) {
             raiseFromBackward();
         }
@@ -633,9 +638,9 @@ struct EmbeddingBackward : TokenNode
     float scale = 1;
     std::string name() const override { return "QmlpEmbeddingBackward"; }
     std::vector<int64_t> tableSizes;
-    void adjoint(const at::Tensor& gradOutput, variable_list& grads) override
+    void adjoint(const at::Tensor& gradOutput, const variable_list& tensors, variable_list& grads) override
     {
-        const at::Tensor index = saved[0].unpack().reshape({-1}), adjOutput = consecutive(gradOutput.reshape({index.size(0), tableSizes[1]}));
+        const at::Tensor index = tensors[0].reshape({-1}), adjOutput = consecutive(gradOutput.reshape({index.size(0), tableSizes[1]}));
         const at::Tensor adjTable = at::empty(tableSizes, adjOutput.options());
         size_t bytes = 0;
         check(qmlp_tokens_embedding_adjoint_memory(index.size(0), tableSizes[0], static_cast<int>(tableSizes[1]), &bytes));
@@ -685,9 +690,9 @@ struct LayerNormBackward : TokenNode
 {
     at::ScalarType weightType = at::kFloat;
     std::string name() const override { return "QmlpLayerNormBackward"; }
-    void adjoint(const at::Tensor& gradOutput, variable_list& grads) override
+    void adjoint(const at::Tensor& gradOutput, const variable_list& tensors, variable_list& grads) override
     {
-        const at::Tensor x = saved[0].unpack(), weight = saved[1].unpack(), statistics = saved[2].unpack();
+        const at::Tensor x = tensors[0], weight = tensors[1], statistics = tensors[2];
         const int64_t channels = x.size(-1);
         const at::Tensor rows = consecutive(x.reshape({statistics.size(1), channels})), adjOutput = consecutive(gradOutput.reshape(rows.sizes()));
         const bool sums = task_should_compute_output(1) || task_should_compute_output(2);
@@ -736,9 +741,9 @@ at::Tensor layerNorm(const at::Tensor& x, const at::Tensor& weight, const at::Te
 struct GroupedLinearBackward : TokenNode
 {
     std::string name() const override { return "QmlpGroupedLinearBackward"; }
-    void adjoint(const at::Tensor& gradOutput, variable_list& grads) override
+    void adjoint(const at::Tensor& gradOutput, const variable_list& tensors, variable_list& grads) override
     {
-        const at::Tensor x = near(saved[0].unpack()), weight = near(saved[1].unpack()), offsets = saved[2].unpack(), adjOutput = near(gradOutput);
+        const at::Tensor x = near(tensors[0]), weight = near(tensors[1]), offsets = tensors[2], adjOutput = near(gradOutput);
         at::Tensor adjX, adjWeight, adjBias;
         if (task_should_compute_output(0)) adjX = emptyLike(x);
         if (task_should_compute_output(1)) adjWeight = emptyLike(weight);
