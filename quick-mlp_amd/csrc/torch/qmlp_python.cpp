@@ -581,6 +581,10 @@ struct TokenNode : torch::autograd::Node
         variable_list tensors;
         tensors.reserve(saved.size());
         for (auto& v : saved) tensors.push_back(v.unpack());
+        // (a hook may have left them anywhere, and a node may be called by hand: kernels read device memory only)
+        TORCH_CHECK(gradOutputs[0].is_cuda(), "QuickMLP tensors must live on the GPU");
+        for (const auto& t : tensors)
+            TORCH_CHECK(!t.defined() || t.device() == gradOutputs[0].device(), "saved tensors came back on another device");
         try {
             at::AutoDispatchBelowADInplaceOrView below;
             const c10::OptionalDeviceGuard guard(gradOutputs[0].device());
@@ -693,6 +697,7 @@ struct LayerNormBackward : TokenNode
     void adjoint(const at::Tensor& gradOutput, const variable_list& tensors, variable_list& grads) override
     {
         const at::Tensor x = tensors[0], weight = tensors[1], statistics = tensors[2];
+        TORCH_CHECK(statistics.dim() == 2 && statistics.size(0) == 2 && statistics.is_contiguous(), "the statistics of the rows came back in another form");
         const int64_t channels = x.size(-1);
         const at::Tensor rows = consecutive(x.reshape({statistics.size(1), channels})), adjOutput = consecutive(gradOutput.reshape(rows.sizes()));
         const bool sums = task_should_compute_output(1) || task_should_compute_output(2);
