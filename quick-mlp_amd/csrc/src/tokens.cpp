@@ -129,6 +129,12 @@ void checkContiguous(const Tensor& t, const char* what)
         stride *= t.size(d);
     }
 }
+/** The kernels go along some sizes in steps of up to 2048 entries, counted in 32 bits: the step behind the last entry has a number too. */
+void checkSteps(const char* what, int64_t size)
+{
+    constexpr int64_t most = (1ll << 31) - (1ll << 12);
+    CHECK_ERROR(size <= most, what, " must not be more than ", most, ", but are ", size);
+}
 void checkIndex(const Tensor& t, const char* what)
 {
     CHECK_ERROR(t.defined() && t.ndim() == 1, what, " must be a tensor with 1 dimension");
@@ -450,6 +456,9 @@ GroupedSizes checkGrouped(const Tensor& input, const Tensor& weight, const Tenso
     CHECK_ERROR(s.inputs > 0 && s.outputs > 0, "experts must have inputs and outputs");
     checkSizes(weight, "weight", {s.experts, s.outputs, s.inputs});
     checkSizes(offsets, "offsets", {s.experts + 1ll});
+    checkSteps("rows", s.rows);
+    checkSteps("inputs", s.inputs);
+    checkSteps("outputs", s.outputs);
     return s;
 }
 
@@ -539,6 +548,7 @@ void Tokens::embedding(const Tensor& index, const Tensor& table, float scale, Te
     checkType(output, "output", table.precision());
     checkSizes(output, "output", {index.size(0), table.size(1)});
     checkOutput(output, "output");
+    checkSteps("channels", table.size(1));
     if (output.numel() == 0) return;
     const int C = table.size(1), vec = C < wide(table.precision()) ? 1 : wide(table.precision()), lanes = lanesPerRow(C, vec);
     const long long rows = index.size(0), vocabulary = table.size(0);
@@ -565,6 +575,7 @@ void Tokens::embeddingAdjoint(const Tensor& index, const Tensor& adjOutput, floa
     checkValues(adjOutput, "adjOutput", 2);
     checkType(adjOutput, "adjOutput", adjTable.precision());
     checkSizes(adjOutput, "adjOutput", {index.size(0), adjTable.size(1)});
+    checkSteps("channels", adjTable.size(1));
     const long long rows = index.size(0), vocabulary = adjTable.size(0);
     const int C = adjTable.size(1);
     checkMemory(memory, embeddingAdjointMemory(rows, vocabulary, C));
@@ -599,6 +610,7 @@ void Tokens::layerNorm(const Tensor& input, const Tensor& weight, const Tensor& 
     checkValues(input, "input", 2);
     const long long rows = input.size(0);
     const int C = input.size(1);
+    checkSteps("channels", C);
     const Tensor::Precision p = input.precision(), weights = weight.defined() ? weight.precision() : bias.defined() ? bias.precision() : p;
     for (const auto& [t, what] : {std::pair<const Tensor&, const char*>{weight, "weight"}, {bias, "bias"}}) {
         if (!t.defined()) continue;
@@ -647,6 +659,7 @@ void Tokens::layerNormAdjoint(const Tensor& input, const Tensor& weight, const T
     checkValues(input, "input", 2);
     const long long rows = input.size(0);
     const int C = input.size(1);
+    checkSteps("channels", C);
     const Tensor::Precision p = input.precision();
     if (weight.defined()) {
         checkValues(weight, "weight", 1);
