@@ -124,7 +124,7 @@ struct EmbeddingBlocks
     const float* sums[SIZES];
 };
 
-constexpr int EMBEDDING_MOST_ROWS = 64;
+constexpr int EMBEDDING_MOST_ROWS = EMBEDDING_THREADS;   // a thread looks up each
 /**
  * The gradient of up to 'each' (EMBEDDING_MOST_ROWS at most) rows of the table per workgroup, G lanes per row. Their spans are
  * looked up together first, with the only term of those that have one. The rows of a workgroup are those of its number and as many as

@@ -227,21 +227,23 @@ LayerNormSumKernel(const float* __restrict__ partial, int count, int C, W* __res
     constexpr int COLUMNS = LAYER_NORM_SUM_COLUMNS, SLICES = LAYER_NORM_SUM_THREADS / COLUMNS;
     __shared__ float sums[SLICES][COLUMNS + 1];
     const int column = threadIdx.x % COLUMNS, slice = threadIdx.x / COLUMNS;
-    const long long c = static_cast<long long>(blockIdx.x) * COLUMNS + column;
-    float sum = 0;
-    if (c < 2ll * C)
+    for (long long first = static_cast<long long>(blockIdx.x) * COLUMNS; first < 2ll * C; first += static_cast<long long>(gridDim.x) * COLUMNS) {
+        const long long c = first + column;
+        float sum = 0;
+        if (c < 2ll * C)
 #pragma unroll 8
-        for (int p = slice; p < count; p += SLICES) sum += partial[static_cast<long long>(p) * 2 * C + c];
-    sums[slice][column] = sum;
-    __syncthreads();
-#pragma unroll
-    for (int half = SLICES / 2; half > 0; half /= 2) {
-        if (slice < half) sums[slice][column] += sums[slice + half][column];
+            for (int p = slice; p < count; p += SLICES) sum += partial[static_cast<long long>(p) * 2 * C + c];
+        sums[slice][column] = sum;
         __syncthreads();
-    }
-    if (slice == 0 && c < 2ll * C) {
-        W* out = c < C ? adjWeight : adjBias;
-        if (out) out[c < C ? c : c - C] = static_cast<W>(sums[0][column]);
+#pragma unroll
+        for (int half = SLICES / 2; half > 0; half /= 2) {
+            if (slice < half) sums[slice][column] += sums[slice + half][column];
+            __syncthreads();
+        }
+        if (slice == 0 && c < 2ll * C) {   // (the total's reader is the one who writes there next)
+            W* out = c < C ? adjWeight : adjBias;
+            if (out) out[c < C ? c : c - C] = static_cast<W>(sums[0][column]);
+        }
     }
 }
 

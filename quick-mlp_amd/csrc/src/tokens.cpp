@@ -153,6 +153,9 @@ T* ptr(const Tensor& t) { return t.defined() ? static_cast<T*>(const_cast<void*>
 /** The stride of a dimension; of one with a single entry it may be anything and is taken to be that of rows side by side. */
 long long strideOf(const Tensor& t, int d) { return t.size(d) <= 1 ? t.size(t.ndim() - 1) : t.stride(d); }
 
+/** A launch counts its threads in 32 bits. */
+bool isLaunch(int64_t groups, int threads) { return groups * threads < (1ll << 32); }
+void checkLaunch(int64_t groups, int threads) { CHECK_ERROR(isLaunch(groups, threads), "the call is too large for one launch"); }
 /** Workgroups for so many pieces of work of their own, no more than 'most' (the kernels go on in steps of the grid). */
 unsigned workgroups(int64_t pieces, int64_t most) { return static_cast<unsigned>(std::max<int64_t>(1, std::min(pieces, most))); }
 
@@ -257,7 +260,7 @@ bool sortByGroup(const Tensor& index, GroupPlan& plan, int* order, unsigned* key
 
 // ------------------------------------------------------------------------------------------------ embeddings
 // as in kernels/embedding.h
-constexpr int EMBEDDING_THREADS = 256, EMBEDDING_BLOCK_BITS = 6, EMBEDDING_MOST_ROWS = 64;
+constexpr int EMBEDDING_THREADS = 256, EMBEDDING_BLOCK_BITS = 6, EMBEDDING_MOST_ROWS = 256;
 struct EmbeddingBlocks
 {
     static constexpr int SIZES = 6;
@@ -275,11 +278,14 @@ int lanesPerRow(int C, int vec)
 
 /** Four rows at a time where that leaves four workgroups for every compute unit. */
 int embeddingRowsAtOnce(int64_t rows, int lanes) { return rows >= 4 * 4 * 256 * (EMBEDDING_THREADS / lanes) ? 4 : 1; }
-/** Rows of the table per workgroup of the adjoint kernel: as many as its lanes take at a time, and more where there are many workgroups. */
+/**
+ * Rows of the table per workgroup of the adjoint kernel: as many as its lanes take at a time, and more where there are many workgroups, up to
+ * 64; all that a workgroup can have where a launch would not take the threads otherwise.
+ */
 int embeddingAdjointRows(int64_t vocabulary, int lanes)
 {
-    const int64_t atATime = EMBEDDING_THREADS / lanes;
-    return static_cast<int>(std::min<int64_t>(EMBEDDING_MOST_ROWS, roundUp(std::max<int64_t>(1, vocabulary / 2048), atATime)));
+    const int64_t atATime = EMBEDDING_THREADS / lanes, most = isLaunch(divUp<int64_t>(vocabulary, 64), EMBEDDING_THREADS) ? 64 : EMBEDDING_MOST_ROWS;
+    return static_cast<int>(std::min<int64_t>(most, roundUp(std::max<int64_t>(1, vocabulary / 2048), atATime)));
 }
 
 struct EmbeddingPlan
@@ -328,9 +334,10 @@ LayerNormShape layerNormShape(int channels, Tensor::Precision p)
 std::string valueTypes(Tensor::Precision p, Tensor::Precision weights) { return std::string(scalarName(p)) + ", " + scalarName(weights); }
 
 /** Workgroups of the adjoint kernel: each leaves a row of sums. Two per compute unit where rows are held by wavefronts, four short of that. */
-unsigned layerNormAdjointWorkgroups(int64_t rows, const LayerNormShape& s)
+unsigned layerNormAdjointWorkgroups(int64_t rows, int channels, const LayerNormShape& s)
 {
-    if (s.lanes == 0) return workgroups(rows, 256);   // slices of the rows
+    // slices of the rows, and no more of them than a launch takes with a thread for each of their sums
+    if (s.lanes == 0) return workgroups(rows, std::min<int64_t>(256, ((1ll << 32) - 1) / roundUp<int64_t>(channels, 256)));
     return workgroups(divUp<int64_t>(rows, s.rows()), s.lanes == 1024 ? 256 : 512);
 }
 
@@ -431,11 +438,6 @@ void checkRows(const Tensor& t, const char* what)
 {
     const int d = t.ndim() - 2;
     CHECK_ERROR(t.size(d) <= 1 || t.stride(d) < (1 << 21), "rows of ", what, " must be less than 2^21 entries apart");
-}
-
-void checkLaunch(int64_t groups, int threads)
-{
-    CHECK_ERROR(groups * threads < (1ll << 32), "the call is too large for one launch");
 }
 
 struct GroupedSizes
@@ -582,6 +584,7 @@ void Tokens::embeddingAdjoint(const Tensor& index, const Tensor& adjOutput, floa
     if (adjTable.numel() == 0) return;
     const Tensor::Precision p = adjTable.precision();
     const int vec = C < wide(p) ? 1 : wide(p), lanes = lanesPerRow(C, vec);
+    checkLaunch(divUp<int64_t>(divUp<int64_t>(rows, 1 << EMBEDDING_BLOCK_BITS), EMBEDDING_THREADS / lanes), EMBEDDING_THREADS);   // (the first blocks)
     auto arguments = [&] { return str("<", scalarName(p), ", ", vec, ", ", lanes); };
     EmbeddingPlan plan(rows, vocabulary, C, memory);
     const void* dy = ptr<void>(adjOutput);
@@ -649,7 +652,7 @@ size_t Tokens::layerNormAdjointMemory(int64_t rows, int channels)
     // (for any precision)
     size_t bytes = 0;
     for (const Tensor::Precision p : {Tensor::FLOAT, Tensor::HALF})
-        bytes = std::max(bytes, sizeof(float) * 2 * channels * layerNormAdjointWorkgroups(rows, layerNormShape(channels, p)));
+        bytes = std::max(bytes, sizeof(float) * 2 * channels * layerNormAdjointWorkgroups(rows, channels, layerNormShape(channels, p)));
     return roundUp(bytes, ALIGNMENT);
 }
 
@@ -699,7 +702,7 @@ void Tokens::layerNormAdjoint(const Tensor& input, const Tensor& weight, const T
     auto types = [&] { return "<" + valueTypes(p, weights); };
     int count = 0;
     if (rows > 0) {
-        const unsigned groups = layerNormAdjointWorkgroups(rows, s);
+        const unsigned groups = layerNormAdjointWorkgroups(rows, C, s);
         count = static_cast<int>(groups);
         const void *x = input.rawPtr(), *w = ptr<void>(weight), *dy = adjOutput.rawPtr();
         const float *m = ptr<float>(mean), *r = ptr<float>(rstd);
@@ -720,7 +723,7 @@ void Tokens::layerNormAdjoint(const Tensor& input, const Tensor& weight, const T
     }
     if (sums)
         tokenKernel("layer_norm.h", kernelKey(LAYER_NORM_SUM, weights), [&] { return str("LayerNormSumKernel<", scalarName(weights), ">"); })
-            .call(static_cast<unsigned>(divUp<int64_t>(2ll * C, LAYER_NORM_SUM_COLUMNS)), LAYER_NORM_SUM_THREADS, 0, stream, static_cast<const float*>(partial), count, C,
+            .call(workgroups(divUp<int64_t>(2ll * C, LAYER_NORM_SUM_COLUMNS), 1 << 20), LAYER_NORM_SUM_THREADS, 0, stream, static_cast<const float*>(partial), count, C,
                   ptr<void>(adjWeight), ptr<void>(adjBias));
 }
 

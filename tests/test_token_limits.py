@@ -51,3 +51,49 @@ def test_sizes_whose_last_step_has_no_number_are_refused(size):
     many = descriptor(H, size, 1)
     for weight in (descriptor(H, 1, 1, 1), none):
         refused(lib.qmlp_tokens_grouped_linear_adjoint(many, descriptor(H, 1, 1, 1), offsets, many, none, weight, few, 256, None), "rows must not be more")
+
+
+def test_a_gradient_of_too_many_rows_for_a_launch_is_refused():
+    """2^31 - 1 rows (all the same one in memory) of more than 512 floats: 2^25 blocks of 64 places, 128 lanes or more for each."""
+    lib, F, I = _lib.lib, _lib.QMLP_FLOAT, _lib.QMLP_INT32
+    rows = 2 ** 31 - 1
+    refused(lib.qmlp_tokens_embedding_adjoint(descriptor(I, rows), descriptor(F, rows, 600, strides=(0, 1)), 1.0, descriptor(F, 4, 600), 256, None),
+            "too large for one launch")
+
+
+@gpu
+def test_gradient_of_a_table_of_more_than_two_to_the_30_rows():
+    vocabulary = (1 << 30) + 5
+    table = torch.zeros(vocabulary, 1, dtype=torch.float16, device="cuda", requires_grad=True)
+    index = torch.tensor([vocabulary - 1, 3, vocabulary, 1 << 29, 3, -1, vocabulary - 2], device="cuda")
+    y = tokens.embedding(index, table)
+    dtable, = torch.autograd.grad(y, table, torch.arange(1, 8, device="cuda").half()[:, None])
+    assert [float(dtable[v]) for v in (vocabulary - 1, 3, 1 << 29, vocabulary - 2)] == [1, 7, 4, 7]
+    assert int(torch.count_nonzero(dtable)) == 4
+
+
+@gpu
+def test_layer_norm_of_more_columns_than_a_launch_takes_in_one_go():
+    """2^26 columns: their sums over the rows have 2^32 threads' work. One row, so that the gradient of the bias is that of the output."""
+    channels = (1 << 26) + 7
+    g = torch.Generator(device="cuda").manual_seed(60)
+    x, grad = (torch.randn(1, channels, device="cuda", generator=g) for _ in range(2))
+    weight, bias = (torch.full((channels,), v, device="cuda", requires_grad=True) for v in (1.0, 0.0))
+    y = tokens.layer_norm(x, weight, bias)
+    dw, db = torch.autograd.grad(y, (weight, bias), grad)
+    assert torch.equal(db, grad[0])
+    # y is the normal here: the same products, rounded once
+    torch.testing.assert_close(dw, (grad * y.detach())[0], rtol=2.0 ** -20, atol=0)
+
+
+@gpu
+def test_layer_norm_of_rows_whose_slices_have_too_many_sums():
+    """256 slices of 2^24 columns: 2^32 threads. 257 rows that are all the same in memory, entries of 1 and -1."""
+    channels, rows = (1 << 24) + 2, 257
+    row = 1 - 2 * (torch.arange(channels, device="cuda") % 2).half()
+    weight, bias = (torch.full((channels,), v, dtype=torch.float16, device="cuda", requires_grad=True) for v in (1.0, 0.0))
+    y = tokens.layer_norm(row.expand(rows, channels), weight, bias, 0.0)
+    dw, db = torch.autograd.grad(y, (weight, bias), torch.ones(1, channels, dtype=torch.float16, device="cuda").expand(rows, channels))
+    # (mean 0 and variance 1 are exact, and so are sums up to 257)
+    assert torch.equal(db, torch.full_like(db, 257))
+    assert torch.equal(dw, 257 * row)
