@@ -32,31 +32,45 @@ const char* scalarName(Tensor::Precision p)
 /** Entries of a 16-byte access. */
 int wide(Tensor::Precision p) { return 16 / Tensor::BytesPerEntry[p]; }
 
-enum KernelId { GROUP_SMALL, GROUP_COUNT, GROUP_SCAN, GROUP_SCATTER, GROUP_OFFSETS, EMBEDDING, EMBEDDING_BLOCKS, EMBEDDING_ADJOINT, LAYER_NORM,
+enum KernelId { GROUP_SMALL = 1, GROUP_COUNT, GROUP_SCAN, GROUP_SCATTER, GROUP_OFFSETS, EMBEDDING, EMBEDDING_BLOCKS, EMBEDDING_ADJOINT, LAYER_NORM,
                 LAYER_NORM_ADJOINT, LAYER_NORM_SUM, LAYER_NORM_LONG, LAYER_NORM_LONG_ADJOINT, LAYER_NORM_LONG_SUMS, GROUPED_ROWS, GROUPED_WEIGHTS,
-                GROUPED_SUM, GROUPED_JOIN };
-/** One number for a kernel and its template arguments, each below 2^11: to build its name takes as long as to launch it. */
+                GROUPED_SUM, GROUPED_JOIN, KERNEL_IDS };
+/**
+ * One number for a kernel and its template arguments, each below 2^11: to build its name takes as long as to launch it. No id is 0, so that
+ * kernels with n arguments have numbers from 2^(11 n) up to less than 2^(11 (n + 1)).
+ */
 template <typename... Args>
-uint64_t kernelKey(KernelId id, Args... args)
+constexpr uint64_t kernelKey(KernelId id, Args... args)
 {
-    static_assert(sizeof...(args) <= 5, "64 bits");
+    static_assert(sizeof...(args) <= 5 && KERNEL_IDS <= 1 << (64 - 5 * 11), "64 bits");
     uint64_t key = id;
     ((key = key << 11 | static_cast<uint64_t>(args)), ...);
     return key;
 }
-/** The kernels stay loaded for the life of the process. File: below kernels/qmlp/kernels; name(): with its template arguments. */
+static_assert(kernelKey(GROUP_SMALL, 0) > kernelKey(KERNEL_IDS), "the smallest number with an argument is above all without");
+/** The kernels in use, which stay loaded for the life of the process. */
+struct TokenKernels
+{
+    std::mutex mutex;
+    std::unordered_map<uint64_t, KernelFunction> loaded;
+};
+TokenKernels& tokenKernels()
+{
+    static TokenKernels kernels;
+    return kernels;
+}
+/** File: below kernels/qmlp/kernels; name(): with its template arguments. */
 template <typename Name>
 KernelFunction& tokenKernel(const char* file, uint64_t key, Name name)
 {
-    static std::mutex mutex;
-    static std::unordered_map<uint64_t, KernelFunction> kernels;
-    std::lock_guard<std::mutex> lock(mutex);
-    auto it = kernels.find(key);
-    if (it == kernels.end()) {
+    TokenKernels& kernels = tokenKernels();
+    std::lock_guard<std::mutex> lock(kernels.mutex);
+    auto it = kernels.loaded.find(key);
+    if (it == kernels.loaded.end()) {
         auto loaded = QuickMLP::Instance().kernelLoader()->getKernel("qmlp::kernel::" + std::string(name()),
                                                                      KernelLoader::MainFile(std::string("qmlp/kernels/") + file),
                                                                      QuickMLP::Instance().getCompileFlags() | KernelLoader::CompileThrowOnError);
-        it = kernels.emplace(key, std::move(*loaded)).first;
+        it = kernels.loaded.emplace(key, std::move(*loaded)).first;
     }
     return it->second;
 }
