@@ -855,10 +855,16 @@ void Tokens::precompile(Tensor::Precision p)
         }
     std::vector<LayerNormShape> shapes = {{8, 1, 1}};
     for (const auto& s : LAYER_NORM_SHAPES) shapes.push_back({s[0], s[1], wide(p)});
-    for (const LayerNormShape& s : shapes)
-        for (const char* kernel : {"LayerNormKernel", "LayerNormAdjointKernel"}) precompileKernel("layer_norm.h", str(kernel, "<", t, ", ", t, ", ", s.arguments(), ">"));
-    for (const char* kernel : {"LayerNormLongKernel", "LayerNormLongAdjointKernel"}) precompileKernel("layer_norm.h", str(kernel, "<", t, ", ", t, ">"));
-    for (const char* kernel : {"LayerNormLongSumsKernel", "LayerNormSumKernel"}) precompileKernel("layer_norm.h", str(kernel, "<", t, ">"));
+    std::vector<Tensor::Precision> weights = {p};   // of a layer norm
+    if (p != Tensor::FLOAT) weights.push_back(Tensor::FLOAT);
+    for (const Tensor::Precision w : weights) {
+        const std::string types = valueTypes(p, w);
+        for (const LayerNormShape& s : shapes)
+            for (const char* kernel : {"LayerNormKernel", "LayerNormAdjointKernel"}) precompileKernel("layer_norm.h", str(kernel, "<", types, ", ", s.arguments(), ">"));
+        for (const char* kernel : {"LayerNormLongKernel", "LayerNormLongAdjointKernel"}) precompileKernel("layer_norm.h", str(kernel, "<", types, ">"));
+        precompileKernel("layer_norm.h", str("LayerNormSumKernel<", scalarName(w), ">"));
+    }
+    precompileKernel("layer_norm.h", str("LayerNormLongSumsKernel<", t, ">"));
     for (const bool direct : {false, true})
         for (const GroupedTiles& tiles : GROUPED_TILES) {
             const bool few = tiles.i == FEW_TILES.i, huge = tiles.i == HUGE_TILES.i, single = p == Tensor::FLOAT;
