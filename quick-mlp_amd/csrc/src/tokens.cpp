@@ -809,26 +809,27 @@ void Tokens::groupedLinearAdjoint(const Tensor& input, const Tensor& weight, con
     const bool inputs = adjInput.defined() && s.rows > 0, weights = s.experts > 0 && (adjWeight.defined() || adjBias.defined());
     if (!inputs && !weights) return;
     checkMemory(memory, groupedLinearAdjointMemory(s.rows, s.experts, s.inputs, s.outputs));
+    const bool direct = isDirect(input) && isDirect(adjOutput);
+    GroupedAdjointPlan plan(p, s.rows, weights ? s.experts : 1, s.inputs, s.outputs, direct, memory);
+    const int64_t groups = plan.places * plan.tilesI * plan.tilesJ;
+    const long long size = static_cast<long long>(s.inputs) * s.outputs;
+    const int64_t pieces = divUp<int64_t>(size + s.outputs, 256);
+    if (weights) {   // (before the input's gradients are launched)
+        checkLaunch(groups, plan.tiles.threads());
+        checkLaunch(plan.partial ? pieces * s.experts : 0, 256);
+    }
     if (inputs) launchRows(false, adjOutput, weight, offsets, {}, adjInput, s, s.inputs, s.outputs, memory, stream);
     if (!weights) return;
-    const bool direct = isDirect(input) && isDirect(adjOutput);
-    GroupedAdjointPlan plan(p, s.rows, s.experts, s.inputs, s.outputs, direct, memory);
-    const int64_t groups = plan.places * plan.tilesI * plan.tilesJ;
-    checkLaunch(groups, plan.tiles.threads());
     const int chunk = static_cast<int>(plan.chunk);
     tokenKernel("grouped_linear.h", kernelKey(GROUPED_WEIGHTS, p * 2 + direct, plan.tiles.i, plan.tiles.j, plan.tiles.wavesI, plan.tiles.wavesJ),
                 [&] { return str("GroupedWeightsKernel<", scalarName(p), ", ", boolName(direct), ", ", plan.tiles.arguments(), ">"); })
         .call(static_cast<unsigned>(groups), plan.tiles.threads(), plan.tiles.lds(s.rows, input.bytesPerEntry(), direct), stream, dy, strideOf(adjOutput, 0), x, strideOf(input, 0), off, s.experts,
               ptr<void>(adjWeight), ptr<void>(adjBias), plan.partial, s.rows, s.outputs, s.inputs,
               static_cast<int>(plan.places), static_cast<int>(plan.tilesI), static_cast<int>(plan.tilesJ), chunk);
-    if (plan.partial) {
-        const long long size = static_cast<long long>(s.inputs) * s.outputs;
-        const int64_t pieces = divUp<int64_t>(size + s.outputs, 256);
-        checkLaunch(pieces * s.experts, 256);
+    if (plan.partial)
         tokenKernel("grouped_linear.h", kernelKey(GROUPED_SUM, p), [&] { return str("GroupedSumKernel<", scalarName(p), ">"); })
             .call(static_cast<unsigned>(pieces * s.experts), 256, 0, stream, static_cast<const float*>(plan.partial), off, ptr<void>(adjWeight),
                   ptr<void>(adjBias), s.rows, size, s.outputs, chunk, static_cast<int>(pieces));
-    }
 }
 
 void Tokens::precompile(Tensor::Precision p)

@@ -61,6 +61,14 @@ def test_a_gradient_of_too_many_rows_for_a_launch_is_refused():
             "too large for one launch")
 
 
+def test_gradients_of_experts_too_large_for_a_launch_are_refused_as_a_whole():
+    """1024 matrices of 2^30 entries have 2^26 tiles: refused before the gradient of the input is launched, which alone were small enough."""
+    lib, H, I = _lib.lib, _lib.QMLP_HALF, _lib.QMLP_INT32
+    rows, weight = descriptor(H, 64, 32768), descriptor(H, 1024, 32768, 32768)
+    none = _lib.TensorDesc()
+    refused(lib.qmlp_tokens_grouped_linear_adjoint(rows, weight, descriptor(I, 1025), rows, rows, weight, none, 256, None), "too large for one launch")
+
+
 @gpu
 def test_gradient_of_a_table_of_more_than_two_to_the_30_rows():
     vocabulary = (1 << 30) + 5
