@@ -267,9 +267,10 @@ int qmlp_utils_pullpush_precompile(int precision);
 
 /* ---- operators on rows of tokens: no counterpart in the reference ----
  * Values are float, half or bfloat16; rows are the first dimension, the last one has stride 1. Indices are 32- or 64-bit
- * integers. Channels, inputs, outputs and the rows of experts are no more than 2^31 - 2^12. Gradients are written as a whole, not added to. These calls allocate nothing and do not synchronise: `memory` is
- * device memory of the caller, aligned to 256 bytes, of the size that the function beside reports (NULL where that is 0). An
- * undefined tensor (NULL or ndim = 0) leaves an optional input or output out. */
+ * integers. Channels, inputs, outputs and the rows of experts are no more than 2^31 - 2^12. Gradients are written as a whole, not
+ * added to. These calls allocate nothing and do not synchronise: `memory` is device memory of the caller, aligned to 256 bytes,
+ * of the size that the function beside reports (NULL where that is 0). An undefined tensor (NULL or ndim = 0) leaves an optional
+ * input or output out. */
 /* order (rows) and offsets (groups + 1), both INT32: the rows by the group that index (rows) names, in their own order within a
  * group; group g has the entries offsets[g] .. offsets[g + 1] - 1. Rows whose index is not in 0 .. groups - 1 come last. */
 int qmlp_tokens_group_memory(long long rows, int groups, size_t* bytes);

@@ -15,11 +15,12 @@
 //
 // Offsets are limited to the rows there are wherever they are read: no access depends on their values.
 //
-// What bounds them: the matrix cores where experts have many rows, and there the power that is left for the clock (fewer cycles
-// for the same tiles came with a lower clock, 2.02 to 1.82 GHz, in the same time); the weights' bytes where experts have few rows;
-// the latency of a tile's first bytes in between. Measured, us for y, dx and dW + db: 32768 rows of 16 experts, 2048 -> 4096, bfloat16 587, 594,
-// 563 (925 to 977 TFLOP/s; a large product of the same card reaches 1390); 2^17 rows of 512 experts, 64 -> 64, half 11.9, 10.2, 12.9; 5003 rows
-// of 12 experts, 333 -> 200, float 21, 21, 22 + 5; y of 24 rows of 64 experts, 1024 -> 4096, bfloat16 33 (the weights: 4.8 TB/s).
+// What bounds them: where experts have many rows, the bytes that a product takes from LDS (the matrix cores are busy 58 % of the cycles also
+// without any loads from memory); the weights' bytes where experts have few rows; the latency of a tile's first bytes in between. Measured, us for
+// y, dx and dW + db: 32768 rows of 16 experts, 2048 -> 4096, bfloat16 566, 567, 535 one after the other, each by itself (970 to 1030 TFLOP/s;
+// a library's products of these sizes, every row with one matrix, in turn with them 392, 430, 508); 2^17 rows of 512 experts, 64 -> 64, half
+// 11.8, 10.3, 12.2; 5003 rows of 12 experts, 333 -> 200, float 21, 21, 22 + 5; y of 24 rows of 64 experts, 1024 -> 4096, bfloat16 33 (the
+// weights: 4.8 TB/s).
 
 #include <qmlp/kernels/token_types.h>
 

@@ -9,8 +9,8 @@
 // Workgroups stay for many rows, with the weights in registers; the adjoint's sums over rows are kept there as well and
 // leave a workgroup once, as a row of 'partial', which a second kernel sums in a fixed order.
 //
-// Measured: 32768 x 4096 bfloat16 102 to 105 us forward and 141 + 5 us adjoint, 5.2 and 5.7 TB/s of what has to be moved (a large copy: 5.1 to
-// 5.5); 4099 x 777 float 6.5 and 11.2 + 3.9 us; one row of 1024 halves 3.0 us.
+// Measured: 32768 x 4096 bfloat16 105 us forward and 143 + 5 us adjoint, 5.1 and 5.6 TB/s of what has to be moved (a large copy: 5.1 to
+// 5.5); 4099 x 777 float 6.6 and 11.7 + 4.0 us; one row of 1024 halves 2.8 us.
 
 #include <qmlp/kernels/token_types.h>
 

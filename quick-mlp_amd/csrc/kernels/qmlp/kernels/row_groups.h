@@ -5,7 +5,7 @@
 // its bytes (2^20 rows: 8 MB). So a digit has as many values as the LDS has counters for, which makes one pass of up to 4399
 // groups, and a batch that fits the registers of a workgroup is sorted by one workgroup in one launch.
 //
-// Measured: 64 rows, 8 groups 4.5 us; 2^20 rows, 4096 groups 28 us: count 5.8, scan 5.3, scatter 17 (2^20 places of 4 bytes, of which a
+// Measured: 64 rows, 8 groups 4.5 us; 2^20 rows, 4096 groups 28 us: count 6.0, scan 5.2, scatter 17 (2^20 places of 4 bytes, of which a
 // tile of 4096 rows has one in a line: the writes); 65536 rows, 65536 groups: two passes of 4.5 + 6.8, without a scan.
 //
 // The place of a row among those of its digit is found by ballots: of the lanes of a wavefront with the same digit, those

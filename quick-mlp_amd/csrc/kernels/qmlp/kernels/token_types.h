@@ -51,9 +51,12 @@ __device__ __forceinline__ void storeFloats(T* __restrict__ p, const float (&v)[
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 /**
  * 16 bytes of a result, at any address that T may have. They are marked as not to be kept: the kernel that reads them comes later, and lines that
- * the L2 would hold until then are in the way of this one's reads and are still to be written when it ends. us without | with the mark: 2^17
- * rows of 512 experts, 64 -> 64, half 17, 16 | 12, 11; 32768 rows of 16 experts, 2048 -> 4096, bfloat16, train 1700 | 1590; 99480 rows
- * of 44 experts, 16 -> 2096, half 182 | 135; layer norm of 32768 x 4096 bfloat16, adjoint 153 | 141; table of 65536 x 1024 bfloat16 65 | 60.
+ * the L2 would hold until then are in the way of this one's reads and are still to be written when it ends. us without | with the mark, one
+ * operator alone, half: lookup of 65536 x 2048 88 | 78, layer norm of them 112 | 92; layer of 2^17 rows of 512 experts, 64 -> 64, 10.8 | 9.2; of
+ * 16384 rows of 16, 256 -> 512, 14.7 | 12.5; of 99480 rows of 44, 16 -> 2096, 182 | 135; three products of 32768 rows of 16, 2048 -> 4096,
+ * bfloat16, 1648 | 1645. With its readers right behind (lookup, layer norm, layer, activation, layer), rows x channels -> hidden: 64 x 256 -> 512
+ * 16.8 | 17.4; 2048 x 256 -> 512 22.0 | 22.8; 16384 x 256 -> 512 62 | 60; 2^17 x 64 -> 64 55.6 | 57.7; 32768 x 1024 -> 2048 513 | 502; 65536 x
+ * 2048 -> 2048 1526 | 1534.
  */
 template <typename T>
 __device__ __forceinline__ void streamPiece(T* __restrict__ p, u32x4 piece)

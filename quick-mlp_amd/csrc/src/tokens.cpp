@@ -347,7 +347,7 @@ LayerNormShape layerNormShape(int channels, Tensor::Precision p)
 }
 std::string valueTypes(Tensor::Precision p, Tensor::Precision weights) { return std::string(scalarName(p)) + ", " + scalarName(weights); }
 
-/** Workgroups of the adjoint kernel: each leaves a row of sums. Two per compute unit where rows are held by wavefronts, four short of that. */
+/** Workgroups of the adjoint kernel: each leaves a row of sums. Two per compute unit, one where a row takes all of its threads. */
 unsigned layerNormAdjointWorkgroups(int64_t rows, int channels, const LayerNormShape& s)
 {
     // slices of the rows, and no more of them than a launch takes with a thread for each of their sums
@@ -373,8 +373,8 @@ const std::array<GroupedTiles, 4> GROUPED_TILES = {HUGE_TILES, LARGE_TILES, SMAL
 /**
  * The tiles for 'rows' of 'each' rows per expert and J results of K terms each, for values of 16 bits. A huge tile takes a compute unit
  * for itself, so that its first loads and its last stores stand alone: it pays where sums are long or where there are many of them, and
- * small ones pay where larger ones would leave compute units without work. us, huge | large | small, bfloat16, 16 or 17 experts (before
- * results were stored past the L2, which took some 6 % off each of them and 15 % where K is short):
+ * small ones pay where larger ones would leave compute units without work. us, huge | large | small, bfloat16, 16 or 17 experts (all of them
+ * before results were stored past the L2, see streamPiece()):
  * 32768 rows, K 2048, J 4096: 610 | 670 | 958; 54272, 2240, 256: 79 | 94 | 140; 54272, 256, 2240: 142 | 139 | 192; 16384, 1024, 1024: 65 | 51 | 64;
  * 4096, 1024, 1024: 34 | 22 | 25; 16384, 4096, 64: 91 | 47 | 38; through registers 32768, 2047, 4095: 840 | 996 | 1467.
  * Single precision is bound by the matrix cores with small tiles as well (16384 rows, 4 experts, 1024, 1024: - | 365 | 343).
@@ -422,7 +422,12 @@ const char* boolName(bool b) { return b ? "true" : "false"; }
 /** Places of tiles (kernels/grouped_linear.h): one more than rows / tileRows for each expert and for the rows behind them. */
 int64_t tilePlaces(int64_t rows, int64_t experts, int64_t tileRows) { return rows / tileRows + experts + 1; }
 
-/** Rows of a chunk of GroupedWeightsKernel: several chunks per expert where its tiles alone are too few for the chip. */
+/**
+ * Rows of a chunk of GroupedWeightsKernel: several chunks per expert where the tiles of all experts are less than two per compute unit. The rule goes by
+ * their number alone, and experts just short of it pay for the second kernel and the memory between: us for dW of 2^17 rows, 64 -> 64, half, of 255,
+ * 256, 511 | 512, 513, 1024 experts with as many rows each: 18, 16, 23 | 6.4, 8.3, 6.8. From there on an expert has one workgroup per tile,
+ * however many rows it has: half of the rows in one of 511 | 512 experts 36 | 417.
+ */
 int64_t weightsChunk(int64_t rows, int64_t experts, int64_t tiles, int tile)
 {
     const int64_t chunks = divUp<int64_t>(512, std::max<int64_t>(1, experts * tiles));   // per expert
