@@ -33,7 +33,7 @@ typedef struct qmlp_activation_s* qmlp_activation_t;
 /* qmlp::Tensor::Precision / ::Usage (src_cpp/include/qmlp/tensor.h:25-38) */
 enum { QMLP_FLOAT = 0, QMLP_HALF = 1, QMLP_DOUBLE = 2 };
 /* Further types of the operators on rows of tokens (qmlp_tokens_*); everything else refuses them. */
-enum { QMLP_BFLOAT16 = 3, QMLP_INT32 = 4, QMLP_INT64 = 5 };
+enum { QMLP_BFLOAT16 = 3, QMLP_INT32 = 4, QMLP_INT64 = 5, QMLP_UINT8 = 6 };
 enum { QMLP_INFERENCE = 0, QMLP_GRADIENTS = 1 };
 /* qmlp::FusedNetwork::AdjointMode (src_cpp/include/qmlp/fused_network.h:22-33) */
 enum { QMLP_GRADIENTS_INPUT = 1, QMLP_GRADIENTS_NETWORK_WEIGHTS = 2, QMLP_GRADIENTS_INPUT_ENCODINGS = 4 };
@@ -303,6 +303,36 @@ int qmlp_tokens_grouped_linear_adjoint_memory(long long rows, int experts, int i
 int qmlp_tokens_grouped_linear_adjoint(const qmlp_tensor* input, const qmlp_tensor* weight, const qmlp_tensor* offsets,
                                        const qmlp_tensor* adj_output, const qmlp_tensor* adj_input, const qmlp_tensor* adj_weight,
                                        const qmlp_tensor* adj_bias, void* memory, void* stream);
+/* As qmlp_tokens_group(), with the same memory; places (rows, INT32, optional): the place of every row in order, -1 - place of rows of no
+ * group. */
+int qmlp_tokens_group_places(const qmlp_tensor* index, int groups, const qmlp_tensor* order, const qmlp_tensor* offsets,
+                             const qmlp_tensor* places, void* memory, void* stream);
+/* The router's choice: index (rows, chosen, INT32) of the largest of logits (rows, experts), the first of equals, and weights (rows, chosen),
+ * their shares of the softmax over all experts or, normalised, over the chosen ones. Logits of -inf are not chosen: -1 and 0 in their place.
+ * 1 <= chosen <= experts, chosen <= 64. */
+int qmlp_tokens_route(const qmlp_tensor* logits, int normalised, const qmlp_tensor* weights, const qmlp_tensor* index, void* stream);
+int qmlp_tokens_route_adjoint(const qmlp_tensor* logits, const qmlp_tensor* index, const qmlp_tensor* adj_weights, int normalised,
+                              const qmlp_tensor* adj_logits, void* stream);
+/* rows[places[t][j]] = input[t]: input (tokens, channels), places (tokens, chosen, INT32) as qmlp_tokens_group_places() leaves them, rows (tokens *
+ * chosen, channels); zeros at places of no expert (-1 - place). */
+int qmlp_tokens_dispatch(const qmlp_tensor* input, const qmlp_tensor* places, const qmlp_tensor* rows, void* stream);
+/* output[t] = residual[t] + the sum of weights[t][j] * rows[places[t][j]]: weights (tokens, chosen) of the rows' type or FLOAT (optional: 1),
+ * residual and output (tokens, channels; residual optional). The gradient of qmlp_tokens_dispatch() with neither weights nor residual. */
+int qmlp_tokens_combine(const qmlp_tensor* rows, const qmlp_tensor* places, const qmlp_tensor* weights, const qmlp_tensor* residual,
+                        const qmlp_tensor* output, void* stream);
+/* The gradients (each optional); that of the residual is adj_output. */
+int qmlp_tokens_combine_adjoint(const qmlp_tensor* rows, const qmlp_tensor* places, const qmlp_tensor* weights, const qmlp_tensor* adj_output,
+                                const qmlp_tensor* adj_rows, const qmlp_tensor* adj_weights, void* stream);
+/* Numbers of 4 bits (MXFP4 of the OCP Microscaling Formats specification 1.0) of input (rows, columns), in blocks of 32 entries of a row: codes
+ * (rows, 16 * blocks, UINT8; two a byte, the first in the low bits) and scales (rows, blocks, UINT8; exponent + 127, 255: NaN). */
+int qmlp_tokens_mx4_quantise(const qmlp_tensor* input, const qmlp_tensor* codes, const qmlp_tensor* scales, void* stream);
+/* The values that they stand for: output (rows, columns). */
+int qmlp_tokens_mx4_values(const qmlp_tensor* codes, const qmlp_tensor* scales, const qmlp_tensor* output, void* stream);
+/* qmlp_tokens_grouped_linear() with weights of 4 bits (experts, outputs, 16 * blocks) and their scales (experts, outputs, blocks): input (rows,
+ * inputs) is quantised by the call, or holds codes with input_scales. offsets optional where there is one expert; memory for values as input. */
+int qmlp_tokens_mx4_linear_memory(long long rows, int inputs, size_t* bytes);
+int qmlp_tokens_mx4_linear(const qmlp_tensor* input, const qmlp_tensor* input_scales, const qmlp_tensor* weight, const qmlp_tensor* scales,
+                           const qmlp_tensor* offsets, const qmlp_tensor* bias, const qmlp_tensor* output, void* memory, void* stream);
 /* Compiles the kernels for values of QMLP_FLOAT, QMLP_HALF or QMLP_BFLOAT16 into the kernel cache without a device. */
 int qmlp_tokens_precompile(int precision);
 

@@ -18,13 +18,13 @@ QUICKMLP_NAMESPACE_BEGIN
 
 /**
  * Describes an N-dimensional strided tensor in device memory.
- * Datatype can be 'float', 'half' or 'double'; the operators on rows of tokens (tokens.h) know 'bfloat16' and integers besides.
+ * Datatype can be 'float', 'half' or 'double'; the operators on rows of tokens (tokens.h) know 'bfloat16', integers and bytes besides.
  * Either wraps external memory (non-owning) or hosts its own allocation.
  */
 class Tensor
 {
 public:
-    enum Precision { FLOAT, HALF, DOUBLE, BFLOAT16, INT32, INT64, _NUM_PRECISION_ };
+    enum Precision { FLOAT, HALF, DOUBLE, BFLOAT16, INT32, INT64, UINT8, _NUM_PRECISION_ };
     static const int BytesPerEntry[];
     static const std::string DatatypePerEntry[];
     static const std::string NamePerEntry[];
@@ -56,6 +56,8 @@ private:
             throw configuration_error("Illegal type, the tensor stores 32-bit integers!");
         if (precision_ == INT64 && !std::is_same_v<int64_t, U>)
             throw configuration_error("Illegal type, the tensor stores 64-bit integers!");
+        if (precision_ == UINT8 && !std::is_same_v<uint8_t, U>)
+            throw configuration_error("Illegal type, the tensor stores bytes!");
     }
 
 public:

@@ -30,6 +30,8 @@ public:
      * \param offsets (groups + 1) INT32: group g has the entries offsets[g] to offsets[g + 1] - 1 of 'order'
      */
     static void group(const Tensor& index, int groups, Tensor& order, Tensor& offsets, void* memory, stream_t stream);
+    /** \param places (rows) INT32, the place of every row in 'order', -1 - place of the rows that belong to no group; or undefined */
+    static void group(const Tensor& index, int groups, Tensor& order, Tensor& offsets, Tensor& places, void* memory, stream_t stream);
 
     /**
      * output[i] = scale * table[index[i]]; a row of zeros where the index names no row of the table.
@@ -78,6 +80,55 @@ public:
      */
     static void groupedLinearAdjoint(const Tensor& input, const Tensor& weight, const Tensor& offsets, const Tensor& adjOutput, Tensor& adjInput,
                                      Tensor& adjWeight, Tensor& adjBias, void* memory, stream_t stream);
+
+    /**
+     * The router's choice: index[r] are the experts with the largest logits of row r, the first of equals, and weights[r] their shares of the softmax
+     * over all experts, or, 'normalised', over the chosen ones. No row takes an expert whose logit is -inf: -1 and a weight of 0 stand in its place. A
+     * NaN counts as the largest; weights of rows with a NaN or +inf are NaN.
+     * \param logits (rows, experts) \param weights (rows, chosen), of the logits' type \param index (rows, chosen) INT32. 1 <= chosen <= experts, <= 64
+     */
+    static void route(const Tensor& logits, bool normalised, Tensor& weights, Tensor& index, stream_t stream);
+    /** Gradient of the logits, written as a whole. index: as the forward pass left it. */
+    static void routeAdjoint(const Tensor& logits, const Tensor& index, const Tensor& adjWeights, bool normalised, Tensor& adjLogits, stream_t stream);
+
+    /**
+     * Rows of tokens to the places of their experts' rows: rows[places[t][j]] = input[t]; rows of zeros at the places of no expert.
+     * \param input (tokens, channels) \param places (tokens, chosen) INT32, as group() returns them for the chosen experts of every token: those of a
+     * permutation, -1 - place where there is no expert \param rows (tokens * chosen, channels)
+     */
+    static void dispatch(const Tensor& input, const Tensor& places, Tensor& rows, stream_t stream);
+    /**
+     * And back: output[t] = residual[t] + sum over j of weights[t][j] rows[places[t][j]], without the terms of no expert. It is the gradient of dispatch(),
+     * too, with neither weights nor residual.
+     * \param weights (tokens, chosen), of the rows' type or FLOAT, or undefined: 1 \param residual (tokens, channels), or undefined: 0
+     */
+    static void combine(const Tensor& rows, const Tensor& places, const Tensor& weights, const Tensor& residual, Tensor& output, stream_t stream);
+    /** Gradients, written as a whole, each of them may be undefined: not wanted. That of the residual is adjOutput. adjWeights: of the weights' type. */
+    static void combineAdjoint(const Tensor& rows, const Tensor& places, const Tensor& weights, const Tensor& adjOutput, Tensor& adjRows,
+                               Tensor& adjWeights, stream_t stream);
+
+    /**
+     * Numbers of 4 bits in blocks of 32 consecutive entries of a row with a common power of two (MXFP4 of the OCP Microscaling Formats specification
+     * 1.0): sign, two bits of exponent and one of mantissa, to the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 times the scale, halfway to the even code.
+     * A block with an infinity or a NaN becomes NaN.
+     * \param input (rows, columns) \param codes (rows, 16 * ceil(columns / 32)) UINT8, two codes a byte, the first in the low bits, zeros behind the last
+     * \param scales (rows, ceil(columns / 32)) UINT8, the exponents plus 127; 255: NaN
+     */
+    static void quantiseMx4(const Tensor& input, Tensor& codes, Tensor& scales, stream_t stream);
+    /** The values that codes and scales stand for, in the output's type (rows, columns). */
+    static void valuesMx4(const Tensor& codes, const Tensor& scales, Tensor& output, stream_t stream);
+
+    /** Bytes of 'memory' for mx4Linear(). */
+    static size_t mx4LinearMemory(int64_t rows, int inputs);
+    /**
+     * groupedLinear() with weights of 4 bits, on rows that are quantised by the call or have been before.
+     * \param input (rows, inputs), or codes as of quantiseMx4() with inputScales \param inputScales undefined where input holds values
+     * \param weight (experts, outputs, 16 * blocks) UINT8, codes of rows along the inputs \param scales (experts, outputs, blocks) UINT8
+     * \param offsets as of groupedLinear(), or undefined: one expert has all rows \param bias (experts, outputs) of the output's type, or undefined
+     * \param output (rows, outputs), of the input's type where that holds values
+     */
+    static void mx4Linear(const Tensor& input, const Tensor& inputScales, const Tensor& weight, const Tensor& scales, const Tensor& offsets,
+                          const Tensor& bias, Tensor& output, void* memory, stream_t stream);
 
     /** Compiles the kernels for values of one precision into the kernel cache; needs no GPU. */
     static void precompile(Tensor::Precision precision);

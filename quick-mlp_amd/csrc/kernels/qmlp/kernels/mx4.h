@@ -1,0 +1,98 @@
+#pragma once
+// Numbers of 4 bits in blocks of 32 with a common scale: MXFP4 as the OCP Microscaling Formats specification 1.0 has it.
+//
+//   block: 32 consecutive entries of a row;  scale 2^e, e = floor(log2(largest magnitude)) - 2, between -127 and 127, kept as e + 127
+//   code: sign, two bits of exponent and one of mantissa: 0, 0.5, 1, 1.5, 2, 3, 4, 6;  nearest to x / 2^e, halfway to the even code, 6 beyond
+//   a block with an infinity or a NaN has the scale 255, which makes all of its entries NaN
+//
+// A row of n entries has ceil(n / 32) blocks: 16 bytes of codes each, the first entry in the low bits, zeros behind the last, and a byte of scale.
+// The hardware's conversions take the exponent bits of a float as the scale, also those of 0 (2^-127).
+//
+// Bound by memory: 4 lanes share a block, so that a wavefront reads and writes consecutive bytes.
+
+#include <qmlp/kernels/token_types.h>
+
+QUICKMLP_KERNEL_NAMESPACE_BEGIN
+
+constexpr int MX4_THREADS = 256, MX4_BLOCK = 32, MX4_LANES = 4, MX4_ENTRIES = MX4_BLOCK / MX4_LANES;
+
+/** The scale (biased exponent) of a block whose largest magnitude has these bits. */
+__device__ __forceinline__ unsigned mx4Scale(unsigned largest)
+{
+    const int exponent = static_cast<int>(largest >> 23);
+    return exponent == 255 ? 255 : max(exponent - 2, 0);
+}
+__device__ __forceinline__ float mx4ScaleBits(unsigned scale) { return __builtin_bit_cast(float, scale << 23); }
+
+/** Eight codes of values that are finite. */
+__device__ __forceinline__ unsigned mx4Codes(const float (&v)[8], float scale)
+{
+    unsigned codes = 0;
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, v[0], v[1], scale, 0);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, v[2], v[3], scale, 1);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, v[4], v[5], scale, 2);
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, v[6], v[7], scale, 3);
+}
+
+/** x (rows, C), rows of any stride; codes (rows, blocks, 16) and scales (rows, blocks), rows of any stride. */
+template <typename T>
+__global__ void __launch_bounds__(MX4_THREADS)
+Mx4QuantiseKernel(const T* __restrict__ x, long long strideX, unsigned char* __restrict__ codes, long long strideCodes, unsigned char* __restrict__ scales,
+                  long long strideScales, long long units, int blocks, int C)
+{
+    const int lane = threadIdx.x % MX4_LANES;
+    for (long long first = static_cast<long long>(blockIdx.x) * MX4_THREADS; first < units * MX4_LANES; first += static_cast<long long>(gridDim.x) * MX4_THREADS) {
+        const long long unit = min((first + threadIdx.x) / MX4_LANES, units - 1);   // (the last ones are written more than once)
+        const long long row = unit / blocks;
+        const int block = static_cast<int>(unit - row * blocks), at = block * MX4_BLOCK + lane * MX4_ENTRIES;
+        float v[MX4_ENTRIES];
+        if (at + MX4_ENTRIES <= C) loadFloats(x + row * strideX + at, v);
+        else
+#pragma unroll
+            for (int k = 0; k < MX4_ENTRIES; ++k) v[k] = at + k < C ? static_cast<float>(x[row * strideX + at + k]) : 0.0f;
+        unsigned largest = 0;
+#pragma unroll
+        for (int k = 0; k < MX4_ENTRIES; ++k) largest = max(largest, __builtin_bit_cast(unsigned, v[k]) & 0x7fffffffu);
+        largest = max(largest, static_cast<unsigned>(__shfl_xor(static_cast<int>(largest), 1)));
+        largest = max(largest, static_cast<unsigned>(__shfl_xor(static_cast<int>(largest), 2)));
+        const unsigned scale = mx4Scale(largest);
+        const unsigned packed = scale == 255 ? 0 : mx4Codes(v, mx4ScaleBits(scale));
+        __builtin_memcpy(codes + row * strideCodes + block * 16 + lane * 4, &packed, 4);
+        if (lane == 0) scales[row * strideScales + block] = static_cast<unsigned char>(scale);
+    }
+}
+
+/** Eight values. */
+__device__ __forceinline__ void mx4Values(unsigned codes, unsigned scale, float (&v)[8])
+{
+    const float s = mx4ScaleBits(scale);
+    const f32x2 pairs[4] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, s, 0), __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, s, 1),
+                            __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, s, 2), __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, s, 3)};
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = scale == 255 ? __builtin_nanf("") : pairs[k / 2][k % 2];
+}
+
+/** What codes and scales stand for: y (rows, C). */
+template <typename T>
+__global__ void __launch_bounds__(MX4_THREADS)
+Mx4ValuesKernel(const unsigned char* __restrict__ codes, long long strideCodes, const unsigned char* __restrict__ scales, long long strideScales,
+                T* __restrict__ y, long long strideY, long long units, int blocks, int C)
+{
+    const int lane = threadIdx.x % MX4_LANES;
+    for (long long i = static_cast<long long>(blockIdx.x) * MX4_THREADS + threadIdx.x; i < units * MX4_LANES; i += static_cast<long long>(gridDim.x) * MX4_THREADS) {
+        const long long unit = i / MX4_LANES, row = unit / blocks;
+        const int block = static_cast<int>(unit - row * blocks), at = block * MX4_BLOCK + lane * MX4_ENTRIES;
+        unsigned packed;
+        __builtin_memcpy(&packed, codes + row * strideCodes + block * 16 + lane * 4, 4);
+        float v[MX4_ENTRIES];
+        mx4Values(packed, scales[row * strideScales + block], v);
+        T* const to = y + row * strideY + at;
+        if (at + MX4_ENTRIES <= C) storeFloats(to, v);
+        else
+#pragma unroll
+            for (int k = 0; k < MX4_ENTRIES; ++k)
+                if (at + k < C) to[k] = static_cast<T>(v[k]);
+    }
+}
+
+QUICKMLP_KERNEL_NAMESPACE_END

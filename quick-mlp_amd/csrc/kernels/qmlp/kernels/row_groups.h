@@ -106,14 +106,20 @@ __device__ __forceinline__ void markSpans(const unsigned* keys, long long i, lon
     if (i == rows - 1 || keys[i + 1] != key) spans[groups + key] = static_cast<unsigned>(i + 1);
 }
 
+/** What is kept of a row's place in the order: the place itself; -1 - place of rows that belong to no group. */
+__device__ __forceinline__ int placeOf(unsigned key, unsigned groups, unsigned place)
+{
+    return static_cast<int>(key < groups ? place : ~place);
+}
+
 /**
  * All of up to GROUP_SMALL_ROWS rows by one workgroup. bits: of the number 'groups'. keys (the groups in order), offsets (groups + 1
- * of them) and spans (see markSpans()) may be null. LDS: GROUP_SMALL_ROWS keys and rows, the counters of the wavefronts.
+ * of them), spans (see markSpans()) and places (see placeOf()) may be null. LDS: GROUP_SMALL_ROWS keys and rows, the counters of the wavefronts.
  */
 template <typename I>
 __global__ void __launch_bounds__(GROUP_SMALL_THREADS)
 GroupSmallKernel(const I* __restrict__ index, long long stride, int rows, unsigned groups, int bits, int* __restrict__ order,
-                 unsigned* __restrict__ keys, int* __restrict__ offsets, unsigned* __restrict__ spans)
+                 unsigned* __restrict__ keys, int* __restrict__ offsets, unsigned* __restrict__ spans, int* __restrict__ places)
 {
     constexpr int WAVES = GROUP_SMALL_THREADS / 64;
     extern __shared__ unsigned groupLds[];
@@ -178,6 +184,7 @@ GroupSmallKernel(const I* __restrict__ index, long long stride, int rows, unsign
         if (i < items && p < rows) {
             order[p] = row[i];
             if (keys) keys[p] = key[i];
+            if (places) places[row[i]] = placeOf(key[i], groups, p);
             if (spans) markSpans(keysLds, p, rows, groups, spans);
         }
     }
@@ -261,13 +268,14 @@ GroupScanKernel(unsigned* __restrict__ counts, int tiles, int digits, unsigned* 
 
 /**
  * Writes the rows of a tile to their places. counts: as GroupScanKernel leaves them, with totals; without totals (up to
- * GROUP_FEW_TILES tiles) as GroupCountKernel does. keysOut, offsets: may be null; offsets for a sort of one pass only, whose digits are
- * the groups. LDS: a start per digit, the counters of the wavefronts.
+ * GROUP_FEW_TILES tiles) as GroupCountKernel does. keysOut, offsets, places (of the last pass): may be null; offsets for a sort of one pass
+ * only, whose digits are the groups. LDS: a start per digit, the counters of the wavefronts.
  */
 template <typename I, int ITEMS>
 __global__ void __launch_bounds__(GROUP_THREADS)
 GroupScatterKernel(GroupSource<I> source, long long rows, int shift, int digitBits, int digits, const unsigned* __restrict__ counts,
-                   const unsigned* __restrict__ totals, int* __restrict__ orderOut, unsigned* __restrict__ keysOut, int* __restrict__ offsets)
+                   const unsigned* __restrict__ totals, int* __restrict__ orderOut, unsigned* __restrict__ keysOut, int* __restrict__ offsets,
+                   int* __restrict__ places)
 {
     constexpr int WAVES = GROUP_THREADS / 64;
     const unsigned mask = (1u << digitBits) - 1;
@@ -346,6 +354,7 @@ GroupScatterKernel(GroupSource<I> source, long long rows, int shift, int digitBi
             if (w < wave) p += counters[w * digits + d];
         orderOut[p] = row[i];
         if (keysOut) keysOut[p] = key[i];
+        if (places) places[row[i]] = placeOf(key[i], source.groups, p);
     }
 }
 

@@ -80,7 +80,7 @@ Tensor wrap(const qmlp_tensor* t, int lastPrecision = QMLP_DOUBLE)
     return Tensor(t->data, static_cast<Tensor::Precision>(t->precision), sizes, strides);
 }
 /** Of the operators on rows of tokens, which know more types. */
-Tensor wrapToken(const qmlp_tensor* t) { return wrap(t, QMLP_INT64); }
+Tensor wrapToken(const qmlp_tensor* t) { return wrap(t, QMLP_UINT8); }
 
 void unwrap(const Tensor& t, qmlp_tensor* out)
 {
@@ -786,6 +786,92 @@ int qmlp_tokens_grouped_linear_adjoint(const qmlp_tensor* input, const qmlp_tens
     Tensor adjInput = wrapToken(adj_input), adjWeight = wrapToken(adj_weight), adjBias = wrapToken(adj_bias);
     Tokens::groupedLinearAdjoint(wrapToken(input), wrapToken(weight), wrapToken(offsets), wrapToken(adj_output), adjInput, adjWeight, adjBias, memory,
                                  static_cast<stream_t>(stream));
+    QMLP_API_END
+}
+
+int qmlp_tokens_group_places(const qmlp_tensor* index, int groups, const qmlp_tensor* order, const qmlp_tensor* offsets, const qmlp_tensor* places,
+                             void* memory, void* stream)
+{
+    QMLP_API_BEGIN
+    Tensor o = wrapToken(order), f = wrapToken(offsets), p = wrapToken(places);
+    Tokens::group(wrapToken(index), groups, o, f, p, memory, static_cast<stream_t>(stream));
+    QMLP_API_END
+}
+
+int qmlp_tokens_route(const qmlp_tensor* logits, int normalised, const qmlp_tensor* weights, const qmlp_tensor* index, void* stream)
+{
+    QMLP_API_BEGIN
+    Tensor w = wrapToken(weights), i = wrapToken(index);
+    Tokens::route(wrapToken(logits), normalised != 0, w, i, static_cast<stream_t>(stream));
+    QMLP_API_END
+}
+
+int qmlp_tokens_route_adjoint(const qmlp_tensor* logits, const qmlp_tensor* index, const qmlp_tensor* adj_weights, int normalised,
+                              const qmlp_tensor* adj_logits, void* stream)
+{
+    QMLP_API_BEGIN
+    Tensor adjLogits = wrapToken(adj_logits);
+    Tokens::routeAdjoint(wrapToken(logits), wrapToken(index), wrapToken(adj_weights), normalised != 0, adjLogits, static_cast<stream_t>(stream));
+    QMLP_API_END
+}
+
+int qmlp_tokens_dispatch(const qmlp_tensor* input, const qmlp_tensor* places, const qmlp_tensor* rows, void* stream)
+{
+    QMLP_API_BEGIN
+    Tensor r = wrapToken(rows);
+    Tokens::dispatch(wrapToken(input), wrapToken(places), r, static_cast<stream_t>(stream));
+    QMLP_API_END
+}
+
+int qmlp_tokens_combine(const qmlp_tensor* rows, const qmlp_tensor* places, const qmlp_tensor* weights, const qmlp_tensor* residual,
+                        const qmlp_tensor* output, void* stream)
+{
+    QMLP_API_BEGIN
+    Tensor out = wrapToken(output);
+    Tokens::combine(wrapToken(rows), wrapToken(places), wrapToken(weights), wrapToken(residual), out, static_cast<stream_t>(stream));
+    QMLP_API_END
+}
+
+int qmlp_tokens_combine_adjoint(const qmlp_tensor* rows, const qmlp_tensor* places, const qmlp_tensor* weights, const qmlp_tensor* adj_output,
+                                const qmlp_tensor* adj_rows, const qmlp_tensor* adj_weights, void* stream)
+{
+    QMLP_API_BEGIN
+    Tensor adjRows = wrapToken(adj_rows), adjWeights = wrapToken(adj_weights);
+    Tokens::combineAdjoint(wrapToken(rows), wrapToken(places), wrapToken(weights), wrapToken(adj_output), adjRows, adjWeights,
+                           static_cast<stream_t>(stream));
+    QMLP_API_END
+}
+
+int qmlp_tokens_mx4_quantise(const qmlp_tensor* input, const qmlp_tensor* codes, const qmlp_tensor* scales, void* stream)
+{
+    QMLP_API_BEGIN
+    Tensor c = wrapToken(codes), s = wrapToken(scales);
+    Tokens::quantiseMx4(wrapToken(input), c, s, static_cast<stream_t>(stream));
+    QMLP_API_END
+}
+
+int qmlp_tokens_mx4_values(const qmlp_tensor* codes, const qmlp_tensor* scales, const qmlp_tensor* output, void* stream)
+{
+    QMLP_API_BEGIN
+    Tensor out = wrapToken(output);
+    Tokens::valuesMx4(wrapToken(codes), wrapToken(scales), out, static_cast<stream_t>(stream));
+    QMLP_API_END
+}
+
+int qmlp_tokens_mx4_linear_memory(long long rows, int inputs, size_t* bytes)
+{
+    QMLP_API_BEGIN
+    *bytes = Tokens::mx4LinearMemory(rows, inputs);
+    QMLP_API_END
+}
+
+int qmlp_tokens_mx4_linear(const qmlp_tensor* input, const qmlp_tensor* input_scales, const qmlp_tensor* weight, const qmlp_tensor* scales,
+                           const qmlp_tensor* offsets, const qmlp_tensor* bias, const qmlp_tensor* output, void* memory, void* stream)
+{
+    QMLP_API_BEGIN
+    Tensor out = wrapToken(output);
+    Tokens::mx4Linear(wrapToken(input), wrapToken(input_scales), wrapToken(weight), wrapToken(scales), wrapToken(offsets), wrapToken(bias), out, memory,
+                      static_cast<stream_t>(stream));
     QMLP_API_END
 }
 

@@ -1,0 +1,350 @@
+#include "token_calls.h"
+
+QUICKMLP_NAMESPACE_BEGIN
+
+using namespace token;
+
+namespace {
+
+// ------------------------------------------------------------------------------------------------ router
+// as in kernels/route.h
+constexpr int ROUTE_THREADS = 256, ROUTE_MOST_CHOSEN = 64;
+
+/** Lanes that share a row, and how many logits each of them holds; none of them: more than a wavefront holds. */
+struct RouteShape
+{
+    int lanes, entries;
+    int rows() const { return ROUTE_THREADS / lanes; }
+    std::string arguments(Tensor::Precision p) const { return str("<", scalarName(p), ", ", lanes, ", ", entries, ">"); }
+};
+constexpr RouteShape ROUTE_SHAPES[] = {{8, 4}, {8, 8}, {16, 8}, {32, 8}, {64, 8}, {64, 16}};
+RouteShape routeShape(int experts)
+{
+    for (const RouteShape& s : ROUTE_SHAPES)
+        if (s.lanes * s.entries >= experts) return s;
+    return {0, 0};
+}
+
+struct RouteSizes
+{
+    long long rows;
+    int experts, chosen;
+};
+RouteSizes checkRoute(const Tensor& logits, const Tensor& weights, const char* what, const Tensor& index)
+{
+    checkValues(logits, "logits", 2);
+    checkValues(weights, what, 2);
+    checkType(weights, what, logits.precision());
+    CHECK_ERROR(index.defined() && index.ndim() == 2, "index must be a tensor with 2 dimensions");
+    checkType(index, "index", Tensor::INT32);
+    checkStrides(index, "index");
+    CHECK_ERROR(index.size(1) <= 1 || index.numel() == 0 || index.stride(1) == 1, "index must be consecutive along its last dimension");
+    const RouteSizes s{logits.size(0), logits.size(1), index.size(1)};
+    CHECK_ERROR(s.chosen >= 1 && s.chosen <= s.experts && s.chosen <= ROUTE_MOST_CHOSEN, "between 1 and ", ROUTE_MOST_CHOSEN,
+                " experts can be chosen, and no more than there are, but they are ", s.chosen, " of ", s.experts);
+    checkSizes(weights, what, {s.rows, s.chosen});
+    checkSizes(index, "index", {s.rows, s.chosen});
+    checkSteps("experts", s.experts);
+    return s;
+}
+
+// ------------------------------------------------------------------------------------------------ rows to experts and back
+// as in kernels/expert_rows.h
+constexpr int EXPERT_ROWS_THREADS = 256;
+
+struct ExpertRowsSizes
+{
+    long long tokens;
+    int chosen, channels;
+    /** Entries of an access and lanes of a token. */
+    int vec(Tensor::Precision p) const { return channels < wide(p) ? 1 : wide(p); }
+    int lanes(Tensor::Precision p, int most) const { return lanesPerRow(channels, vec(p), most); }
+};
+ExpertRowsSizes checkExpertRows(const Tensor& rows, const Tensor& places)
+{
+    checkValues(rows, "rows", 2);
+    CHECK_ERROR(places.defined() && places.ndim() == 2, "places must be a tensor with 2 dimensions");
+    checkType(places, "places", Tensor::INT32);
+    checkStrides(places, "places");
+    CHECK_ERROR(places.size(1) <= 1 || places.numel() == 0 || places.stride(1) == 1, "places must be consecutive along its last dimension");
+    const ExpertRowsSizes s{places.size(0), places.size(1), rows.size(1)};
+    CHECK_ERROR(places.numel() < (1ll << 31), "tokens times chosen experts must fit into 32 bits");
+    checkSizes(rows, "rows", {places.numel(), s.channels});
+    checkSteps("channels", s.channels);
+    return s;
+}
+void checkTokens(const Tensor& t, const char* what, const Tensor& rows, const ExpertRowsSizes& s)
+{
+    checkValues(t, what, 2);
+    checkType(t, what, rows.precision());
+    checkSizes(t, what, {s.tokens, s.channels});
+}
+/** Weights or their gradients. */
+void checkExpertWeights(const Tensor& t, const char* what, const Tensor& rows, const ExpertRowsSizes& s)
+{
+    if (!t.defined()) return;
+    checkValues(t, what, 2);
+    CHECK_ERROR(t.precision() == rows.precision() || t.precision() == Tensor::FLOAT, what, " must be of the rows' type or FLOAT");
+    checkSizes(t, what, {s.tokens, s.chosen});
+}
+long long strideOrNone(const Tensor& t) { return t.defined() ? strideOf(t, 0) : 0; }
+
+/** Values are moved as they are: a name of a type of their size. */
+const char* bitsName(Tensor::Precision p) { return p == Tensor::FLOAT ? "unsigned" : "unsigned short"; }
+
+// ------------------------------------------------------------------------------------------------ numbers of 4 bits
+// as in kernels/mx4.h and kernels/mx4_linear.h
+constexpr int MX4_THREADS = 256, MX4_BLOCK = 32, MX4_LANES = 4, MX4_FEW_WAVES = 4;
+struct Mx4Matrix
+{
+    const unsigned char *codes, *scales;
+    long long codesExpert, scalesExpert, codesRow, scalesRow;
+};
+
+/** Codes and scales of 'dims' dimensions; returns the blocks of a row. */
+int checkMx4(const Tensor& codes, const char* whatCodes, const Tensor& scales, const char* whatScales, int dims)
+{
+    for (const auto& [t, what] : {std::pair<const Tensor&, const char*>{codes, whatCodes}, {scales, whatScales}}) {
+        CHECK_ERROR(t.defined() && t.ndim() == dims, what, " must be a tensor with ", dims, " dimensions");
+        checkType(t, what, Tensor::UINT8);
+        checkStrides(t, what);
+        CHECK_ERROR(t.size(dims - 1) <= 1 || t.numel() == 0 || t.stride(dims - 1) == 1, what, " must be consecutive along its last dimension");
+    }
+    const int blocks = scales.size(dims - 1);
+    for (int d = 0; d + 1 < dims; ++d)
+        CHECK_ERROR(codes.size(d) == scales.size(d), whatCodes, " and ", whatScales, " must be of one size, but have ", codes.size(d), " and ",
+                    scales.size(d), " entries at dimension ", d);
+    CHECK_ERROR(codes.size(dims - 1) == 16ll * blocks, whatCodes, " must have 16 bytes for each of the ", blocks, " blocks of a row, but has ",
+                codes.size(dims - 1));
+    return blocks;
+}
+int mx4Blocks(int64_t columns) { return static_cast<int>(divUp<int64_t>(columns, MX4_BLOCK)); }
+unsigned mx4Workgroups(long long units) { return workgroups(divUp<int64_t>(units * MX4_LANES, MX4_THREADS), 1 << 16); }
+
+void launchQuantise(const Tensor& input, unsigned char* codes, long long strideCodes, unsigned char* scales, long long strideScales, stream_t stream)
+{
+    const int blocks = mx4Blocks(input.size(1));
+    const long long units = static_cast<long long>(input.size(0)) * blocks;
+    if (units == 0) return;
+    const Tensor::Precision p = input.precision();
+    tokenKernel("mx4.h", kernelKey(MX4_QUANTISE, p), [&] { return str("Mx4QuantiseKernel<", scalarName(p), ">"); })
+        .call(mx4Workgroups(units), MX4_THREADS, 0, stream, input.rawPtr(), strideOf(input, 0), codes, strideCodes, scales, strideScales, units, blocks,
+              static_cast<int>(input.size(1)));
+}
+
+/** Rows of the 4-bit operand as a call makes them in its memory. */
+struct Mx4Rows
+{
+    Workspace memory;
+    unsigned char *codes, *scales;
+    Mx4Rows(int64_t rows, int blocks, void* base)
+        : memory{static_cast<char*>(base)}, codes(memory.take<unsigned char>(rows * blocks * 16)), scales(memory.take<unsigned char>(rows * blocks))
+    {
+    }
+};
+
+} // namespace
+
+// ------------------------------------------------------------------------------------------------ entry points
+void Tokens::route(const Tensor& logits, bool normalised, Tensor& weights, Tensor& index, stream_t stream)
+{
+    const RouteSizes s = checkRoute(logits, weights, "weights", index);
+    checkOutput(weights, "weights");
+    checkOutput(index, "index");
+    if (s.rows == 0) return;
+    const Tensor::Precision p = logits.precision();
+    const RouteShape shape = routeShape(s.experts);
+    const bool isLong = shape.lanes == 0;
+    tokenKernel("route.h", isLong ? kernelKey(ROUTE_LONG, p) : kernelKey(ROUTE, p, shape.lanes, shape.entries),
+                [&] { return isLong ? str("RouteLongKernel<", scalarName(p), ">") : "RouteKernel" + shape.arguments(p); })
+        .call(isLong ? workgroups(s.rows, 4096) : workgroups(divUp<int64_t>(s.rows, shape.rows()), 1 << 16), ROUTE_THREADS,
+              8 * s.chosen * (isLong ? 1 : shape.rows()), stream, logits.rawPtr(), strideOf(logits, 0), weights.rawPtr(), strideOf(weights, 0),
+              ptr<int>(index), strideOf(index, 0), s.rows, s.experts, s.chosen, static_cast<int>(normalised));
+}
+
+void Tokens::routeAdjoint(const Tensor& logits, const Tensor& index, const Tensor& adjWeights, bool normalised, Tensor& adjLogits, stream_t stream)
+{
+    const RouteSizes s = checkRoute(logits, adjWeights, "adjWeights", index);
+    checkValues(adjLogits, "adjLogits", 2);
+    checkType(adjLogits, "adjLogits", logits.precision());
+    checkSizes(adjLogits, "adjLogits", {s.rows, s.experts});
+    checkOutput(adjLogits, "adjLogits");
+    if (s.rows == 0) return;
+    const Tensor::Precision p = logits.precision();
+    const RouteShape shape = routeShape(s.experts);
+    const bool isLong = shape.lanes == 0;
+    tokenKernel("route.h", isLong ? kernelKey(ROUTE_LONG_ADJOINT, p) : kernelKey(ROUTE_ADJOINT, p, shape.lanes, shape.entries),
+                [&] { return isLong ? str("RouteLongAdjointKernel<", scalarName(p), ">") : "RouteAdjointKernel" + shape.arguments(p); })
+        .call(isLong ? workgroups(s.rows, 4096) : workgroups(divUp<int64_t>(s.rows, shape.rows()), 1 << 16), ROUTE_THREADS, 0, stream, logits.rawPtr(),
+              strideOf(logits, 0), static_cast<const int*>(ptr<int>(index)), strideOf(index, 0), adjWeights.rawPtr(), strideOf(adjWeights, 0),
+              adjLogits.rawPtr(), strideOf(adjLogits, 0), s.rows, s.experts, s.chosen, static_cast<int>(normalised));
+}
+
+void Tokens::dispatch(const Tensor& input, const Tensor& places, Tensor& rows, stream_t stream)
+{
+    const ExpertRowsSizes s = checkExpertRows(rows, places);
+    checkTokens(input, "input", rows, s);
+    checkOutput(rows, "rows");
+    if (rows.numel() == 0) return;
+    const Tensor::Precision p = rows.precision();
+    const int vec = s.vec(p), lanes = s.lanes(p, EXPERT_ROWS_THREADS);
+    tokenKernel("expert_rows.h", kernelKey(DISPATCH, rows.bytesPerEntry(), vec, lanes),
+                [&] { return str("DispatchKernel<", bitsName(p), ", ", vec, ", ", lanes, ">"); })
+        .call(workgroups(divUp<int64_t>(s.tokens, EXPERT_ROWS_THREADS / lanes), 1 << 20), EXPERT_ROWS_THREADS, 0, stream, input.rawPtr(), strideOf(input, 0),
+              static_cast<const int*>(ptr<int>(places)), strideOf(places, 0), s.chosen, rows.rawPtr(), strideOf(rows, 0), s.tokens, s.channels);
+}
+
+void Tokens::combine(const Tensor& rows, const Tensor& places, const Tensor& weights, const Tensor& residual, Tensor& output, stream_t stream)
+{
+    const ExpertRowsSizes s = checkExpertRows(rows, places);
+    checkExpertWeights(weights, "weights", rows, s);
+    if (residual.defined()) checkTokens(residual, "residual", rows, s);
+    checkTokens(output, "output", rows, s);
+    checkOutput(output, "output");
+    if (output.numel() == 0) return;
+    const Tensor::Precision p = rows.precision();
+    const int vec = s.vec(p), lanes = s.lanes(p, EXPERT_ROWS_THREADS);
+    tokenKernel("expert_rows.h", kernelKey(COMBINE, p, vec, lanes), [&] { return str("CombineKernel<", scalarName(p), ", ", vec, ", ", lanes, ">"); })
+        .call(workgroups(divUp<int64_t>(s.tokens, EXPERT_ROWS_THREADS / lanes), 1 << 20), EXPERT_ROWS_THREADS, 0, stream, rows.rawPtr(), strideOf(rows, 0),
+              static_cast<const int*>(ptr<int>(places)), strideOf(places, 0), s.chosen, static_cast<const void*>(ptr<void>(weights)), strideOrNone(weights),
+              static_cast<int>(weights.defined() && weights.precision() == Tensor::FLOAT), static_cast<const void*>(ptr<void>(residual)),
+              strideOrNone(residual), output.rawPtr(), strideOf(output, 0), s.tokens, s.channels);
+}
+
+void Tokens::combineAdjoint(const Tensor& rows, const Tensor& places, const Tensor& weights, const Tensor& adjOutput, Tensor& adjRows, Tensor& adjWeights,
+                            stream_t stream)
+{
+    const ExpertRowsSizes s = checkExpertRows(rows, places);
+    checkExpertWeights(weights, "weights", rows, s);
+    checkExpertWeights(adjWeights, "adjWeights", rows, s);
+    if (weights.defined() && adjWeights.defined()) checkType(adjWeights, "adjWeights", weights.precision());
+    checkTokens(adjOutput, "adjOutput", rows, s);
+    if (adjRows.defined()) {
+        checkValues(adjRows, "adjRows", 2);
+        checkType(adjRows, "adjRows", rows.precision());
+        checkSizes(adjRows, "adjRows", {rows.size(0), s.channels});
+        checkOutput(adjRows, "adjRows");
+    }
+    if (adjWeights.defined()) checkOutput(adjWeights, "adjWeights");
+    if (places.numel() == 0 || (!adjRows.defined() && !adjWeights.defined())) return;
+    const Tensor::Precision p = rows.precision();
+    const int vec = s.vec(p), lanes = s.lanes(p, 64);
+    const Tensor& typed = weights.defined() ? weights : adjWeights;
+    tokenKernel("expert_rows.h", kernelKey(COMBINE_ADJOINT, p, vec, lanes),
+                [&] { return str("CombineAdjointKernel<", scalarName(p), ", ", vec, ", ", lanes, ">"); })
+        .call(workgroups(divUp<int64_t>(s.tokens, EXPERT_ROWS_THREADS / lanes), 1 << 20), EXPERT_ROWS_THREADS, 0, stream, rows.rawPtr(), strideOf(rows, 0),
+              static_cast<const int*>(ptr<int>(places)), strideOf(places, 0), s.chosen, static_cast<const void*>(ptr<void>(weights)), strideOrNone(weights),
+              static_cast<int>(typed.defined() && typed.precision() == Tensor::FLOAT), adjOutput.rawPtr(), strideOf(adjOutput, 0), ptr<void>(adjRows),
+              strideOrNone(adjRows), ptr<void>(adjWeights), strideOrNone(adjWeights), s.tokens, s.channels);
+}
+
+void Tokens::quantiseMx4(const Tensor& input, Tensor& codes, Tensor& scales, stream_t stream)
+{
+    checkValues(input, "input", 2);
+    checkSteps("columns", input.size(1));
+    const int blocks = checkMx4(codes, "codes", scales, "scales", 2);
+    CHECK_ERROR(blocks == mx4Blocks(input.size(1)), "scales must have ", mx4Blocks(input.size(1)), " entries at dimension 1, but has ", blocks);
+    checkSizes(scales, "scales", {input.size(0), blocks});
+    checkOutput(codes, "codes");
+    checkOutput(scales, "scales");
+    launchQuantise(input, ptr<unsigned char>(codes), strideOf(codes, 0), ptr<unsigned char>(scales), strideOf(scales, 0), stream);
+}
+
+void Tokens::valuesMx4(const Tensor& codes, const Tensor& scales, Tensor& output, stream_t stream)
+{
+    checkValues(output, "output", 2);
+    checkOutput(output, "output");
+    checkSteps("columns", output.size(1));
+    const int blocks = checkMx4(codes, "codes", scales, "scales", 2);
+    CHECK_ERROR(blocks == mx4Blocks(output.size(1)), "scales must have ", mx4Blocks(output.size(1)), " entries at dimension 1, but has ", blocks);
+    checkSizes(scales, "scales", {output.size(0), blocks});
+    const long long units = static_cast<long long>(output.size(0)) * blocks;
+    if (units == 0) return;
+    const Tensor::Precision p = output.precision();
+    tokenKernel("mx4.h", kernelKey(MX4_VALUES, p), [&] { return str("Mx4ValuesKernel<", scalarName(p), ">"); })
+        .call(mx4Workgroups(units), MX4_THREADS, 0, stream, static_cast<const unsigned char*>(ptr<unsigned char>(codes)), strideOf(codes, 0),
+              static_cast<const unsigned char*>(ptr<unsigned char>(scales)), strideOf(scales, 0), output.rawPtr(), strideOf(output, 0), units, blocks,
+              static_cast<int>(output.size(1)));
+}
+
+size_t Tokens::mx4LinearMemory(int64_t rows, int inputs)
+{
+    CHECK_ERROR(rows >= 0 && inputs >= 0, "sizes must not be negative");
+    return Mx4Rows(rows, mx4Blocks(inputs), nullptr).memory.bytes;
+}
+
+void Tokens::mx4Linear(const Tensor& input, const Tensor& inputScales, const Tensor& weight, const Tensor& scales, const Tensor& offsets, const Tensor& bias,
+                       Tensor& output, void* memory, stream_t stream)
+{
+    const int blocks = checkMx4(weight, "weight", scales, "scales", 3);
+    const bool quantised = inputScales.defined();
+    if (quantised) {
+        const int of = checkMx4(input, "input", inputScales, "inputScales", 2);
+        CHECK_ERROR(of == blocks, "input must have the weights' ", blocks, " blocks in a row, but has ", of);
+    } else {
+        checkValues(input, "input", 2);
+        CHECK_ERROR(mx4Blocks(input.size(1)) == blocks, "input must have the weights' ", blocks, " blocks in a row, but has ", mx4Blocks(input.size(1)));
+    }
+    const int rows = input.size(0), experts = weight.size(0), outputs = weight.size(1);
+    CHECK_ERROR(blocks > 0 && outputs > 0, "experts must have inputs and outputs");
+    if (offsets.defined()) {
+        CHECK_ERROR(offsets.ndim() == 1, "offsets must be a tensor with 1 dimension");
+        checkType(offsets, "offsets", Tensor::INT32);
+        CHECK_ERROR(offsets.size(0) <= 1 || offsets.stride(0) == 1, "offsets must be contiguous");
+        checkSizes(offsets, "offsets", {experts + 1ll});
+    } else
+        CHECK_ERROR(experts == 1, "without offsets there must be one expert, but there are ", experts);
+    checkValues(output, "output", 2);
+    if (!quantised) checkType(output, "output", input.precision());
+    checkSizes(output, "output", {rows, outputs});
+    checkOutput(output, "output");
+    if (bias.defined()) {
+        checkValues(bias, "bias", 2);
+        checkType(bias, "bias", output.precision());
+        checkSizes(bias, "bias", {experts, outputs});
+    }
+    checkSteps("rows", rows);
+    checkSteps("inputs", static_cast<int64_t>(blocks) * MX4_BLOCK);
+    checkSteps("outputs", outputs);
+    if (rows == 0) return;
+    const Tensor::Precision p = output.precision();
+    const int64_t places = static_cast<int64_t>(rows) / 16 + experts + 1, tilesJ = divUp<int64_t>(outputs, 16 * MX4_FEW_WAVES);
+    checkLaunch(places * tilesJ, 64 * MX4_FEW_WAVES);
+    Mx4Rows x(rows, blocks, memory);
+    long long strideX = blocks * 16ll, strideScalesX = blocks;
+    if (quantised) {
+        x.codes = ptr<unsigned char>(input);
+        x.scales = ptr<unsigned char>(inputScales);
+        strideX = strideOf(input, 0);
+        strideScalesX = strideOf(inputScales, 0);
+    } else {
+        checkMemory(memory, x.memory.bytes);
+        launchQuantise(input, x.codes, strideX, x.scales, strideScalesX, stream);
+    }
+    const Mx4Matrix w{ptr<unsigned char>(weight), ptr<unsigned char>(scales), strideOf(weight, 0), strideOf(scales, 0), strideOf(weight, 1), strideOf(scales, 1)};
+    tokenKernel("mx4_linear.h", kernelKey(MX4_FEW, p), [&] { return str("Mx4FewKernel<", scalarName(p), ">"); })
+        .call(static_cast<unsigned>(places * tilesJ), 64 * MX4_FEW_WAVES, 0, stream, static_cast<const unsigned char*>(x.codes),
+              static_cast<const unsigned char*>(x.scales), strideX, strideScalesX, w, static_cast<const void*>(ptr<void>(bias)), strideOrNone(bias),
+              static_cast<const int*>(ptr<int>(offsets)), experts, output.rawPtr(), strideOf(output, 0), rows, outputs, blocks, static_cast<int>(places),
+              static_cast<int>(tilesJ));
+}
+
+void token::precompileExperts(Tensor::Precision p)
+{
+    const std::string t = scalarName(p);
+    for (const RouteShape& s : ROUTE_SHAPES)
+        for (const char* kernel : {"RouteKernel", "RouteAdjointKernel"}) precompileKernel("route.h", kernel + s.arguments(p));
+    for (const char* kernel : {"RouteLongKernel", "RouteLongAdjointKernel"}) precompileKernel("route.h", str(kernel, "<", t, ">"));
+    for (const int vec : {1, wide(p)})
+        for (const int lanes : {8, 16, 32, 64, 128, 256}) {
+            if (vec == 1 && lanes > 8) continue;
+            const std::string shape = str(", ", vec, ", ", lanes, ">");
+            precompileKernel("expert_rows.h", str("DispatchKernel<", bitsName(p), shape));
+            precompileKernel("expert_rows.h", str("CombineKernel<", t, shape));
+            if (lanes <= 64) precompileKernel("expert_rows.h", str("CombineAdjointKernel<", t, shape));
+        }
+    for (const char* kernel : {"Mx4QuantiseKernel", "Mx4ValuesKernel"}) precompileKernel("mx4.h", str(kernel, "<", t, ">"));
+    precompileKernel("mx4_linear.h", str("Mx4FewKernel<", t, ">"));
+}
+
+QUICKMLP_NAMESPACE_END

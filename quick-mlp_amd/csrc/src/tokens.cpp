@@ -1,177 +1,12 @@
-#include <qmlp/tokens.h>
+#include "token_calls.h"
 
-#include <qmlp/errors.h>
-#include <qmlp/qmlp.h>
-
-#include "qmlp_hip.h"
-
-#include <algorithm>
 #include <array>
-#include <mutex>
-#include <unordered_map>
 
 QUICKMLP_NAMESPACE_BEGIN
 
+using namespace token;
+
 namespace {
-
-constexpr size_t ALIGNMENT = 256;
-
-// ------------------------------------------------------------------------------------------------ kernels
-const char* scalarName(Tensor::Precision p)
-{
-    switch (p) {
-        case Tensor::FLOAT: return "float";
-        case Tensor::HALF: return "_Float16";
-        case Tensor::BFLOAT16: return "__bf16";
-        case Tensor::INT32: return "int";
-        case Tensor::INT64: return "long long";
-        default: throw std::runtime_error("values must be float, half or bfloat16, indices 32- or 64-bit integers");
-    }
-}
-
-/** Entries of a 16-byte access. */
-int wide(Tensor::Precision p) { return 16 / Tensor::BytesPerEntry[p]; }
-
-enum KernelId { GROUP_SMALL = 1, GROUP_COUNT, GROUP_SCAN, GROUP_SCATTER, GROUP_OFFSETS, EMBEDDING, EMBEDDING_BLOCKS, EMBEDDING_ADJOINT, LAYER_NORM,
-                LAYER_NORM_ADJOINT, LAYER_NORM_SUM, LAYER_NORM_LONG, LAYER_NORM_LONG_ADJOINT, LAYER_NORM_LONG_SUMS, GROUPED_ROWS, GROUPED_WEIGHTS,
-                GROUPED_SUM, GROUPED_JOIN, KERNEL_IDS };
-/**
- * One number for a kernel and its template arguments, each below 2^11: to build its name takes as long as to launch it. No id is 0, so that
- * kernels with n arguments have numbers from 2^(11 n) up to less than 2^(11 (n + 1)).
- */
-template <typename... Args>
-constexpr uint64_t kernelKey(KernelId id, Args... args)
-{
-    static_assert(sizeof...(args) <= 5 && KERNEL_IDS <= 1 << (64 - 5 * 11), "64 bits");
-    uint64_t key = id;
-    ((key = key << 11 | static_cast<uint64_t>(args)), ...);
-    return key;
-}
-static_assert(kernelKey(GROUP_SMALL, 0) > kernelKey(KERNEL_IDS), "the smallest number with an argument is above all without");
-/** The kernels in use, which stay loaded for the life of the process. */
-struct TokenKernels
-{
-    std::mutex mutex;
-    std::unordered_map<uint64_t, KernelFunction> loaded;
-};
-TokenKernels& tokenKernels()
-{
-    static TokenKernels kernels;
-    return kernels;
-}
-/** File: below kernels/qmlp/kernels; name(): with its template arguments. */
-template <typename Name>
-KernelFunction& tokenKernel(const char* file, uint64_t key, Name name)
-{
-    TokenKernels& kernels = tokenKernels();
-    std::lock_guard<std::mutex> lock(kernels.mutex);
-    auto it = kernels.loaded.find(key);
-    if (it == kernels.loaded.end()) {
-        auto loaded = QuickMLP::Instance().kernelLoader()->getKernel("qmlp::kernel::" + std::string(name()),
-                                                                     KernelLoader::MainFile(std::string("qmlp/kernels/") + file),
-                                                                     QuickMLP::Instance().getCompileFlags() | KernelLoader::CompileThrowOnError);
-        it = kernels.loaded.emplace(key, std::move(*loaded)).first;
-    }
-    return it->second;
-}
-void precompileKernel(const char* file, const std::string& name)
-{
-    QuickMLP::Instance().kernelLoader()->getKernel("qmlp::kernel::" + name, KernelLoader::MainFile(std::string("qmlp/kernels/") + file),
-                                                   QuickMLP::Instance().getCompileFlags() | KernelLoader::CompileThrowOnError | KernelLoader::CompileOnly);
-}
-
-/** Hands out a workspace piece by piece; without a base only its size is wanted. */
-struct Workspace
-{
-    char* base;
-    size_t bytes = 0;
-    template <typename T>
-    T* take(int64_t count)
-    {
-        T* p = base ? reinterpret_cast<T*>(base + bytes) : nullptr;
-        bytes += roundUp(static_cast<size_t>(std::max<int64_t>(count, 0)) * sizeof(T), ALIGNMENT);
-        return p;
-    }
-};
-
-// ------------------------------------------------------------------------------------------------ checks
-bool isValue(Tensor::Precision p) { return p == Tensor::FLOAT || p == Tensor::HALF || p == Tensor::BFLOAT16; }
-
-void checkStrides(const Tensor& t, const char* what)
-{
-    for (int d = 0; d < t.ndim(); ++d) {
-        CHECK_ERROR(t.size(d) >= 0, what, " has a negative size");
-        if (t.size(d) <= 1) continue;   // its stride is not used
-        CHECK_ERROR(t.stride(d) >= 0, what, " has a negative stride");
-    }
-}
-/** Values, whose last dimension is consecutive. */
-void checkValues(const Tensor& t, const char* what, int dims)
-{
-    CHECK_ERROR(t.defined(), what, " is undefined");
-    CHECK_ERROR(t.ndim() == dims, what, " must be a tensor with ", dims, " dimensions, but has ", t.ndim());
-    CHECK_ERROR(isValue(t.precision()), what, " must be of type float, half or bfloat16, but is ", Tensor::NamePerEntry[t.precision()]);
-    checkStrides(t, what);
-    CHECK_ERROR(t.size(dims - 1) <= 1 || t.numel() == 0 || t.stride(dims - 1) == 1, what, " must be consecutive along its last dimension");
-}
-void checkSizes(const Tensor& t, const char* what, std::initializer_list<int64_t> sizes)
-{
-    int d = 0;
-    for (const int64_t s : sizes) {
-        CHECK_ERROR(t.size(d) == s, what, " must have ", s, " entries at dimension ", d, ", but has ", t.size(d));
-        ++d;
-    }
-}
-void checkType(const Tensor& t, const char* what, Tensor::Precision p)
-{
-    CHECK_ERROR(t.precision() == p, what, " must be of type ", Tensor::NamePerEntry[p], ", but is ", Tensor::NamePerEntry[t.precision()]);
-}
-/** Something is written: no two entries may be one. */
-void checkOutput(const Tensor& t, const char* what)
-{
-    for (int d = 0; d + 1 < t.ndim(); ++d) {
-        int64_t inner = 1;
-        for (int k = d + 1; k < t.ndim(); ++k) inner += static_cast<int64_t>(t.size(k) - 1) * t.stride(k);
-        CHECK_ERROR(t.numel() == 0 || t.size(d) <= 1 || t.stride(d) >= inner, what, " has entries that share memory");
-    }
-}
-void checkContiguous(const Tensor& t, const char* what)
-{
-    int64_t stride = 1;
-    for (int d = t.ndim() - 1; d >= 0; --d) {
-        CHECK_ERROR(t.size(d) <= 1 || t.stride(d) == stride, what, " must be contiguous");
-        stride *= t.size(d);
-    }
-}
-/** The kernels go along some sizes in steps of up to 2048 entries, counted in 32 bits: the step behind the last entry has a number too. */
-void checkSteps(const char* what, int64_t size)
-{
-    constexpr int64_t most = (1ll << 31) - (1ll << 12);
-    CHECK_ERROR(size <= most, what, " must not be more than ", most, ", but are ", size);
-}
-void checkIndex(const Tensor& t, const char* what)
-{
-    CHECK_ERROR(t.defined() && t.ndim() == 1, what, " must be a tensor with 1 dimension");
-    CHECK_ERROR(t.precision() == Tensor::INT32 || t.precision() == Tensor::INT64, what, " must hold 32- or 64-bit integers, but is ",
-                Tensor::NamePerEntry[t.precision()]);
-    checkStrides(t, what);
-}
-void checkMemory(const void* memory, size_t bytes)
-{
-    CHECK_ERROR(bytes == 0 || memory != nullptr, "the call needs ", bytes, " bytes of memory");
-    CHECK_ERROR(reinterpret_cast<uintptr_t>(memory) % ALIGNMENT == 0, "memory must be aligned to ", ALIGNMENT, " bytes");
-}
-
-template <typename T>
-T* ptr(const Tensor& t) { return t.defined() ? static_cast<T*>(const_cast<void*>(t.rawPtr())) : nullptr; }
-/** The stride of a dimension; of one with a single entry it may be anything and is taken to be that of rows side by side. */
-long long strideOf(const Tensor& t, int d) { return t.size(d) <= 1 ? t.size(t.ndim() - 1) : t.stride(d); }
-
-/** A launch counts its threads in 32 bits. */
-bool isLaunch(int64_t groups, int threads) { return groups * threads < (1ll << 32); }
-void checkLaunch(int64_t groups, int threads) { CHECK_ERROR(isLaunch(groups, threads), "the call is too large for one launch"); }
-/** Workgroups for so many pieces of work of their own, no more than 'most' (the kernels go on in steps of the grid). */
-unsigned workgroups(int64_t pieces, int64_t most) { return static_cast<unsigned>(std::max<int64_t>(1, std::min(pieces, most))); }
 
 // ------------------------------------------------------------------------------------------------ groups
 // as in kernels/row_groups.h
@@ -227,8 +62,8 @@ struct GroupPlan
     }
 };
 
-/** Sorts; keysOut (the groups in order) and offsets may be null. spans, if not null, are written for small batches: true. */
-bool sortByGroup(const Tensor& index, GroupPlan& plan, int* order, unsigned* keysOut, int* offsets, unsigned* spans, stream_t stream)
+/** Sorts; keysOut (the groups in order), offsets and places may be null. spans, if not null, are written for small batches: true. */
+bool sortByGroup(const Tensor& index, GroupPlan& plan, int* order, unsigned* keysOut, int* offsets, unsigned* spans, int* places, stream_t stream)
 {
     const Tensor::Precision type = index.precision();
     const long long stride = strideOf(index, 0);
@@ -237,7 +72,7 @@ bool sortByGroup(const Tensor& index, GroupPlan& plan, int* order, unsigned* key
         const size_t lds = plan.rows * 6 + 64 + (static_cast<size_t>(GROUP_SMALL_THREADS / 64 * 4) << std::min(bits, GROUP_SMALL_BITS)) + 4;
         tokenKernel("row_groups.h", kernelKey(GROUP_SMALL, type), [&] { return str("GroupSmallKernel<", scalarName(type), ">"); })
             .call(1, GROUP_SMALL_THREADS, static_cast<unsigned>(lds), stream, index.rawPtr(), stride, static_cast<int>(plan.rows), plan.groups, bits, order,
-                  keysOut, offsets, spans);
+                  keysOut, offsets, spans, places);
         return spans != nullptr;
     }
     auto arguments = [&] { return str("<", scalarName(type), ", ", plan.items, ">"); };
@@ -262,7 +97,8 @@ bool sortByGroup(const Tensor& index, GroupPlan& plan, int* order, unsigned* key
         const unsigned lds = digits * 4 + digits * 2 * (GROUP_THREADS / 64);
         tokenKernel("row_groups.h", kernelKey(GROUP_SCATTER, type, plan.items), [&] { return "GroupScatterKernel" + arguments(); })
             .call(tiles, GROUP_THREADS, lds, stream, source, rows, shift, digitBits, digits, static_cast<const unsigned*>(plan.counts),
-                  few ? nullptr : static_cast<const unsigned*>(plan.totals), to, toKeys, plan.passes == 1 ? offsets : nullptr);
+                  few ? nullptr : static_cast<const unsigned*>(plan.totals), to, toKeys, plan.passes == 1 ? offsets : nullptr,
+                  last ? places : nullptr);
         source.keys = toKeys;
         source.order = to;
     }
@@ -281,14 +117,6 @@ struct EmbeddingBlocks
     int sizes;
     const float* sums[SIZES];
 };
-
-/** Lanes per row of C entries. */
-int lanesPerRow(int C, int vec)
-{
-    int lanes = 8;
-    while (lanes < EMBEDDING_THREADS && lanes * vec < C) lanes *= 2;
-    return lanes;
-}
 
 /** Four rows at a time where that leaves four workgroups for every compute unit. */
 int embeddingRowsAtOnce(int64_t rows, int lanes) { return rows >= 4 * 4 * 256 * (EMBEDDING_THREADS / lanes) ? 4 : 1; }
@@ -547,9 +375,17 @@ size_t Tokens::groupMemory(int64_t rows, int groups)
 
 void Tokens::group(const Tensor& index, int groups, Tensor& order, Tensor& offsets, void* memory, stream_t stream)
 {
+    Tensor places;
+    group(index, groups, order, offsets, places, memory, stream);
+}
+
+void Tokens::group(const Tensor& index, int groups, Tensor& order, Tensor& offsets, Tensor& places, void* memory, stream_t stream)
+{
     checkIndex(index, "index");
     CHECK_ERROR(groups >= 0, "the number of groups must not be negative");
-    for (const auto& [t, what, size] : {std::tuple<const Tensor&, const char*, int64_t>{order, "order", index.size(0)}, {offsets, "offsets", groups + 1ll}}) {
+    for (const auto& [t, what, size] : {std::tuple<const Tensor&, const char*, int64_t>{order, "order", index.size(0)}, {offsets, "offsets", groups + 1ll},
+                                        {places, "places", index.size(0)}}) {
+        if (&t == &places && !t.defined()) continue;
         CHECK_ERROR(t.defined() && t.ndim() == 1, what, " must be a tensor with 1 dimension");
         checkType(t, what, Tensor::INT32);
         checkSizes(t, what, {size});
@@ -558,7 +394,7 @@ void Tokens::group(const Tensor& index, int groups, Tensor& order, Tensor& offse
     checkMemory(memory, groupMemory(index.size(0), groups));
     Workspace workspace{static_cast<char*>(memory)};
     GroupPlan plan(index.size(0), static_cast<unsigned>(groups), false, workspace);
-    sortByGroup(index, plan, ptr<int>(order), nullptr, ptr<int>(offsets), nullptr, stream);
+    sortByGroup(index, plan, ptr<int>(order), nullptr, ptr<int>(offsets), nullptr, ptr<int>(places), stream);
 }
 
 void Tokens::embedding(const Tensor& index, const Tensor& table, float scale, Tensor& output, stream_t stream)
@@ -608,7 +444,7 @@ void Tokens::embeddingAdjoint(const Tensor& index, const Tensor& adjOutput, floa
     EmbeddingPlan plan(rows, vocabulary, C, memory);
     const void* dy = ptr<void>(adjOutput);
     if (rows > 0) {
-        const bool marked = sortByGroup(index, plan.sort, plan.order, plan.keys, nullptr, plan.spans, stream);
+        const bool marked = sortByGroup(index, plan.sort, plan.order, plan.keys, nullptr, plan.spans, nullptr, stream);
         for (int s = 0; s < plan.blocks.sizes; ++s) {
             // (the first kernel looks at every place for the spans)
             const int64_t blocks = s == 0 && !marked ? divUp<int64_t>(rows, 1 << EMBEDDING_BLOCK_BITS) : rows >> (EMBEDDING_BLOCK_BITS * (s + 1));
@@ -881,6 +717,7 @@ void Tokens::precompile(Tensor::Precision p)
             if (!few && (direct || !huge)) precompileKernel("grouped_linear.h", str("GroupedWeightsKernel<", types, ", ", tiles.arguments(), ">"));
         }
     for (const char* kernel : {"GroupedSumKernel", "GroupedJoinKernel"}) precompileKernel("grouped_linear.h", str(kernel, "<", t, ">"));
+    precompileExperts(p);
 }
 
 QUICKMLP_NAMESPACE_END

@@ -87,6 +87,7 @@ qmlp_tensor wrap(const at::Tensor& t, bool token = false)
             if (token && t.scalar_type() == at::kBFloat16) d.precision = QMLP_BFLOAT16;
             else if (token && t.scalar_type() == at::kInt) d.precision = QMLP_INT32;
             else if (token && t.scalar_type() == at::kLong) d.precision = QMLP_INT64;
+            else if (token && t.scalar_type() == at::kByte) d.precision = QMLP_UINT8;
             else throw py::type_error("unsupported dtype " + std::string(c10::toString(t.scalar_type())));
     }
     d.data = t.data_ptr();
@@ -619,7 +620,7 @@ void refuseRecording()
     if (at::tracer::impl::is_dispatch_enabled()) throw std::runtime_error("operators on tokens cannot be recorded by torch.jit.trace");
 }
 
-py::tuple group(const at::Tensor& index, int64_t groups)
+py::tuple group(const at::Tensor& index, int64_t groups, bool withPlaces)
 {
     refuseRecording();
     checkDevices({&index});
@@ -628,12 +629,14 @@ py::tuple group(const at::Tensor& index, int64_t groups)
         const at::Tensor flat = index.reshape({-1});
         const auto options = flat.options().dtype(at::kInt);
         const at::Tensor order = at::empty({flat.size(0)}, options), offsets = at::empty({groups + 1}, options);
+        const at::Tensor places = withPlaces ? at::empty({flat.size(0)}, options) : at::Tensor();
         size_t bytes = 0;
         check(qmlp_tokens_group_memory(flat.size(0), static_cast<int>(groups), &bytes));
         const at::Tensor memory = temporary(flat, bytes);
-        const qmlp_tensor in = wrapToken(flat), ord = wrapToken(order), off = wrapToken(offsets);
-        check(qmlp_tokens_group(&in, static_cast<int>(groups), &ord, &off, dataOf(memory), currentStream(flat)));
-        return py::make_tuple(order, offsets);
+        const qmlp_tensor in = wrapToken(flat), ord = wrapToken(order), off = wrapToken(offsets), at = wrapToken(places);
+        check(qmlp_tokens_group_places(&in, static_cast<int>(groups), &ord, &off, &at, dataOf(memory), currentStream(flat)));
+        if (!withPlaces) return py::make_tuple(order, offsets);
+        return py::make_tuple(order, offsets, places.view(index.sizes()));
     });
 }
 
@@ -788,6 +791,205 @@ at::Tensor groupedLinear(const at::Tensor& x, const at::Tensor& weight, const at
     return output;
 }
 
+// ------------------------------------------------------------------------------------------------ around the experts
+/** (..., columns) as rows of the last dimension, whose entries lie side by side. */
+at::Tensor asRows(const at::Tensor& t)
+{
+    const int64_t columns = t.size(-1);
+    return consecutive(t.dim() == 2 ? t : t.reshape({columns > 0 ? t.numel() / columns : c10::multiply_integers(t.sizes().slice(0, t.dim() - 1)), columns}));
+}
+/** The shape of t with another last dimension. */
+std::vector<int64_t> withLast(const at::Tensor& t, int64_t last)
+{
+    auto sizes = t.sizes().vec();
+    sizes.back() = last;
+    return sizes;
+}
+/** Rows as a result of the given shape. */
+at::Tensor shaped(const at::Tensor& rows, at::IntArrayRef sizes) { return rows.sizes() == sizes ? rows : rows.view(sizes); }
+
+struct RouteBackward : TokenNode
+{
+    bool normalised = false;
+    std::string name() const override { return "QmlpRouteBackward"; }
+    void adjoint(const at::Tensor& gradOutput, const variable_list& tensors, variable_list& grads) override
+    {
+        const at::Tensor logits = asRows(tensors[0]), index = asRows(tensors[1]), adjWeights = asRows(gradOutput);
+        const at::Tensor adjLogits = emptyLike(logits);
+        const qmlp_tensor in = wrapToken(logits), i = wrapToken(index), dw = wrapToken(adjWeights), dl = wrapToken(adjLogits);
+        check(qmlp_tokens_route_adjoint(&in, &i, &dw, normalised, &dl, currentStream(logits)));
+        grads[0] = shaped(adjLogits, tensors[0].sizes());
+    }
+};
+
+py::tuple route(const at::Tensor& logits, int64_t chosen, bool normalised)
+{
+    refuseRecording();
+    checkDevices({&logits});
+    refuseOtherModes({logits});
+    if (logits.dim() < 1) throw std::runtime_error("logits must have a dimension of experts");
+    if (chosen < 1 || chosen > logits.size(-1) || chosen > 64)
+        throw py::value_error("between 1 and 64 experts can be chosen, and no more than there are");
+    at::Tensor index;
+    const at::Tensor weights = guarded(logits, [&] {
+        const at::Tensor rows = asRows(logits);
+        const at::Tensor w = at::empty({rows.size(0), chosen}, logits.options().requires_grad(false)), i = at::empty({rows.size(0), chosen}, w.options().dtype(at::kInt));
+        const qmlp_tensor in = wrapToken(rows), wt = wrapToken(w), it = wrapToken(i);
+        check(qmlp_tokens_route(&in, normalised, &wt, &it, currentStream(logits)));
+        const auto sizes = withLast(logits, chosen);
+        index = shaped(i, sizes);
+        return shaped(w, sizes);
+    });
+    if (wantsGradient(logits)) attach<RouteBackward>(weights, {logits}, {logits, index})->normalised = normalised;
+    return py::make_tuple(weights, index);
+}
+
+struct DispatchBackward : TokenNode
+{
+    std::vector<int64_t> sizes;   // of the tokens' rows
+    std::string name() const override { return "QmlpDispatchBackward"; }
+    void adjoint(const at::Tensor& gradOutput, const variable_list& tensors, variable_list& grads) override
+    {
+        const at::Tensor places = asRows(tensors[0]), adjRows = consecutive(gradOutput);
+        const at::Tensor adjX = at::empty({places.size(0), adjRows.size(1)}, adjRows.options());
+        const qmlp_tensor none{}, dr = wrapToken(adjRows), p = wrapToken(places), dx = wrapToken(adjX);
+        check(qmlp_tokens_combine(&dr, &p, &none, &none, &dx, currentStream(adjRows)));
+        grads[0] = shaped(adjX, sizes);
+    }
+};
+
+at::Tensor dispatchRows(const at::Tensor& x, const at::Tensor& places)
+{
+    refuseRecording();
+    checkDevices({&x, &places});
+    refuseOtherModes({x, places});
+    if (x.dim() < 1 || places.dim() != x.dim()) throw std::runtime_error("places must have the dimensions of the tokens' rows, with those of a token's experts in the last one");
+    if (places.size(-1) < 1) throw std::runtime_error("a token must have at least one expert");
+    if (x.sizes().slice(0, x.dim() - 1) != places.sizes().slice(0, places.dim() - 1)) throw std::runtime_error("places must be those of the tokens");
+    const at::Tensor output = guarded(x, [&] {
+        const at::Tensor rows = asRows(x), p = asRows(places);
+        const at::Tensor out = at::empty({places.numel(), x.size(-1)}, x.options().requires_grad(false));
+        const qmlp_tensor in = wrapToken(rows), pt = wrapToken(p), o = wrapToken(out);
+        check(qmlp_tokens_dispatch(&in, &pt, &o, currentStream(x)));
+        return out;
+    });
+    if (wantsGradient(x)) attach<DispatchBackward>(output, {x}, {places})->sizes = x.sizes().vec();
+    return output;
+}
+
+struct CombineBackward : TokenNode
+{
+    std::string name() const override { return "QmlpCombineBackward"; }
+    void adjoint(const at::Tensor& gradOutput, const variable_list& tensors, variable_list& grads) override
+    {
+        const at::Tensor rows = consecutive(tensors[0]), places = asRows(tensors[1]), adjOutput = asRows(gradOutput);
+        const at::Tensor weights = tensors[2].defined() ? asRows(tensors[2]) : at::Tensor();
+        at::Tensor adjRows, adjWeights;
+        if (task_should_compute_output(0)) adjRows = at::empty(rows.sizes(), rows.options().requires_grad(false));
+        if (task_should_compute_output(1)) adjWeights = at::empty(weights.sizes(), weights.options().requires_grad(false));
+        const qmlp_tensor in = wrapToken(rows), p = wrapToken(places), w = wrapToken(weights), dy = wrapToken(adjOutput), dr = wrapToken(adjRows),
+                          dw = wrapToken(adjWeights);
+        check(qmlp_tokens_combine_adjoint(&in, &p, &w, &dy, &dr, &dw, currentStream(rows)));
+        grads[0] = adjRows;
+        if (adjWeights.defined()) grads[1] = shaped(adjWeights, tensors[2].sizes());
+        if (task_should_compute_output(2)) grads[2] = gradOutput;
+    }
+};
+
+at::Tensor combine(const at::Tensor& rows, const at::Tensor& places, const at::Tensor& weights, const at::Tensor& residual)
+{
+    refuseRecording();
+    checkDevices({&rows, &places, &weights, &residual});
+    refuseOtherModes({rows, places, weights, residual});
+    if (rows.dim() != 2) throw std::runtime_error("rows must be a tensor with 2 dimensions (tokens * chosen, channels)");
+    if (places.dim() < 1 || places.size(-1) < 1) throw std::runtime_error("a token must have at least one expert");
+    if (weights.defined() && weights.sizes() != places.sizes()) throw std::runtime_error("weights must be of the shape of places");
+    const auto sizes = withLast(places, rows.size(1));
+    if (residual.defined() && residual.sizes() != at::IntArrayRef(sizes)) throw std::runtime_error("residual must have a row of the same channels for every token");
+    const at::Tensor output = guarded(rows, [&] {
+        const at::Tensor r = consecutive(rows), p = asRows(places), w = weights.defined() ? asRows(weights) : at::Tensor(),
+                         x = residual.defined() ? asRows(residual) : at::Tensor();
+        const at::Tensor out = at::empty({p.size(0), rows.size(1)}, rows.options().requires_grad(false));
+        const qmlp_tensor in = wrapToken(r), pt = wrapToken(p), wt = wrapToken(w), xt = wrapToken(x), o = wrapToken(out);
+        check(qmlp_tokens_combine(&in, &pt, &wt, &xt, &o, currentStream(rows)));
+        return shaped(out, sizes);
+    });
+    if (wantsGradient(rows) || wantsGradient(weights) || wantsGradient(residual)) attach<CombineBackward>(output, {rows, weights, residual}, {rows, places, weights});
+    return output;
+}
+
+at::ScalarType dtypeOf(const py::object& dtype)
+{
+    if (!THPDtype_Check(dtype.ptr())) throw py::type_error("a dtype is wanted");
+    return reinterpret_cast<THPDtype*>(dtype.ptr())->scalar_type;
+}
+
+/** Operators whose results know no gradient refuse inputs that want one. */
+void refuseGradients(std::initializer_list<const at::Tensor*> tensors)
+{
+    for (const at::Tensor* t : tensors)
+        if (wantsGradient(*t)) throw std::runtime_error("numbers of 4 bits have no gradient: detach what they are made of, or call within torch.no_grad()");
+}
+
+py::tuple mx4Quantise(const at::Tensor& x)
+{
+    refuseRecording();
+    checkDevices({&x});
+    refuseOtherModes({x});
+    refuseGradients({&x});
+    if (x.dim() < 1) throw std::runtime_error("input must have a dimension of columns");
+    return guarded(x, [&] {
+        const at::Tensor rows = asRows(x);
+        const int64_t blocks = (x.size(-1) + 31) / 32;
+        const auto options = x.options().dtype(at::kByte).requires_grad(false);
+        const at::Tensor codes = at::empty({rows.size(0), 16 * blocks}, options), scales = at::empty({rows.size(0), blocks}, options);
+        const qmlp_tensor in = wrapToken(rows), c = wrapToken(codes), s = wrapToken(scales);
+        check(qmlp_tokens_mx4_quantise(&in, &c, &s, currentStream(x)));
+        return py::make_tuple(shaped(codes, withLast(x, 16 * blocks)), shaped(scales, withLast(x, blocks)));
+    });
+}
+
+at::Tensor mx4Values(const at::Tensor& codes, const at::Tensor& scales, int64_t columns, const py::object& dtype)
+{
+    refuseRecording();
+    checkDevices({&codes, &scales});
+    if (codes.dim() < 1 || codes.dim() != scales.dim()) throw std::runtime_error("codes and scales must have the same dimensions");
+    if (codes.sizes().slice(0, codes.dim() - 1) != scales.sizes().slice(0, scales.dim() - 1)) throw std::runtime_error("codes and scales must be of the same rows");
+    if (columns < 0) throw py::value_error("columns must not be negative");
+    const at::ScalarType type = dtypeOf(dtype);
+    return guarded(codes, [&] {
+        const at::Tensor c = asRows(codes), s = asRows(scales), out = at::empty({c.size(0), columns}, codes.options().dtype(type));
+        const qmlp_tensor ct = wrapToken(c), st = wrapToken(s), o = wrapToken(out);
+        check(qmlp_tokens_mx4_values(&ct, &st, &o, currentStream(codes)));
+        return shaped(out, withLast(codes, columns));
+    });
+}
+
+/** \param inputScales undefined: input holds values \param dtype of the result, where input holds codes */
+at::Tensor mx4Linear(const at::Tensor& input, const at::Tensor& inputScales, const at::Tensor& weight, const at::Tensor& scales, const at::Tensor& offsets,
+                     const at::Tensor& bias, const py::object& dtype)
+{
+    refuseRecording();
+    checkDevices({&input, &inputScales, &weight, &scales, &offsets, &bias});
+    refuseOtherModes({input, bias});
+    refuseGradients({&input, &bias});
+    if (input.dim() != 2) throw std::runtime_error("input must be a tensor with 2 dimensions (rows, inputs)");
+    if (weight.dim() != 3 || scales.dim() != 3) throw std::runtime_error("weight must have 3 dimensions (experts, outputs, inputs)");
+    const at::ScalarType type = inputScales.defined() ? dtypeOf(dtype) : input.scalar_type();
+    return guarded(input, [&] {
+        const at::Tensor rows = consecutive(input), rowScales = consecutive(inputScales), w = consecutive(weight), s = consecutive(scales), b = consecutive(bias),
+                         off = consecutive(offsets);
+        const at::Tensor out = at::empty({input.size(0), weight.size(1)}, input.options().dtype(type).requires_grad(false));
+        size_t bytes = 0;
+        const qmlp_tensor in = wrapToken(rows), is = wrapToken(rowScales), wt = wrapToken(w), st = wrapToken(s), of = wrapToken(off), bt = wrapToken(b),
+                          o = wrapToken(out);
+        if (!inputScales.defined()) check(qmlp_tokens_mx4_linear_memory(in.sizes[0], in.sizes[1], &bytes));
+        const at::Tensor memory = temporary(rows, bytes);
+        check(qmlp_tokens_mx4_linear(&in, &is, &wt, &st, &of, &bt, &o, dataOf(memory), currentStream(input)));
+        return out;
+    });
+}
+
 at::Tensor tensorOrNone(const py::object& o) { return o.is_none() ? at::Tensor() : o.cast<at::Tensor>(); }
 py::object noneOr(const at::Tensor& t) { return t.defined() ? py::cast(t) : py::none(); }
 
@@ -873,6 +1075,17 @@ PYBIND11_MODULE(_native, m)
              },
              "Gradients (input, parameter), the latter in floats; None where flags do not ask for them.");
     m.def("group", group);
+    m.def("route", route);
+    m.def("dispatch", dispatchRows);
+    m.def("combine", [](const at::Tensor& rows, const at::Tensor& places, const py::object& weights, const py::object& residual) {
+        return combine(rows, places, tensorOrNone(weights), tensorOrNone(residual));
+    });
+    m.def("mx4_quantise", mx4Quantise);
+    m.def("mx4_values", mx4Values);
+    m.def("mx4_linear", [](const at::Tensor& input, const py::object& inputScales, const at::Tensor& weight, const at::Tensor& scales, const py::object& offsets,
+                           const py::object& bias, const py::object& dtype) {
+        return mx4Linear(input, tensorOrNone(inputScales), weight, scales, tensorOrNone(offsets), tensorOrNone(bias), dtype);
+    });
     m.def("embedding", embedding);
     m.def("layer_norm", [](const at::Tensor& x, const py::object& weight, const py::object& bias, double epsilon) {
         return layerNorm(x, tensorOrNone(weight), tensorOrNone(bias), epsilon);

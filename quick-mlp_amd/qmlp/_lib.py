@@ -12,7 +12,7 @@ LIB_PATH = os.path.join(_HERE, "libqmlp.so")
 DEFAULT_CACHE_DIR = os.path.join(os.path.dirname(_HERE), ".kernel_cache")
 
 QMLP_FLOAT, QMLP_HALF, QMLP_DOUBLE = 0, 1, 2
-QMLP_BFLOAT16, QMLP_INT32, QMLP_INT64 = 3, 4, 5   # of the operators on rows of tokens alone
+QMLP_BFLOAT16, QMLP_INT32, QMLP_INT64, QMLP_UINT8 = 3, 4, 5, 6   # of the operators on rows of tokens alone
 QMLP_INFERENCE, QMLP_GRADIENTS = 0, 1
 GRADIENTS_INPUT, GRADIENTS_NETWORK_WEIGHTS, GRADIENTS_INPUT_ENCODINGS = 1, 2, 4
 
@@ -133,6 +133,16 @@ _SIGNATURES = {
     "qmlp_tokens_grouped_linear": [_TD, _TD, _TD, _TD, _TD, _vp, _vp],
     "qmlp_tokens_grouped_linear_adjoint_memory": [ctypes.c_longlong, _ci, _ci, _ci, _P(ctypes.c_size_t)],
     "qmlp_tokens_grouped_linear_adjoint": [_TD, _TD, _TD, _TD, _TD, _TD, _TD, _vp, _vp],
+    "qmlp_tokens_group_places": [_TD, _ci, _TD, _TD, _TD, _vp, _vp],
+    "qmlp_tokens_route": [_TD, _ci, _TD, _TD, _vp],
+    "qmlp_tokens_route_adjoint": [_TD, _TD, _TD, _ci, _TD, _vp],
+    "qmlp_tokens_dispatch": [_TD, _TD, _TD, _vp],
+    "qmlp_tokens_combine": [_TD, _TD, _TD, _TD, _TD, _vp],
+    "qmlp_tokens_combine_adjoint": [_TD, _TD, _TD, _TD, _TD, _TD, _vp],
+    "qmlp_tokens_mx4_quantise": [_TD, _TD, _TD, _vp],
+    "qmlp_tokens_mx4_values": [_TD, _TD, _TD, _vp],
+    "qmlp_tokens_mx4_linear_memory": [ctypes.c_longlong, _ci, _P(ctypes.c_size_t)],
+    "qmlp_tokens_mx4_linear": [_TD, _TD, _TD, _TD, _TD, _TD, _TD, _vp, _vp],
     "qmlp_tokens_precompile": [_ci],
 }
 for _name, _args in _SIGNATURES.items():

@@ -1,8 +1,8 @@
 """Operators on rows of tokens: what a model of tokens with experts needs beside networks and encodings.
 
 All of them work on GPU tensors of type float32, float16 or bfloat16, run on torch's current stream, hold their sums in
-32 bits and round once. They are differentiable (once, in reverse mode) in every floating-point argument; the same inputs give
-the same bits. They have no counterpart in the reference.
+32 bits and round once. They are differentiable (once, in reverse mode) in every floating-point argument, those on numbers of 4 bits
+(:class:`Mx4`) excepted; the same inputs give the same bits. They have no counterpart in the reference.
 """
 import math
 
@@ -14,16 +14,18 @@ from ._lib import check, lib
 _PRECISION_OF = {torch.float32: _lib.QMLP_FLOAT, torch.float16: _lib.QMLP_HALF, torch.bfloat16: _lib.QMLP_BFLOAT16}
 
 
-def group(index: torch.Tensor, groups: int):
+def group(index: torch.Tensor, groups: int, places: bool = False):
     """
     Rows in the order of the group that they belong to, in their own order within a group.
 
     :param index: (rows) int32 or int64, the group of a row; rows whose index is not in 0 .. groups - 1 belong to none
     :param groups: number of groups
+    :param places: whether the place of every row in the order is returned, too
     :return: ``(order, offsets)``, both int32: ``order[offsets[g]:offsets[g + 1]]`` are the rows of group g;
-        ``order[offsets[groups]:]`` those of no group
+        ``order[offsets[groups]:]`` those of no group. With places ``(order, offsets, places)``: places, int32 of the shape of index,
+        for :func:`dispatch` and :func:`combine`; -1 - place for the rows of no group
     """
-    return _native.group(index, groups)
+    return _native.group(index, groups, places)
 
 
 def embedding(index: torch.Tensor, table: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
@@ -59,6 +61,107 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
     :return: (rows, outputs)
     """
     return _native.grouped_linear(x, weight, offsets, bias)
+
+
+def route(logits: torch.Tensor, chosen: int, normalised: bool = False):
+    """
+    The router's choice: for every row of logits the experts with the largest ones, the first of equals, in that order, and their shares of the
+    softmax. Differentiable in the logits.
+
+    No row takes an expert whose logit is -inf: where a row has fewer others than are chosen, -1 and a weight of 0 stand for the rest. A NaN counts
+    as the largest logit; weights of a row with a NaN or +inf are NaN.
+
+    :param logits: (..., experts)
+    :param chosen: experts of a row, 1 to 64
+    :param normalised: softmax over the chosen experts alone, so that the weights of a row add up to 1
+    :return: ``(weights, index)``, both (..., chosen): weights of the logits' type, index int32, for :func:`group`
+    """
+    return _native.route(logits, chosen, normalised)
+
+
+def dispatch(x: torch.Tensor, places: torch.Tensor) -> torch.Tensor:
+    """
+    Rows of tokens to their experts: ``rows[places[..., j]] = x[...]``, zeros at places of no expert. Differentiable in x.
+
+    :param x: (..., channels)
+    :param places: (..., chosen) int32, as :func:`group` returns them for the chosen experts: those of a permutation (what any others than that
+        leave in the rows is undefined, though nothing beside them is written)
+    :return: (tokens * chosen, channels), rows by expert, for :func:`grouped_linear` and :func:`mx4_linear`
+    """
+    return _native.dispatch(x, places)
+
+
+def combine(rows: torch.Tensor, places: torch.Tensor, weights: torch.Tensor = None, residual: torch.Tensor = None) -> torch.Tensor:
+    """
+    And back: ``residual[...] + sum over j of weights[..., j] * rows[places[..., j]]``, without the terms of no expert. Differentiable in rows,
+    weights and residual.
+
+    :param rows: (tokens * chosen, channels)
+    :param places: (..., chosen) as for :func:`dispatch`
+    :param weights: (..., chosen), of the type of the rows or float32; None: 1
+    :param residual: (..., channels), of the type of the rows; None: 0
+    :return: (..., channels)
+    """
+    return _native.combine(rows, places, weights, residual)
+
+
+class Mx4:
+    """
+    A tensor of 4-bit numbers, blocks of 32 consecutive entries of its last dimension with a common power of two: MXFP4 as the OCP Microscaling
+    Formats specification 1.0 has it.
+
+    :param codes: (..., 16 * blocks) uint8, two numbers a byte, the first in the low bits: sign, two bits of exponent, one of mantissa. Zeros
+        behind the last column
+    :param scales: (..., blocks) uint8, the exponents of the blocks plus 127; 255: a block of NaN
+    :param columns: entries of the last dimension, in ceil(columns / 32) blocks
+    """
+    __slots__ = ("codes", "scales", "columns")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, columns: int):
+        if scales.shape[-1] != (columns + 31) // 32 or codes.shape[-1] != 16 * scales.shape[-1]:
+            raise ValueError("%d columns are %d blocks of 16 bytes of codes and a scale, but there are %d bytes and %d scales"
+                             % (columns, (columns + 31) // 32, codes.shape[-1], scales.shape[-1]))
+        self.codes, self.scales, self.columns = codes, scales, columns
+
+    @property
+    def shape(self):
+        return torch.Size((*self.scales.shape[:-1], self.columns))
+
+    def dequantise(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """The values that the numbers stand for, rounded once to the type (float32 and bfloat16 hold all of them)."""
+        return _native.mx4_values(self.codes, self.scales, self.columns, dtype)
+
+    def __repr__(self):
+        return "Mx4(%s)" % (tuple(self.shape),)
+
+
+def quantise_mx4(x: torch.Tensor) -> Mx4:
+    """
+    x in numbers of 4 bits. The scale of a block is the power of two that brings its largest magnitude to 4 .. 8; its entries go to the nearest of 0,
+    0.5, 1, 1.5, 2, 3, 4, 6 times the scale, halfway to the even code. A block with an infinity or a NaN becomes NaN. No gradient: inputs that want
+    one are refused.
+
+    :param x: (..., columns)
+    """
+    return Mx4(*_native.mx4_quantise(x), x.shape[-1])
+
+
+def mx4_linear(x, weight: Mx4, offsets: torch.Tensor = None, bias: torch.Tensor = None, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """
+    :func:`grouped_linear` with weights of 4 bits, for serving: both operands of the product are numbers of 4 bits, sums are held in 32. No gradient:
+    inputs that want one are refused.
+
+    :param x: (rows, inputs), which the call quantises as :func:`quantise_mx4` does, or :class:`Mx4`
+    :param weight: (experts, outputs, inputs), quantised along the inputs
+    :param offsets: as for :func:`grouped_linear`; None: one expert has all rows
+    :param bias: (experts, outputs) of the type of the result, or None
+    :param dtype: of the result, where x is :class:`Mx4`; otherwise it has the type of x
+    :return: (rows, outputs)
+    """
+    values, scales, inputs = (x.codes, x.scales, x.columns) if isinstance(x, Mx4) else (x, None, x.shape[-1])
+    if inputs != weight.columns:
+        raise ValueError("x has rows of %d, the weights of %d inputs" % (inputs, weight.columns))
+    return _native.mx4_linear(values, scales, weight.codes, weight.scales, offsets, bias, dtype)
 
 
 def precompile(dtype: torch.dtype = torch.float32) -> None:
@@ -114,3 +217,24 @@ class FusedGroupedLinear(torch.nn.Module):
     def extra_repr(self):
         experts, outputs, inputs = self.weight.shape
         return "%d experts, %d -> %d, bias=%s" % (experts, inputs, outputs, self.bias is not None)
+
+
+class FusedMx4GroupedLinear(torch.nn.Module):
+    """The layers of a :class:`FusedGroupedLinear` with weights of 4 bits, for serving: :func:`mx4_linear` with them. Made once from the trained
+    layer; codes and scales are buffers."""
+
+    def __init__(self, layer: FusedGroupedLinear):
+        super().__init__()
+        weight = quantise_mx4(layer.weight.detach())
+        self.inputs = weight.columns
+        self.register_buffer("codes", weight.codes)
+        self.register_buffer("scales", weight.scales)
+        self.register_buffer("bias", layer.bias.detach().clone() if layer.bias is not None else None)
+
+    def forward(self, x: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
+        bias = self.bias.to(x.dtype) if self.bias is not None else None
+        return mx4_linear(x, Mx4(self.codes, self.scales, self.inputs), offsets, bias)
+
+    def extra_repr(self):
+        experts, outputs = self.scales.shape[:2]
+        return "%d experts, %d -> %d, bias=%s" % (experts, self.inputs, outputs, self.bias is not None)
