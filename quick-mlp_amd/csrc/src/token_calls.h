@@ -36,7 +36,7 @@ inline int wide(Tensor::Precision p) { return 16 / Tensor::BytesPerEntry[p]; }
 
 enum KernelId { GROUP_SMALL = 1, GROUP_COUNT, GROUP_SCAN, GROUP_SCATTER, GROUP_OFFSETS, EMBEDDING, EMBEDDING_BLOCKS, EMBEDDING_ADJOINT, LAYER_NORM,
                 LAYER_NORM_ADJOINT, LAYER_NORM_SUM, LAYER_NORM_LONG, LAYER_NORM_LONG_ADJOINT, LAYER_NORM_LONG_SUMS, GROUPED_ROWS, GROUPED_WEIGHTS,
-                GROUPED_SUM, GROUPED_JOIN, ROUTE, ROUTE_ADJOINT, ROUTE_LONG, ROUTE_LONG_ADJOINT, DISPATCH, COMBINE, COMBINE_ADJOINT, MX4_QUANTISE, MX4_VALUES, MX4_FEW,
+                GROUPED_SUM, GROUPED_JOIN, ROUTE, ROUTE_ADJOINT, ROUTE_LONG, ROUTE_LONG_ADJOINT, DISPATCH, COMBINE, COMBINE_ADJOINT, MX4_QUANTISE, MX4_VALUES, MX4_FEW, MX4_TILES_OF,
                 KERNEL_IDS };
 /**
  * One number for a kernel and its template arguments, each below 2^11: to build its name takes as long as to launch it. No id is 0, so that

@@ -118,6 +118,26 @@ int checkMx4(const Tensor& codes, const char* whatCodes, const Tensor& scales, c
                 codes.size(dims - 1));
     return blocks;
 }
+struct Mx4Tiles
+{
+    int i, j, wavesI, wavesJ;
+    int threads() const { return 64 * wavesI * wavesJ; }
+    /** Two tiles of each operand and two pairs of tiles' scales, later the results. */
+    unsigned lds(int entry) const { return static_cast<unsigned>(std::max((2 * 128 + 2 * 16) * (i + j), i * j * entry)); }
+    std::string arguments() const { return str(i, ", ", j, ", ", wavesI, ", ", wavesJ); }
+};
+constexpr Mx4Tiles MX4_HUGE = {256, 256, 2, 4}, MX4_LARGE = {128, 128, 2, 2}, MX4_SMALL = {64, 64, 2, 2}, MX4_FEWEST = {16, 64, 1, 4};
+constexpr Mx4Tiles MX4_TILES[] = {MX4_HUGE, MX4_LARGE, MX4_SMALL};
+
+Mx4Tiles mx4Tiles(Tensor::Precision p, int64_t rows, int64_t experts, int64_t J, bool direct)
+{
+    const int64_t each = rows / std::max<int64_t>(experts, 1);
+    if (each <= 32 || !direct) return MX4_FEWEST;
+    auto count = [&](const Mx4Tiles& t) { return (rows / t.i + experts) * divUp<int64_t>(J, t.j); };
+    if (p != Tensor::FLOAT && each > 128 && J > 128 && count(MX4_HUGE) >= 256) return MX4_HUGE;
+    return each > 64 && J > 64 && count(MX4_LARGE) >= 256 ? MX4_LARGE : MX4_SMALL;
+}
+
 int mx4Blocks(int64_t columns) { return static_cast<int>(divUp<int64_t>(columns, MX4_BLOCK)); }
 unsigned mx4Workgroups(long long units) { return workgroups(divUp<int64_t>(units * MX4_LANES, MX4_THREADS), 1 << 16); }
 
@@ -308,8 +328,17 @@ void Tokens::mx4Linear(const Tensor& input, const Tensor& inputScales, const Ten
     checkSteps("outputs", outputs);
     if (rows == 0) return;
     const Tensor::Precision p = output.precision();
-    const int64_t places = static_cast<int64_t>(rows) / 16 + experts + 1, tilesJ = divUp<int64_t>(outputs, 16 * MX4_FEW_WAVES);
-    checkLaunch(places * tilesJ, 64 * MX4_FEW_WAVES);
+    // pieces of 16 bytes, rows that do not overlap and whose tiles have 32-bit offsets: straight to LDS
+    const auto direct = [](const Tensor& t) {
+        const int n = t.ndim();
+        for (int d = 0; d + 1 < n; ++d)
+            if (t.size(d) > 1 && t.stride(d) % 16 != 0) return false;
+        return reinterpret_cast<uintptr_t>(t.rawPtr()) % 16 == 0 && (t.size(n - 2) <= 1 || (t.stride(n - 2) >= t.size(n - 1) && t.stride(n - 2) < 1 << 22));
+    };
+    const bool isDirect = direct(weight) && (!quantised || direct(input)) && blocks < 1 << 17;
+    const Mx4Tiles tiles = mx4Tiles(p, rows, experts, outputs, isDirect);
+    const int64_t places = static_cast<int64_t>(rows) / tiles.i + experts + 1, tilesJ = divUp<int64_t>(outputs, tiles.j);
+    checkLaunch(places * tilesJ, tiles.threads());
     Mx4Rows x(rows, blocks, memory);
     long long strideX = blocks * 16ll, strideScalesX = blocks;
     if (quantised) {
@@ -322,11 +351,13 @@ void Tokens::mx4Linear(const Tensor& input, const Tensor& inputScales, const Ten
         launchQuantise(input, x.codes, strideX, x.scales, strideScalesX, stream);
     }
     const Mx4Matrix w{ptr<unsigned char>(weight), ptr<unsigned char>(scales), strideOf(weight, 0), strideOf(scales, 0), strideOf(weight, 1), strideOf(scales, 1)};
-    tokenKernel("mx4_linear.h", kernelKey(MX4_FEW, p), [&] { return str("Mx4FewKernel<", scalarName(p), ">"); })
-        .call(static_cast<unsigned>(places * tilesJ), 64 * MX4_FEW_WAVES, 0, stream, static_cast<const unsigned char*>(x.codes),
-              static_cast<const unsigned char*>(x.scales), strideX, strideScalesX, w, static_cast<const void*>(ptr<void>(bias)), strideOrNone(bias),
-              static_cast<const int*>(ptr<int>(offsets)), experts, output.rawPtr(), strideOf(output, 0), rows, outputs, blocks, static_cast<int>(places),
-              static_cast<int>(tilesJ));
+    const bool few = tiles.i == MX4_FEWEST.i;
+    tokenKernel("mx4_linear.h", few ? kernelKey(MX4_FEW, p) : kernelKey(MX4_TILES_OF, p, tiles.i, tiles.j, tiles.wavesI, tiles.wavesJ),
+                [&] { return few ? str("Mx4FewKernel<", scalarName(p), ">") : str("Mx4TilesKernel<", scalarName(p), ", ", tiles.arguments(), ">"); })
+        .call(static_cast<unsigned>(places * tilesJ), tiles.threads(), few ? 0 : tiles.lds(output.bytesPerEntry()), stream,
+              static_cast<const unsigned char*>(x.codes), static_cast<const unsigned char*>(x.scales), strideX, strideScalesX, w,
+              static_cast<const void*>(ptr<void>(bias)), strideOrNone(bias), static_cast<const int*>(ptr<int>(offsets)), experts, output.rawPtr(),
+              strideOf(output, 0), rows, outputs, blocks, static_cast<int>(places), static_cast<int>(tilesJ));
 }
 
 void token::precompileExperts(Tensor::Precision p)
@@ -345,6 +376,8 @@ void token::precompileExperts(Tensor::Precision p)
         }
     for (const char* kernel : {"Mx4QuantiseKernel", "Mx4ValuesKernel"}) precompileKernel("mx4.h", str(kernel, "<", t, ">"));
     precompileKernel("mx4_linear.h", str("Mx4FewKernel<", t, ">"));
+    for (const Mx4Tiles& tiles : MX4_TILES)
+        if (p != Tensor::FLOAT || tiles.i < MX4_HUGE.i) precompileKernel("mx4_linear.h", str("Mx4TilesKernel<", t, ", ", tiles.arguments(), ">"));
 }
 
 QUICKMLP_NAMESPACE_END
