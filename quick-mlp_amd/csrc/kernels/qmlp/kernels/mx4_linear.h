@@ -52,50 +52,108 @@ __device__ __forceinline__ f32x16 mx4Multiply(u32x4 a, u32x4 b, f32x16 c, unsign
 }
 
 /**
+ * Moves tiles of SIZE rows of 128 bytes straight to LDS, laid out as by Tile; address and strides are multiples of 16 bytes, and rows do not
+ * overlap. What is not there is zero: rows behind the last lie behind the buffer.
+ */
+template <int SIZE, int THREADS>
+struct Mx4Loads
+{
+    static constexpr int TURN = THREADS / 8, EACH = SIZE / TURN;   // rows of a turn, turns
+    static_assert(SIZE % TURN == 0 && TURN % 16 == 0, "a thread's pieces lie in one column, which the order of pieces in LDS does not change");
+    const unsigned char* p;
+    int indices;
+    unsigned stride, first, turn;
+    u32x4 buffer;
+    unsigned to, from;
+
+    static __device__ __forceinline__ int column()
+    {
+        const int row = threadIdx.x / 8;
+        return (static_cast<int>(threadIdx.x) % 8 ^ (row >> 1 & 7)) * 16;
+    }
+    __device__ __forceinline__ void begin(const Source<unsigned char>& s)
+    {
+        p = s.p;
+        stride = static_cast<unsigned>(s.stride);
+        indices = s.indices;
+        first = threadIdx.x / 8 * stride + column();
+        turn = TURN * stride;
+    }
+    /** Turns to the tile of the next 'ks' bytes of every row, which goes to LDS from 'lds' on with the calls of load(0) to load(EACH - 1). */
+    __device__ __forceinline__ void next(unsigned lds, int ks)
+    {
+        buffer = bufferAt(p, (indices - 1) * stride + ks);
+        to = __builtin_amdgcn_readfirstlane(lds + threadIdx.x / 64 * 1024);
+        from = column() < ks ? first : 0x80000000u;
+        p += 128;
+    }
+    __device__ __forceinline__ void load(int n) const { loadToLds(buffer, from + n * turn, to + n * THREADS * 16); }
+};
+
+/**
  * The scales of a matrix' rows for two tiles of 8 blocks each: a thread takes the 16 bytes of a row at a time, its half of every tile side by side
- * for the lanes that read them.
+ * for the lanes that read them. Scales behind the last block are 1.
  */
 template <int TI, int TJ, int THREADS>
 struct Mx4Scales
 {
     static constexpr int ROWS = TI + TJ, EACH = (ROWS + THREADS - 1) / THREADS, BYTES = ROWS * 16;
+    static constexpr unsigned ONES = 0x7f7f7f7fu;
     const unsigned char* p[EACH];
     u32x4 raw[EACH];
-    __device__ __forceinline__ void begin(const unsigned char* a, long long strideA, int ni, const unsigned char* b, long long strideB, int nj)
+    int blocks, next, away;   // the first block that has not been asked for; bytes before the first one asked for
+    /** Asks for the first pair. */
+    __device__ __forceinline__ void begin(const unsigned char* a, long long strideA, int ni, const unsigned char* b, long long strideB, int nj, int blocks_)
     {
+        blocks = blocks_;
+        next = away = 0;
 #pragma unroll
         for (int n = 0; n < EACH; ++n) {
             const int row = n * THREADS + threadIdx.x;
             p[n] = row < TI ? a + min(row, ni - 1) * strideA : b + min(row - TI, nj - 1) * strideB;
         }
-    }
-    /** Asks for the next 16 blocks, of which 'left' are there; the others' scales are 1. */
-    __device__ __forceinline__ void load(int left)
-    {
+        if (blocks >= 16) {
+            ask();
+            return;
+        }
+        next = 16;
 #pragma unroll
-        for (int n = 0; n < EACH; ++n) {
-            if (left >= 16) __builtin_memcpy(&raw[n], p[n], 16);
-            else
+            for (int n = 0; n < EACH; ++n)
 #pragma unroll
                 for (int d = 0; d < 4; ++d) {
-                    unsigned v = 0x7f7f7f7fu;
-                    if (left >= 4 * d + 4) __builtin_memcpy(&v, p[n] + 4 * d, 4);
+                    unsigned v = ONES;
+                    if (blocks >= 4 * d + 4) __builtin_memcpy(&v, p[n] + 4 * d, 4);
                     else
 #pragma unroll
                         for (int k = 0; k < 3; ++k)
-                            if (4 * d + k < left) v = (v & ~(0xffu << (8 * k))) | static_cast<unsigned>(p[n][4 * d + k]) << (8 * k);
+                            if (4 * d + k < blocks) v = (v & ~(0xffu << (8 * k))) | static_cast<unsigned>(p[n][4 * d + k]) << (8 * k);
                     raw[n][d] = v;
                 }
-            p[n] += 16;
-        }
+    }
+    /** Asks for the next pair, if there is one; for the last one with blocks before it. */
+    __device__ __forceinline__ void ask()
+    {
+        if (next >= blocks) return;
+        const int from = min(next, blocks - 16);
+        away = next - from;
+        next += 16;
+#pragma unroll
+        for (int n = 0; n < EACH; ++n) __builtin_memcpy(&raw[n], p[n] + from, 16);
     }
     __device__ __forceinline__ void write(char* lds) const
     {
 #pragma unroll
         for (int n = 0; n < EACH; ++n) {
             const int row = n * THREADS + threadIdx.x;
-            const u32x4 ordered = {raw[n][0], raw[n][2], raw[n][1], raw[n][3]};
-            if (row < ROWS) __builtin_memcpy(__builtin_assume_aligned(lds + row * 16, 16), &ordered, 16);
+            unsigned v[4] = {raw[n][0], raw[n][1], raw[n][2], raw[n][3]};
+#pragma unroll
+            for (int d = 0; d < 4; ++d) v[d] = away & 8 ? (d < 2 ? v[d + 2] : ONES) : v[d];
+#pragma unroll
+            for (int d = 0; d < 4; ++d) v[d] = away & 4 ? (d < 3 ? v[d + 1] : ONES) : v[d];
+#pragma unroll
+            for (int d = 0; d < 4; ++d) v[d] = __builtin_amdgcn_alignbyte(d < 3 ? v[d + 1] : ONES, v[d], away & 3);
+            const u32x4 ordered = {v[0], v[2], v[1], v[3]};
+            if (ROWS >= (n + 1) * THREADS || row < ROWS) __builtin_memcpy(__builtin_assume_aligned(lds + row * 16, 16), &ordered, 16);
         }
     }
     /** Of the lane's row among the 32 from 'row' on: its half of two tiles. */
@@ -105,6 +163,13 @@ struct Mx4Scales
         __builtin_memcpy(&v, __builtin_assume_aligned(lds + (row + threadIdx.x % 32) * 16 + threadIdx.x % 64 / 32 * 8, 8), 8);
         return v;
     }
+};
+
+/** Which tile of a pair. */
+template <int W>
+struct Mx4Which
+{
+    static constexpr int value = W;
 };
 
 /**
@@ -118,8 +183,8 @@ struct Mx4Product
     typedef unsigned char Byte;
     typedef Tile<Byte, true, TI, THREADS> TileA;
     typedef Tile<Byte, true, TJ, THREADS> TileB;
-    typedef DirectTile<Byte, true, TI, THREADS> LoadsA;
-    typedef DirectTile<Byte, true, TJ, THREADS> LoadsB;
+    typedef Mx4Loads<TI, THREADS> LoadsA;
+    typedef Mx4Loads<TJ, THREADS> LoadsB;
     typedef Mx4Scales<TI, TJ, THREADS> Scales;
     static constexpr unsigned BYTES_A = TileA::BYTES, BYTES = BYTES_A + TileB::BYTES;
 
@@ -132,20 +197,42 @@ struct Mx4Product
     {
         u32x4 a[NI], b[NJ];
     };
-    template <int SIZE>
-    static __device__ __forceinline__ u32x4 operand(const char* lds, int i, int step)
+    /**
+     * Where in LDS the lane finds its pieces of every step of a tile, for the first 32 rows of each operand; those of the next 32 lie 4096 bytes
+     * behind (Tile::place() orders pieces by 16 rows), which needs no register.
+     */
+    struct Places
     {
-        const int lane = threadIdx.x % 64;
-        u32x4 v;
-        __builtin_memcpy(&v, __builtin_assume_aligned(lds + Tile<Byte, true, SIZE, THREADS>::place(i + lane % 32, (lane / 32 * 4 + step) * 16), 16), 16);
-        return v;
-    }
-    static __device__ __forceinline__ void readStep(Operands& o, const char* lds, int step)
+        unsigned a[STEPS], b[STEPS];
+        __device__ __forceinline__ void begin(unsigned lds)
+        {
+            const int lane = threadIdx.x % 64;
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s) {
+                const unsigned piece = TileA::place(lane % 32, (lane / 32 * 4 + s) * 16);
+                a[s] = lds + firstI() * 128 + piece;
+                b[s] = lds + BYTES_A + firstJ() * 128 + piece;
+            }
+        }
+        /** To the other tile. */
+        __device__ __forceinline__ void turn(unsigned by)
+        {
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s) {
+                a[s] += by;
+                b[s] += by;
+                // (otherwise the compiler keeps a register for each of their reads)
+                asm volatile("" : "+v"(a[s]), "+v"(b[s]));
+            }
+        }
+    };
+    static __device__ __forceinline__ u32x4 pieceAt(unsigned place) { return *(const __attribute__((address_space(3))) u32x4*)(place); }
+    static __device__ __forceinline__ void readStep(Operands& o, const Places& places, int step)
     {
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) o.b[j] = operand<TJ>(lds + BYTES_A, firstJ() + j * 32, step);
+        for (int j = 0; j < NJ; ++j) o.b[j] = pieceAt(places.b[step] + j * 4096);
 #pragma unroll
-        for (int i = 0; i < NI; ++i) o.a[i] = operand<TI>(lds, firstI() + i * 32, step);
+        for (int i = 0; i < NI; ++i) o.a[i] = pieceAt(places.a[step] + i * 4096);
         __builtin_amdgcn_sched_barrier(0);   // the compiler would move the reads to where they are used
     }
     template <int S, typename Between>
@@ -156,29 +243,33 @@ struct Mx4Product
 #pragma unroll
             for (int j = 0; j < NJ; ++j) {
                 sums[i][j] = mx4Multiply<S>(o.b[j], o.a[i], sums[i][j], scalesB[j], scalesA[i]);
+                // here and not behind the next barrier
+                if constexpr (NI * NJ > 8) asm volatile("" : "+a"(sums[i][j]));
+                else asm volatile("" : "+v"(sums[i][j]));
                 between(i * NJ + j);
             }
     }
 
-    /** LDS: two tiles of each operand, two pairs of tiles' scales. */
-    __device__ __forceinline__ void run(char* lds, const Source<Byte>& a, const Source<Byte>& b, Scales& scales, int blocks)
+    __device__ __forceinline__ void clear()
     {
 #pragma unroll
         for (int i = 0; i < NI; ++i)
 #pragma unroll
             for (int j = 0; j < NJ; ++j) sums[i][j] = f32x16{};
-        if (blocks <= 0) return;
+    }
+    /** LDS: two tiles of each operand, two pairs of tiles' scales. */
+    __device__ __forceinline__ void run(char* lds, const Source<Byte>& a, const Source<Byte>& b, Scales& scales, int blocks)
+    {
+        if (blocks <= 0) {
+            clear();
+            return;
+        }
         LoadsA tileA;
         LoadsB tileB;
         constexpr int LOADS = LoadsA::EACH + LoadsB::EACH, PRODUCTS = NI * NJ;
         const unsigned at = static_cast<unsigned>(reinterpret_cast<unsigned long long>((__attribute__((address_space(3))) char*)lds));
         char* const scalesLds = lds + 2 * BYTES;
-        int ahead = blocks, scalesAhead = blocks;   // blocks that have not been asked for
-        auto askScales = [&] {
-            if (scalesAhead > 0) scales.load(scalesAhead);
-            scalesAhead -= 16;
-        };
-        askScales();
+        int ahead = blocks;   // blocks that have not been asked for
         tileA.begin(a);
         tileB.begin(b);
         auto ask = [&](unsigned buffer) {
@@ -197,11 +288,9 @@ struct Mx4Product
         ask(0);
         load(0, LOADS);
         scales.write(scalesLds);
-        askScales();
-        if (ahead > 0) {
-            ask(BYTES);
-            load(0, LOADS);
-        }
+        scales.ask();
+        ask(BYTES);
+        load(0, LOADS);
         waitForTiles<0>();
         Operands operands[2];   // of a step and of the one behind it
         u32x2 pairsA[NI], pairsB[NJ];
@@ -211,52 +300,124 @@ struct Mx4Product
 #pragma unroll
             for (int j = 0; j < NJ; ++j) pairsB[j] = Scales::read(scalesLds + from, TI + firstJ() + j * 32);
         };
+        clear();
         readScales(0);
-        readStep(operands[0], lds, 0);
+        Places places;
+        places.begin(at);
+        readStep(operands[0], places, 0);
         const auto nothing = [](int) {};
-        unsigned buffer = 0, pair = 0;   // (where the tile and the scales of its pair lie)
-        bool second = false;             // of a pair
-        for (int k = 0; k < blocks; k += 8) {
+        unsigned pair = 0;   // (where the scales lie)
+        // All tiles go through the same code, without a branch that products would wait for: behind the last one lie tiles of zeros, which are not
+        // read from memory.
+        auto tile = [&](auto which) {
+            constexpr int W = decltype(which)::value;
             unsigned scalesA[NI], scalesB[NJ];
 #pragma unroll
-            for (int i = 0; i < NI; ++i) scalesA[i] = second ? pairsA[i][1] : pairsA[i][0];
+            for (int i = 0; i < NI; ++i) scalesA[i] = pairsA[i][W];
 #pragma unroll
-            for (int j = 0; j < NJ; ++j) scalesB[j] = second ? pairsB[j][1] : pairsB[j][0];
-            readStep(operands[1], lds + buffer, 1);
+            for (int j = 0; j < NJ; ++j) scalesB[j] = pairsB[j][W];
+            readStep(operands[1], places, 1);
             multiplyStep<0>(operands[0], scalesA, scalesB, nothing);
             __builtin_amdgcn_sched_barrier(0);
-            readStep(operands[0], lds + buffer, 2);
+            readStep(operands[0], places, 2);
             multiplyStep<1>(operands[1], scalesA, scalesB, nothing);
             __builtin_amdgcn_sched_barrier(0);
-            readStep(operands[1], lds + buffer, 3);
+            readStep(operands[1], places, 3);
             multiplyStep<2>(operands[0], scalesA, scalesB, nothing);
             __builtin_amdgcn_sched_barrier(0);
-            const bool more = ahead > 0, last = k + 8 >= blocks;
-            if (!last) {
-                if (more) ask(buffer);
-                buffer ^= BYTES;
-                waitForTiles<0>();
-            }
+            ask(W == 0 ? 0 : BYTES);
+            places.turn(W == 0 ? BYTES : 0u - BYTES);
+            waitForTiles<0>();
             // Behind the barrier the matrix cores go on at once; what else there is to do stands between the products. The scales of a pair are
             // asked for two barriers before it begins, written to LDS behind the first of them and read behind the second. (The compiler, which
             // does not know of the loads to LDS, waits for all loads when it waits for these: none are under way where they are written.)
             multiplyStep<3>(operands[1], scalesA, scalesB, [&](int n) {
-                if (n == 0 && !last) {
-                    readStep(operands[0], lds + buffer, 0);
-                    if (second) {
-                        pair ^= Scales::BYTES;
-                        readScales(pair);
-                        askScales();
-                    } else if (k + 16 < blocks)
-                        scales.write(scalesLds + (pair ^ Scales::BYTES));
+                if (n == 0) {
+                    readStep(operands[0], places, 0);
+                    if constexpr (W == 0) scales.write(scalesLds + (pair ^ Scales::BYTES));
                 }
-                if (more) load(n * LOADS / PRODUCTS, (n + 1) * LOADS / PRODUCTS);
+                load(n * LOADS / PRODUCTS, (n + 1) * LOADS / PRODUCTS);
                 __builtin_amdgcn_sched_barrier(0);
             });
-            second = !second;
+            if constexpr (W == 1) {
+                pair ^= Scales::BYTES;
+                readScales(pair);
+                scales.ask();
+            }
+        };
+        for (int k = 0;;) {
+            tile(Mx4Which<0>{});
+            if ((k += 8) >= blocks) break;
+            tile(Mx4Which<1>{});
+            if ((k += 8) >= blocks) break;
         }
+        waitForTiles<0>();
     }
 };
+
+/**
+ * As storeTile(), for few steps of K behind which there is little else to do: of a whole tile eight pieces a lane are on their way at a time.
+ */
+template <typename Product, typename T>
+__device__ __forceinline__ void mx4Store(const Product& product, char* lds, const T* __restrict__ bias, T* __restrict__ to, long long stride, int ni, int nj)
+{
+    constexpr int NI = Product::NI, NJ = Product::NJ, ROW = NJ * 32, PIECE = WIDE<T>, PIECES = ROW / PIECE, MASK = PIECES < 8 ? PIECES - 1 : 7;
+    constexpr int TURNS = NI * 32 * PIECES / 64, BATCH = TURNS < 8 ? TURNS : 8, TURN = 64 / PIECES;   // rows of a turn
+    const int lane = threadIdx.x % 64;
+    const int fromI = Product::firstI(), fromJ = Product::firstJ();
+    T* const part = reinterpret_cast<T*>(lds) + threadIdx.x / 64 * (NI * 32 * ROW);
+    __syncthreads();   // the last tiles have been read
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+        float b[16] = {};
+        if (bias)
+#pragma unroll
+            for (int n = 0; n < 16; ++n) b[n] = static_cast<float>(bias[min(fromJ + j * 32 + n / 4 * 8 + lane / 32 * 4 + n % 4, nj - 1)]);   // (columns behind: any)
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+#pragma unroll
+            for (int n = 0; n < 16; n += 4) {
+                const int row = i * 32 + lane % 32, column = j * 32 + n * 2 + lane / 32 * 4;
+                float v[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] = product.sums[i][j][n + k] + b[n + k];
+                // (a row's pieces in an order that depends on the row, for the banks)
+                T* at = part + row * ROW + ((column / PIECE ^ (row & MASK)) * PIECE + column % PIECE);
+                storeFloats(static_cast<T*>(__builtin_assume_aligned(at, 4 * sizeof(T))), v);
+            }
+    }
+    waveLdsSync();
+    const int row = lane / PIECES, piece = lane % PIECES, j = fromJ + piece * PIECE;
+    T* out = to + (fromI + row) * stride + j;
+    const bool whole = ni - fromI >= NI * 32 && nj - fromJ >= ROW;   // (of the wavefront's part)
+#pragma unroll 1
+    for (int n = 0; n < TURNS; n += BATCH) {
+        u32x4 raw[BATCH];
+#pragma unroll
+        for (int m = 0; m < BATCH; ++m) {
+            const int r = (n + m) * TURN + row;
+            __builtin_memcpy(&raw[m], __builtin_assume_aligned(part + r * ROW + (piece ^ (r & MASK)) * PIECE, 16), 16);
+        }
+        if (whole) {
+#pragma unroll
+            for (int m = 0; m < BATCH; ++m) streamPiece(out + m * TURN * stride, raw[m]);
+        } else
+#pragma unroll
+            for (int m = 0; m < BATCH; ++m) {
+                if (fromI + (n + m) * TURN + row >= ni || j >= nj) continue;
+                T* const at = out + m * TURN * stride;
+                if (j + PIECE <= nj) streamPiece(at, raw[m]);
+                else {
+                    T entries[PIECE];
+                    __builtin_memcpy(entries, &raw[m], 16);
+#pragma unroll
+                    for (int k = 0; k < PIECE - 1; ++k)
+                        if (j + k < nj) at[k] = entries[k];
+                }
+            }
+        out += BATCH * TURN * stride;
+    }
+}
 
 /** Workgroups: places of tiles x tiles of J. */
 template <typename T, int TI, int TJ, int WI, int WJ>
@@ -279,9 +440,9 @@ Mx4TilesKernel(const unsigned char* __restrict__ x, const unsigned char* __restr
     const Source<unsigned char> b = {weights.codes + expert * weights.codesExpert + j0 * weights.codesRow, weights.codesRow, nj, J - j0};
     typename Product::Scales scales;
     scales.begin(scalesX + at.from * strideScalesX, strideScalesX, ni, weights.scales + expert * weights.scalesExpert + j0 * weights.scalesRow,
-                 weights.scalesRow, nj);
+                 weights.scalesRow, nj, blocks);
     product.run(groupedLds, a, b, scales, none ? 0 : blocks);
-    storeTile(product, groupedLds, bias && !none ? bias + expert * strideBias + j0 : nullptr, y + at.from * strideY + j0, strideY, ni, nj);
+    mx4Store(product, groupedLds, bias && !none ? bias + expert * strideBias + j0 : nullptr, y + at.from * strideY + j0, strideY, ni, nj);
 }
 
 // ------------------------------------------------------------------------------------------------ few rows
