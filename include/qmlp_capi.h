@@ -330,7 +330,7 @@ int qmlp_tokens_mx4_quantise(const qmlp_tensor* input, const qmlp_tensor* codes,
 int qmlp_tokens_mx4_values(const qmlp_tensor* codes, const qmlp_tensor* scales, const qmlp_tensor* output, void* stream);
 /* qmlp_tokens_grouped_linear() with weights of 4 bits (experts, outputs, 16 * blocks) and their scales (experts, outputs, blocks): input (rows,
  * inputs) is quantised by the call, or holds codes with input_scales. offsets optional where there is one expert; memory for values as input. */
-int qmlp_tokens_mx4_linear_memory(long long rows, int inputs, size_t* bytes);
+int qmlp_tokens_mx4_linear_memory(long long rows, int experts, int inputs, int outputs, size_t* bytes);
 int qmlp_tokens_mx4_linear(const qmlp_tensor* input, const qmlp_tensor* input_scales, const qmlp_tensor* weight, const qmlp_tensor* scales,
                            const qmlp_tensor* offsets, const qmlp_tensor* bias, const qmlp_tensor* output, void* memory, void* stream);
 /* Compiles the kernels for values of QMLP_FLOAT, QMLP_HALF or QMLP_BFLOAT16 into the kernel cache without a device. */

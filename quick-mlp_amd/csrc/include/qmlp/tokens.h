@@ -118,8 +118,8 @@ public:
     /** The values that codes and scales stand for, in the output's type (rows, columns). */
     static void valuesMx4(const Tensor& codes, const Tensor& scales, Tensor& output, stream_t stream);
 
-    /** Bytes of 'memory' for mx4Linear(). */
-    static size_t mx4LinearMemory(int64_t rows, int inputs);
+    /** Bytes of 'memory' for mx4Linear() where input holds values; codes need none. */
+    static size_t mx4LinearMemory(int64_t rows, int experts, int inputs, int outputs);
     /**
      * groupedLinear() with weights of 4 bits, on rows that are quantised by the call or have been before.
      * \param input (rows, inputs), or codes as of quantiseMx4() with inputScales \param inputScales undefined where input holds values

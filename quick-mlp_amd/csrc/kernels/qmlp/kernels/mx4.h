@@ -34,6 +34,28 @@ __device__ __forceinline__ unsigned mx4Codes(const float (&v)[8], float scale)
     return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, v[6], v[7], scale, 3);
 }
 
+/** The lane's entries of a row of C, zeros behind the last. */
+template <typename T>
+__device__ __forceinline__ void mx4Load(const T* __restrict__ row, int at, int C, float (&v)[MX4_ENTRIES])
+{
+    if (at + MX4_ENTRIES <= C) loadFloats(row + at, v);
+    else
+#pragma unroll
+        for (int k = 0; k < MX4_ENTRIES; ++k) v[k] = at + k < C ? static_cast<float>(row[at + k]) : 0.0f;
+}
+/** The codes of the lane's entries and the scale of the block, which four lanes share: all of them call it. */
+__device__ __forceinline__ unsigned mx4Pack(const float (&v)[MX4_ENTRIES], unsigned& scale)
+{
+    unsigned largest = 0;
+#pragma unroll
+    for (int k = 0; k < MX4_ENTRIES; ++k) largest = max(largest, __builtin_bit_cast(unsigned, v[k]) & 0x7fffffffu);
+    // (lanes 1 0 3 2 and 2 3 0 1 of every four)
+    largest = max(largest, static_cast<unsigned>(__builtin_amdgcn_mov_dpp(static_cast<int>(largest), 0xb1, 0xf, 0xf, true)));
+    largest = max(largest, static_cast<unsigned>(__builtin_amdgcn_mov_dpp(static_cast<int>(largest), 0x4e, 0xf, 0xf, true)));
+    scale = mx4Scale(largest);
+    return scale == 255 ? 0 : mx4Codes(v, mx4ScaleBits(scale));
+}
+
 /** x (rows, C), rows of any stride; codes (rows, blocks, 16) and scales (rows, blocks), rows of any stride. */
 template <typename T>
 __global__ void __launch_bounds__(MX4_THREADS)
@@ -44,19 +66,11 @@ Mx4QuantiseKernel(const T* __restrict__ x, long long strideX, unsigned char* __r
     for (long long first = static_cast<long long>(blockIdx.x) * MX4_THREADS; first < units * MX4_LANES; first += static_cast<long long>(gridDim.x) * MX4_THREADS) {
         const long long unit = min((first + threadIdx.x) / MX4_LANES, units - 1);   // (the last ones are written more than once)
         const long long row = unit / blocks;
-        const int block = static_cast<int>(unit - row * blocks), at = block * MX4_BLOCK + lane * MX4_ENTRIES;
+        const int block = static_cast<int>(unit - row * blocks);
         float v[MX4_ENTRIES];
-        if (at + MX4_ENTRIES <= C) loadFloats(x + row * strideX + at, v);
-        else
-#pragma unroll
-            for (int k = 0; k < MX4_ENTRIES; ++k) v[k] = at + k < C ? static_cast<float>(x[row * strideX + at + k]) : 0.0f;
-        unsigned largest = 0;
-#pragma unroll
-        for (int k = 0; k < MX4_ENTRIES; ++k) largest = max(largest, __builtin_bit_cast(unsigned, v[k]) & 0x7fffffffu);
-        largest = max(largest, static_cast<unsigned>(__shfl_xor(static_cast<int>(largest), 1)));
-        largest = max(largest, static_cast<unsigned>(__shfl_xor(static_cast<int>(largest), 2)));
-        const unsigned scale = mx4Scale(largest);
-        const unsigned packed = scale == 255 ? 0 : mx4Codes(v, mx4ScaleBits(scale));
+        mx4Load(x + row * strideX, block * MX4_BLOCK + lane * MX4_ENTRIES, C, v);
+        unsigned scale;
+        const unsigned packed = mx4Pack(v, scale);
         __builtin_memcpy(codes + row * strideCodes + block * 16 + lane * 4, &packed, 4);
         if (lane == 0) scales[row * strideScales + block] = static_cast<unsigned char>(scale);
     }

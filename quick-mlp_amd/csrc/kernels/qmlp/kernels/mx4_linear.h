@@ -243,9 +243,7 @@ struct Mx4Product
 #pragma unroll
             for (int j = 0; j < NJ; ++j) {
                 sums[i][j] = mx4Multiply<S>(o.b[j], o.a[i], sums[i][j], scalesB[j], scalesA[i]);
-                // here and not behind the next barrier
-                if constexpr (NI * NJ > 8) asm volatile("" : "+a"(sums[i][j]));
-                else asm volatile("" : "+v"(sums[i][j]));
+                asm volatile("" : "+v"(sums[i][j]));   // here and not behind the next barrier
                 between(i * NJ + j);
             }
     }
@@ -419,9 +417,10 @@ __device__ __forceinline__ void mx4Store(const Product& product, char* lds, cons
     }
 }
 
-/** Workgroups: places of tiles x tiles of J. */
+/** Workgroups: places of tiles x tiles of J. (Two wavefronts per SIMD at least: with all of its registers the compiler would keep the sums where each
+ *  product has to fetch them from.) */
 template <typename T, int TI, int TJ, int WI, int WJ>
-__global__ void __launch_bounds__(64 * WI * WJ)
+__global__ void __launch_bounds__(64 * WI * WJ, 2)
 Mx4TilesKernel(const unsigned char* __restrict__ x, const unsigned char* __restrict__ scalesX, long long strideX, long long strideScalesX, Mx4Matrix weights,
                const T* __restrict__ bias, long long strideBias, const int* __restrict__ offsets, int experts, T* __restrict__ y, long long strideY, int rows,
                int J, int blocks, int places, int tilesJ)
@@ -447,47 +446,161 @@ Mx4TilesKernel(const unsigned char* __restrict__ x, const unsigned char* __restr
 
 // ------------------------------------------------------------------------------------------------ few rows
 constexpr int MX4_FEW_WAVES = 4;
-/**
- * 16 rows by 16 outputs per wavefront, operands straight from memory: lane l has block l / 16 of every four of row l % 16. Results: lane l has
- * outputs 4 (l / 16) .. + 3 of row l % 16.
- */
-template <typename T>
-__global__ void __launch_bounds__(64 * MX4_FEW_WAVES)
-Mx4FewKernel(const unsigned char* __restrict__ x, const unsigned char* __restrict__ scalesX, long long strideX, long long strideScalesX, Mx4Matrix weights,
-             const T* __restrict__ bias, long long strideBias, const int* __restrict__ offsets, int experts, T* __restrict__ y, long long strideY, int rows,
-             int J, int blocks, int places, int tilesJ)
+/** Where experts have few rows: blocks of K at a time, their steps of 4 blocks, and what a row of them takes in LDS (no two of 16 in one bank). */
+constexpr int MX4_FEW_BLOCKS = 32, MX4_FEW_STEPS = MX4_FEW_BLOCKS / 4, MX4_FEW_CODES = MX4_FEW_BLOCKS * 16 + 16, MX4_FEW_SCALES = MX4_FEW_BLOCKS + 16;
+
+/** Rows of a chunk of MX4_FEW_BLOCKS blocks from block 'first' on, in LDS: quantised, or as they are where X holds codes. Blocks behind the last: zeros. */
+template <typename X>
+__device__ __forceinline__ void mx4Stage(const X* __restrict__ x, const unsigned char* __restrict__ scalesX, long long strideX, long long strideScalesX, int count,
+                                         int first, int blocks, int inputs, char* codesLds, char* scalesLds)
 {
-    const int place = static_cast<int>(blockIdx.x % places), tile = static_cast<int>(blockIdx.x / places);
-    const ExpertTile at = mx4Tile(offsets, experts, rows, 16, place);
-    if (at.to <= at.from) return;
-    const int lane = threadIdx.x % 64, i = lane % 16, g = lane / 16;
-    const int j0 = (tile * MX4_FEW_WAVES + static_cast<int>(threadIdx.x) / 64) * 16;
-    if (j0 >= J) return;
-    const bool none = at.expert >= experts;
-    f32x4 sum = {};
-    if (!none) {
-        const long long row = min(at.from + i, at.to - 1), output = min(j0 + i, J - 1);   // (rows and outputs behind the last: any, not written)
-        const unsigned char* const ownX = x + row * strideX;
-        const unsigned char* const ownScalesX = scalesX + row * strideScalesX;
-        const unsigned char* const own = weights.codes + at.expert * weights.codesExpert + output * weights.codesRow;
-        const unsigned char* const ownScales = weights.scales + at.expert * weights.scalesExpert + output * weights.scalesRow;
-        for (int b = g; b < (blocks + 3) / 4 * 4; b += 4) {
-            i32x8 codesW = {}, codesX = {};
-            unsigned scaleW = 127, scaleX = 127;
+    constexpr bool CODES = sizeof(X) == 1;
+    constexpr int LANES = CODES ? 1 : MX4_LANES;
+    for (int unit = threadIdx.x / LANES; unit < count * MX4_FEW_BLOCKS; unit += 64 * MX4_FEW_WAVES / LANES) {
+        const int row = unit / MX4_FEW_BLOCKS, block = unit % MX4_FEW_BLOCKS, b = first + block;
+        char* const toCodes = codesLds + row * MX4_FEW_CODES + block * 16;
+        char* const toScale = scalesLds + row * MX4_FEW_SCALES + block;
+        if constexpr (CODES) {
+            u32x4 codes = {};
+            unsigned char scale = 127;
             if (b < blocks) {
-                __builtin_memcpy(&codesW, own + b * 16ll, 16);
-                __builtin_memcpy(&codesX, ownX + b * 16ll, 16);
-                scaleW = ownScales[b];
-                scaleX = ownScalesX[b];
+                __builtin_memcpy(&codes, x + row * strideX + b * 16ll, 16);
+                scale = scalesX[row * strideScalesX + b];
             }
-            sum = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(codesW, codesX, sum, 4, 4, 0, scaleW, 0, scaleX);
+            __builtin_memcpy(__builtin_assume_aligned(toCodes, 16), &codes, 16);
+            *toScale = static_cast<char>(scale);
+        } else {
+            const int lane = threadIdx.x % MX4_LANES, at = b * MX4_BLOCK + lane * MX4_ENTRIES;
+            float v[MX4_ENTRIES];
+            mx4Load(x + row * strideX, at, inputs, v);
+            unsigned scale;
+            const unsigned packed = mx4Pack(v, scale);
+            __builtin_memcpy(__builtin_assume_aligned(toCodes + lane * 4, 4), &packed, 4);
+            if (lane == 0) *toScale = static_cast<char>(scale);
         }
     }
-    if (at.from + i >= at.to) return;
+}
+
+/**
+ * The tile of 16 rows that begins at the given row; to <= from: there is none. So there are no more places of tiles than rows, however many experts
+ * have none.
+ */
+__device__ __forceinline__ ExpertTile mx4TileAt(const int* __restrict__ offsets, int experts, int rows, int row)
+{
+    int from = 0, begin = 0, end = rows;   // of the last expert that begins at the row or before it, as in expertTile()
+    const int lane = threadIdx.x % 64;
+    for (int count = offsets ? experts : 0; count > 0;) {
+        const int step = (count + 63) / 64, ahead = (lane + 1) * step, e = from + min(ahead, count);
+        const int begins = expertBegin(offsets, e, rows);
+        const int reached = __popcll(__ballot(ahead <= count && begins <= row));
+        if (reached > 0) begin = __builtin_amdgcn_readlane(begins, reached - 1);
+        if (reached < 64 && (reached + 1) * step <= count) end = __builtin_amdgcn_readlane(begins, reached);
+        from += reached * step;
+        count = min(step - 1, count - reached * step);
+    }
+    ExpertTile t;
+    t.expert = from;
+    t.index = (row - begin) / 16;
+    t.from = row;
+    t.to = (row - begin) % 16 == 0 ? min(end, static_cast<int>(min(row + 16ll, static_cast<long long>(rows)))) : row;
+    t.expertRows = max(0, end - begin);
+    return t;
+}
+
+/**
+ * 16 rows by 16 outputs per wavefront, the weights straight from memory: lane l has block l / 16 of every four of output l % 16, a chunk ahead of the
+ * matrix cores. WJ wavefronts take outputs of their own, WK share the chunk's steps and add up what they have. Results: lane l has outputs
+ * 4 (l / 16) .. + 3 of row l % 16. X: T, or bytes of codes. byRow: places are rows, of which those work that a tile begins at.
+ */
+template <typename T, typename X, int WJ, int WK>
+__global__ void __launch_bounds__(64 * MX4_FEW_WAVES)
+Mx4FewKernel(const X* __restrict__ x, const unsigned char* __restrict__ scalesX, long long strideX, long long strideScalesX, Mx4Matrix weights,
+             const T* __restrict__ bias, long long strideBias, const int* __restrict__ offsets, int experts, T* __restrict__ y, long long strideY, int rows,
+             int J, int blocks, int inputs, int byRow, int tilesJ)
+{
+    static_assert(WJ * WK == MX4_FEW_WAVES, "wavefronts of a workgroup");
+    constexpr int STEPS = MX4_FEW_STEPS / WK, ROWS = 16;
+    __shared__ __attribute__((aligned(16))) char codesLds[2][ROWS * MX4_FEW_CODES];
+    __shared__ __attribute__((aligned(16))) char scalesLds[2][ROWS * MX4_FEW_SCALES];
+    const int place = static_cast<int>(blockIdx.x / tilesJ), tile = static_cast<int>(blockIdx.x % tilesJ);
+    const ExpertTile at = byRow ? mx4TileAt(offsets, experts, rows, place) : mx4Tile(offsets, experts, rows, ROWS, place);
+    if (at.to <= at.from) return;
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, i = lane % 16, g = lane / 16;
+    const int j0 = (tile * WJ + wave / WK) * 16, step0 = wave % WK * STEPS;
+    const int count = at.to - at.from;
+    f32x4 sum = {};
+    if (at.expert < experts) {
+        const long long output = min(j0 + i, J - 1);   // (outputs behind the last: any, not written)
+        const unsigned char* const own = weights.codes + at.expert * weights.codesExpert + output * weights.codesRow;
+        const unsigned char* const ownScales = weights.scales + at.expert * weights.scalesExpert + output * weights.scalesRow;
+        u32x4 codes[2][STEPS];
+        unsigned scales[2][STEPS];   // in the lane's byte g
+        auto load = [&](int first, u32x4 (&c)[STEPS], unsigned (&s)[STEPS]) {
+            const int b = first + step0 * 4;
+            if (b + STEPS * 4 <= blocks) {
+#pragma unroll
+                for (int n = 0; n < STEPS; ++n) __builtin_memcpy(&c[n], own + (b + n * 4 + g) * 16ll, 16);
+                __builtin_memcpy(s, ownScales + b, sizeof(s));
+            } else
+#pragma unroll
+                for (int n = 0; n < STEPS; ++n) {
+                    const int block = b + n * 4 + g;
+                    c[n] = u32x4{};
+                    s[n] = 127u << (8 * g);
+                    if (block >= blocks) continue;
+                    __builtin_memcpy(&c[n], own + block * 16ll, 16);
+                    s[n] = static_cast<unsigned>(ownScales[block]) << (8 * g);
+                }
+        };
+        auto stage = [&](int first, int buffer) {
+            mx4Stage(x + at.from * strideX, scalesX + at.from * strideScalesX, strideX, strideScalesX, count, first, blocks, inputs, codesLds[buffer], scalesLds[buffer]);
+        };
+        auto multiply = [&](int buffer, const u32x4 (&c)[STEPS], const unsigned (&s)[STEPS]) {
+            // (rows behind the last of the tile hold anything, and so do their results)
+            const char* const rowCodes = codesLds[buffer] + i * MX4_FEW_CODES;
+            const char* const rowScales = scalesLds[buffer] + i * MX4_FEW_SCALES;
+#pragma unroll
+            for (int n = 0; n < STEPS; ++n) {
+                u32x4 other;
+                unsigned otherScale;
+                __builtin_memcpy(&other, __builtin_assume_aligned(rowCodes + ((step0 + n) * 4 + g) * 16, 16), 16);
+                __builtin_memcpy(&otherScale, __builtin_assume_aligned(rowScales + (step0 + n) * 4, 4), 4);
+                const i32x8 wideW = __builtin_bit_cast(i32x8, __builtin_shufflevector(c[n], c[n], 0, 1, 2, 3, -1, -1, -1, -1));
+                const i32x8 wideX = __builtin_bit_cast(i32x8, __builtin_shufflevector(other, other, 0, 1, 2, 3, -1, -1, -1, -1));
+                sum = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wideW, wideX, sum, 4, 4, 0, s[n] >> (8 * g), 0, otherScale >> (8 * g));
+            }
+        };
+        load(0, codes[0], scales[0]);
+        stage(0, 0);
+        __syncthreads();
+        for (int first = 0;; first += 2 * MX4_FEW_BLOCKS) {
+            const bool second = first + MX4_FEW_BLOCKS < blocks, third = first + 2 * MX4_FEW_BLOCKS < blocks;
+            if (second) load(first + MX4_FEW_BLOCKS, codes[1], scales[1]);
+            multiply(0, codes[0], scales[0]);
+            if (!second) break;
+            stage(first + MX4_FEW_BLOCKS, 1);
+            __syncthreads();
+            if (third) load(first + 2 * MX4_FEW_BLOCKS, codes[0], scales[0]);
+            multiply(1, codes[1], scales[1]);
+            if (!third) break;
+            stage(first + 2 * MX4_FEW_BLOCKS, 0);
+            __syncthreads();
+        }
+    }
+    if constexpr (WK > 1) {
+        __shared__ f32x4 others[WJ][WK - 1][64];
+        if (wave % WK > 0) others[wave / WK][wave % WK - 1][lane] = sum;
+        __syncthreads();
+        if (wave % WK > 0) return;
+#pragma unroll
+        for (int k = 0; k < WK - 1; ++k) sum += others[wave / WK][k][lane];
+    }
     const int j = j0 + 4 * g;
+    if (j >= J || i >= count) return;
     float v[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = sum[k] + (bias && !none && j + k < J ? static_cast<float>(bias[at.expert * strideBias + j + k]) : 0.0f);
+    for (int k = 0; k < 4; ++k)
+        v[k] = sum[k] + (bias && at.expert < experts ? static_cast<float>(bias[at.expert * strideBias + min(j + k, J - 1)]) : 0.0f);
     storeUpToFour(y + (at.from + i) * strideY + j, v, J - j);
 }
 

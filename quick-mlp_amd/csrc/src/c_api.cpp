@@ -858,10 +858,10 @@ int qmlp_tokens_mx4_values(const qmlp_tensor* codes, const qmlp_tensor* scales, 
     QMLP_API_END
 }
 
-int qmlp_tokens_mx4_linear_memory(long long rows, int inputs, size_t* bytes)
+int qmlp_tokens_mx4_linear_memory(long long rows, int experts, int inputs, int outputs, size_t* bytes)
 {
     QMLP_API_BEGIN
-    *bytes = Tokens::mx4LinearMemory(rows, inputs);
+    *bytes = Tokens::mx4LinearMemory(rows, experts, inputs, outputs);
     QMLP_API_END
 }
 

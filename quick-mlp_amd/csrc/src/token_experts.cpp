@@ -121,21 +121,46 @@ int checkMx4(const Tensor& codes, const char* whatCodes, const Tensor& scales, c
 struct Mx4Tiles
 {
     int i, j, wavesI, wavesJ;
-    int threads() const { return 64 * wavesI * wavesJ; }
+    int wavesK = 0;   // few rows: wavefronts that share a chunk of K; otherwise 0
+    int threads() const { return wavesK ? 64 * MX4_FEW_WAVES : 64 * wavesI * wavesJ; }
     /** Two tiles of each operand and two pairs of tiles' scales, later the results. */
-    unsigned lds(int entry) const { return static_cast<unsigned>(std::max((2 * 128 + 2 * 16) * (i + j), i * j * entry)); }
+    unsigned lds(int entry) const { return wavesK ? 0 : static_cast<unsigned>(std::max((2 * 128 + 2 * 16) * (i + j), i * j * entry)); }
     std::string arguments() const { return str(i, ", ", j, ", ", wavesI, ", ", wavesJ); }
 };
-constexpr Mx4Tiles MX4_HUGE = {256, 256, 2, 4}, MX4_LARGE = {128, 128, 2, 2}, MX4_SMALL = {64, 64, 2, 2}, MX4_FEWEST = {16, 64, 1, 4};
+constexpr Mx4Tiles MX4_HUGE = {256, 256, 2, 4}, MX4_LARGE = {128, 128, 2, 2}, MX4_SMALL = {64, 64, 2, 2};
 constexpr Mx4Tiles MX4_TILES[] = {MX4_HUGE, MX4_LARGE, MX4_SMALL};
+/** 16 rows at a time, as many outputs for each of the wavefronts that do not share K. */
+constexpr Mx4Tiles mx4Few(int wavesK) { return {16, 16 * MX4_FEW_WAVES / wavesK, 1, MX4_FEW_WAVES / wavesK, wavesK}; }
+constexpr int MX4_FEW_SHARES[] = {1, 4};
 
-Mx4Tiles mx4Tiles(Tensor::Precision p, int64_t rows, int64_t experts, int64_t J, bool direct)
+struct Mx4Plan
+{
+    Mx4Tiles tiles;
+    bool inPlace = false;   // the product's workgroups quantise the rows, each for its own outputs
+};
+/**
+ * How the product of 'rows' rows, 'blocks' blocks each, with J outputs of every expert is made. us with rows that are codes | with values, bfloat16,
+ * rows, experts, inputs, outputs:
+ * Few rows or tiles: the weights straight from memory, one wavefront or four for a chunk of K; then tiles of 64. 24, 64, 1024, 4096: 14.6 | 14.9 in
+ * place, 16.9 before; 15.3 | 16.0; 19.9 | 22.2. 256, 64, 1024, 4096: 33.9 | 38.7, 36.3; 37.8 | 46.6; 32.0 | 34.5. 16, 1, 4096, 4096: 9.6 | 17.3,
+ * 12.7; 6.3 | 13.9, 9.5; 12.4 | 15.0. 60, 4, 2048, 2048: 6.3 | 10.1, 9.0; 5.8 | 9.8, 8.2; 6.7 | 10.1. 32, 1, 1024, 1024: 4.6 | 6.5, 7.0; 4.0 |
+ * 5.7, 6.3; 5.1 | 8.0. 200, 100, 200, 300: 5.2 | 6.1, 7.7; 6.7 | 8.2; 6.0 | 8.6.
+ * Tiles of 64, 128 and 256, codes: 5003, 12, 333, 200: 6.3, 7.2, 10.5; 256, 1, 4096, 4096: 10.4, 17.8, 28; 6400, 64, 512, 512: 8.6, 7.5, 9.7; 3200,
+ * 64, 2048, 2048: 33, 37, 52; 6400, 64, 2048, 2048: 51, 46, 53; 16384, 16, 1024, 1024: 30, 24, 27; 8192, 16, 2048, 4096: 89, 66, 61; 32768, 16,
+ * 2048, 4096: 342, 240, 215. Single precision, whose results take too much LDS for tiles of 256: 32768, 16, 2048, 4096: 359, 269; 5003, 12, 333,
+ * 200: 6.5, 7.8.
+ */
+Mx4Plan mx4Plan(Tensor::Precision p, int64_t rows, int64_t experts, int64_t J, int64_t blocks, bool values, bool direct)
 {
     const int64_t each = rows / std::max<int64_t>(experts, 1);
-    if (each <= 32 || !direct) return MX4_FEWEST;
-    auto count = [&](const Mx4Tiles& t) { return (rows / t.i + experts) * divUp<int64_t>(J, t.j); };
-    if (p != Tensor::FLOAT && each > 128 && J > 128 && count(MX4_HUGE) >= 256) return MX4_HUGE;
-    return each > 64 && J > 64 && count(MX4_LARGE) >= 256 ? MX4_LARGE : MX4_SMALL;
+    auto count = [&](const Mx4Tiles& t) { return (rows / t.i + std::min(experts, rows)) * divUp<int64_t>(J, t.j); };
+    auto whole = [&](const Mx4Tiles& t) { return rows / t.i * divUp<int64_t>(J, t.j); };
+    const Mx4Tiles few = mx4Few(blocks >= 16 && count(mx4Few(1)) < 700 ? 4 : 1);
+    // (what a workgroup and what all of them have to quantise)
+    const bool inPlace = values && rows <= 256 && each <= 16 && each * blocks <= 512 && rows * blocks * divUp<int64_t>(J, few.j) <= 1 << 18;
+    if (inPlace || !direct || each <= 1 || (each <= 64 && count(MX4_SMALL) <= 128)) return {few, inPlace};
+    if (p != Tensor::FLOAT && each > 128 && J > 128 && whole(MX4_HUGE) >= 512) return {MX4_HUGE};
+    return {each > 64 && J > 64 && whole(MX4_LARGE) >= 128 ? MX4_LARGE : MX4_SMALL};
 }
 
 int mx4Blocks(int64_t columns) { return static_cast<int>(divUp<int64_t>(columns, MX4_BLOCK)); }
@@ -150,6 +175,11 @@ void launchQuantise(const Tensor& input, unsigned char* codes, long long strideC
     tokenKernel("mx4.h", kernelKey(MX4_QUANTISE, p), [&] { return str("Mx4QuantiseKernel<", scalarName(p), ">"); })
         .call(mx4Workgroups(units), MX4_THREADS, 0, stream, input.rawPtr(), strideOf(input, 0), codes, strideCodes, scales, strideScales, units, blocks,
               static_cast<int>(input.size(1)));
+}
+
+std::string mx4FewName(Tensor::Precision p, bool inPlace, const Mx4Tiles& t)
+{
+    return str("Mx4FewKernel<", scalarName(p), ", ", inPlace ? scalarName(p) : "unsigned char", ", ", t.wavesJ, ", ", t.wavesK, ">");
 }
 
 /** Rows of the 4-bit operand as a call makes them in its memory. */
@@ -287,10 +317,11 @@ void Tokens::valuesMx4(const Tensor& codes, const Tensor& scales, Tensor& output
               static_cast<int>(output.size(1)));
 }
 
-size_t Tokens::mx4LinearMemory(int64_t rows, int inputs)
+size_t Tokens::mx4LinearMemory(int64_t rows, int experts, int inputs, int outputs)
 {
-    CHECK_ERROR(rows >= 0 && inputs >= 0, "sizes must not be negative");
-    return Mx4Rows(rows, mx4Blocks(inputs), nullptr).memory.bytes;
+    CHECK_ERROR(rows >= 0 && experts >= 0 && inputs >= 0 && outputs >= 0, "sizes must not be negative");
+    const int blocks = mx4Blocks(inputs);
+    return mx4Plan(Tensor::FLOAT, rows, experts, outputs, blocks, true, true).inPlace ? 0 : Mx4Rows(rows, blocks, nullptr).memory.bytes;
 }
 
 void Tokens::mx4Linear(const Tensor& input, const Tensor& inputScales, const Tensor& weight, const Tensor& scales, const Tensor& offsets, const Tensor& bias,
@@ -336,28 +367,37 @@ void Tokens::mx4Linear(const Tensor& input, const Tensor& inputScales, const Ten
         return reinterpret_cast<uintptr_t>(t.rawPtr()) % 16 == 0 && (t.size(n - 2) <= 1 || (t.stride(n - 2) >= t.size(n - 1) && t.stride(n - 2) < 1 << 22));
     };
     const bool isDirect = direct(weight) && (!quantised || direct(input)) && blocks < 1 << 17;
-    const Mx4Tiles tiles = mx4Tiles(p, rows, experts, outputs, isDirect);
-    const int64_t places = static_cast<int64_t>(rows) / tiles.i + experts + 1, tilesJ = divUp<int64_t>(outputs, tiles.j);
+    const Mx4Plan plan = mx4Plan(p, rows, experts, outputs, blocks, !quantised, isDirect);
+    const Mx4Tiles& tiles = plan.tiles;
+    const bool few = tiles.wavesK > 0;
+    const int64_t all = static_cast<int64_t>(rows) / tiles.i + experts + 1, places = few ? std::min<int64_t>(all, rows) : all, tilesJ = divUp<int64_t>(outputs, tiles.j);
     checkLaunch(places * tilesJ, tiles.threads());
-    Mx4Rows x(rows, blocks, memory);
-    long long strideX = blocks * 16ll, strideScalesX = blocks;
-    if (quantised) {
-        x.codes = ptr<unsigned char>(input);
-        x.scales = ptr<unsigned char>(inputScales);
-        strideX = strideOf(input, 0);
-        strideScalesX = strideOf(inputScales, 0);
-    } else {
-        checkMemory(memory, x.memory.bytes);
-        launchQuantise(input, x.codes, strideX, x.scales, strideScalesX, stream);
-    }
     const Mx4Matrix w{ptr<unsigned char>(weight), ptr<unsigned char>(scales), strideOf(weight, 0), strideOf(scales, 0), strideOf(weight, 1), strideOf(scales, 1)};
-    const bool few = tiles.i == MX4_FEWEST.i;
-    tokenKernel("mx4_linear.h", few ? kernelKey(MX4_FEW, p) : kernelKey(MX4_TILES_OF, p, tiles.i, tiles.j, tiles.wavesI, tiles.wavesJ),
-                [&] { return few ? str("Mx4FewKernel<", scalarName(p), ">") : str("Mx4TilesKernel<", scalarName(p), ", ", tiles.arguments(), ">"); })
-        .call(static_cast<unsigned>(places * tilesJ), tiles.threads(), few ? 0 : tiles.lds(output.bytesPerEntry()), stream,
-              static_cast<const unsigned char*>(x.codes), static_cast<const unsigned char*>(x.scales), strideX, strideScalesX, w,
-              static_cast<const void*>(ptr<void>(bias)), strideOrNone(bias), static_cast<const int*>(ptr<int>(offsets)), experts, output.rawPtr(),
-              strideOf(output, 0), rows, outputs, blocks, static_cast<int>(places), static_cast<int>(tilesJ));
+    const void* const b = ptr<void>(bias);
+    const int* const off = ptr<int>(offsets);
+    const int count = static_cast<int>(places), countJ = static_cast<int>(tilesJ), byRow = places < all;
+    const unsigned groups = static_cast<unsigned>(places * tilesJ);
+    const void* x = input.rawPtr();
+    const unsigned char* scalesX = ptr<unsigned char>(inputScales);
+    long long strideX = strideOf(input, 0), strideScalesX = strideOrNone(inputScales);
+    if (!quantised && !plan.inPlace) {
+        const Mx4Rows codes(rows, blocks, memory);
+        checkMemory(memory, codes.memory.bytes);
+        strideX = blocks * 16ll;
+        strideScalesX = blocks;
+        launchQuantise(input, codes.codes, strideX, codes.scales, strideScalesX, stream);
+        x = codes.codes;
+        scalesX = codes.scales;
+    }
+    if (few)
+        tokenKernel("mx4_linear.h", kernelKey(MX4_FEW, p, plan.inPlace, tiles.wavesK), [&] { return mx4FewName(p, plan.inPlace, tiles); })
+            .call(groups, tiles.threads(), 0, stream, x, scalesX, strideX, strideScalesX, w, b, strideOrNone(bias), off, experts, output.rawPtr(),
+                  strideOf(output, 0), rows, outputs, blocks, plan.inPlace ? static_cast<int>(input.size(1)) : 0, byRow, countJ);
+    else
+        tokenKernel("mx4_linear.h", kernelKey(MX4_TILES_OF, p, tiles.i, tiles.j, tiles.wavesI, tiles.wavesJ),
+                    [&] { return str("Mx4TilesKernel<", scalarName(p), ", ", tiles.arguments(), ">"); })
+            .call(groups, tiles.threads(), tiles.lds(output.bytesPerEntry()), stream, x, scalesX, strideX, strideScalesX, w, b, strideOrNone(bias), off,
+                  experts, output.rawPtr(), strideOf(output, 0), rows, outputs, blocks, count, countJ);
 }
 
 void token::precompileExperts(Tensor::Precision p)
@@ -375,7 +415,8 @@ void token::precompileExperts(Tensor::Precision p)
             if (lanes <= 64) precompileKernel("expert_rows.h", str("CombineAdjointKernel<", t, shape));
         }
     for (const char* kernel : {"Mx4QuantiseKernel", "Mx4ValuesKernel"}) precompileKernel("mx4.h", str(kernel, "<", t, ">"));
-    precompileKernel("mx4_linear.h", str("Mx4FewKernel<", t, ">"));
+    for (const bool inPlace : {false, true})
+        for (const int share : MX4_FEW_SHARES) precompileKernel("mx4_linear.h", mx4FewName(p, inPlace, mx4Few(share)));
     for (const Mx4Tiles& tiles : MX4_TILES)
         if (p != Tensor::FLOAT || tiles.i < MX4_HUGE.i) precompileKernel("mx4_linear.h", str("Mx4TilesKernel<", t, ", ", tiles.arguments(), ">"));
 }

@@ -983,7 +983,7 @@ at::Tensor mx4Linear(const at::Tensor& input, const at::Tensor& inputScales, con
         size_t bytes = 0;
         const qmlp_tensor in = wrapToken(rows), is = wrapToken(rowScales), wt = wrapToken(w), st = wrapToken(s), of = wrapToken(off), bt = wrapToken(b),
                           o = wrapToken(out);
-        if (!inputScales.defined()) check(qmlp_tokens_mx4_linear_memory(in.sizes[0], in.sizes[1], &bytes));
+        if (!inputScales.defined()) check(qmlp_tokens_mx4_linear_memory(in.sizes[0], wt.sizes[0], in.sizes[1], wt.sizes[1], &bytes));
         const at::Tensor memory = temporary(rows, bytes);
         check(qmlp_tokens_mx4_linear(&in, &is, &wt, &st, &of, &bt, &o, dataOf(memory), currentStream(input)));
         return out;

@@ -141,7 +141,7 @@ _SIGNATURES = {
     "qmlp_tokens_combine_adjoint": [_TD, _TD, _TD, _TD, _TD, _TD, _vp],
     "qmlp_tokens_mx4_quantise": [_TD, _TD, _TD, _vp],
     "qmlp_tokens_mx4_values": [_TD, _TD, _TD, _vp],
-    "qmlp_tokens_mx4_linear_memory": [ctypes.c_longlong, _ci, _P(ctypes.c_size_t)],
+    "qmlp_tokens_mx4_linear_memory": [ctypes.c_longlong, _ci, _ci, _ci, _P(ctypes.c_size_t)],
     "qmlp_tokens_mx4_linear": [_TD, _TD, _TD, _TD, _TD, _TD, _TD, _vp, _vp],
     "qmlp_tokens_precompile": [_ci],
 }

@@ -212,11 +212,23 @@ def test_layers_of_few_rows(inputs, outputs, counts, dtype):
 @pytest.mark.parametrize("inputs,outputs", [(520, 264), (1024, 640), (96, 136), (2100, 300)])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_layers_of_many_rows(inputs, outputs, dtype):
-    """Enough work for the largest tiles; experts whose rows end anywhere in one."""
+    """Enough work for larger tiles; experts whose rows end anywhere in one."""
     say("many rows", inputs, outputs, dtype)
     counts = [450 + (37 * e) % 140 for e in range(60)]
     counts[7], counts[20], counts[59] = 0, 1, 3000
     check_linear(counts, inputs, outputs, dtype, outputs, 5)
+
+
+@gpu
+@pytest.mark.parametrize("inputs", [1, 40, 256, 257, 500, 512, 520, 768, 1030, 1536, 2100])
+@pytest.mark.parametrize("outputs", [1300, 1301])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_layers_of_the_largest_tiles(inputs, outputs, dtype):
+    """One tile of K and part of one, an odd and an even number of them; rows and outputs that end anywhere in one."""
+    say("largest tiles", inputs, outputs, dtype)
+    counts = [450 + (37 * e) % 140 for e in range(60)]
+    counts[7], counts[20], counts[59] = 0, 1, 3000
+    check_linear(counts, inputs, outputs, dtype, inputs + outputs, 5)
 
 
 @gpu
@@ -305,7 +317,7 @@ def test_nothing_beside_the_results_is_written(offsets, dtype, rows, inputs, out
     _lib.check(lib.qmlp_tokens_mx4_quantise(described(w), described(codes), described(scales), stream))
     values, y = margins.tensor(dtype, 4 * outputs, inputs), margins.tensor(dtype, rows, outputs)
     _lib.check(lib.qmlp_tokens_mx4_values(described(codes), described(scales), described(values), stream))
-    _lib.check(lib.qmlp_tokens_mx4_linear_memory(rows, inputs, ctypes.byref(size)))
+    _lib.check(lib.qmlp_tokens_mx4_linear_memory(rows, 4, inputs, outputs, ctypes.byref(size)))
     memory = margins.bytes(size.value)
     off = torch.tensor(offsets, dtype=torch.int32, device="cuda")
     _lib.check(lib.qmlp_tokens_mx4_linear(described(x), none, described(codes.view(4, outputs, -1)), described(scales.view(4, outputs, -1)), described(off), none,
@@ -451,8 +463,9 @@ def test_c_interface_refuses_before_any_launch():
     refused(lib.qmlp_tokens_mx4_values(codes, descriptor(B, 3, 2), x, None), "of one size")
     w, s, off, y = descriptor(B, 3, 5, 32), descriptor(B, 3, 5, 2), descriptor(I, 4), descriptor(F, 4, 5)
     linear = lambda *a: lib.qmlp_tokens_mx4_linear(*a)  # noqa: E731
-    refused(linear(x, none, w, s, off, none, y, None, None), "bytes of memory")
-    refused(linear(x, none, w, s, off, none, y, 264, None), "aligned")
+    many, ymany = descriptor(F, 400, 40), descriptor(F, 400, 5)
+    refused(linear(many, none, w, s, off, none, ymany, None, None), "bytes of memory")
+    refused(linear(many, none, w, s, off, none, ymany, 264, None), "aligned")
     refused(linear(x, none, w, s, none, none, y, 256, None), "one expert")
     refused(linear(descriptor(F, 4, 65), none, w, s, off, none, y, 256, None), "2 blocks")
     refused(linear(codes, scales, descriptor(B, 3, 5, 48), descriptor(B, 3, 5, 3), off, none, y, 256, None), "3 blocks")
@@ -461,7 +474,7 @@ def test_c_interface_refuses_before_any_launch():
     refused(linear(x, none, w, s, off, none, descriptor(F, 4, 5, strides=(4, 1)), 256, None), "share memory")
     refused(linear(x, none, descriptor(B, 3, 0, 32), descriptor(B, 3, 0, 2), off, none, descriptor(F, 4, 0), 256, None), "inputs and outputs")
     refused(linear(descriptor(F, 2 ** 31 - 1, 40, strides=(0, 1)), none, w, s, off, none, descriptor(F, 2 ** 31 - 1, 5), 256, None), "rows must not be more")
-    refused(lib.qmlp_tokens_mx4_linear_memory(-1, 4, ctypes.byref(ctypes.c_size_t())), "must not be negative")
+    refused(lib.qmlp_tokens_mx4_linear_memory(-1, 4, 4, 4, ctypes.byref(ctypes.c_size_t())), "must not be negative")
 
 
 def test_other_entry_points_refuse_bytes():
