@@ -66,59 +66,161 @@ __device__ __forceinline__ void loadLogits(const T* __restrict__ row, int first,
         for (int i = 0; i < ENTRIES; ++i) v[i] = first + i < experts ? static_cast<float>(row[first + i]) : -__builtin_inff();
 }
 
-/** G lanes per row, ENTRIES logits each. LDS: 8 bytes for every chosen expert of the workgroup's rows. */
+/**
+ * exp(d) for d <= 0, to 2 units of the last place: what the product with log2(e) loses comes back as the first term of its exponential. 0 below -200.
+ */
+__device__ __forceinline__ float routeExp(float d)
+{
+    constexpr float LOG2E = 1.44269502f, REST = 1.92596303e-8f, LN2 = 0.693147182f;   // log2(e) = LOG2E + REST
+    d = fmaxf(d, -200.0f);
+    const float t = d * LOG2E;
+    const float lost = __builtin_fmaf(d, REST, __builtin_fmaf(d, LOG2E, -t));
+    const float e = __builtin_amdgcn_exp2f(t);
+    return __builtin_fmaf(e, lost * LN2, e);
+}
+/** A row with a NaN or +inf has no weights. */
+__device__ __forceinline__ float routeTotal(float total, unsigned top) { return top < 0xff800000u ? total : __builtin_nanf(""); }
+
+/** Sorted with the largest first: Batcher's merge exchange, by instructions for the smaller and the larger of two. */
+template <int N>
+struct RouteSort
+{
+    template <int I, int J>
+    static __device__ __forceinline__ void exchange(unsigned (&k)[N])
+    {
+        const unsigned larger = max(k[I], k[J]);
+        k[J] = min(k[I], k[J]);
+        k[I] = larger;
+    }
+    /** Entries I, I + 2 R, ... before END, each with the one R behind it. */
+    template <int I, int R, int END>
+    static __device__ __forceinline__ void exchanges(unsigned (&k)[N])
+    {
+        if constexpr (I + R < END) {
+            exchange<I, I + R>(k);
+            exchanges<I + 2 * R, R, END>(k);
+        }
+    }
+    /** Entries FROM, FROM + R, ..., COUNT / R of them, whose halves are sorted. */
+    template <int FROM, int COUNT, int R>
+    static __device__ __forceinline__ void merge(unsigned (&k)[N])
+    {
+        if constexpr (2 * R < COUNT) {
+            merge<FROM, COUNT, 2 * R>(k);
+            merge<FROM + R, COUNT, 2 * R>(k);
+            exchanges<FROM + R, R, FROM + COUNT>(k);
+        } else
+            exchange<FROM, FROM + R>(k);
+    }
+    template <int FROM, int COUNT>
+    static __device__ __forceinline__ void sort(unsigned (&k)[N])
+    {
+        if constexpr (COUNT > 1) {
+            sort<FROM, COUNT / 2>(k);
+            sort<FROM + COUNT / 2, COUNT / 2>(k);
+            merge<FROM, COUNT, 1>(k);
+        }
+    }
+};
+
+/** The chosen experts of a row and their keys, by keys as they are: the lowest lane with the largest one has the first of equals. All lanes call it. */
+template <int G, int ENTRIES>
+__device__ __forceinline__ void chooseExactly(const float (&v)[ENTRIES], int chosen, unsigned* keys, int* indices)
+{
+    const int lane = threadIdx.x % G;
+    unsigned key[ENTRIES];
+#pragma unroll
+    for (int i = 0; i < ENTRIES; ++i) key[i] = routeKey(v[i]);
+    for (int j = 0; j < chosen; ++j) {
+        unsigned own = key[0];
+#pragma unroll
+        for (int i = 1; i < ENTRIES; ++i) own = max(own, key[i]);
+        const unsigned best = largestOfLanes<G>(own);
+        const unsigned long long have = __ballot(own == best) >> (threadIdx.x % 64 / G * G);
+        if (lane == __ffsll(have) - 1) {
+            int at = 0;
+#pragma unroll
+            for (int i = ENTRIES - 1; i >= 0; --i) at = key[i] == best ? i : at;
+#pragma unroll
+            for (int i = 0; i < ENTRIES; ++i) key[i] = i == at ? 0 : key[i];
+            keys[j] = best;
+            indices[j] = best > ROUTE_KEY_NONE ? lane * ENTRIES + at : -1;
+        }
+    }
+    waveLdsSync();
+}
+
+/**
+ * G lanes per row, ENTRIES logits each. The expert's number takes the place of the last bits of a key, so that a key is all that a lane has to sort and
+ * to pass on, and equal logits come in the order of their experts. Of 16-bit logits these bits are all the same; in single precision rows of which
+ * two that count differ in them alone are chosen from once more, by whole keys. LDS: 8 bytes for every chosen expert of the workgroup's rows.
+ */
 template <typename T, int G, int ENTRIES>
 __global__ void __launch_bounds__(ROUTE_THREADS)
 RouteKernel(const T* __restrict__ logits, long long strideLogits, T* __restrict__ weights, long long strideWeights, int* __restrict__ index,
             long long strideIndex, long long rows, int experts, int chosen, int normalised)
 {
     constexpr int ROWS = ROUTE_THREADS / G;
+    constexpr unsigned LAST = G * ENTRIES - 1;   // bits of an expert's number
+    static_assert(LAST < 1u << 13, "bits that are free in a key of a half");
     extern __shared__ unsigned routeLds[];
     const int lane = threadIdx.x % G;
     unsigned* const keys = routeLds + threadIdx.x / G * (2 * chosen);
     int* const indices = reinterpret_cast<int*>(keys + chosen);
     for (long long first = static_cast<long long>(blockIdx.x) * ROWS; first < rows; first += static_cast<long long>(gridDim.x) * ROWS) {
         const long long row = min(first + threadIdx.x / G, rows - 1);   // (lanes behind the last row do its work once more)
+        const T* const own = logits + row * strideLogits;
         float v[ENTRIES];
-        loadLogits(logits + row * strideLogits, lane * ENTRIES, experts, v);
-        unsigned key[ENTRIES];
+        loadLogits(own, lane * ENTRIES, experts, v);
+        unsigned key[ENTRIES], top = 0;
 #pragma unroll
-        for (int i = 0; i < ENTRIES; ++i) key[i] = routeKey(v[i]);
-        unsigned top = 0;
-        for (int j = 0; j < chosen; ++j) {
-            unsigned own = key[0];
-#pragma unroll
-            for (int i = 1; i < ENTRIES; ++i) own = max(own, key[i]);
-            const unsigned best = largestOfLanes<G>(own);
-            if (j == 0) top = best;
-            // (the lowest lane has the first of equals)
-            const unsigned long long have = __ballot(own == best) >> (threadIdx.x % 64 / G * G);
-            if (lane == __ffsll(have) - 1) {
-                int at = 0;
-#pragma unroll
-                for (int i = ENTRIES - 1; i >= 0; --i) at = key[i] == best ? i : at;
-#pragma unroll
-                for (int i = 0; i < ENTRIES; ++i) key[i] = i == at ? 0 : key[i];
-                keys[j] = best;
-                indices[j] = best > ROUTE_KEY_NONE ? lane * ENTRIES + at : -1;
-            }
+        for (int i = 0; i < ENTRIES; ++i) {
+            key[i] = routeKey(v[i]);
+            top = max(top, key[i]);
+            key[i] = (key[i] & ~LAST) | (LAST - (lane * ENTRIES + i));
         }
-        waveLdsSync();
+        top = largestOfLanes<G>(top);
         const bool any = top > ROUTE_KEY_NONE;
-        const float largest = routeValue(top);
+        const float largest = any ? routeValue(top) : 0.0f;
+        RouteSort<ENTRIES>::template sort<0, ENTRIES>(key);
+        unsigned before = 0;
+        bool close = false;
+        for (int j = 0; j < chosen; ++j) {
+            const unsigned best = largestOfLanes<G>(key[0]);
+            // (by bits: of a choice between entries the compiler makes one between their numbers)
+            const unsigned mine = key[0] == best ? ~0u : 0u;
+#pragma unroll
+            for (int i = 0; i + 1 < ENTRIES; ++i) key[i] = (mine & key[i + 1]) | (~mine & key[i]);
+            key[ENTRIES - 1] &= ~mine;
+            if (lane == 0) keys[j] = best;
+            if (sizeof(T) == 4) close |= (best ^ before) <= LAST && best > ROUTE_KEY_NONE;
+            before = best;
+        }
+        if (sizeof(T) == 4) close |= (largestOfLanes<G>(key[0]) ^ before) <= LAST && before > ROUTE_KEY_NONE;
+        waveLdsSync();
+        if (sizeof(T) == 4 && __ballot(close) != 0) chooseExactly<G>(v, chosen, keys, indices);
+        else
+            for (int j = lane; j < chosen; j += G) {
+                const unsigned k = keys[j];
+                const int e = k > ROUTE_KEY_NONE ? static_cast<int>(LAST - (k & LAST)) : -1;
+                indices[j] = e;
+                // (the logit itself, or the bits of it that there are)
+                if (sizeof(T) == 4) keys[j] = e >= 0 ? routeKey(static_cast<float>(own[e])) : k;
+                else keys[j] = k & 0x80000000u ? k & ~LAST : k | LAST;
+            }
         float total = 0;
         if (normalised) {
-            for (int j = lane; j < chosen; j += G) total += indices[j] >= 0 ? expf(routeValue(keys[j]) - largest) : 0.0f;
+            for (int j = lane; j < chosen; j += G) total += indices[j] >= 0 ? routeExp(routeValue(keys[j]) - largest) : 0.0f;
         } else {
 #pragma unroll
-            for (int i = 0; i < ENTRIES; ++i) total += any ? expf(v[i] - largest) : 0.0f;
+            for (int i = 0; i < ENTRIES; ++i) total += routeExp(v[i] - largest);
         }
-        total = totalOfLanes<G>(total);
+        total = routeTotal(totalOfLanes<G>(total), top);
         if (first + threadIdx.x / G < rows)
             for (int j = lane; j < chosen; j += G) {
                 const int e = indices[j];
                 index[row * strideIndex + j] = e;
-                weights[row * strideWeights + j] = static_cast<T>(e >= 0 ? expf(routeValue(keys[j]) - largest) / total : 0.0f);
+                weights[row * strideWeights + j] = static_cast<T>(e >= 0 ? routeExp(routeValue(keys[j]) - largest) / total : 0.0f);
             }
         waveLdsSync();
     }
@@ -146,14 +248,15 @@ RouteAdjointKernel(const T* __restrict__ logits, long long strideLogits, const i
 #pragma unroll
         for (int i = 0; i < ENTRIES; ++i) top = max(top, routeKey(v[i]));
         top = largestOfLanes<G>(top);
-        const float largest = routeValue(top);
+        const bool any = top > ROUTE_KEY_NONE;
+        const float largest = any ? routeValue(top) : 0.0f;
         float total = 0;
 #pragma unroll
         for (int i = 0; i < ENTRIES; ++i) {
-            v[i] = top > ROUTE_KEY_NONE ? expf(v[i] - largest) : 0.0f;
+            v[i] = routeExp(v[i] - largest);
             total += v[i];
-            own[from + i] = v[i];
         }
+        __builtin_memcpy(__builtin_assume_aligned(own + from, 16), v, sizeof(v));
         waveLdsSync();
         float taken = 0, inner = 0;
         const int* const indices = index + row * strideIndex;
@@ -164,11 +267,13 @@ RouteAdjointKernel(const T* __restrict__ logits, long long strideLogits, const i
             taken += own[e];
             inner += own[e] * static_cast<float>(gradients[j]);
         }
-        total = totalOfLanes<G>(normalised ? taken : total);
-        inner = totalOfLanes<G>(inner) / total;
+        const float share = 1.0f / routeTotal(totalOfLanes<G>(normalised ? taken : total), top);
+        inner = totalOfLanes<G>(inner) * share;
         waveLdsSync();
+        unsigned none[ENTRIES];
 #pragma unroll
-        for (int i = 0; i < ENTRIES; ++i) own[from + i] = __builtin_bit_cast(float, ROUTE_NOT_CHOSEN);
+        for (int i = 0; i < ENTRIES; ++i) none[i] = ROUTE_NOT_CHOSEN;
+        __builtin_memcpy(__builtin_assume_aligned(own + from, 16), none, sizeof(none));
         waveLdsSync();
         for (int j = lane; j < chosen; j += G) {
             const int e = indices[j];
@@ -177,13 +282,15 @@ RouteAdjointKernel(const T* __restrict__ logits, long long strideLogits, const i
         }
         waveLdsSync();
         float out[ENTRIES];
+        unsigned gradient[ENTRIES];
+        __builtin_memcpy(gradient, __builtin_assume_aligned(own + from, 16), sizeof(gradient));
 #pragma unroll
         for (int i = 0; i < ENTRIES; ++i) {
-            const unsigned bits = __builtin_bit_cast(unsigned, own[from + i]);
+            const unsigned bits = gradient[i];
             const bool held = bits != ROUTE_NOT_CHOSEN;
             const float g = held ? __builtin_bit_cast(float, bits) : 0.0f;
             // (rows without experts have no total)
-            out[i] = top > ROUTE_KEY_NONE && (held || !normalised) ? v[i] / total * (g - inner) : 0.0f;
+            out[i] = any && (held || !normalised) ? v[i] * share * (g - inner) : 0.0f;
         }
         if (first + threadIdx.x / G < rows) {
             T* const to = adjLogits + row * strideAdjLogits + from;
