@@ -470,9 +470,9 @@ __device__ __forceinline__ void mx4Stage(const X* __restrict__ x, const unsigned
             __builtin_memcpy(__builtin_assume_aligned(toCodes, 16), &codes, 16);
             *toScale = static_cast<char>(scale);
         } else {
-            const int lane = threadIdx.x % MX4_LANES, at = b * MX4_BLOCK + lane * MX4_ENTRIES;
+            const int lane = threadIdx.x % LANES;
             float v[MX4_ENTRIES];
-            mx4Load(x + row * strideX, at, inputs, v);
+            mx4Load(x + row * strideX, b * MX4_BLOCK + lane * MX4_ENTRIES, inputs, v);
             unsigned scale;
             const unsigned packed = mx4Pack(v, scale);
             __builtin_memcpy(__builtin_assume_aligned(toCodes + lane * 4, 4), &packed, 4);

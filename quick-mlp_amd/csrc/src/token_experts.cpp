@@ -164,7 +164,7 @@ Mx4Plan mx4Plan(Tensor::Precision p, int64_t rows, int64_t experts, int64_t J, i
 }
 
 int mx4Blocks(int64_t columns) { return static_cast<int>(divUp<int64_t>(columns, MX4_BLOCK)); }
-unsigned mx4Workgroups(long long units) { return workgroups(divUp<int64_t>(units * MX4_LANES, MX4_THREADS), 1 << 16); }
+unsigned mx4Workgroups(long long units, int lanes) { return workgroups(divUp<int64_t>(units * lanes, MX4_THREADS), 1 << 16); }
 
 void launchQuantise(const Tensor& input, unsigned char* codes, long long strideCodes, unsigned char* scales, long long strideScales, stream_t stream)
 {
@@ -173,7 +173,7 @@ void launchQuantise(const Tensor& input, unsigned char* codes, long long strideC
     if (units == 0) return;
     const Tensor::Precision p = input.precision();
     tokenKernel("mx4.h", kernelKey(MX4_QUANTISE, p), [&] { return str("Mx4QuantiseKernel<", scalarName(p), ">"); })
-        .call(mx4Workgroups(units), MX4_THREADS, 0, stream, input.rawPtr(), strideOf(input, 0), codes, strideCodes, scales, strideScales, units, blocks,
+        .call(mx4Workgroups(units, MX4_LANES), MX4_THREADS, 0, stream, input.rawPtr(), strideOf(input, 0), codes, strideCodes, scales, strideScales, units, blocks,
               static_cast<int>(input.size(1)));
 }
 
@@ -312,7 +312,7 @@ void Tokens::valuesMx4(const Tensor& codes, const Tensor& scales, Tensor& output
     if (units == 0) return;
     const Tensor::Precision p = output.precision();
     tokenKernel("mx4.h", kernelKey(MX4_VALUES, p), [&] { return str("Mx4ValuesKernel<", scalarName(p), ">"); })
-        .call(mx4Workgroups(units), MX4_THREADS, 0, stream, static_cast<const unsigned char*>(ptr<unsigned char>(codes)), strideOf(codes, 0),
+        .call(mx4Workgroups(units, MX4_BLOCK / wide(p)), MX4_THREADS, 0, stream, static_cast<const unsigned char*>(ptr<unsigned char>(codes)), strideOf(codes, 0),
               static_cast<const unsigned char*>(ptr<unsigned char>(scales)), strideOf(scales, 0), output.rawPtr(), strideOf(output, 0), units, blocks,
               static_cast<int>(output.size(1)));
 }
