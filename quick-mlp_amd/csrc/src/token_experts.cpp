@@ -59,6 +59,12 @@ struct ExpertRowsSizes
     /** Entries of an access and lanes of a token. */
     int vec(Tensor::Precision p) const { return channels < wide(p) ? 1 : wide(p); }
     int lanes(Tensor::Precision p, int most) const { return lanesPerRow(channels, vec(p), most); }
+    /** Workgroups that share the columns of their tokens: as many as have some, where there are few tokens. */
+    int parts(Tensor::Precision p, int lanes) const
+    {
+        const int64_t all = divUp<int64_t>(channels, lanes * vec(p)), blocks = divUp<int64_t>(tokens, EXPERT_ROWS_THREADS / lanes);
+        return static_cast<int>(blocks * all <= 2048 ? all : 1);
+    }
 };
 ExpertRowsSizes checkExpertRows(const Tensor& rows, const Tensor& places)
 {
@@ -88,6 +94,9 @@ void checkExpertWeights(const Tensor& t, const char* what, const Tensor& rows, c
     checkSizes(t, what, {s.tokens, s.chosen});
 }
 long long strideOrNone(const Tensor& t) { return t.defined() ? strideOf(t, 0) : 0; }
+
+/** Pieces of a row that a lane of the adjoint kernel has at a time. */
+int expertRowsBatch(int channels, int vec, int lanes) { return channels <= vec * lanes ? 1 : 4; }
 
 /** Values are moved as they are: a name of a type of their size. */
 const char* bitsName(Tensor::Precision p) { return p == Tensor::FLOAT ? "unsigned" : "unsigned short"; }
@@ -237,11 +246,12 @@ void Tokens::dispatch(const Tensor& input, const Tensor& places, Tensor& rows, s
     checkOutput(rows, "rows");
     if (rows.numel() == 0) return;
     const Tensor::Precision p = rows.precision();
-    const int vec = s.vec(p), lanes = s.lanes(p, EXPERT_ROWS_THREADS);
+    const int vec = s.vec(p), lanes = s.lanes(p, EXPERT_ROWS_THREADS), parts = s.parts(p, lanes);
     tokenKernel("expert_rows.h", kernelKey(DISPATCH, rows.bytesPerEntry(), vec, lanes),
                 [&] { return str("DispatchKernel<", bitsName(p), ", ", vec, ", ", lanes, ">"); })
-        .call(workgroups(divUp<int64_t>(s.tokens, EXPERT_ROWS_THREADS / lanes), 1 << 20), EXPERT_ROWS_THREADS, 0, stream, input.rawPtr(), strideOf(input, 0),
-              static_cast<const int*>(ptr<int>(places)), strideOf(places, 0), s.chosen, rows.rawPtr(), strideOf(rows, 0), s.tokens, s.channels);
+        .call(workgroups(divUp<int64_t>(s.tokens, EXPERT_ROWS_THREADS / lanes), 1 << 20) * parts, EXPERT_ROWS_THREADS, 0, stream, input.rawPtr(),
+              strideOf(input, 0), static_cast<const int*>(ptr<int>(places)), strideOf(places, 0), s.chosen, rows.rawPtr(), strideOf(rows, 0), s.tokens, s.channels,
+              parts);
 }
 
 void Tokens::combine(const Tensor& rows, const Tensor& places, const Tensor& weights, const Tensor& residual, Tensor& output, stream_t stream)
@@ -253,12 +263,12 @@ void Tokens::combine(const Tensor& rows, const Tensor& places, const Tensor& wei
     checkOutput(output, "output");
     if (output.numel() == 0) return;
     const Tensor::Precision p = rows.precision();
-    const int vec = s.vec(p), lanes = s.lanes(p, EXPERT_ROWS_THREADS);
+    const int vec = s.vec(p), lanes = s.lanes(p, EXPERT_ROWS_THREADS), parts = s.parts(p, lanes);
     tokenKernel("expert_rows.h", kernelKey(COMBINE, p, vec, lanes), [&] { return str("CombineKernel<", scalarName(p), ", ", vec, ", ", lanes, ">"); })
-        .call(workgroups(divUp<int64_t>(s.tokens, EXPERT_ROWS_THREADS / lanes), 1 << 20), EXPERT_ROWS_THREADS, 0, stream, rows.rawPtr(), strideOf(rows, 0),
-              static_cast<const int*>(ptr<int>(places)), strideOf(places, 0), s.chosen, static_cast<const void*>(ptr<void>(weights)), strideOrNone(weights),
-              static_cast<int>(weights.defined() && weights.precision() == Tensor::FLOAT), static_cast<const void*>(ptr<void>(residual)),
-              strideOrNone(residual), output.rawPtr(), strideOf(output, 0), s.tokens, s.channels);
+        .call(workgroups(divUp<int64_t>(s.tokens, EXPERT_ROWS_THREADS / lanes), 1 << 20) * parts, EXPERT_ROWS_THREADS, 0, stream, rows.rawPtr(),
+              strideOf(rows, 0), static_cast<const int*>(ptr<int>(places)), strideOf(places, 0), s.chosen, static_cast<const void*>(ptr<void>(weights)),
+              strideOrNone(weights), static_cast<int>(weights.defined() && weights.precision() == Tensor::FLOAT),
+              static_cast<const void*>(ptr<void>(residual)), strideOrNone(residual), output.rawPtr(), strideOf(output, 0), s.tokens, s.channels, parts);
 }
 
 void Tokens::combineAdjoint(const Tensor& rows, const Tensor& places, const Tensor& weights, const Tensor& adjOutput, Tensor& adjRows, Tensor& adjWeights,
@@ -280,12 +290,14 @@ void Tokens::combineAdjoint(const Tensor& rows, const Tensor& places, const Tens
     const Tensor::Precision p = rows.precision();
     const int vec = s.vec(p), lanes = s.lanes(p, 64);
     const Tensor& typed = weights.defined() ? weights : adjWeights;
-    tokenKernel("expert_rows.h", kernelKey(COMBINE_ADJOINT, p, vec, lanes),
-                [&] { return str("CombineAdjointKernel<", scalarName(p), ", ", vec, ", ", lanes, ">"); })
-        .call(workgroups(divUp<int64_t>(s.tokens, EXPERT_ROWS_THREADS / lanes), 1 << 20), EXPERT_ROWS_THREADS, 0, stream, rows.rawPtr(), strideOf(rows, 0),
+    const int batch = expertRowsBatch(s.channels, vec, lanes);
+    const int split = s.tokens <= 4096 ? s.chosen : 1;   // (fewer than 4 wavefronts per SIMD otherwise)
+    tokenKernel("expert_rows.h", kernelKey(COMBINE_ADJOINT, p, vec, lanes, batch),
+                [&] { return str("CombineAdjointKernel<", scalarName(p), ", ", vec, ", ", lanes, ", ", batch, ">"); })
+        .call(workgroups(divUp<int64_t>(s.tokens * split, EXPERT_ROWS_THREADS / lanes), 1 << 20), EXPERT_ROWS_THREADS, 0, stream, rows.rawPtr(), strideOf(rows, 0),
               static_cast<const int*>(ptr<int>(places)), strideOf(places, 0), s.chosen, static_cast<const void*>(ptr<void>(weights)), strideOrNone(weights),
               static_cast<int>(typed.defined() && typed.precision() == Tensor::FLOAT), adjOutput.rawPtr(), strideOf(adjOutput, 0), ptr<void>(adjRows),
-              strideOrNone(adjRows), ptr<void>(adjWeights), strideOrNone(adjWeights), s.tokens, s.channels);
+              strideOrNone(adjRows), ptr<void>(adjWeights), strideOrNone(adjWeights), s.tokens, s.channels, split);
 }
 
 void Tokens::quantiseMx4(const Tensor& input, Tensor& codes, Tensor& scales, stream_t stream)
@@ -412,7 +424,9 @@ void token::precompileExperts(Tensor::Precision p)
             const std::string shape = str(", ", vec, ", ", lanes, ">");
             precompileKernel("expert_rows.h", str("DispatchKernel<", bitsName(p), shape));
             precompileKernel("expert_rows.h", str("CombineKernel<", t, shape));
-            if (lanes <= 64) precompileKernel("expert_rows.h", str("CombineAdjointKernel<", t, shape));
+            for (const int batch : {1, 4})
+                if (lanes < 64 ? batch == 1 : lanes == 64)
+                    precompileKernel("expert_rows.h", str("CombineAdjointKernel<", t, ", ", vec, ", ", lanes, ", ", batch, ">"));
         }
     for (const char* kernel : {"Mx4QuantiseKernel", "Mx4ValuesKernel"}) precompileKernel("mx4.h", str(kernel, "<", t, ">"));
     for (const bool inPlace : {false, true})
