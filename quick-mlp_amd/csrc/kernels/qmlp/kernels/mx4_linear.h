@@ -255,13 +255,9 @@ struct Mx4Product
 #pragma unroll
             for (int j = 0; j < NJ; ++j) sums[i][j] = f32x16{};
     }
-    /** LDS: two tiles of each operand, two pairs of tiles' scales. */
+    /** LDS: two tiles of each operand, two pairs of tiles' scales. blocks > 0. */
     __device__ __forceinline__ void run(char* lds, const Source<Byte>& a, const Source<Byte>& b, Scales& scales, int blocks)
     {
-        if (blocks <= 0) {
-            clear();
-            return;
-        }
         LoadsA tileA;
         LoadsB tileB;
         constexpr int LOADS = LoadsA::EACH + LoadsB::EACH, PRODUCTS = NI * NJ;
@@ -432,15 +428,18 @@ Mx4TilesKernel(const unsigned char* __restrict__ x, const unsigned char* __restr
     if (at.to <= at.from) return;
     const int j0 = work.tile * TJ;
     const int ni = at.to - at.from, nj = min(J - j0, TJ);
-    const bool none = at.expert >= experts;
+    const bool none = at.expert >= experts;   // (then there may be no weights at all)
     const long long expert = none ? 0 : at.expert;
     Product product;
-    const Source<unsigned char> a = {x + at.from * strideX, strideX, ni, rows - at.from};
-    const Source<unsigned char> b = {weights.codes + expert * weights.codesExpert + j0 * weights.codesRow, weights.codesRow, nj, J - j0};
-    typename Product::Scales scales;
-    scales.begin(scalesX + at.from * strideScalesX, strideScalesX, ni, weights.scales + expert * weights.scalesExpert + j0 * weights.scalesRow,
-                 weights.scalesRow, nj, blocks);
-    product.run(groupedLds, a, b, scales, none ? 0 : blocks);
+    if (none) product.clear();
+    else {
+        const Source<unsigned char> a = {x + at.from * strideX, strideX, ni, rows - at.from};
+        const Source<unsigned char> b = {weights.codes + expert * weights.codesExpert + j0 * weights.codesRow, weights.codesRow, nj, J - j0};
+        typename Product::Scales scales;
+        scales.begin(scalesX + at.from * strideScalesX, strideScalesX, ni, weights.scales + expert * weights.scalesExpert + j0 * weights.scalesRow,
+                     weights.scalesRow, nj, blocks);
+        product.run(groupedLds, a, b, scales, blocks);
+    }
     mx4Store(product, groupedLds, bias && !none ? bias + expert * strideBias + j0 : nullptr, y + at.from * strideY + j0, strideY, ni, nj);
 }
 

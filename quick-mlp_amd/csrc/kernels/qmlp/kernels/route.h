@@ -329,10 +329,10 @@ __device__ __forceinline__ float totalOfGroup(float v, float* lds)
     return v;
 }
 
-/** A key and, below it, the expert: of equal keys the first is the largest. */
+/** A key and, below it, the expert: of equal keys the first is the largest. Less than 2^64 - 1. */
 __device__ __forceinline__ unsigned long long routePair(float v, int expert)
 {
-    return static_cast<unsigned long long>(routeKey(v)) << 32 | (0xffffffffu - static_cast<unsigned>(expert));
+    return static_cast<unsigned long long>(routeKey(v)) << 32 | (0xfffffffeu - static_cast<unsigned>(expert));
 }
 
 /** A workgroup per row, which is read once more for every chosen expert: the largest pair below the one before. */
@@ -347,7 +347,7 @@ RouteLongKernel(const T* __restrict__ logits, long long strideLogits, T* __restr
     int* const indices = reinterpret_cast<int*>(routeLds + chosen);
     for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
         const T* const own = logits + row * strideLogits;
-        unsigned long long last = ~0ull;   // (above every pair: the last expert's number is not 2^32 - 1)
+        unsigned long long last = ~0ull;   // (above every pair)
         float largest = 0;
         bool any = false;
         for (int j = 0; j < chosen; ++j) {
@@ -364,7 +364,7 @@ RouteLongKernel(const T* __restrict__ logits, long long strideLogits, T* __restr
             }
             if (threadIdx.x == 0) {
                 routeLds[j] = key;
-                indices[j] = key > ROUTE_KEY_NONE ? static_cast<int>(0xffffffffu - static_cast<unsigned>(last)) : -1;
+                indices[j] = key > ROUTE_KEY_NONE ? static_cast<int>(0xfffffffeu - static_cast<unsigned>(last)) : -1;
             }
         }
         float total = 0;

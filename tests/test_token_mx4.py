@@ -239,6 +239,20 @@ def test_numbers_of_experts(experts):
 
 
 @gpu
+@pytest.mark.parametrize("rows,outputs", [(5, 40), (70, 40), (3000, 300), (33000, 1030)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_of_no_expert_are_zeros(rows, outputs, dtype):
+    """Without any expert, and behind the last one's rows: no weights are read for them."""
+    weight = tokens.Mx4(torch.zeros(0, outputs, 32, dtype=torch.uint8, device="cuda"), torch.zeros(0, outputs, 2, dtype=torch.uint8, device="cuda"), 60)
+    x = torch.ones(rows, 60, dtype=dtype, device="cuda")
+    assert not bool(tokens.mx4_linear(x, weight, offsets_of([])).any())
+    weight = tokens.Mx4(torch.full((2, outputs, 32), 0x22, dtype=torch.uint8, device="cuda"), torch.full((2, outputs, 2), 127, dtype=torch.uint8, device="cuda"), 60)
+    bias = torch.ones(2, outputs, dtype=dtype, device="cuda")
+    y = tokens.mx4_linear(x, weight, offsets_of([0, rows // 3]), bias)
+    assert bool((y[:rows // 3] == 61).all()) and not bool(y[rows // 3:].any())
+
+
+@gpu
 @pytest.mark.parametrize("rows", [1, 15, 16, 17, 300, 3000])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_one_layer_needs_no_offsets(rows, dtype):
