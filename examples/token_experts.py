@@ -1,9 +1,9 @@
 """A field per object, learned with the operators on tokens in front of a coordinate network.
 
 Every object has a token. Its learned code (embedding) is normalised (layer norm) and refined by experts: a router picks two of
-them per token, the tokens are sorted by expert (group), gathered (embedding once more, with the tokens' rows as the table) and
-go through the experts' linear layers, with one of the framework's activations in between. A fused coordinate network decodes the
-code and a position to the value of the field there.
+them per token (route), the tokens are sorted by expert (group), go to their places there (dispatch), through the experts' linear
+layers, with one of the framework's activations in between, and back (combine). A fused coordinate network decodes the code and a
+position to the value of the field there. Once trained, the experts are served with weights of 4 bits.
 
     python examples/token_experts.py [steps]
 """
@@ -23,7 +23,7 @@ class Experts(torch.nn.Module):
 
     def __init__(self, experts, channels, hidden, chosen=2):
         super().__init__()
-        self.chosen = chosen
+        self.count, self.chosen = experts, chosen
         self.norm = qmlp.FusedLayerNorm(channels)
         self.router = torch.nn.Linear(channels, experts, bias=False, device="cuda")
         self.first = qmlp.FusedGroupedLinear(experts, channels, hidden)
@@ -32,15 +32,16 @@ class Experts(torch.nn.Module):
 
     def forward(self, x):
         normal = self.norm(x)
-        weights, experts = torch.softmax(self.router(normal), 1).topk(self.chosen, 1)
-        # the rows (token, choice) by expert, and where each of them went
-        order, offsets = tokens.group(experts.flatten(), self.first.weight.shape[0])
-        places = torch.empty_like(order)
-        places[order.long()] = torch.arange(len(order), dtype=order.dtype, device=order.device)
-        rows = tokens.embedding(order // self.chosen, normal.half())
-        rows = self.second(self.activation(self.first(rows, offsets)), offsets)   # in 16 bits, as the activation works
-        back = tokens.embedding(places.view(len(x), self.chosen), rows)
-        return x + (back * weights[..., None]).sum(1)
+        weights, experts = tokens.route(self.router(normal), self.chosen)
+        # the rows (token, choice) by expert, and where each of them goes
+        _, offsets, places = tokens.group(experts, self.count, places=True)
+        rows = tokens.dispatch(normal.half(), places)   # in 16 bits, as the activation works
+        rows = self.second(self.activation(self.first(rows, offsets)), offsets)
+        return tokens.combine(rows.to(x.dtype), places, weights, x)
+
+    def quantise(self):
+        """For serving: the experts' weights in 4 bits."""
+        self.first, self.second = (qmlp.FusedMx4GroupedLinear(layer) for layer in (self.first, self.second))
 
 
 class ObjectFields(torch.nn.Module):
@@ -64,17 +65,24 @@ class ObjectFields(torch.nn.Module):
         return self.decoder(inputs.reshape(-1, inputs.shape[2])).view(positions.shape[:2])
 
 
-def train(steps=300, objects=500, batch=256, points=64, seed=0):
-    """Fits balls of different places and sizes (signed distances); returns the losses."""
-    torch.manual_seed(seed)
-    centres, radii = torch.rand(objects, 3, device="cuda"), 0.1 + 0.3 * torch.rand(objects, device="cuda")
-    model = ObjectFields(objects)
+def balls(objects):
+    """Centres and radii."""
+    return torch.rand(objects, 3, device="cuda"), 0.1 + 0.3 * torch.rand(objects, device="cuda")
+
+
+def batch_of(centres, radii, batch, points):
+    """Objects, positions and the signed distances there."""
+    index = torch.randint(0, len(radii), (batch,), device="cuda")
+    positions = torch.rand(batch, points, 3, device="cuda")
+    return index, positions, (positions - centres[index][:, None]).norm(dim=2) - radii[index][:, None]
+
+
+def fit(model, centres, radii, steps, batch=256, points=64):
+    """Returns the losses."""
     optimizer = torch.optim.Adam(model.parameters(), lr=1e-2)
     losses = []
     for _ in range(steps):
-        index = torch.randint(0, objects, (batch,), device="cuda")
-        positions = torch.rand(batch, points, 3, device="cuda")
-        target = (positions - centres[index][:, None]).norm(dim=2) - radii[index][:, None]
+        index, positions, target = batch_of(centres, radii, batch, points)
         loss = (model(index, positions) - target).square().mean()
         optimizer.zero_grad(set_to_none=True)
         loss.backward()
@@ -83,8 +91,24 @@ def train(steps=300, objects=500, batch=256, points=64, seed=0):
     return torch.stack(losses).tolist()
 
 
+def train(steps=300, objects=500, batch=256, points=64, seed=0):
+    """Fits balls of different places and sizes (signed distances); returns the losses."""
+    torch.manual_seed(seed)
+    shapes = balls(objects)
+    return fit(ObjectFields(objects), *shapes, steps, batch, points)
+
+
 if __name__ == "__main__":
-    history = train(int(sys.argv[1]) if len(sys.argv) > 1 else 300)
+    torch.manual_seed(0)
+    shapes = balls(500)
+    model = ObjectFields(500)
+    history = fit(model, *shapes, int(sys.argv[1]) if len(sys.argv) > 1 else 300)
     for step in range(0, len(history), max(1, len(history) // 10)):
         print("step %4d: mean squared error %.5f" % (step, history[step]))
     print("step %4d: mean squared error %.5f" % (len(history) - 1, history[-1]))
+    with torch.no_grad():
+        index, positions, target = batch_of(*shapes, 500, 256)
+        for name in ("as they are", "in 4 bits"):
+            if name == "in 4 bits":
+                model.experts.quantise()
+            print("experts' weights %s: %.5f" % (name, (model(index, positions) - target).square().mean()))

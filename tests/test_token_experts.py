@@ -3,6 +3,8 @@
 Tolerances: sums of n terms in 32 bits are off by at most n 2^-23 of the sum of their magnitudes, a result is rounded once to its type.
 """
 import ctypes
+import importlib.util
+import os
 
 import numpy as np
 import pytest
@@ -514,6 +516,49 @@ def test_an_index_that_was_changed_has_no_gradient():
     index.add_(1)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         weights.sum().backward()
+
+
+@gpu
+def test_no_kernel_is_compiled_late():
+    """Calls of every kind of size find their kernels where qmlp.tokens.precompile left them."""
+    g = generator(70)
+    before = _lib.kernel_cache_stats()[0]
+    for dtype in DTYPES:
+        for experts in (3, 40, 100, 200, 500, 900, 2000):
+            logits = normal(g, 9, experts, dtype=dtype).requires_grad_()
+            weights, index = tokens.route(logits, 2)
+            weights.sum().backward()
+        places = tokens.group(index, 2000, places=True)[2]
+        for channels in (1, 5, 20, 70, 150, 300, 600, 3000):
+            x = normal(g, 9, channels, dtype=dtype).requires_grad_()
+            tokens.combine(tokens.dispatch(x, places), places, weights.detach().requires_grad_(), x).sum().backward()
+    assert _lib.kernel_cache_stats()[0] == before
+
+
+@gpu
+def test_example_serves_numbers_of_four_bits():
+    """Trained for a few steps, then with the experts' weights in 4 bits: it runs, and refuses to be trained."""
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "token_experts.py")
+    spec = importlib.util.spec_from_file_location("token_experts", path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    torch.manual_seed(1)
+    shapes = module.balls(20)
+    model = module.ObjectFields(20)
+    module.fit(model, *shapes, 3, batch=8, points=16)
+    assert all(p.grad is not None and bool(p.grad.isfinite().all()) for p in model.experts.parameters())
+    x = torch.randn(30, 32, device="cuda")
+    layer = model.experts
+    weights = [tokens.quantise_mx4(l.weight.detach()).dequantise() for l in (layer.first, layer.second)]
+    layer.quantise()
+    with torch.no_grad():
+        assert bool(layer(x).isfinite().all())
+        index, positions, _ = module.batch_of(*shapes, 8, 16)
+        assert bool(model(index, positions).isfinite().all())
+        for l, w in zip((layer.first, layer.second), weights):
+            assert torch.equal(tokens.Mx4(l.codes, l.scales, l.inputs).dequantise(), w)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        layer(x)
 
 
 # ------------------------------------------------------------------------------------------------ refusals

@@ -417,6 +417,22 @@ def test_calls_run_on_the_current_stream_and_can_be_captured():
 
 
 @gpu
+def test_no_kernel_is_compiled_late():
+    """Calls of every kind of size find their kernels where qmlp.tokens.precompile left them."""
+    g = generator(71)
+    before = _lib.kernel_cache_stats()[0]
+    for dtype in DTYPES:
+        for rows, experts, inputs, outputs in ((4, 8, 100, 100), (4, 1, 4096, 64), (16, 1, 4096, 512), (1, 300, 64, 1024), (300, 2, 64, 64), (9000, 2, 64, 256),
+                                               (33000, 2, 64, 1030)):
+            x, weight = normal(g, rows, inputs, dtype=dtype), tokens.quantise_mx4(normal(g, experts, outputs, inputs))
+            offsets = offsets_of([rows] + [0] * (experts - 1))
+            for values in (x, tokens.quantise_mx4(x)):
+                tokens.mx4_linear(values, weight, offsets, None, dtype)
+            tokens.quantise_mx4(x).dequantise(dtype)
+    assert _lib.kernel_cache_stats()[0] == before
+
+
+@gpu
 def test_module_keeps_its_numbers():
     first, _ = layers(3)
     state = first.state_dict()
