@@ -118,17 +118,17 @@ struct Mx4Scales
         }
         next = 16;
 #pragma unroll
-            for (int n = 0; n < EACH; ++n)
+        for (int n = 0; n < EACH; ++n)
 #pragma unroll
-                for (int d = 0; d < 4; ++d) {
-                    unsigned v = ONES;
-                    if (blocks >= 4 * d + 4) __builtin_memcpy(&v, p[n] + 4 * d, 4);
-                    else
+            for (int d = 0; d < 4; ++d) {
+                unsigned v = ONES;
+                if (blocks >= 4 * d + 4) __builtin_memcpy(&v, p[n] + 4 * d, 4);
+                else
 #pragma unroll
-                        for (int k = 0; k < 3; ++k)
-                            if (4 * d + k < blocks) v = (v & ~(0xffu << (8 * k))) | static_cast<unsigned>(p[n][4 * d + k]) << (8 * k);
-                    raw[n][d] = v;
-                }
+                    for (int k = 0; k < 3; ++k)
+                        if (4 * d + k < blocks) v = (v & ~(0xffu << (8 * k))) | static_cast<unsigned>(p[n][4 * d + k]) << (8 * k);
+                raw[n][d] = v;
+            }
     }
     /** Asks for the next pair, if there is one; for the last one with blocks before it. */
     __device__ __forceinline__ void ask()
