@@ -59,7 +59,10 @@ struct ExpertRowsSizes
     /** Entries of an access and lanes of a token. */
     int vec(Tensor::Precision p) const { return channels < wide(p) ? 1 : wide(p); }
     int lanes(Tensor::Precision p, int most) const { return lanesPerRow(channels, vec(p), most); }
-    /** Workgroups that share the columns of their tokens: as many as have some, where there are few tokens. */
+    /**
+     * Workgroups that share the columns of their tokens: as many as have some, where there are few tokens. us of dispatch() by one | by several, 4096
+     * channels, bfloat16: 24 tokens of 8 experts 6.1 | 4.1, 256 of 4 4.6 | 3.7, 1024 of 4 7.8 | 7.4, 4096 of 4 25.5 | 25.8.
+     */
     int parts(Tensor::Precision p, int lanes) const
     {
         const int64_t all = divUp<int64_t>(channels, lanes * vec(p)), blocks = divUp<int64_t>(tokens, EXPERT_ROWS_THREADS / lanes);
@@ -95,8 +98,19 @@ void checkExpertWeights(const Tensor& t, const char* what, const Tensor& rows, c
 }
 long long strideOrNone(const Tensor& t) { return t.defined() ? strideOf(t, 0) : 0; }
 
-/** Pieces of a row that a lane of the adjoint kernel has at a time. */
-int expertRowsBatch(int channels, int vec, int lanes) { return channels <= vec * lanes ? 1 : 4; }
+/**
+ * Pieces of a row that a lane of the adjoint kernel has at a time, and the wavefronts that share the rows of a token (all of them or one). us of one
+ * and one piece | one, 4 | all, 1 | all, 4: bfloat16, 24 tokens of 8 experts, 4096 channels 31 | 27 | 6.5 | 5.8; 2048, 8, 512 11.4 | 12.3 | 8.7 |
+ * 12.7; 4096, 8, 512 14.7 | 15.8 | 15.6 | 22; 16384, 8, 512 45 | 55 | 53 | 79; 16384, 4, 768 39 | 41 | 38 | 54; 4096, 8, 1024 23.9 | 24.2 | 24.6 |
+ * 30; 16384, 8, 1024 110 | 122 | 98 | 159; 32768, 2, 2048 134 | 130 | 122 | 143; 8192, 4, 4096 133 | 130 | 109 | 107. Single precision, 1024, 4,
+ * 1024 13.8 | 10.0 | 6.8 | 6.9; 4096, 4, 1024 29 | 23.7 | 25 | 23.8; 5003, 3, 333 11.7 | 10.5 | 11.9 | 11.8; 8192, 8, 1024 121 | 106 | 107 | 105;
+ * 16384, 8, 512 114 | 103 | 105 | 116.
+ */
+int expertRowsBatch(Tensor::Precision p, int channels, int vec, int lanes) { return p == Tensor::FLOAT && channels > vec * lanes ? 4 : 1; }
+int expertRowsSplit(Tensor::Precision p, const ExpertRowsSizes& s, int vec, int lanes)
+{
+    return s.tokens <= 2048 || (p != Tensor::FLOAT && s.channels >= 2 * vec * lanes) ? s.chosen : 1;
+}
 
 /** Values are moved as they are: a name of a type of their size. */
 const char* bitsName(Tensor::Precision p) { return p == Tensor::FLOAT ? "unsigned" : "unsigned short"; }
@@ -290,8 +304,7 @@ void Tokens::combineAdjoint(const Tensor& rows, const Tensor& places, const Tens
     const Tensor::Precision p = rows.precision();
     const int vec = s.vec(p), lanes = s.lanes(p, 64);
     const Tensor& typed = weights.defined() ? weights : adjWeights;
-    const int batch = expertRowsBatch(s.channels, vec, lanes);
-    const int split = s.tokens <= 4096 ? s.chosen : 1;   // (fewer than 4 wavefronts per SIMD otherwise)
+    const int batch = expertRowsBatch(p, s.channels, vec, lanes), split = expertRowsSplit(p, s, vec, lanes);
     tokenKernel("expert_rows.h", kernelKey(COMBINE_ADJOINT, p, vec, lanes, batch),
                 [&] { return str("CombineAdjointKernel<", scalarName(p), ", ", vec, ", ", lanes, ", ", batch, ">"); })
         .call(workgroups(divUp<int64_t>(s.tokens * split, EXPERT_ROWS_THREADS / lanes), 1 << 20), EXPERT_ROWS_THREADS, 0, stream, rows.rawPtr(), strideOf(rows, 0),
@@ -425,7 +438,7 @@ void token::precompileExperts(Tensor::Precision p)
             precompileKernel("expert_rows.h", str("DispatchKernel<", bitsName(p), shape));
             precompileKernel("expert_rows.h", str("CombineKernel<", t, shape));
             for (const int batch : {1, 4})
-                if (lanes < 64 ? batch == 1 : lanes == 64)
+                if (batch == 1 ? lanes <= 64 : lanes == 64 && p == Tensor::FLOAT)
                     precompileKernel("expert_rows.h", str("CombineAdjointKernel<", t, ", ", vec, ", ", lanes, ", ", batch, ">"));
         }
     for (const char* kernel : {"Mx4QuantiseKernel", "Mx4ValuesKernel"}) precompileKernel("mx4.h", str(kernel, "<", t, ">"));

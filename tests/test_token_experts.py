@@ -252,6 +252,15 @@ def test_rows_to_experts_and_back(tokens_, chosen, channels, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("channels", [40, 520, 1023, 1024, 1032])
+@pytest.mark.parametrize("tokens_", [2048, 2049])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_of_tokens_that_are_shared_out_and_not(tokens_, channels, dtype):
+    """Tokens and channels at which wavefronts begin to share the rows of a token, or to take them one after the other."""
+    test_rows_to_experts_and_back(tokens_, 3, channels, dtype)
+
+
+@gpu
 def test_rows_of_other_shapes_and_strides():
     g = generator(5)
     wide = normal(g, 6, 7, 90)
