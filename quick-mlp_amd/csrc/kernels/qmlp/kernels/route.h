@@ -7,8 +7,8 @@
 //
 // A row lies in the registers of 8 to 64 lanes, so that reading it is one access each, and every lane sorts what it has. What bounds the forward pass
 // then is the choice, one after the other: the largest of the lanes' first keys by operations between neighbouring lanes, and a step of the list
-// it came from. Measured, single precision, us: 65536 rows of 128 experts, 8 chosen 15.7 (2 chosen 11.5), gradient 14.7 (67 MB, 4.6 TB/s); 65536 of
-// 16, 2 chosen 5.6 and 4.8; 8192 of 1024, 8 chosen 17.6 and 19; 500 of 2000, which no wavefront holds, 16.7 and 8.8; bfloat16, 24 rows of 64 2.5. By a
+// it came from. Measured, single precision, us: 65536 rows of 128 experts, 8 chosen 15.8 (2 chosen 12.0), gradient 15.0 (72 MB, 4.8 TB/s); 65536 of
+// 16, 2 chosen 5.9 and 5.8; 8192 of 1024, 8 chosen 17.8 and 19.6; 500 of 2000, which no wavefront holds, 17.3 and 9.2; bfloat16, 24 rows of 64 2.6. By a
 // search for the largest key and its entry in every step the first of them took 20.4, its gradient with a division for every logit 17.2.
 
 #include <qmlp/kernels/token_types.h>

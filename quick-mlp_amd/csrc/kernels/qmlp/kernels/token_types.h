@@ -1,6 +1,6 @@
 #pragma once
 // Element types and vector accesses shared by the operators on rows of tokens (layer_norm.h, embedding.h, row_groups.h,
-// grouped_linear.h). Values are read and written in float, half or bfloat16 and computed in float.
+// grouped_linear.h, route.h, expert_rows.h, mx4.h). Values are read and written in float, half or bfloat16 and computed in float.
 
 #include <qmlp/kernels/common.h>
 
