@@ -32,7 +32,7 @@ typedef struct qmlp_activation_s* qmlp_activation_t;
 
 /* qmlp::Tensor::Precision / ::Usage (src_cpp/include/qmlp/tensor.h:25-38) */
 enum { QMLP_FLOAT = 0, QMLP_HALF = 1, QMLP_DOUBLE = 2 };
-/* Further types of the operators on rows of tokens (qmlp_tokens_*); everything else refuses them. */
+/* Further types of the operators on rows of tokens (qmlp_tokens_*), whose results share no memory with arguments; everything else refuses them. */
 enum { QMLP_BFLOAT16 = 3, QMLP_INT32 = 4, QMLP_INT64 = 5, QMLP_UINT8 = 6 };
 enum { QMLP_INFERENCE = 0, QMLP_GRADIENTS = 1 };
 /* qmlp::FusedNetwork::AdjointMode (src_cpp/include/qmlp/fused_network.h:22-33) */

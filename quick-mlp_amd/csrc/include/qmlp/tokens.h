@@ -11,6 +11,7 @@ QUICKMLP_NAMESPACE_BEGIN
  *
  * Values are float, half or bfloat16, sums are held in float and rounded once. Rows are the first dimension; the last one has
  * to be consecutive in memory (stride 1), the others may have any stride that is not negative. Indices are 32- or 64-bit integers.
+ * Results share no memory with arguments.
  * Channels, inputs, outputs and the rows of experts are no more than 2^31 - 2^12.
  *
  * Every call only enqueues kernels on the stream: it allocates nothing, does not wait and can be captured into a graph once its kernels are

@@ -8,9 +8,9 @@
 //
 // What bounds them. Few rows: the weights that are read (24 rows of 64 experts, 1024 -> 4096, bfloat16: 11 us for 54 MB, 4.8 TB/s). Many rows: what the
 // matrix cores take from LDS, and their own rate at the clock that the power allows. 32768 rows of 16 experts, 2048 -> 4096, bfloat16: 199 us, 2.8
-// PFLOP/s, behind 28 us that quantise the rows. The same tiles with 8192 inputs take 680 us, without the loads to LDS 519, without the reads from it
-// 626, with the products alone, without barriers too, 448 (4.9 PFLOP/s; operands that stay the same reach 7.6), with a third more reads, by wavefronts of 64 x 64, 964. Tiles of
-// K that were in the L2 already save nothing with 2048 inputs.
+// PFLOP/s, behind 28 us that quantise the rows; 159 without the stores. The same tiles with 8192 inputs take 680 us, without the loads to LDS 519,
+// without the reads from it 626, with the products alone, without barriers too, 448 (4.9 PFLOP/s; operands that stay the same reach 7.6), with a third
+// more reads, by wavefronts of 64 x 64, 964. Tiles of K that were in the L2 already save nothing with 2048 inputs.
 
 #include <qmlp/kernels/grouped_linear.h>
 #include <qmlp/kernels/mx4.h>

@@ -953,6 +953,7 @@ at::Tensor mx4Values(const at::Tensor& codes, const at::Tensor& scales, int64_t 
 {
     refuseRecording();
     checkDevices({&codes, &scales});
+    refuseOtherModes({codes, scales});
     if (codes.dim() < 1 || codes.dim() != scales.dim()) throw std::runtime_error("codes and scales must have the same dimensions");
     if (codes.sizes().slice(0, codes.dim() - 1) != scales.sizes().slice(0, scales.dim() - 1)) throw std::runtime_error("codes and scales must be of the same rows");
     if (columns < 0) throw py::value_error("columns must not be negative");

@@ -595,6 +595,20 @@ def test_arguments_that_do_not_fit_are_refused():
             call()
 
 
+@gpu
+def test_function_transforms_and_tangents_are_refused():
+    x, places = torch.randn(2, 3, 4, device="cuda"), torch.arange(6, dtype=torch.int32, device="cuda").view(3, 2)
+    for call, v in ((lambda v: tokens.route(v, 2)[0], x), (lambda v: tokens.dispatch(v, places), x),
+                    (lambda v: tokens.combine(v, places), torch.randn(2, 6, 4, device="cuda"))):
+        with pytest.raises(RuntimeError):
+            torch.func.vmap(call)(v)
+        with pytest.raises(RuntimeError):
+            torch.func.grad(lambda t: call(t).sum())(v[0])
+        with torch.autograd.forward_ad.dual_level(), pytest.raises(NotImplementedError):
+            call(torch.autograd.forward_ad.make_dual(v[0], torch.ones_like(v[0])))
+        call(v[0])
+
+
 def test_tensors_on_the_host_are_refused():
     places = torch.zeros(3, 2, dtype=torch.int32)
     for call in (lambda: tokens.route(torch.zeros(3, 4), 2), lambda: tokens.dispatch(torch.zeros(3, 4), places),

@@ -473,6 +473,21 @@ def test_arguments_that_do_not_fit_are_refused():
             call()
 
 
+@gpu
+def test_function_transforms_and_tangents_are_refused():
+    x, offsets = torch.randn(2, 3, 40, device="cuda"), torch.tensor([0, 1, 3], dtype=torch.int32, device="cuda")
+    weight = tokens.quantise_mx4(torch.randn(2, 5, 40, device="cuda"))
+    rows = tokens.quantise_mx4(x)
+    for call in (lambda v: tokens.quantise_mx4(v).codes, lambda v: tokens.mx4_linear(v, weight, offsets)):
+        with pytest.raises(RuntimeError):
+            torch.func.vmap(call)(x)
+        with torch.autograd.forward_ad.dual_level(), pytest.raises(NotImplementedError):
+            call(torch.autograd.forward_ad.make_dual(x[0], torch.ones_like(x[0])))
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda c, s: tokens.Mx4(c, s, 40).dequantise())(rows.codes, rows.scales)
+    assert tokens.mx4_linear(x[0], weight, offsets).shape == (3, 5)
+
+
 def test_tensors_on_the_host_are_refused():
     weight = tokens.Mx4(torch.zeros(1, 5, 16, dtype=torch.uint8), torch.zeros(1, 5, 1, dtype=torch.uint8), 30)
     for call in (lambda: tokens.quantise_mx4(torch.zeros(3, 4)), lambda: weight.dequantise(), lambda: tokens.mx4_linear(torch.zeros(3, 30), weight)):
