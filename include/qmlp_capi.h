@@ -320,7 +320,8 @@ int qmlp_tokens_dispatch(const qmlp_tensor* input, const qmlp_tensor* places, co
  * residual and output (tokens, channels; residual optional). The gradient of qmlp_tokens_dispatch() with neither weights nor residual. */
 int qmlp_tokens_combine(const qmlp_tensor* rows, const qmlp_tensor* places, const qmlp_tensor* weights, const qmlp_tensor* residual,
                         const qmlp_tensor* output, void* stream);
-/* The gradients (each optional); that of the residual is adj_output. */
+/* The gradients (each optional); that of the residual is adj_output. rows are read for adj_weights only and optional without it; weights for
+ * adj_rows. */
 int qmlp_tokens_combine_adjoint(const qmlp_tensor* rows, const qmlp_tensor* places, const qmlp_tensor* weights, const qmlp_tensor* adj_output,
                                 const qmlp_tensor* adj_rows, const qmlp_tensor* adj_weights, void* stream);
 /* Numbers of 4 bits (MXFP4 of the OCP Microscaling Formats specification 1.0) of input (rows, columns), in blocks of 32 entries of a row: codes

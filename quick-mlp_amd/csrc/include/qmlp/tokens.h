@@ -104,7 +104,10 @@ public:
      * \param weights (tokens, chosen), of the rows' type or FLOAT, or undefined: 1 \param residual (tokens, channels), or undefined: 0
      */
     static void combine(const Tensor& rows, const Tensor& places, const Tensor& weights, const Tensor& residual, Tensor& output, stream_t stream);
-    /** Gradients, written as a whole, each of them may be undefined: not wanted. That of the residual is adjOutput. adjWeights: of the weights' type. */
+    /**
+     * Gradients, written as a whole, each of them may be undefined: not wanted. That of the residual is adjOutput. adjWeights: of the weights' type.
+     * \param rows may be undefined where adjWeights is \param weights only adjRows depends on them
+     */
     static void combineAdjoint(const Tensor& rows, const Tensor& places, const Tensor& weights, const Tensor& adjOutput, Tensor& adjRows,
                                Tensor& adjWeights, stream_t stream);
 

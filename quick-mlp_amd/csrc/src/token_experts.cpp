@@ -288,27 +288,29 @@ void Tokens::combine(const Tensor& rows, const Tensor& places, const Tensor& wei
 void Tokens::combineAdjoint(const Tensor& rows, const Tensor& places, const Tensor& weights, const Tensor& adjOutput, Tensor& adjRows, Tensor& adjWeights,
                             stream_t stream)
 {
-    const ExpertRowsSizes s = checkExpertRows(rows, places);
-    checkExpertWeights(weights, "weights", rows, s);
-    checkExpertWeights(adjWeights, "adjWeights", rows, s);
+    const Tensor& like = rows.defined() || adjWeights.defined() ? rows : adjRows;   // (only the weights' gradient reads the rows)
+    const ExpertRowsSizes s = checkExpertRows(like, places);
+    checkExpertWeights(weights, "weights", like, s);
+    checkExpertWeights(adjWeights, "adjWeights", like, s);
     if (weights.defined() && adjWeights.defined()) checkType(adjWeights, "adjWeights", weights.precision());
-    checkTokens(adjOutput, "adjOutput", rows, s);
+    checkTokens(adjOutput, "adjOutput", like, s);
     if (adjRows.defined()) {
         checkValues(adjRows, "adjRows", 2);
-        checkType(adjRows, "adjRows", rows.precision());
-        checkSizes(adjRows, "adjRows", {rows.size(0), s.channels});
+        checkType(adjRows, "adjRows", like.precision());
+        checkSizes(adjRows, "adjRows", {like.size(0), s.channels});
         checkOutput(adjRows, "adjRows");
     }
     if (adjWeights.defined()) checkOutput(adjWeights, "adjWeights");
     if (places.numel() == 0 || (!adjRows.defined() && !adjWeights.defined())) return;
-    const Tensor::Precision p = rows.precision();
+    const Tensor::Precision p = like.precision();
     const int vec = s.vec(p), lanes = s.lanes(p, 64);
     const Tensor& typed = weights.defined() ? weights : adjWeights;
     const int batch = expertRowsBatch(p, s.channels, vec, lanes), split = expertRowsSplit(p, s, vec, lanes);
     tokenKernel("expert_rows.h", kernelKey(COMBINE_ADJOINT, p, vec, lanes, batch),
                 [&] { return str("CombineAdjointKernel<", scalarName(p), ", ", vec, ", ", lanes, ", ", batch, ">"); })
-        .call(workgroups(divUp<int64_t>(s.tokens * split, EXPERT_ROWS_THREADS / lanes), 1 << 20), EXPERT_ROWS_THREADS, 0, stream, rows.rawPtr(), strideOf(rows, 0),
-              static_cast<const int*>(ptr<int>(places)), strideOf(places, 0), s.chosen, static_cast<const void*>(ptr<void>(weights)), strideOrNone(weights),
+        .call(workgroups(divUp<int64_t>(s.tokens * split, EXPERT_ROWS_THREADS / lanes), 1 << 20), EXPERT_ROWS_THREADS, 0, stream,
+              static_cast<const void*>(ptr<void>(rows)), strideOrNone(rows), static_cast<const int*>(ptr<int>(places)), strideOf(places, 0), s.chosen,
+              static_cast<const void*>(ptr<void>(weights)), strideOrNone(weights),
               static_cast<int>(typed.defined() && typed.precision() == Tensor::FLOAT), adjOutput.rawPtr(), strideOf(adjOutput, 0), ptr<void>(adjRows),
               strideOrNone(adjRows), ptr<void>(adjWeights), strideOrNone(adjWeights), s.tokens, s.channels, split);
 }

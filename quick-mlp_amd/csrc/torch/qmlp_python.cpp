@@ -877,22 +877,27 @@ at::Tensor dispatchRows(const at::Tensor& x, const at::Tensor& places)
     return output;
 }
 
+/** Saved: places; the rows for the weights' gradient and the weights for the rows', where those are wanted. */
 struct CombineBackward : TokenNode
 {
+    at::ScalarType weightType = at::kFloat;
     std::string name() const override { return "QmlpCombineBackward"; }
     void adjoint(const at::Tensor& gradOutput, const variable_list& tensors, variable_list& grads) override
     {
-        const at::Tensor rows = consecutive(tensors[0]), places = asRows(tensors[1]), adjOutput = asRows(gradOutput);
+        const bool wantsRows = task_should_compute_output(0), wantsWeights = task_should_compute_output(1);
+        if (task_should_compute_output(2)) grads[2] = gradOutput;
+        if (!wantsRows && !wantsWeights) return;
+        const at::Tensor places = asRows(tensors[0]), adjOutput = asRows(gradOutput), rows = consecutive(tensors[1]);
         const at::Tensor weights = tensors[2].defined() ? asRows(tensors[2]) : at::Tensor();
+        const auto options = adjOutput.options().requires_grad(false);
         at::Tensor adjRows, adjWeights;
-        if (task_should_compute_output(0)) adjRows = at::empty(rows.sizes(), rows.options().requires_grad(false));
-        if (task_should_compute_output(1)) adjWeights = at::empty(weights.sizes(), weights.options().requires_grad(false));
+        if (wantsRows) adjRows = at::empty({places.numel(), adjOutput.size(1)}, options);
+        if (wantsWeights) adjWeights = at::empty(places.sizes(), options.dtype(weightType));
         const qmlp_tensor in = wrapToken(rows), p = wrapToken(places), w = wrapToken(weights), dy = wrapToken(adjOutput), dr = wrapToken(adjRows),
                           dw = wrapToken(adjWeights);
-        check(qmlp_tokens_combine_adjoint(&in, &p, &w, &dy, &dr, &dw, currentStream(rows)));
+        check(qmlp_tokens_combine_adjoint(&in, &p, &w, &dy, &dr, &dw, currentStream(adjOutput)));
         grads[0] = adjRows;
-        if (adjWeights.defined()) grads[1] = shaped(adjWeights, tensors[2].sizes());
-        if (task_should_compute_output(2)) grads[2] = gradOutput;
+        if (wantsWeights) grads[1] = shaped(adjWeights, tensors[0].sizes());
     }
 };
 
@@ -914,7 +919,11 @@ at::Tensor combine(const at::Tensor& rows, const at::Tensor& places, const at::T
         check(qmlp_tokens_combine(&in, &pt, &wt, &xt, &o, currentStream(rows)));
         return shaped(out, sizes);
     });
-    if (wantsGradient(rows) || wantsGradient(weights) || wantsGradient(residual)) attach<CombineBackward>(output, {rows, weights, residual}, {rows, places, weights});
+    const bool trainRows = wantsGradient(rows), trainWeights = wantsGradient(weights);
+    if (trainRows || trainWeights || wantsGradient(residual)) {
+        auto node = attach<CombineBackward>(output, {rows, weights, residual}, {places, trainWeights ? rows : at::Tensor(), trainRows ? weights : at::Tensor()});
+        if (weights.defined()) node->weightType = weights.scalar_type();
+    }
     return output;
 }
 

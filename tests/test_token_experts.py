@@ -528,6 +528,43 @@ def test_an_index_that_was_changed_has_no_gradient():
 
 
 @gpu
+@pytest.mark.parametrize("weighted", [False, True])
+def test_combine_keeps_only_what_its_gradients_read(weighted):
+    """Rows are read for the weights' gradient, weights for the rows': what no wanted gradient reads may change, and is not held."""
+    g = generator(8)
+    places = places_of(g, 30, 2)
+    place, token, has, _ = rows_reference(places, 5)
+    values = {"rows": normal(g, 60, 5), "weights": normal(g, 30, 2) if weighted else None, "residual": normal(g, 30, 5)}
+    dy = normal(g, 30, 5)
+    flat = values["weights"].flatten()[has].double()[:, None] if weighted else 1.0
+    drows, dweights, size = (torch.zeros(60, n, dtype=torch.float64, device="cuda") for n in (5, 1, 1))
+    drows[place] = dy[token].double() * flat
+    products = dy[token].double() * values["rows"][place].double()
+    dweights[has], size[has] = products.sum(1, keepdim=True), products.abs().sum(1, keepdim=True)
+    expected = {"rows": (drows, U * drows.abs()), "weights": (dweights.view(30, 2), 9 * U * size.view(30, 2)), "residual": (dy.double(), torch.zeros_like(dy))}
+    reads = {"rows": {"weights"}, "weights": {"rows"}, "residual": set()}
+    for wanted in ("rows", "weights", "residual")[::1 if weighted else 2]:
+        for changed in ("rows", "weights", "residual")[::1 if weighted else 2]:
+            given = {name: v.clone() if v is not None else None for name, v in values.items()}
+            given[wanted].requires_grad_()
+            y = tokens.combine(given["rows"], places, given["weights"], given["residual"])
+            with torch.no_grad():
+                given[changed].fill_(float("nan"))
+            if changed in reads[wanted]:
+                with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                    torch.autograd.grad(y, given[wanted], dy)
+            else:
+                near(torch.autograd.grad(y, given[wanted], dy)[0], *expected[wanted], wanted)
+    rows = torch.zeros(60, 1 << 16, device="cuda")   # 16 MB
+    residual = torch.zeros(30, 1 << 16, device="cuda", requires_grad=True)
+    y = tokens.combine(rows, places, values["weights"], residual)
+    held = torch.cuda.memory_allocated()
+    del rows
+    assert held - torch.cuda.memory_allocated() >= 60 << 18
+    assert y.grad_fn is not None
+
+
+@gpu
 def test_no_kernel_is_compiled_late():
     """Calls of every kind of size find their kernels where qmlp.tokens.precompile left them."""
     g = generator(70)
@@ -654,3 +691,16 @@ def test_c_interface_refuses_before_any_launch():
     order, offsets = descriptor(I, 8), descriptor(I, 4)
     refused(lib.qmlp_tokens_group_places(descriptor(I, 8), 3, order, offsets, descriptor(I, 7), None, None), "must have 8 entries")
     refused(lib.qmlp_tokens_group_places(descriptor(I, 8), 3, order, offsets, descriptor(F, 8), None, None), "must be of type INT32")
+
+
+def test_gradients_of_combine_refuse_missing_rows():
+    """Rows are needed for the weights' gradient; without it the rows' gradient has the sizes (these calls need no device)."""
+    lib, F, I = _lib.lib, _lib.QMLP_FLOAT, _lib.QMLP_INT32
+    none, places, dy, drows, w = _lib.TensorDesc(), descriptor(I, 4, 2), descriptor(F, 4, 6), descriptor(F, 8, 6), descriptor(F, 4, 2)
+    adjoint = lambda *a: lib.qmlp_tokens_combine_adjoint(*a, None)  # noqa: E731
+    refused(adjoint(none, places, w, dy, drows, w), "rows is undefined")
+    refused(adjoint(none, places, w, dy, none, none), "rows is undefined")
+    refused(adjoint(none, places, w, dy, descriptor(F, 7, 6), none), "must have 8 entries")
+    refused(adjoint(none, places, w, descriptor(F, 4, 5), drows, none), "must have 6 entries")
+    refused(adjoint(none, places, descriptor(_lib.QMLP_HALF, 4, 2), dy, drows, none), "rows' type or FLOAT")
+    refused(adjoint(none, places, none, dy, descriptor(F, 8, 6, strides=(3, 1)), none), "share memory")
