@@ -137,6 +137,35 @@ def test_masked_experts_are_taken_by_no_row(experts, normalised, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("experts", [8, 33, 200, 500, 1024, 1025])
+@pytest.mark.parametrize("normalised", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_weights_below_the_normal_numbers(experts, normalised, dtype):
+    """Shares from 2^-115 down to the smallest number there is: the exponential and its quotient are each off by half of 2^-149 besides what they are
+    relative to their size. In gradients up to 1024 experts count shares below 2^-126 as 0."""
+    logits = torch.full((3, experts), -200.0)
+    logits[0, :8] = torch.tensor([0.0, -80.0, -87.25, -87.5, -90.0, -95.0, -100.0, -103.0])
+    logits[1, :8] = torch.tensor([-0.5, -60.0, -86.0, -88.0, -93.0, -97.0, -101.5, -102.5])
+    logits[2, -8:] = torch.tensor([-102.0, -99.0, -98.0, -94.0, -92.0, -89.0, -87.0, 1.0])
+    logits = logits.to(dtype).cuda().requires_grad_()
+    grad = (torch.tensor([1.0, -2.0, 3.0, -1.0, 2.0, -3.0, 1.0, 4.0]) * torch.tensor([1.0] + [2.0 ** 30] * 7)).to(dtype).expand(3, 8).contiguous().cuda()
+    weights, index = tokens.route(logits, 8, normalised)
+    dlogits, = torch.autograd.grad(weights, logits, grad)
+    w, e_w, expected, dl, _ = route_reference(logits.detach(), 8, normalised, grad)
+    assert torch.equal(index, expected)
+    near(weights.detach(), w, e_w - 2.0 ** -126 + 2.0 ** -150, "weights")
+    relative = 2 * (220 + experts + 8 + 16) * U
+    l = logits.detach().double()
+    p = torch.exp(l - l.max(1, keepdim=True)[0])
+    p = p / torch.gather(p, 1, index.long()).sum(1, keepdim=True) if normalised else p / p.sum(1, keepdim=True)
+    full = torch.zeros_like(l).scatter_(1, index.long(), grad.double())
+    size = full.abs() + 2 * (p * full).abs().sum(1, keepdim=True)
+    near(dlogits, dl, (p * relative + (2.0 ** -126 if experts <= 1024 else 2.0 ** -149)) * size, "gradient")
+    if dtype == torch.float32:
+        assert int((weights > 0).sum()) == 24 and int((weights < 2.0 ** -126).sum()) == 17
+
+
+@gpu
 @pytest.mark.parametrize("experts", [5, 64, 300, 1024, 3000])
 def test_rows_that_are_not_numbers_stay_alone(experts):
     g = generator(experts + 1)
