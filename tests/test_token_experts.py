@@ -206,6 +206,22 @@ def test_route_takes_any_shape_and_stride():
             near(dlogits.reshape(-1, logits.shape[-1]), dl, e_dl, "gradient")
 
 
+@gpu
+@pytest.mark.parametrize("rows,experts,chosen", [(65536 * 32 + 33, 3, 2), (4096 + 5, 1025, 3)])
+@pytest.mark.parametrize("normalised", [False, True])
+def test_more_rows_than_workgroups_of_a_launch(rows, experts, chosen, normalised):
+    """The kernels go on in steps of the grid: 65536 workgroups of 32 rows, 4096 of a row where no wavefront holds one."""
+    g = generator(rows)
+    logits = normal(g, rows, experts, dtype=torch.float16).requires_grad_()
+    grad = normal(g, rows, chosen, dtype=torch.float16)
+    weights, index = tokens.route(logits, chosen, normalised)
+    dlogits, = torch.autograd.grad(weights, logits, grad)
+    w, e_w, expected, dl, e_dl = route_reference(logits.detach(), chosen, normalised, grad)
+    assert torch.equal(index, expected)
+    near(weights.detach(), w, e_w, "weights")
+    near(dlogits, dl, e_dl, "gradient")
+
+
 # ------------------------------------------------------------------------------------------------ rows to experts and back
 def places_of(g, tokens_, chosen, dropped=0.1):
     index = torch.randint(0, 6, (tokens_, chosen), device="cuda", generator=g)
@@ -336,6 +352,24 @@ def test_rows_of_more_than_two_to_the_31_entries():
     assert bool((dx[0] == 6).all()) and bool((dx[-1] == 10).all()) and int(torch.count_nonzero(dx)) == 2 * channels
     drows, = torch.autograd.grad(y.sum(), [y.grad_fn.next_functions[0][0].variable])
     assert bool((drows[-1] == 0.5).all()) and bool((drows[0] == 2).all())
+
+
+@gpu
+def test_more_tokens_than_workgroups_of_a_launch():
+    """2^20 workgroups of 32 tokens, and a second turn."""
+    tokens_ = (1 << 25) + 37
+    places = torch.arange(tokens_, dtype=torch.int32, device="cuda").flip(0).view(tokens_, 1).contiguous()
+    x = (torch.arange(tokens_, device="cuda") % 251).half().view(tokens_, 1).requires_grad_()
+    rows = tokens.dispatch(x, places)
+    assert torch.equal(rows.detach(), x.detach().flip(0))
+    dx, = torch.autograd.grad(rows, x, x.detach())
+    assert torch.equal(dx, x.detach().flip(0))
+    r, w = rows.detach().requires_grad_(), (torch.arange(tokens_, device="cuda") % 4).half().view(tokens_, 1).requires_grad_()
+    y = tokens.combine(r, places, w)
+    assert torch.equal(y.detach(), w.detach() * x.detach())   # (products of numbers of 8 and 2 bits: exact)
+    drows, dweights = torch.autograd.grad(y, (r, w), x.detach())
+    assert torch.equal(drows, (w.detach() * x.detach()).flip(0))
+    assert torch.equal(dweights, (x.detach().float() ** 2).half())   # (below 2^16; one rounding)
 
 
 @gpu

@@ -320,6 +320,62 @@ def test_layers_of_other_strides(dtype):
 
 
 @gpu
+@pytest.mark.parametrize("block", [0, 1, 3])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_weights_that_begin_at_any_block_of_others(block, dtype):
+    """Parts of wider matrices of codes, whose scales then begin at any byte, of all experts or of every other one."""
+    g = generator(15 + block)
+    counts = [70, 0, 200, 31]
+    wide = normal(g, 310, 200, dtype=dtype)
+    stack = tokens.quantise_mx4(normal(g, 8, 90, 192))
+    for x in (wide[:, 1:65], wide[5:, :64]):
+        x = x[:301]
+        for part in (slice(0, 4), slice(1, 8, 2)):
+            weight = tokens.Mx4(stack.codes[part, 5:72, 16 * block:16 * block + 32], stack.scales[part, 5:72, block:block + 2], 64)
+            packed = tokens.Mx4(weight.codes.contiguous(), weight.scales.contiguous(), 64)
+            exact, error = linear_reference(tokens.quantise_mx4(x).dequantise().double(), packed.dequantise().double(), counts, None)
+            near(tokens.mx4_linear(x, weight, offsets_of(counts)), exact, error, "y")
+
+
+@gpu
+@pytest.mark.parametrize("counts,outputs", [([2, 1], 40), ([37, 70, 0, 5], 72), ([900, 0, 2101], 300)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_of_codes_of_other_strides(counts, outputs, dtype):
+    """Rows that are numbers of 4 bits already: parts of wider ones, every other one, one and the same, codes at odd addresses."""
+    say("codes of rows", counts, outputs, dtype)
+    g = generator(16 + outputs)
+    rows = sum(counts) + 3
+    stack, weight = tokens.quantise_mx4(normal(g, 2 * rows + 4, 700)), tokens.quantise_mx4(normal(g, len(counts), outputs, 600))
+    bias = normal(g, len(counts), outputs, dtype=dtype)
+    odd = torch.zeros(rows * 19 * 16 + 1, dtype=torch.uint8, device="cuda")[1:].view(rows, 19 * 16)
+    odd.copy_(stack.codes[:rows, :19 * 16])
+    odd_row = torch.zeros(rows, 19 * 16 + 8, dtype=torch.uint8, device="cuda")[:, :19 * 16]
+    odd_row.copy_(stack.codes[:rows, :19 * 16])
+    one = lambda t: t[3:4].expand(rows, t.shape[1])  # noqa: E731
+    # (codes of 600 of the 700 columns: the last 8 numbers of block 18 meet weights that are zeros)
+    for codes, scales in ((stack.codes[1:rows + 1, :19 * 16], stack.scales[1:rows + 1, :19]), (stack.codes[3:2 * rows + 3:2, 16:20 * 16], stack.scales[3:2 * rows + 3:2, 1:20]),
+                          (odd, stack.scales[:rows, :19]), (odd_row, stack.scales[:rows, :19]), (one(stack.codes[:, :19 * 16]), one(stack.scales[:, :19]))):
+        values = tokens.Mx4(codes.contiguous(), scales.contiguous(), 600).dequantise().double()
+        exact, error = linear_reference(values, weight.dequantise().double(), counts, bias)
+        near(tokens.mx4_linear(tokens.Mx4(codes, scales, 600), weight, offsets_of(counts), bias, dtype), exact, error, "y")
+
+
+@gpu
+@pytest.mark.parametrize("inputs", [40, 700])
+@pytest.mark.parametrize("experts", [65, 128, 513, 4096, 4097])
+def test_more_experts_than_rows(experts, inputs):
+    """Tiles begin at the first rows of experts, which are found among all of them: the first, the last, some in between, of more than a tile."""
+    say("experts", experts, inputs)
+    counts = [0] * experts
+    for e, n in ((0, 3), (1, 1), (experts // 2, 17), (experts // 2 + 1, 2), (experts - 2, 1), (experts - 1, 20)):
+        counts[e] += n
+    for dtype in (torch.float32, torch.bfloat16):
+        check_linear(counts, inputs, 24, dtype, experts + inputs, 3)
+    counts[0], counts[experts - 1], counts[63] = 0, 0, 16
+    check_linear(counts, inputs, 24, torch.float16, experts + inputs, 0, False)
+
+
+@gpu
 @pytest.mark.parametrize("offsets", [[0, 50, 1 << 30, 1 << 30, 1 << 30], [0, -5, -7, 1000, 20], [90, 80, 70, 60, 50], [2 ** 31 - 1] * 5, [-2 ** 31] * 5,
                                      [0, 33, 33, 64, 97]])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
