@@ -11,7 +11,7 @@
 // All of them are bound by memory, and go by token: what a token has of its own (x, dy) is read once, however many experts it has. Results are stored
 // past the L2. Where there are few tokens, workgroups share out their columns, wavefronts of the adjoint kernel their rows. Measured, us: 32768 tokens
 // of 2 experts, 2048 channels, bfloat16 70 (dispatch, 403 MB, 5.8 TB/s), 72 (its gradient), 91 (combine with residual, 537 MB, 5.9 TB/s), 121 (its
-// gradients, 671 MB, 5.5 TB/s); 5003 tokens of 3, 333 floats 8.5 (combine), 11 (gradients); 24 tokens of 2, 1024 channels, bfloat16 2.8 and 3.2.
+// gradients, 671 MB, 5.5 TB/s); 5003 tokens of 3, 333 floats 8.1 (combine), 10.8 (gradients); 24 tokens of 2, 1024 channels, bfloat16 2.8 and 3.2.
 
 #include <qmlp/kernels/token_types.h>
 

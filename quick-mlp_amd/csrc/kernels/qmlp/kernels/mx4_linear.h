@@ -6,7 +6,8 @@
 // The matrix cores multiply blocks of 32 codes with their scales: an operand has a block of a row in each lane, 16 bytes and a byte of scale, as
 // they lie in memory. Sums are held in floats.
 //
-// What bounds them. Few rows: the weights that are read (24 rows of 64 experts, 1024 -> 4096, bfloat16: 11 us for 54 MB, 4.8 TB/s). Many rows: what the
+// What bounds them. Few rows: the weights that are read, 2.2 MB for every expert that has rows of 1024 -> 4096, bfloat16: 3.8 us for one expert, 6.6 for
+// 8, 11.4 for 17, 14.7 for 23 (4.6 TB/s behind the 3.3 that a launch, the offsets and the first loads take). Many rows: what the
 // matrix cores take from LDS, and their own rate at the clock that the power allows. 32768 rows of 16 experts, 2048 -> 4096, bfloat16: 199 us, 2.8
 // PFLOP/s, behind 28 us that quantise the rows; 159 without the stores. The same tiles with 8192 inputs take 680 us, without the loads to LDS 519,
 // without the reads from it 626, with the products alone, without barriers too, 448 (4.9 PFLOP/s; operands that stay the same reach 7.6), with a third

@@ -5,11 +5,15 @@
 //   normalised: w = softmax over the chosen ones alone.  An expert whose logit is -inf is taken by no row: index -1 and w 0 in its place.
 //   dl = p (G - sum over j of g[j] w[j]),  G the g[j] at their experts;  normalised: the same with p = 0 at experts that were not chosen
 //
-// A row lies in the registers of 8 to 64 lanes, so that reading it is one access each, and every lane sorts what it has. What bounds the forward pass
-// then is the choice, one after the other: the largest of the lanes' first keys by operations between neighbouring lanes, and a step of the list
-// it came from. Measured, single precision, us: 65536 rows of 128 experts, 8 chosen 15.8 (2 chosen 12.0), gradient 15.0 (72 MB, 4.8 TB/s); 65536 of
-// 16, 2 chosen 5.9 and 5.8; 8192 of 1024, 8 chosen 17.8 and 19.6; 500 of 2000, which no wavefront holds, 17.3 and 9.2; bfloat16, 24 rows of 64 2.6. By a
-// search for the largest key and its entry in every step the first of them took 20.4, its gradient with a division for every logit 17.2.
+// A row lies in the registers of 8 to 64 lanes, so that reading it is one access each, and every lane sorts what it has. A choice then is the largest
+// of the lanes' first keys by operations between neighbouring lanes, and a step of the list it came from.
+//
+// What bounds the forward pass is what a row takes besides its bytes and choices: 65536 rows of 128 floats with 1, 2, 4, 8 chosen take 11.9, 12.1, 13.3,
+// 15.9 us, 0.6 a choice and 11 without any, of which the bytes would be 7; of bfloat16, half the bytes, 10.3 and 13.2 with 1 and 8. Keys, sort and
+// exponentials of a row follow each other, and a wavefront has no other row under way. The gradient is bound by memory: 14.9 (72 MB, 4.8 TB/s).
+// Others, single precision, us forward and gradient: 65536 of 16, 2 chosen 5.6 and 5.6; 8192 of 1024, 8 chosen 18.3 and 19.0; 500 of 2000, which no
+// wavefront holds and which is read again for every choice, with two barriers, 17.1 (1 chosen 6.1) and 9.1; bfloat16, 24 rows of 64 2.6. By a search for
+// the largest key and its entry in every step 65536 of 128, 8 chosen, took 20.4, its gradient with a division for every logit 17.2.
 
 #include <qmlp/kernels/token_types.h>
 

@@ -106,7 +106,11 @@ __device__ __forceinline__ void markSpans(const unsigned* keys, long long i, lon
     if (i == rows - 1 || keys[i + 1] != key) spans[groups + key] = static_cast<unsigned>(i + 1);
 }
 
-/** What is kept of a row's place in the order: the place itself; -1 - place of rows that belong to no group. */
+/**
+ * What is kept of a row's place in the order: the place itself; -1 - place of rows that belong to no group. Its store goes to a line of its own where rows
+ * next to each other in the order lie apart: us of all kernels without | with places 4.8 | 4.9 for 48 rows, 13.1 | 15.2 for 8192 of 64 groups, 16.2 | 16.5
+ * for 2^19 of 128, 28 | 29 for 2^20 of 4096, 58 | 72 for 2^20 of 70000, whose second pass takes rows in the order of the first.
+ */
 __device__ __forceinline__ int placeOf(unsigned key, unsigned groups, unsigned place)
 {
     return static_cast<int>(key < groups ? place : ~place);

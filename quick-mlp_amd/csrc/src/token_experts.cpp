@@ -162,16 +162,21 @@ struct Mx4Plan
     bool inPlace = false;   // the product's workgroups quantise the rows, each for its own outputs
 };
 /**
- * How the product of 'rows' rows, 'blocks' blocks each, with J outputs of every expert is made. us with rows that are codes | with values, bfloat16,
- * rows, experts, inputs, outputs:
- * Few rows or tiles: the weights straight from memory, one wavefront or four for a chunk of K; then tiles of 64. 24, 64, 1024, 4096: 14.6 | 14.9 in
- * place, 16.9 before; 15.3 | 16.0; 19.9 | 22.2. 256, 64, 1024, 4096: 33.9 | 38.7, 36.3; 37.8 | 46.6; 32.0 | 34.5. 16, 1, 4096, 4096: 9.6 | 17.3,
- * 12.7; 6.3 | 13.9, 9.5; 12.4 | 15.0. 60, 4, 2048, 2048: 6.3 | 10.1, 9.0; 5.8 | 9.8, 8.2; 6.7 | 10.1. 32, 1, 1024, 1024: 4.6 | 6.5, 7.0; 4.0 |
- * 5.7, 6.3; 5.1 | 8.0. 200, 100, 200, 300: 5.2 | 6.1, 7.7; 6.7 | 8.2; 6.0 | 8.6.
- * Tiles of 64, 128 and 256, codes: 5003, 12, 333, 200: 6.3, 7.2, 10.5; 256, 1, 4096, 4096: 10.4, 17.8, 28; 6400, 64, 512, 512: 8.6, 7.5, 9.7; 3200,
- * 64, 2048, 2048: 33, 37, 52; 6400, 64, 2048, 2048: 51, 46, 53; 16384, 16, 1024, 1024: 30, 24, 27; 8192, 16, 2048, 4096: 89, 66, 61; 32768, 16,
- * 2048, 4096: 342, 240, 215. Single precision, whose results take too much LDS for tiles of 256: 32768, 16, 2048, 4096: 359, 269; 5003, 12, 333,
- * 200: 6.5, 7.8.
+ * How the product of 'rows' rows, 'blocks' blocks each, with J outputs of every expert is made. us of the call in a captured graph, bfloat16; rows,
+ * experts, inputs, outputs; rows spread evenly at random (23 of 64 experts have some of 24, all of 256, 87 of 100 of 200):
+ * Few rows or tiles: the weights straight from memory, one wavefront for a chunk of K; four of them; tiles of 64. Each with rows that are codes | with
+ * values, quantised in place, before. 24, 64, 1024, 4096: 14.4 | 14.7, 16.9; 14.9 | 15.6, 17.7; 19.3 | 22.1. 8 of them: 5.4 | 5.6, 7.4; 6.3 | 6.6, 8.4;
+ * 10.4 | 12.9. One: 4.3 | 4.5, 6.2; 3.6 | 3.8, 5.5; 6.8 | 8.9. 256, 64, 1024, 4096: 32.8 | 38.0, 36.3; 37.0 | 45.8, 39.4; 32.1 | 34.7. 1, 1, 1024, 1024:
+ * 4.3 | 4.5, 6.2; 3.8 | 3.8, 5.5; 5.0 | 7.2. 1, 1, 4096, 4096: 8.8 | 9.4, 11.0; 5.4 | 6.2, 7.7; 12.4 | 14.4. 8, 1, 4096, 4096: 8.9 | 12.7, 11.3; 5.8 |
+ * 9.6, 8.1; 12.2 | 14.4. 16, 1, 4096, 4096: 9.6 | 17.2, 12.7; 6.4 | 14.0, 9.5; 12.1 | 14.9. 16, 1, 1024, 1024: 4.6 | 6.5, 7.0; 3.9 | 5.7, 6.3; 5.1 | 7.8.
+ * 32, 1, 1024, 1024: 4.6 | 6.5, 6.9; 4.0 | 5.7, 6.3; 5.1 | 7.8. 60, 4, 2048, 2048: 6.3 | 10.1, 9.0; 5.8 | 9.9, 8.2; 6.6 | 10.0. 200, 100, 200, 300:
+ * 5.1 | 6.1, 7.6; 6.6 | 8.1, 9.3; 6.0 | 8.6.
+ * The rule takes the slower side of 8, 64, 1024, 4096 (four wavefronts, 6.6 with values for 5.6), 200, 100, 200, 300 with codes (tiles, 6.0 for 5.1) and
+ * 32, 1, 1024, 1024 with values (before, 6.3 for 5.7).
+ * Tiles of 64, 128 and 256, codes: 5003, 12, 333, 200: 6.3, 7.2, 10.7; 256, 1, 4096, 4096: 10.5, 17.9, 28.4; 6400, 64, 512, 512: 9.0, 7.6, 10.0; 3200,
+ * 64, 2048, 2048: 34, 37, 52; 6400, 64, 2048, 2048: 52, 46, 53; 16384, 16, 1024, 1024: 29.5, 24.0, 26.5; 8192, 16, 2048, 4096: 87, 62, 62; 32768, 16,
+ * 2048, 4096: 306, 204, 183. Single precision, whose results take too much LDS for tiles of 256: 32768, 16, 2048, 4096: 329, 237; 5003, 12, 333,
+ * 200: 6.6, 8.0.
  */
 Mx4Plan mx4Plan(Tensor::Precision p, int64_t rows, int64_t experts, int64_t J, int64_t blocks, bool values, bool direct)
 {

@@ -94,7 +94,7 @@ def dispatch(x: torch.Tensor, places: torch.Tensor) -> torch.Tensor:
 def combine(rows: torch.Tensor, places: torch.Tensor, weights: torch.Tensor = None, residual: torch.Tensor = None) -> torch.Tensor:
     """
     And back: ``residual[...] + sum over j of weights[..., j] * rows[places[..., j]]``, without the terms of no expert. Differentiable in rows,
-    weights and residual.
+    weights and residual; for the backward pass rows are kept where weights want a gradient, weights where rows do.
 
     :param rows: (tokens * chosen, channels)
     :param places: (..., chosen) as for :func:`dispatch`
